@@ -908,6 +908,53 @@ int sdx_controller_update(sdx_ctrl_state* state, int64_t nstate, const int64_t* 
   return hip_status(sdx::launch_controller(a, (hipStream_t)stream), "controller");
 }
 
+// ------------------------------------------------------------------ log probabilities
+size_t sdx_token_logprobs_workspace(int64_t rows, int64_t vocab, int32_t top_n) {
+  if (rows < 1 || vocab < 1 || top_n < 0) return 0;
+  const int parts = sdx::logprob_parts(rows, vocab);
+  if (parts == 1) return 0;
+  return align256((size_t)rows * parts * 16) + (size_t)rows * parts * top_n * sizeof(uint64_t);
+}
+
+int sdx_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld,
+                       float temperature, const int64_t* ids, int32_t n_ids, int32_t top_n,
+                       float* logp, float* entropy, float* top_logp, int64_t* top_ids,
+                       void* workspace, size_t workspace_bytes, sdx_stream_t stream) {
+  if (!dtype_ok(dtype) || rows < 0 || vocab < 1 || ld < vocab || n_ids < 0 || top_n < 0 ||
+      top_n > vocab)
+    return fail(SDX_EINVAL, "sdx_token_logprobs: bad arguments");
+  const float c = 1.4426950408889634f / temperature;
+  if (!(temperature > 0.0f) || !(temperature < INFINITY) || !(c < INFINITY))
+    return fail(SDX_EINVAL, "sdx_token_logprobs: temperature must be positive and finite");
+  if (top_n > sdx::LP_MAX_TOP || vocab > 0x7FFFFFF0)
+    return fail(SDX_EUNSUPPORTED, "sdx_token_logprobs: top_n <= %d and vocab < 2^31 - 16",
+                sdx::LP_MAX_TOP);
+  if (rows > (1 << 23))  // a launch has less than 2^32 threads
+    return fail(SDX_EUNSUPPORTED, "sdx_token_logprobs: more than 2^23 rows");
+  if (rows == 0) return SDX_OK;
+  if (!logits || !entropy || (n_ids > 0 && (!ids || !logp)) ||
+      (top_n > 0 && (!top_logp || !top_ids)))
+    return fail(SDX_EINVAL, "sdx_token_logprobs: bad arguments");
+  if (((uintptr_t)logits % dsize(dtype)) != 0)
+    return fail(SDX_EINVAL, "sdx_token_logprobs: logits not aligned to their type");
+  const size_t need = sdx_token_logprobs_workspace(rows, vocab, top_n);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(SDX_EWORKSPACE, "sdx_token_logprobs: needs a 16-byte aligned workspace of %zu "
+                                "bytes (got %zu)", need, workspace_bytes);
+  sdx::LogprobArgs a = {};
+  a.logits = logits; a.rows = rows; a.V = vocab; a.ld = ld;
+  a.ids = ids; a.n_ids = n_ids; a.top_n = top_n;
+  a.parts = sdx::logprob_parts(rows, vocab);
+  a.T = temperature; a.c = c;
+  a.logp = logp; a.entropy = entropy; a.top_logp = top_logp; a.top_ids = top_ids;
+  Carve w{(uint8_t*)workspace};
+  if (a.parts > 1) {
+    a.part = w.take<float4>((size_t)rows * a.parts);
+    a.part_keys = w.take<uint64_t>((size_t)rows * a.parts * top_n);
+  }
+  return hip_status(sdx::launch_logprob(dtype, a, (hipStream_t)stream), "logprob");
+}
+
 // ------------------------------------------------------------------ proposer
 int sdx_argmax(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld,
                int64_t* ids, sdx_stream_t stream) {
@@ -988,6 +1035,61 @@ int sdx_kv_append_paged(void* pool, int64_t layer_stride, int64_t side_stride, c
                                                 max_blocks, block_size, num_blocks, lengths, error,
                                                 (hipStream_t)stream),
                     "kv_append_paged");
+}
+
+// ------------------------------------------------------------------ paged layout
+int sdx_build_block_tables(const int64_t* kv_len, int64_t batch, const int32_t* free_blocks,
+                           int64_t num_free, int32_t block_size, int64_t max_blocks,
+                           const int64_t* cu_group, const int64_t* prefix_len, int64_t num_groups,
+                           int32_t* block_table, int64_t* used, int32_t* error,
+                           sdx_stream_t stream) {
+  if (!kv_len || !block_table || batch < 0 || num_free < 0 || (num_free > 0 && !free_blocks) ||
+      block_size < 1 || max_blocks < 1 || (cu_group && (!prefix_len || num_groups < 1)))
+    return fail(SDX_EINVAL, "sdx_build_block_tables: bad arguments");
+  if (batch > (1 << 23) || max_blocks > (1 << 27))  // a launch has less than 2^32 threads
+    return fail(SDX_EUNSUPPORTED, "sdx_build_block_tables: more than 2^23 rows or 2^27 blocks");
+  if (batch == 0) return SDX_OK;
+  sdx::BlockTableArgs a{kv_len, free_blocks, cu_group, prefix_len, batch, num_free, num_groups,
+                        max_blocks, block_size, block_table, used, error};
+  return hip_status(sdx::launch_block_tables(a, (hipStream_t)stream), "block_tables");
+}
+
+int sdx_paged_slot_mapping(const int32_t* block_table, int64_t batch, int64_t max_blocks,
+                           const int64_t* cu_q, const int64_t* kv_len, int32_t block_size,
+                           int64_t num_tokens, int64_t padding_slot, int64_t* positions,
+                           int64_t* slots, int32_t* error, sdx_stream_t stream) {
+  if (!block_table || !cu_q || !kv_len || batch < 0 || num_tokens < 0 || max_blocks < 1 ||
+      block_size < 1 || (num_tokens > 0 && (!positions || !slots)))
+    return fail(SDX_EINVAL, "sdx_paged_slot_mapping: bad arguments");
+  if (max_blocks > ((int64_t)1 << 31) || num_tokens > ((int64_t)1 << 31))
+    return fail(SDX_EUNSUPPORTED, "sdx_paged_slot_mapping: more than 2^31 blocks or tokens");
+  if (num_tokens == 0) return SDX_OK;
+  if (batch == 0)
+    return fail(SDX_EINVAL, "sdx_paged_slot_mapping: %lld tokens of no row", (long long)num_tokens);
+  sdx::PagedSlotArgs a{block_table, cu_q, kv_len, batch, max_blocks, num_tokens, padding_slot,
+                       block_size, positions, slots, error};
+  return hip_status(sdx::launch_paged_slots(a, (hipStream_t)stream), "paged_slots");
+}
+
+int sdx_append_slots(void* pool, int64_t layer_stride, int64_t side_stride, const void* staged,
+                     int dtype, int32_t layers, int64_t num_tokens, int64_t row_elems,
+                     int64_t num_slots, const int64_t* slots, int32_t* error,
+                     sdx_stream_t stream) {
+  if (!pool || !dtype_ok(dtype) || layers < 1 || num_tokens < 0 || row_elems < 1 ||
+      num_slots < 1 || (num_tokens > 0 && (!staged || !slots)))
+    return fail(SDX_EINVAL, "sdx_append_slots: bad arguments");
+  const int64_t es = (int64_t)dsize(dtype);
+  if ((row_elems * es) % 16 != 0 || !aligned16(pool) || !aligned16(staged) ||
+      (layer_stride * es) % 16 != 0 || (side_stride * es) % 16 != 0)
+    return fail(SDX_EINVAL, "sdx_append_slots: rows and strides must be 16-byte multiples");
+  if (layers > 32767 || row_elems > ((int64_t)1 << 30) ||
+      num_tokens > ((int64_t)1 << 33) / (row_elems * es / 16))
+    return fail(SDX_EUNSUPPORTED, "sdx_append_slots: more than 32767 layers or 2^37 staged bytes "
+                                  "per layer and side");
+  if (num_tokens == 0) return SDX_OK;
+  sdx::AppendSlotArgs a{(uint8_t*)pool, (const uint8_t*)staged, slots, layer_stride * es,
+                        side_stride * es, row_elems * es, num_tokens, num_slots, layers, error};
+  return hip_status(sdx::launch_append_slots(a, (hipStream_t)stream), "append_slots");
 }
 
 // ------------------------------------------------------------------ verify attention

@@ -464,4 +464,56 @@ hipError_t launch_slot_mapping(const int32_t* bt, int64_t rows, int64_t max_bloc
                                const int64_t* positions, int32_t bs, int64_t max_len,
                                int64_t pad_slot, int64_t* clamped, int64_t* slots, hipStream_t s);
 
+// sdx_paged.hip
+struct BlockTableArgs {
+  const int64_t* kv_len;        // [batch]
+  const int32_t* free_blocks;   // [num_free] pages to hand out, in order
+  const int64_t* cu_group;      // [groups + 1] rows of a group are consecutive, or null
+  const int64_t* prefix_len;    // [groups] tokens that a group's rows share
+  int64_t batch, num_free, groups, max_blocks;
+  int32_t bs;
+  int32_t* table;               // [batch, max_blocks]
+  int64_t* used;                // [1] pages handed out, or null
+  int32_t* error;
+};
+hipError_t launch_block_tables(const BlockTableArgs& a, hipStream_t s);
+struct PagedSlotArgs {
+  const int32_t* table;         // [batch, max_blocks]
+  const int64_t* cu_q;          // [batch + 1] token offsets
+  const int64_t* kv_len;        // [batch] keys per row, the new tokens included
+  int64_t batch, max_blocks, tokens, padding_slot;
+  int32_t bs;
+  int64_t* positions;           // [tokens]
+  int64_t* slots;               // [tokens]
+  int32_t* error;
+};
+hipError_t launch_paged_slots(const PagedSlotArgs& a, hipStream_t s);
+struct AppendSlotArgs {
+  uint8_t* pool;                // (layer, side) at layer * layer_bytes + side * side_bytes
+  const uint8_t* staged;        // [layers, 2, tokens, row_bytes]
+  const int64_t* slots;         // [tokens]
+  int64_t layer_bytes, side_bytes, row_bytes, tokens, num_slots;
+  int32_t layers;
+  int32_t* error;
+};
+hipError_t launch_append_slots(const AppendSlotArgs& a, hipStream_t s);
+
+// sdx_logprob.hip
+constexpr int LP_MAX_PARTS = 32, LP_MAX_TOP = 64;
+struct LogprobArgs {
+  const void* logits;   // [rows, ld]
+  int64_t rows, V, ld;
+  const int64_t* ids;   // [rows, n_ids]
+  int32_t n_ids, top_n, parts;
+  float T, c;           // temperature, log2(e) / T
+  float* logp;          // [rows, n_ids]
+  float* entropy;       // [rows]
+  float* top_logp;      // [rows, top_n]
+  int64_t* top_ids;
+  void* part;           // [rows, parts] 16-byte records (several parts)
+  uint64_t* part_keys;  // [rows, parts, top_n]
+};
+int logprob_parts(int64_t rows, int64_t V);  // workgroups per row
+hipError_t launch_logprob(int dtype, const LogprobArgs& a, hipStream_t s);
+
 }  // namespace sdx

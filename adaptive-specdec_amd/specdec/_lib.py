@@ -61,6 +61,8 @@ _SIGS = {
                              P]),
     "sdx_round_commit": (INT, [I64, I32, P, P, P, P, P, P, P, I64, P, I32, P, P, P, P, P, P]),
     "sdx_controller_update": (INT, [P, I64, P, I64, P, D, I32, I32, I32, I32, P, P, P, P]),
+    "sdx_token_logprobs_workspace": (SZ, [I64, I64, I32]),
+    "sdx_token_logprobs": (INT, [P, INT, I64, I64, I64, F, P, I32, I32, P, P, P, P, P, SZ, P]),
     "sdx_argmax": (INT, [P, INT, I64, I64, I64, P, P]),
     "sdx_slot_mapping": (INT, [P, I64, I64, P, I32, I64, I64, P, P, P]),
     "sdx_kv_advance": (INT, [P, I64, I64, P]),
@@ -69,6 +71,9 @@ _SIGS = {
     "sdx_attn_mask": (INT, [P, P, I64, I64, I64, F, INT, P, P]),
     "sdx_kv_append_paged": (INT, [P, I64, I64, P, INT, I32, I64, I64, I64, P, I64, I32, I64, P,
                                   P, P]),
+    "sdx_build_block_tables": (INT, [P, I64, P, I64, I32, I64, P, P, I64, P, P, P, P]),
+    "sdx_paged_slot_mapping": (INT, [P, I64, I64, P, P, I32, I64, I64, P, P, P, P]),
+    "sdx_append_slots": (INT, [P, I64, I64, P, INT, I32, I64, I64, I64, P, P, P]),
     "sdx_verify_attention_paged": (INT, [P, INT, I64, P, I32, I32, I32, I32, P, P, I64, I32, P,
                                          I64, P, F, I32, P, SZ, P, P, P]),
     "sdx_verify_attention_workspace": (SZ, [I64, I32, I32, I32, I32, I64, I32]),
@@ -122,6 +127,31 @@ def require_gpu(*tensors):
             raise RuntimeError(
                 "specdec (MI355X build) runs on ROCm device tensors only; got "
                 f"{getattr(t, 'device', type(t))}")
+
+
+def same_device(first, *others):
+    """Every tensor on the first one's device."""
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on several devices: {first.device} and {t.device}")
+
+
+class _Here:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *a):
+        pass
+
+
+_HERE = _Here()
+
+
+def on_device(t):
+    """A context in which t's device is the current one (kernels launch on the current
+    device, whatever stream they are given)."""
+    d = t.device.index
+    return _HERE if d is None or d == torch.cuda.current_device() else torch.cuda.device(d)
 
 
 def ptr(t):

@@ -12,6 +12,11 @@ is the sync-free variant for counts that stay on the device.
 all layers of the target+draft pair share one block table; a step appends
 q candidate positions per row into every layer with one kernel, then commits
 and rolls back by per-row counts without touching K/V bytes.
+
+`build_block_tables` lays out a batch's block tables from its lengths, with the
+pages that the rows of a group share; `paged_slot_mapping` gives the positions
+and slots of a step's packed new tokens (the slot formula of `proposer.py:295-314`
+at a different count per row); `append_paged_slots` writes their K/V there.
 """
 import torch
 
@@ -22,7 +27,8 @@ try:  # HF integration is optional: the cache works standalone
 except Exception:  # pragma: no cover - transformers absent
     _HFCache, _HFLayer = object, object
 
-__all__ = ["RaggedCache", "PagedKVCache"]
+__all__ = ["RaggedCache", "PagedKVCache", "build_block_tables", "paged_slot_mapping",
+           "append_paged_slots"]
 
 
 class _RaggedLayer(_HFLayer):
@@ -289,6 +295,11 @@ class PagedKVCache:
             _lib.ptr(self.error), _lib.stream_of(st))
         _lib.check(rc, "PagedKVCache.append")
 
+    def append_slots(self, staged, slots):
+        """`append` for packed tokens with given slots: staged [L, 2, T, row_elems] -> slots
+        [T] (`append_paged_slots`)."""
+        append_paged_slots(self.pool, staged, slots, error=self.error)
+
     def commit(self, q):
         """lengths += q (`kvcache.py:165-168`)."""
         rc = _lib.lib().sdx_kv_advance(_lib.ptr(self.lengths), self.batch_size, int(q),
@@ -314,3 +325,113 @@ class PagedKVCache:
         """Contiguous [length, row_elems] view of row b's first `length` positions."""
         flat = self.pool[layer, side].reshape(-1, self.row_elems)
         return flat[self.slots(b, length)]
+
+
+def _error_word(error, like):
+    if error is not None and (error.dtype != torch.int32 or error.numel() < 1):
+        raise TypeError("error must be an int32 device tensor of one element")
+    _lib.same_device(like, error)
+
+
+def build_block_tables(kv_len, free_blocks, block_size, max_blocks, cu_group=None, prefix_len=None,
+                       out=None, error=None):
+    """Block tables of a batch from its lengths, on the device.
+
+    kv_len [B] int64: row b gets ceil(kv_len[b] / block_size) pages, taken from free_blocks
+    (int32 page ids) row after row, in order. With cu_group [G+1] and prefix_len [G] (int64)
+    the rows of group g, cu_group[g] .. cu_group[g+1] - 1, share their first prefix_len[g]
+    tokens: the rows after a group's first take over its floor(prefix_len / block_size)
+    whole prefix pages (no more than they need). Returns (block_table [B, max_blocks] int32,
+    -1 behind a row's last page; used [1] int64, the pages taken: free_blocks[used:] are
+    free). All or nothing: lengths, groups or free pages that do not fit give a table of -1
+    and used 0, and set `error` (an int32 [1] device tensor) when given.
+    """
+    _lib.require_gpu(kv_len, free_blocks, cu_group, prefix_len, out, error)
+    _lib.same_device(kv_len, free_blocks, cu_group, prefix_len, out)
+    _error_word(error, kv_len)
+    block_size, max_blocks = int(block_size), int(max_blocks)
+    if (cu_group is None) != (prefix_len is None):
+        raise ValueError("cu_group and prefix_len go together")
+    kl = _lib.as_dtype(kv_len, torch.int64)
+    fb = _lib.as_dtype(free_blocks, torch.int32)
+    B = kl.numel()
+    cu = pl = None
+    G = 0
+    if cu_group is not None:
+        cu, pl = _lib.as_dtype(cu_group, torch.int64), _lib.as_dtype(prefix_len, torch.int64)
+        G = pl.numel()
+        if cu.numel() != G + 1:
+            raise ValueError(f"cu_group has {cu.numel()} offsets, prefix_len {G} groups")
+        if G == 0:
+            if B > 0:
+                raise ValueError(f"{B} rows in no group")
+            cu = pl = None
+    if out is None:
+        out = torch.empty((B, max_blocks), dtype=torch.int32, device=kl.device)
+    elif out.dtype != torch.int32 or tuple(out.shape) != (B, max_blocks) or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous int32 [{B}, {max_blocks}]")
+    if B == 0:
+        return out, torch.zeros(1, dtype=torch.int64, device=kl.device)
+    used = torch.empty(1, dtype=torch.int64, device=kl.device)
+    with _lib.on_device(kl):
+        rc = _lib.lib().sdx_build_block_tables(
+            _lib.ptr(kl), B, _lib.ptr(fb), fb.numel(), block_size, max_blocks, _lib.ptr(cu),
+            _lib.ptr(pl), G, _lib.ptr(out), _lib.ptr(used), _lib.ptr(error), _lib.stream_of(kl))
+    _lib.check(rc, "build_block_tables")
+    return out, used
+
+
+def paged_slot_mapping(block_table, cu_q, kv_len, block_size, num_tokens, padding_slot_id=-1,
+                       error=None):
+    """Positions and slots [num_tokens] (int64) of a step's packed new tokens.
+
+    block_table [B, max_blocks] int32; cu_q [B+1] int64: row b's tokens are cu_q[b] ..
+    cu_q[b+1] - 1, the last of its kv_len[b] (int64) positions. Tokens behind cu_q[B] are
+    padding (position 0, slot padding_slot_id), and so are those of a row whose length or
+    pages are out of range, which set `error` (an int32 [1] device tensor) when given.
+    """
+    _lib.require_gpu(block_table, cu_q, kv_len, error)
+    _lib.same_device(block_table, cu_q, kv_len)
+    _error_word(error, block_table)
+    bt = _lib.as_dtype(block_table, torch.int32)
+    cu = _lib.as_dtype(cu_q, torch.int64)
+    kl = _lib.as_dtype(kv_len, torch.int64)
+    B, T = kl.numel(), int(num_tokens)
+    if bt.dim() != 2 or bt.shape[0] != B or cu.numel() != B + 1:
+        raise ValueError(f"block_table must be [{B}, max_blocks] and cu_q [{B + 1}] for {B} "
+                         f"lengths, got {tuple(bt.shape)} and {cu.numel()} offsets")
+    pos, slots = torch.empty((2, T), dtype=torch.int64, device=bt.device).unbind(0)
+    if T:
+        with _lib.on_device(bt):
+            rc = _lib.lib().sdx_paged_slot_mapping(
+                _lib.ptr(bt), B, bt.shape[1], _lib.ptr(cu), _lib.ptr(kl), int(block_size), T,
+                int(padding_slot_id), _lib.ptr(pos), _lib.ptr(slots), _lib.ptr(error),
+                _lib.stream_of(bt))
+        _lib.check(rc, "paged_slot_mapping")
+    return pos, slots
+
+
+def append_paged_slots(pool, staged, slots, error=None):
+    """Write staged [L, 2, T, row_elems] at rows slots [T] (int64) of every layer and side of
+    pool [L, 2, num_blocks, block_size, row_elems] (contiguous; written in place). Negative
+    slots are padding and skipped; slots past the pool are skipped and set `error` (an int32
+    [1] device tensor) when given."""
+    _lib.require_gpu(pool, staged, slots, error)
+    _lib.same_device(pool, staged, slots)
+    _error_word(error, pool)
+    if pool.dim() != 5 or pool.shape[1] != 2 or not pool.is_contiguous():
+        raise ValueError("pool must be a contiguous [L, 2, num_blocks, block_size, row_elems]")
+    L, _, nb, bs, re = pool.shape
+    T = slots.numel()
+    if tuple(staged.shape) != (L, 2, T, re):
+        raise ValueError(f"staged must be [{L}, 2, {T}, {re}], got {tuple(staged.shape)}")
+    st = _lib.as_dtype(staged, pool.dtype)
+    if st.data_ptr() % 16:
+        st = st.clone()
+    sl = _lib.as_dtype(slots, torch.int64)
+    side = nb * bs * re
+    with _lib.on_device(pool):
+        rc = _lib.lib().sdx_append_slots(
+            _lib.ptr(pool), 2 * side, side, _lib.ptr(st), _lib.dtype_code(pool), L, T, re, nb * bs,
+            _lib.ptr(sl), _lib.ptr(error), _lib.stream_of(pool))
+    _lib.check(rc, "append_paged_slots")

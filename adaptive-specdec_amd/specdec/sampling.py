@@ -26,8 +26,8 @@ import torch
 
 from . import _lib
 
-__all__ = ["to_probs", "sample_from_probs", "residual_probs", "gather_prob", "rejection_sample",
-           "rejection_sample_ragged", "Verifier", "draft_step"]
+__all__ = ["to_probs", "sample_from_probs", "residual_probs", "gather_prob", "token_logprobs",
+           "rejection_sample", "rejection_sample_ragged", "Verifier", "draft_step"]
 
 # per-row flags of the verify calls (the SDX_FLAG_* bits of the C ABI)
 FLAG_ACCEPT_NEAR_TIE = 1   # an evaluated accept test had |u - min(p/q, 1)| < 1e-5
@@ -145,6 +145,60 @@ def gather_prob(probs, ids):
                                _lib.stream_of(p))
         _lib.check(rc, "gather_prob")
     return out.reshape(ids.shape)
+
+
+def token_logprobs(logits, ids, temperature=1.0, top_n=0):
+    """Log probabilities of given tokens with the entropy of their distribution and its
+    likeliest tokens, in one read of the logits: softmax(logits / temperature), no filter.
+
+    logits [..., V] (fp32/bf16/fp16, any row stride and alignment), ids [...] or [..., n].
+    Returns (logp, entropy, top_logp, top_ids): logp fp32 of the shape of ids (-inf at an id
+    outside [0, V)), entropy fp32 [...] in nats, and with top_n > 0 (at most 64 and V) the
+    top_n largest logits' log probabilities and ids [..., top_n], by decreasing value and
+    lowest id first among equals (else None, None). temperature > 0: the greedy limit has no
+    finite scores. Rows without a finite maximum, or with NaN, score NaN.
+    """
+    _lib.require_gpu(logits, ids)
+    _lib.same_device(logits, ids)
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    if tuple(ids.shape) != tuple(lead) and tuple(ids.shape[:-1]) != tuple(lead):
+        raise ValueError(f"ids must be {tuple(lead)} or {tuple(lead)} + (n,), got "
+                         f"{tuple(ids.shape)}")
+    if ids.dtype.is_floating_point or ids.dtype is torch.bool:
+        raise TypeError(f"ids must be whole numbers, got {ids.dtype}")
+    T, top_n = float(temperature), int(top_n)
+    if not 0.0 < T < float("inf"):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not 0 <= top_n <= min(V, 64):
+        raise ValueError(f"top_n must lie in [0, min(64, V = {V})], got {top_n}")
+    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        x = x.float()
+    rows = x.shape[0]
+    if x.stride(1) != 1 or (rows > 1 and x.stride(0) < V):
+        x = x.contiguous()
+    dev = x.device
+    i = _lib.as_dtype(ids, torch.int64)
+    n = 1 if ids.dim() == len(lead) else ids.shape[-1]
+    logp = torch.empty(ids.shape, dtype=torch.float32, device=dev)
+    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+    top_logp = top_ids = None
+    if top_n:
+        top_logp = torch.empty((*lead, top_n), dtype=torch.float32, device=dev)
+        top_ids = torch.empty((*lead, top_n), dtype=torch.int64, device=dev)
+    if rows == 0:
+        return logp, entropy, top_logp, top_ids
+    L = _lib.lib()
+    with _lib.on_device(x):
+        need = L.sdx_token_logprobs_workspace(rows, V, top_n)
+        ws = _lib.cached_workspace(need, dev, "logprobs") if need else None
+        rc = L.sdx_token_logprobs(_lib.ptr(x), _lib.dtype_code(x), rows, V,
+                                  x.stride(0) if rows > 1 else V, T, _lib.ptr(i), n, top_n,
+                                  _lib.ptr(logp), _lib.ptr(entropy), _lib.ptr(top_logp),
+                                  _lib.ptr(top_ids), _lib.ptr(ws), ws.numel() if need else 0,
+                                  _lib.stream_of(x))
+    _lib.check(rc, "token_logprobs")
+    return logp, entropy, top_logp, top_ids
 
 
 def rejection_sample(target_logits, draft_logits, draft_ids, u_accept, u_final, *,

@@ -120,6 +120,25 @@ int sdx_residual_probs(const float* p, const float* q, int64_t rows, int64_t voc
 int sdx_gather_prob(const float* probs, int64_t rows, int64_t vocab, int64_t ld, const int64_t* ids,
                     float* out, sdx_stream_t stream);
 
+/* Log probabilities of given tokens, without the probabilities: logits [rows, ld] (dtype; any
+ * alignment and stride) under softmax(x / temperature), no filter.
+ *   logp [rows, n_ids]      ln softmax at ids [rows, n_ids] (int64; -inf at an id outside the
+ *                           vocabulary)
+ *   entropy [rows]          -sum p ln p in nats (terms of p = 0 are 0)
+ *   top_logp, top_ids       [rows, top_n] the top_n largest logits by decreasing value, the
+ *                           lowest id first among equal ones (-0 == +0), with their ln softmax
+ * all fp32, ids int64. fp32 sums. A row whose logits are all -inf, or that holds a +inf or
+ * NaN, has NaN log probabilities and entropy; its list orders the values all the same, NaN
+ * last (id -1 where a row with NaN leaves none). top_n up to 64 and at most vocab;
+ * temperature positive and finite. Rows split over workgroups keep their parts in the
+ * workspace (16-byte aligned, no initial contents; 0 bytes where rows are many). One kernel,
+ * or two. What to_probs + gather_prob (sampling.py:34-67,93-95) would be composed for. */
+size_t sdx_token_logprobs_workspace(int64_t rows, int64_t vocab, int32_t top_n);
+int sdx_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld,
+                       float temperature, const int64_t* ids, int32_t n_ids, int32_t top_n,
+                       float* logp, float* entropy, float* top_logp, int64_t* top_ids,
+                       void* workspace, size_t workspace_bytes, sdx_stream_t stream);
+
 /* ---- verify: specdec/engine.py:281-312 ----------------------------------
  * The engine's accept block factored out as one call. Inputs:
  *   target_logits [batch, k+1, vocab], draft_logits [batch, k, vocab] (dtype, contiguous),
@@ -348,6 +367,49 @@ int sdx_kv_append_paged(void* pool, int64_t layer_stride, int64_t side_stride,
                         int64_t q, int64_t row_elems, const int32_t* block_table,
                         int64_t max_blocks, int32_t block_size, int64_t num_blocks,
                         const int64_t* lengths, int32_t* error, sdx_stream_t stream);
+
+/* ---- layout of a batch in the paged cache, from its lengths --------------- */
+
+/* Block tables of a batch whose groups share a prefix: row b needs ceil(kv_len[b] /
+ * block_size) pages. Groups are consecutive rows, cu_group [num_groups + 1] int64 from 0 to
+ * batch (null: no row shares); the rows of group g share the prefix_len[g] (int64) first
+ * tokens, and a row that is not its group's first takes over the first row's whole prefix
+ * pages, floor(prefix_len / block_size) of them but no more than it needs. All other pages
+ * come from free_blocks [num_free] int32, row after row, in order. The whole of block_table
+ * [batch, max_blocks] int32 is written, -1 behind a row's last page; *used (nullable, int64)
+ * = pages taken, free_blocks[0 .. used). All or nothing: where a length is negative or past
+ * max_blocks pages, offsets do not run from 0 to batch, a prefix is longer than its group's
+ * first row or the free pages do not suffice, the table is -1 throughout, *used 0 and
+ * *error (nullable, device int32) 1. One kernel, no workspace. No reference counterpart (the
+ * reference leaves block tables to vLLM's host-side manager). */
+int sdx_build_block_tables(const int64_t* kv_len, int64_t batch, const int32_t* free_blocks,
+                           int64_t num_free, int32_t block_size, int64_t max_blocks,
+                           const int64_t* cu_group, const int64_t* prefix_len, int64_t num_groups,
+                           int32_t* block_table, int64_t* used, int32_t* error,
+                           sdx_stream_t stream);
+
+/* Positions and slots of a step's packed new tokens: row b's q_b = cu_q[b+1] - cu_q[b]
+ * tokens (cu_q int64 [batch + 1] from 0) are the last of its kv_len[b] positions; token t of
+ * row b has position kv_len[b] - q_b + (t - cu_q[b]) and slot block_table[b, pos / bs] * bs +
+ * pos % bs, the formula of proposer.py:295-314 with a length per row. positions and slots
+ * [num_tokens] int64. Tokens behind the last row (t >= cu_q[batch]) are padding: position 0,
+ * slot padding_slot. So are the tokens of a row whose length is out of range or whose page
+ * is negative, and those set *error (nullable). */
+int sdx_paged_slot_mapping(const int32_t* block_table, int64_t batch, int64_t max_blocks,
+                           const int64_t* cu_q, const int64_t* kv_len, int32_t block_size,
+                           int64_t num_tokens, int64_t padding_slot, int64_t* positions,
+                           int64_t* slots, int32_t* error, sdx_stream_t stream);
+
+/* sdx_kv_append_paged for packed tokens with given slots (a different number per row):
+ * staged [layers, 2, num_tokens, row_elems] -> row slots[t] (int64, of num_slots =
+ * num_blocks * block_size) of every (layer, side) of the pool. A negative slot is padding
+ * and skipped; a slot of num_slots or more is skipped and sets *error (nullable). Tokens with
+ * the same slot leave a mix of theirs in it. Pool strides, element types and 16-byte rules
+ * as sdx_kv_append_paged. */
+int sdx_append_slots(void* pool, int64_t layer_stride, int64_t side_stride, const void* staged,
+                     int dtype, int32_t layers, int64_t num_tokens, int64_t row_elems,
+                     int64_t num_slots, const int64_t* slots, int32_t* error,
+                     sdx_stream_t stream);
 
 /* ---- verify attention: the target's multi-query attention of one verify
  * forward (bench/bench_engine.py:170-174 -> specdec/engine.py:273-275 through
