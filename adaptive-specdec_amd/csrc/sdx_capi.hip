@@ -1200,4 +1200,68 @@ int sdx_verify_attention_paged(const void* q, int dtype, int64_t batch, const in
   return hip_status(sdx::launch_verify_attn(a, (hipStream_t)stream), "verify_attn");
 }
 
+// ------------------------------------------------------------------ shared prefixes
+size_t sdx_prefix_attention_workspace(int64_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads,
+                                      int32_t head_dim) {
+  if (num_tokens < 1 || num_q_heads < 1 || num_kv_heads < 1 || num_q_heads % num_kv_heads != 0 ||
+      (head_dim != 64 && head_dim != 128))
+    return 0;
+  const size_t parts = sdx::prefix_attn_parts(num_tokens, num_q_heads, num_kv_heads, head_dim);
+  const size_t rows = parts * (size_t)num_tokens * num_q_heads;
+  return 256 + align256(rows * sizeof(float2)) + rows * head_dim * sizeof(float);
+}
+
+int sdx_prefix_attention_paged(const void* q, int dtype, int64_t num_tokens, int64_t batch,
+                               const int64_t* cu_q, int32_t num_q_heads, int32_t num_kv_heads,
+                               int32_t head_dim, const void* k_pool, const void* v_pool,
+                               int64_t num_blocks, int32_t block_size, const int32_t* block_table,
+                               int64_t max_blocks, const int64_t* kv_len, const int64_t* cu_group,
+                               const int64_t* prefix_len, int64_t num_groups, float scale,
+                               void* workspace, size_t workspace_bytes, void* out, int32_t* error,
+                               sdx_stream_t stream) {
+  if (num_tokens < 0 || batch < 0 || num_groups < 0 || num_q_heads < 1 || num_kv_heads < 1 ||
+      block_size < 1 || max_blocks < 1 || num_blocks < 1 || !(scale > 0.0f) || !(scale < INFINITY))
+    return fail(SDX_EINVAL, "sdx_prefix_attention_paged: bad arguments");
+  if (num_q_heads % num_kv_heads != 0)
+    return fail(SDX_EINVAL, "sdx_prefix_attention_paged: query heads must be a multiple of KV heads");
+  if ((dtype != SDX_BF16 && dtype != SDX_F16) || (head_dim != 64 && head_dim != 128))
+    return fail(SDX_EUNSUPPORTED, "sdx_prefix_attention_paged: bf16 or fp16 with head_dim 64 or 128");
+  if (num_tokens == 0) return SDX_OK;
+  if (batch == 0 || num_groups == 0)
+    return fail(SDX_EINVAL, "sdx_prefix_attention_paged: %lld tokens of no row or group",
+                (long long)num_tokens);
+  if (!q || !cu_q || !k_pool || !v_pool || !block_table || !kv_len || !cu_group || !prefix_len || !out)
+    return fail(SDX_EINVAL, "sdx_prefix_attention_paged: null pointer");
+  if (max_blocks > 0x7FFFFFFF / block_size || num_blocks > (int64_t)0xFFFFFFFE / block_size)
+    return fail(SDX_EUNSUPPORTED, "sdx_prefix_attention_paged: rows of 2^31 or a pool of 2^32 - 1 "
+                                  "tokens or more");
+  // query rows index 32-bit tiles, the join's grid has less than 2^32 threads
+  if (num_tokens > ((int64_t)1 << 25) / num_q_heads || batch > (1 << 24) || num_groups > (1 << 24))
+    return fail(SDX_EUNSUPPORTED, "sdx_prefix_attention_paged: more than 2^25 query vectors or 2^24 rows");
+  if (!aligned16(q) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out))
+    return fail(SDX_EINVAL, "sdx_prefix_attention_paged: tensors must be 16-byte aligned");
+  const size_t need = sdx_prefix_attention_workspace(num_tokens, num_q_heads, num_kv_heads, head_dim);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < need)
+    return fail(SDX_EWORKSPACE, "sdx_prefix_attention_paged: needs a 16-byte aligned workspace of %zu "
+                                "bytes (got %zu)", need, workspace_bytes);
+  sdx::PrefixAttnArgs a = {};
+  a.q = (const uint16_t*)q; a.cu_q = cu_q;
+  a.k_pool = (const uint16_t*)k_pool; a.v_pool = (const uint16_t*)v_pool;
+  a.block_table = block_table; a.kv_len = kv_len;
+  a.cu_group = cu_group; a.prefix_len = prefix_len;
+  a.batch = batch; a.groups = num_groups; a.tokens = num_tokens;
+  a.max_blocks = max_blocks; a.num_blocks = num_blocks;
+  a.hq = num_q_heads; a.hkv = num_kv_heads; a.group = num_q_heads / num_kv_heads; a.bs = block_size;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = (uint16_t*)out; a.error = error;
+  a.parts = sdx::prefix_attn_parts(num_tokens, num_q_heads, num_kv_heads, head_dim);
+  a.min_chunk = 2;
+  Carve c{(uint8_t*)workspace};
+  const size_t rows = (size_t)a.parts * num_tokens * num_q_heads;
+  a.head = c.take<int32_t>(2);
+  a.part_ml = c.take<float2>(rows);
+  a.part_o = c.take<float>(rows * head_dim);
+  return hip_status(sdx::launch_prefix_attn(dtype, head_dim, a, (hipStream_t)stream), "prefix_attn");
+}
+
 }  // extern "C"

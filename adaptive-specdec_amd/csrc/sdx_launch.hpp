@@ -516,4 +516,28 @@ struct LogprobArgs {
 int logprob_parts(int64_t rows, int64_t V);  // workgroups per row
 hipError_t launch_logprob(int dtype, const LogprobArgs& a, hipStream_t s);
 
+// sdx_prefix_attn.hip: attention of groups of rows that share a prefix's keys
+struct PrefixAttnArgs {
+  const uint16_t* q;           // [tokens, hq, d] bf16 or fp16
+  const int64_t* cu_q;         // [batch + 1] token offsets
+  const uint16_t* k_pool;      // [num_blocks, bs, hkv * d]
+  const uint16_t* v_pool;
+  const int32_t* block_table;  // [batch, max_blocks]
+  const int64_t* kv_len;       // [batch] keys per row, prefix and new tokens included
+  const int64_t* cu_group;     // [groups + 1] rows of a group are consecutive
+  const int64_t* prefix_len;   // [groups] keys read through the group's first row
+  int64_t batch, groups, tokens, max_blocks, num_blocks;
+  int32_t hq, hkv, group, bs;  // group: query heads per KV head
+  float scale_log2;            // softmax scale * log2(e)
+  uint16_t* out;               // [tokens, hq, d]
+  int32_t* error;
+  int32_t* head;               // [2] tiles per chunk (for the join)
+  float2* part_ml;             // [parts, tokens * hq] max and sum of each part
+  float* part_o;               // [parts, tokens * hq, d]
+  int32_t parts;               // the first half the prefix's, the second the rows' own
+  int32_t min_chunk;           // fewest 64-key tiles per chunk
+};
+int prefix_attn_parts(int64_t tokens, int32_t hq, int32_t hkv, int32_t d);
+hipError_t launch_prefix_attn(int dtype, int d, const PrefixAttnArgs& a, hipStream_t s);
+
 }  // namespace sdx

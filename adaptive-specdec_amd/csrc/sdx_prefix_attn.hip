@@ -1,0 +1,810 @@
+// Attention of a batch whose rows share prefixes over the paged cache, one layer: the
+// multi-query attention of sdx_attn.hip (bench/bench_engine.py:170-174, the mask of
+// specdec/kvcache.py:138-162) for groups of rows that hold a prefix's keys once.
+//
+// out_t = sum_s p_s v_s / sum_s p_s,  p_s = 2^(scale log2(e) q_t k_s - m), over the keys
+// s < P of the group's first row and P <= s of the row itself, s <= kv_len - q_b + j.
+// The two ranges are segments with their own running maximum and sum: a group's prefix
+// against all of the group's queries, a row's own keys against the row's.
+//
+// A segment's query rows (tokens x the query heads of a KV head) against its keys are cut
+// into units: a tile of query rows, a chunk of keys, a KV head. Two forms:
+//   rows > 32   the four waves of a workgroup hold 32 query rows each and share 64-key
+//               tiles in LDS. Bound by the matrix instructions and the exponentials.
+//   rows <= 32  every wave holds the same rows and takes 32 keys of each 128 by itself,
+//               without a workgroup barrier; the waves' results are joined at the end.
+//               Bound by the read of the keys.
+// Both compute S^T = K Q^T with v_mfma_f32_32x32x16: lane l then holds 16 keys' scores of
+// query l % 32, so maxima and sums stay in the lane (one exchange with lane l ^ 32), and
+// the weights, rounded to 16 bits, are the second operand of O^T = V^T P^T as they lie:
+// its 16 keys are contracted in the order in which the scores hold them. V is read from
+// its rows in LDS by the transposing 64-bit reads. The running maximum moves only when a
+// score passes it by 2^8 (weights up to 2^8 lose nothing), which spares rescaling O.
+//
+// Units are dealt to a fixed grid, each XCD a contiguous share of them, so that the units
+// of one chunk of keys read it from one L2. Every workgroup derives the units from the
+// lengths itself: chunk sizes from the total work, then offsets by a scan over segments.
+// A unit leaves (O, max, sum) in fp32, a second kernel joins them; a row without a prefix
+// whose keys fit one unit is written directly.
+#include <algorithm>
+
+#include "sdx_launch.hpp"
+
+namespace sdx {
+
+constexpr int PA_NT = 256;
+constexpr int PA_NW = PA_NT / kWave;
+constexpr int PA_TILE = 64;       // keys per tile of the shared form, and the chunks' unit
+constexpr int PA_STEP = 128;      // keys per step of the other: 32 per wave
+constexpr int PA_ROWS = 128;      // query rows per unit of the shared form
+constexpr int PA_WROWS = 32;      // query rows per wave
+constexpr int PA_GRID = 512;      // two workgroups on each of 256 CUs
+constexpr uint32_t PA_NOSLOT = 0xFFFFFFFFu;
+constexpr float PA_SLACK = 8.0f;  // log2 by which a weight may pass 1
+
+typedef short pa_s4 __attribute__((ext_vector_type(4)));
+typedef uint32_t pa_u4 __attribute__((ext_vector_type(4)));
+typedef __bf16 pa_bf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 pa_h8 __attribute__((ext_vector_type(8)));
+typedef float pa_f16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) pa_s4 pa_lds_s4;
+
+// v_mfma_f32_32x32x16: lane l holds A[l % 32][8 (l / 32) .. + 7], B[8 (l / 32) .. + 7][l % 32]
+// and D[8 (i / 4) + 4 (l / 32) + i % 4][l % 32] in element i.
+template <int FMT>
+__device__ __forceinline__ pa_f16 pa_mfma(pa_u4 a, pa_u4 b, pa_f16 c) {
+  if constexpr (FMT == SDX_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pa_bf8, a),
+                                                   __builtin_bit_cast(pa_bf8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(pa_h8, a),
+                                                  __builtin_bit_cast(pa_h8, b), c, 0, 0, 0);
+}
+// two fp32 rounded to 16 bits (nearest even), x in the low half
+template <int FMT>
+__device__ __forceinline__ uint32_t pa_pack(float x, float y) {
+  if constexpr (FMT == SDX_BF16) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, (b2){(__bf16)x, (__bf16)y});
+  } else {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, (h2){(_Float16)x, (_Float16)y});
+  }
+}
+// the values of lanes l and l ^ 32 in both
+__device__ __forceinline__ float pa_max_halves(float x) {
+  typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+  const u2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pa_sum_halves(float x) {
+  typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+  const u2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// ---- the batch's shape
+
+// the last i in [0, n) with cu[i] <= x, or 0
+__device__ __forceinline__ int64_t pa_find(const int64_t* cu, int64_t n, int64_t x) {
+  int64_t lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int64_t mid = (lo + hi) / 2;
+    if (cu[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+struct PaGroup {
+  int64_t first, rows, prefix;  // rows of the batch, and their shared keys (0 in a group of one)
+  int64_t t0, nt;               // tokens
+  bool ok;
+};
+__device__ __forceinline__ PaGroup pa_group(const PrefixAttnArgs& a, int64_t g) {
+  PaGroup r;
+  const int64_t f = a.cu_group[g], e = a.cu_group[g + 1], p = a.prefix_len[g];
+  r.first = f;
+  r.rows = e - f;
+  r.ok = f >= 0 && e >= f && e <= a.batch && p >= 0 && p <= a.max_blocks * a.bs;
+  r.prefix = r.ok && r.rows > 1 ? p : 0;
+  r.t0 = r.nt = 0;
+  if (r.ok) {
+    const int64_t t0 = a.cu_q[f], t1 = a.cu_q[e];
+    r.ok = t0 >= 0 && t1 >= t0 && t1 <= a.tokens;
+    if (r.ok) r.t0 = t0, r.nt = t1 - t0;
+  }
+  return r;
+}
+struct PaRow {
+  int64_t t0, nt, kv, prefix;
+  bool ok;
+};
+__device__ __forceinline__ PaRow pa_row(const PrefixAttnArgs& a, int64_t b) {
+  PaRow r;
+  const int64_t g = pa_find(a.cu_group, a.groups, b);
+  const PaGroup gr = pa_group(a, g);
+  const int64_t t0 = a.cu_q[b], t1 = a.cu_q[b + 1];
+  r.kv = a.kv_len[b];
+  r.t0 = t0;
+  r.nt = t1 - t0;
+  r.prefix = gr.prefix;
+  r.ok = gr.ok && b >= gr.first && b < gr.first + gr.rows && t0 >= 0 && t1 >= t0 &&
+         t1 <= a.tokens && r.kv >= r.nt && r.kv <= a.max_blocks * a.bs;
+  return r;
+}
+
+// A segment's size: tiles of query rows, 64-key tiles.
+struct PaSeg {
+  int32_t qt, kt;
+  bool shared;  // the form of more than 32 rows
+};
+__device__ __forceinline__ PaSeg pa_seg(const PrefixAttnArgs& a, int64_t nt, int64_t keys) {
+  PaSeg s;
+  const int64_t m = nt * a.group;
+  s.shared = m > PA_WROWS;
+  s.qt = keys > 0 ? (int32_t)((m + PA_ROWS - 1) / PA_ROWS) : 0;
+  s.kt = nt > 0 ? (int32_t)((keys + PA_TILE - 1) / PA_TILE) : 0;
+  return s;
+}
+
+// Work of a 64-key tile, in units of one of the shared form.
+constexpr int PA_COST = 1, PA_COST_ALONE = 2;
+// Tiles per chunk of the two forms, for all segments of a call.
+struct PaChunks {
+  int32_t shared, alone;
+};
+__device__ __forceinline__ int32_t pa_chunk(const PaSeg& s, const PaChunks& c) {
+  return s.shared ? c.shared : c.alone;
+}
+__device__ __forceinline__ int32_t pa_nchunk(const PaSeg& s, const PaChunks& c) {
+  const int32_t n = pa_chunk(s, c);
+  return s.qt > 0 ? (s.kt + n - 1) / n : 0;
+}
+
+// What a workgroup keeps of the batch: the units before each thread's run of segments.
+// Segments 0 .. G - 1 are the groups', G .. G + B - 1 the rows'.
+struct PaPlan {
+  PaChunks chunks;
+  int64_t run;             // segments per thread
+  int64_t units[2];        // in all: of groups, of rows
+  uint32_t before[2][PA_NT + 1];
+  uint64_t red[2][PA_NW + 1];
+  int32_t most;
+  int32_t masked;          // some token does not see its whole prefix
+};
+
+__device__ __forceinline__ PaSeg pa_segment(const PrefixAttnArgs& a, int64_t i, bool* ok,
+                                            bool* masked) {
+  *ok = true;
+  if (i < a.groups) {
+    const PaGroup g = pa_group(a, i);
+    *ok = g.ok;
+    return pa_seg(a, g.ok ? g.nt : 0, g.prefix);
+  }
+  const PaRow r = pa_row(a, i - a.groups);
+  *ok = r.ok;
+  if (!r.ok) return PaSeg{0, 0, false};
+  if (r.nt > 0 && r.kv - r.nt < r.prefix - 1) *masked = true;
+  return pa_seg(a, r.nt, max((int64_t)0, r.kv - r.prefix));
+}
+
+// exclusive scan over the workgroup's threads; total to every thread
+__device__ __forceinline__ uint32_t pa_scan(uint32_t v, uint32_t* wave_sum, uint32_t* total) {
+  const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
+  const uint32_t inc = wave_incl_scan_u32(v, lane);
+  if (lane == kWave - 1) wave_sum[w] = inc;
+  __syncthreads();
+  uint32_t ex = inc - v, t = 0;
+#pragma unroll
+  for (int i = 0; i < PA_NW; ++i) {
+    if (i < w) ex += wave_sum[i];
+    t += wave_sum[i];
+  }
+  *total = t;
+  __syncthreads();
+  return ex;
+}
+
+__device__ __forceinline__ void pa_plan(const PrefixAttnArgs& a, PaPlan& p, bool report) {
+  const int tid = threadIdx.x;
+  const int64_t n = a.groups + a.batch, run = (n + PA_NT - 1) / PA_NT;
+  if (tid == 0) p.most = 0, p.masked = 0;
+  __syncthreads();
+  uint64_t cost = 0;
+  int32_t most = 0;
+  bool masked = false, bad = false;
+  for (int64_t i = tid * run; i < min(n, (tid + 1) * run); ++i) {
+    bool ok;
+    const PaSeg s = pa_segment(a, i, &ok, &masked);
+    bad |= !ok;
+    cost += (uint64_t)s.qt * s.kt * (s.shared ? PA_COST : PA_COST_ALONE);
+    most = max(most, s.kt);
+  }
+  if (tid == 0 && (a.cu_group[0] != 0 || a.cu_group[a.groups] != a.batch)) bad = true;
+  if (bad && report && a.error) *a.error = 1;
+  if (masked) p.masked = 1;
+  atomicMax(&p.most, most);
+  cost = wave_sum_u64(cost);
+  if ((tid & (kWave - 1)) == 0) p.red[0][tid / kWave] = cost;
+  __syncthreads();
+  cost = 0;
+#pragma unroll
+  for (int w = 0; w < PA_NW; ++w) cost += p.red[0][w];
+  // chunks of equal work that fill the grid, few enough for the parts there is room for
+  const int32_t half = a.parts / 2, least = (p.most + half - 1) / half;
+  const uint64_t each = (cost * a.hkv + PA_GRID - 1) / PA_GRID;
+  PaChunks c;
+  c.shared = (int32_t)min((uint64_t)0x3FFFFFFF, (each + PA_COST - 1) / PA_COST);
+  c.alone = (int32_t)min((uint64_t)0x3FFFFFFF, (each + PA_COST_ALONE - 1) / PA_COST_ALONE);
+  c.shared = max(max(c.shared, least), a.min_chunk);
+  c.alone = (max(max(c.alone, least), a.min_chunk) + 1) / 2 * 2;  // whole steps of 128 keys
+  uint32_t u[2] = {0, 0};
+  for (int64_t i = tid * run; i < min(n, (tid + 1) * run); ++i) {
+    bool ok;
+    const PaSeg s = pa_segment(a, i, &ok, &masked);
+    u[i >= a.groups] += (uint32_t)s.qt * (uint32_t)pa_nchunk(s, c) * (uint32_t)a.hkv;
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    uint32_t total;
+    p.before[k][tid] = pa_scan(u[k], reinterpret_cast<uint32_t*>(p.red[1]), &total);
+    if (tid == 0) p.before[k][PA_NT] = total, p.units[k] = total;
+  }
+  if (tid == 0) p.chunks = c, p.run = run;
+  __syncthreads();
+}
+
+struct PaUnit {
+  int64_t table;       // row of the block table
+  int64_t key0;        // first key
+  int64_t t0;          // first token of the segment
+  int64_t base;        // rows: the last key that the segment's first token sees
+  int32_t n;           // keys
+  int32_t r0, m;       // first query row of the tile, rows in it
+  int32_t kvh, part;
+  bool shared, group, direct;
+};
+
+// Unit u of kind k (0 groups: query tiles of one chunk follow each other; 1 rows: KV heads).
+__device__ __forceinline__ PaUnit pa_unit(const PrefixAttnArgs& a, const PaPlan& p, int k, uint32_t u) {
+  // the thread whose run holds it: the last with before <= u
+  const int lane = threadIdx.x & (kWave - 1);
+  int t = -1;
+#pragma unroll
+  for (int w = 0; w < PA_NT / kWave; ++w) t += __popcll(__ballot(p.before[k][w * kWave + lane] <= u));
+  u -= p.before[k][t];
+  const int64_t n = a.groups + a.batch;
+  int64_t i = t * p.run;
+  const int64_t end = min(n, i + p.run);
+  PaSeg s;
+  uint32_t units = 0;
+  for (; i < end; ++i) {  // uniform
+    if ((i >= a.groups) != (k == 1)) continue;
+    bool ok, masked = false;
+    s = pa_segment(a, i, &ok, &masked);
+    units = (uint32_t)s.qt * (uint32_t)pa_nchunk(s, p.chunks) * (uint32_t)a.hkv;
+    if (u < units) break;
+    u -= units;
+  }
+  if (i >= end) {  // lengths that changed under the call
+    PaUnit none = {};
+    return none;
+  }
+  const uint32_t nch = (uint32_t)pa_nchunk(s, p.chunks);
+  PaUnit r;
+  uint32_t qt, ch;
+  int64_t keys, nt;
+  r.group = k == 0;
+  if (k == 0) {
+    qt = u % s.qt;
+    ch = (u / s.qt) % nch;
+    r.kvh = u / s.qt / nch;
+    const PaGroup g = pa_group(a, i);
+    r.table = g.first;
+    r.key0 = 0;
+    keys = g.prefix;
+    r.t0 = g.t0;
+    nt = g.nt;
+    r.base = 0;
+    r.direct = false;
+    r.part = (int32_t)ch;
+  } else {
+    r.kvh = u % a.hkv;
+    qt = (u / a.hkv) % s.qt;
+    ch = u / a.hkv / s.qt;
+    const int64_t b = i - a.groups;
+    const PaRow w = pa_row(a, b);
+    r.table = b;
+    r.key0 = w.prefix;
+    keys = w.kv - w.prefix;
+    r.t0 = w.t0;
+    nt = w.nt;
+    r.base = w.kv - w.nt;
+    r.direct = w.prefix == 0 && nch == 1;
+    r.part = a.parts / 2 + (int32_t)ch;
+  }
+  r.shared = s.shared;
+  const int64_t c = (int64_t)pa_chunk(s, p.chunks) * PA_TILE;
+  r.n = (int32_t)min(c, keys - ch * c);
+  r.key0 += ch * c;
+  r.r0 = (int32_t)qt * PA_ROWS;
+  r.m = (int32_t)min((int64_t)PA_ROWS, nt * a.group - r.r0);
+  return r;
+}
+
+// ---- a unit's arithmetic
+
+// The running state of a wave's 32 query rows: lane l holds row l % 32, and of O^T the
+// dims 32 db + 8 (i / 4) + 4 (l / 32) + i % 4 in o[db][i]. l is of the lane's own keys.
+template <int D>
+struct PaState {
+  pa_f16 o[D / 32];
+  float m, l;
+};
+
+// Weights of NB x 32 scores s (keys t0 + 32 nb + 8 (i / 4) + 4 (l / 32) + i % 4 of the
+// chunk), in s. MASK: keys past the lane's lim weigh nothing.
+template <int D, int NB, bool MASK>
+__device__ __forceinline__ void pa_softmax(PaState<D>& st, pa_f16 (&s)[NB], float scale, int t0,
+                                           int lim, int hi) {
+  if constexpr (MASK) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (t0 + 32 * nb + 8 * (i / 4) + 4 * hi + i % 4 > lim) s[nb][i] = -INFINITY;
+  }
+  float mx = s[0][0];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[nb][i]);
+  mx = pa_max_halves(mx) * scale;
+  if (__any(mx > st.m + PA_SLACK)) {
+    const float mn = fmaxf(st.m, mx);
+    const float alpha = st.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.m - mn);
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.o[db][i] *= alpha;
+    st.l *= alpha;
+    st.m = mn;
+  }
+  const float off = st.m == -INFINITY ? 0.0f : -st.m;  // no key seen yet: all weights 0
+  float sum = 0.0f;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[nb][i] = __builtin_amdgcn_exp2f(fmaf(s[nb][i], scale, off));
+      sum += s[nb][i];
+    }
+  st.l += sum;
+}
+
+// 16-byte chunk c of row r of a tile in LDS lies in chunk c ^ swizzle(r): the operand reads
+// of consecutive rows then fall into different banks. K rows are read 16 bytes a lane, 8
+// rows at a time; V rows 32 bytes, 4 rows at a time.
+template <int D>
+__device__ __forceinline__ int pa_swz_k(int r) { return r & (D / 8 - 1); }
+template <int D>
+__device__ __forceinline__ int pa_swz_v(int r) { return D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3); }
+
+// O^T += V^T P^T for NB x 32 keys. va: the lane's byte address in V's first row block.
+template <int D, int FMT, int NB>
+__device__ __forceinline__ void pa_pv(PaState<D>& st, const pa_f16 (&s)[NB], const uint8_t* sV,
+                                      uint32_t va) {
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      pa_u4 p;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[e] = pa_pack<FMT>(s[nb][8 * k + 2 * e], s[nb][8 * k + 2 * e + 1]);
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db) {
+        const uint8_t* const at = sV + (va ^ (db << 6)) + (32 * nb + 16 * k) * 2 * D;
+        const pa_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s4*)at);
+        const pa_s4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s4*)(at + 8 * 2 * D));
+        typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+        const u2 x = __builtin_bit_cast(u2, lo), y = __builtin_bit_cast(u2, up);
+        st.o[db] = pa_mfma<FMT>((pa_u4){x[0], x[1], y[0], y[1]}, p, st.o[db]);
+      }
+    }
+}
+
+constexpr int PA_LDS_TILES = 2 * 2 * PA_TILE * 2 * 128;          // two tiles of K and V
+constexpr int PA_LDS_JOIN = PA_NW * PA_WROWS * (128 + 4) * 4;     // four waves' O
+constexpr int PA_LDS = PA_LDS_JOIN > PA_LDS_TILES ? PA_LDS_JOIN : PA_LDS_TILES;
+constexpr int PA_RING = 8;                                        // tiles of slots
+
+// row of the pool of the key at position pos of table row `table`, or PA_NOSLOT
+__device__ __forceinline__ uint32_t pa_slot(const PrefixAttnArgs& a, int32_t page, uint32_t pos) {
+  return page >= 0 && page < a.num_blocks ? (uint32_t)page * (uint32_t)a.bs + pos % (uint32_t)a.bs
+                                          : PA_NOSLOT;
+}
+
+// lim of query row i of a unit: the last key it sees, of the chunk (-1: none)
+__device__ __forceinline__ int pa_lim(const PrefixAttnArgs& a, const PaUnit& u, bool masked, int i) {
+  if (i >= u.m) return -1;
+  const int64_t j = (u.r0 + i) / a.group;
+  int64_t lim;
+  if (!u.group) {
+    lim = u.base + j;
+  } else if (!masked) {
+    return u.n - 1;
+  } else {  // the token's own row
+    const int64_t t = u.t0 + j, b = pa_find(a.cu_q, a.batch, t);
+    lim = a.kv_len[b] - (a.cu_q[b + 1] - t);
+  }
+  return (int)max((int64_t)-1, min(lim - u.key0, (int64_t)u.n - 1));
+}
+
+// Results of query row `i` (lane l % 32's): O / l to out, or the part.
+template <int D, int FMT>
+__device__ __forceinline__ void pa_store4(const PrefixAttnArgs& a, const PaUnit& u, int64_t qrow, int d,
+                                          float4 v) {
+  if (u.direct) {
+    uint2 w = make_uint2(pa_pack<FMT>(v.x, v.y), pa_pack<FMT>(v.z, v.w));
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + qrow * D + d) = w;
+  } else {
+    *reinterpret_cast<float4*>(a.part_o + ((int64_t)u.part * a.tokens * a.hq + qrow) * D + d) = v;
+  }
+}
+__device__ __forceinline__ int64_t pa_qrow(const PrefixAttnArgs& a, const PaUnit& u, int i) {
+  const int r = u.r0 + i;
+  return (u.t0 + r / a.group) * a.hq + u.kvh * a.group + r % a.group;
+}
+
+template <int D, int FMT>
+__global__ void __launch_bounds__(PA_NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
+prefix_attn_kernel(PrefixAttnArgs a) {
+  constexpr int NC = D / 8;            // 16-byte chunks of a row
+  constexpr int RB = 2 * D;            // bytes of a row
+  __shared__ __align__(256) uint8_t sMem[PA_LDS];
+  __shared__ uint32_t sSlot[PA_RING * PA_TILE];
+  __shared__ PaPlan sPlan;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), w = tid / kWave;
+  const int hi = lane / 32, l31 = lane & 31;
+  pa_plan(a, sPlan, blockIdx.x == 0);
+  if (blockIdx.x == 0 && tid == 0) a.head[0] = sPlan.chunks.shared, a.head[1] = sPlan.chunks.alone;
+  const int64_t row_elems = (int64_t)a.hkv * D;
+  // addresses of the lane's operands in LDS tiles
+  const uint32_t ka = l31 * RB + ((hi ^ pa_swz_k<D>(l31)) << 4);
+  const int vr = 4 * hi + ((lane & 15) >> 2), vd = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  const uint32_t va = vr * RB + (((vd >> 3) ^ pa_swz_v<D>(vr)) << 4) + (vd & 7) * 2;
+
+  // the XCD's share of both kinds of units
+  const int x = blockIdx.x % 8;
+  const uint32_t g0 = (uint32_t)(sPlan.units[0] * x / 8), ng = (uint32_t)(sPlan.units[0] * (x + 1) / 8) - g0;
+  const uint32_t b0 = (uint32_t)(sPlan.units[1] * x / 8), nb = (uint32_t)(sPlan.units[1] * (x + 1) / 8) - b0;
+  for (uint32_t at = blockIdx.x / 8; at < ng + nb; at += PA_GRID / 8) {  // uniform
+    const PaUnit u = at < ng ? pa_unit(a, sPlan, 0, g0 + at) : pa_unit(a, sPlan, 1, b0 + at - ng);
+    if (u.n <= 0 || u.m <= 0) continue;  // uniform
+    const int32_t* const table = a.block_table + u.table * a.max_blocks;
+    const uint16_t* const kp = a.k_pool + u.kvh * D;
+    const uint16_t* const vp = a.v_pool + u.kvh * D;
+    const uint32_t pos0 = (uint32_t)u.key0;
+    int bad = 0;
+    PaState<D> st;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.o[db][i] = 0.0f;
+    st.m = -INFINITY;
+    st.l = 0.0f;
+    // the wave's rows: 32 w .. of the shared form, all of the other
+    const int r0 = u.shared ? PA_WROWS * w : 0;
+    const bool active = r0 < u.m;
+    const int lim = pa_lim(a, u, sPlan.masked, r0 + l31);
+    // keys that every query row of the unit sees
+    const int seen = u.group ? (sPlan.masked ? 0 : u.n)
+                             : (int)max((int64_t)0, min((int64_t)u.n, u.base + u.r0 / a.group + 1 - u.key0));
+    pa_u4 qa[D / 16];
+    {
+      const uint16_t* src = a.q + (r0 + l31 < u.m ? pa_qrow(a, u, r0 + l31) * D : 0);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        qa[ks] = *reinterpret_cast<const pa_u4*>(src + 16 * ks + 8 * hi);
+        if (r0 + l31 >= u.m) qa[ks] = (pa_u4){0, 0, 0, 0};
+      }
+    }
+
+    if (u.shared) {
+      constexpr int H = NC / 4, TPR = PA_NT / NC;  // passes, rows per pass
+      const int ntile = (u.n + PA_TILE - 1) / PA_TILE;
+      const int lr = tid / NC, lc = tid % NC;
+      // slots of the chunk's tiles, by the first wave: page ids are loaded a tile before
+      // they are needed here, four tiles before their keys
+      auto page_of = [&](int tile) {
+        const int t = tile * PA_TILE + lane;
+        return t < u.n ? table[(pos0 + t) / (uint32_t)a.bs] : 0;
+      };
+      auto put_slot = [&](int tile, int32_t page) {
+        const int t = tile * PA_TILE + lane;
+        uint32_t s = PA_NOSLOT;
+        if (t < u.n) {
+          s = pa_slot(a, page, pos0 + t);
+          bad |= s == PA_NOSLOT;
+        }
+        sSlot[(tile % PA_RING) * PA_TILE + lane] = s;
+      };
+      pa_u4 kk[H], vv[H];
+      uint32_t vok = 0;
+      auto gather = [&](int tile) {
+        vok = 0;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          const uint32_t s = sSlot[(tile % PA_RING) * PA_TILE + lr + TPR * h];
+          const int64_t off = (int64_t)(s == PA_NOSLOT ? 0u : s) * row_elems + lc * 8;
+          vok |= (uint32_t)(s != PA_NOSLOT) << h;
+          kk[h] = *reinterpret_cast<const pa_u4*>(kp + off);
+          vv[h] = *reinterpret_cast<const pa_u4*>(vp + off);
+        }
+      };
+      auto stage = [&](int tile) {
+        uint8_t* const k = sMem + (tile & 1) * (2 * PA_TILE * RB);
+        uint8_t* const v = k + PA_TILE * RB;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          const int r = lr + TPR * h;
+          *reinterpret_cast<pa_u4*>(k + r * RB + ((lc ^ pa_swz_k<D>(r)) << 4)) = kk[h];
+          // keys past the chunk, or without a page, weigh 0: their V must not be NaN
+          *reinterpret_cast<pa_u4*>(v + r * RB + ((lc ^ pa_swz_v<D>(r)) << 4)) =
+              (vok >> h) & 1u ? vv[h] : (pa_u4){0, 0, 0, 0};
+        }
+      };
+      int32_t page = 0;
+      if (w == 0) {
+        int32_t pg[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) pg[i] = page_of(i);
+        page = page_of(3);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) put_slot(i, pg[i]);
+      }
+      __syncthreads();
+      gather(0);
+      stage(0);
+      gather(1);
+      __syncthreads();
+      for (int t = 0; t < ntile; ++t) {
+        if (w == 0) {  // tile t + 3
+          put_slot(t + 3, page);
+          page = page_of(t + 4);
+        }
+        if (active) {
+          const uint8_t* const k = sMem + (t & 1) * (2 * PA_TILE * RB);
+          pa_f16 s[2] = {};
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+              s[n] = pa_mfma<FMT>(*reinterpret_cast<const pa_u4*>(k + (ka ^ (ks << 5)) + n * 32 * RB),
+                                  qa[ks], s[n]);
+          if ((t + 1) * PA_TILE <= seen) pa_softmax<D, 2, false>(st, s, a.scale_log2, 0, 0, hi);
+          else pa_softmax<D, 2, true>(st, s, a.scale_log2, t * PA_TILE, lim, hi);
+          pa_pv<D, FMT, 2>(st, s, k + PA_TILE * RB, va);
+        }
+        if (t + 1 < ntile) {  // uniform
+          stage(t + 1);
+          if (t + 2 < ntile) gather(t + 2);
+        }
+        __syncthreads();
+      }
+      st.l = pa_sum_halves(st.l);
+      const int i = r0 + l31;
+      if (active && i < u.m) {
+        const int64_t qrow = pa_qrow(a, u, i);
+        const float f = u.direct ? (st.l > 0.0f || st.l != st.l ? 1.0f / st.l : 0.0f) : 1.0f;
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            pa_store4<D, FMT>(a, u, qrow, 32 * db + 8 * e + 4 * hi,
+                              make_float4(st.o[db][4 * e] * f, st.o[db][4 * e + 1] * f,
+                                          st.o[db][4 * e + 2] * f, st.o[db][4 * e + 3] * f));
+        if (!u.direct && hi == 0)
+          a.part_ml[(int64_t)u.part * a.tokens * a.hq + qrow] = make_float2(st.m, st.l);
+      }
+    } else {
+      constexpr int H = NC / 2, TPR = kWave / NC;  // passes and rows per pass of a wave's V
+      const int nstep = (u.n + PA_STEP - 1) / PA_STEP;
+      uint8_t* const v = sMem + w * (32 * RB);
+      const int lr = lane / NC, lc = lane % NC;
+      // the lane's key of a step is 32 w + l % 32
+      auto page_of = [&](int step) {
+        const int t = step * PA_STEP + 32 * w + l31;
+        return t < u.n ? table[(pos0 + t) / (uint32_t)a.bs] : 0;
+      };
+      auto slot_of = [&](int step, int32_t page) {
+        const int t = step * PA_STEP + 32 * w + l31;
+        if (t >= u.n) return PA_NOSLOT;
+        const uint32_t s = pa_slot(a, page, pos0 + t);
+        bad |= s == PA_NOSLOT;
+        return s;
+      };
+      pa_u4 kk[D / 16], vv[H];
+      uint32_t vok = 0;
+      auto gather_k = [&](uint32_t slot) {
+        const uint16_t* src = kp + (int64_t)(slot == PA_NOSLOT ? 0u : slot) * row_elems + 8 * hi;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) kk[ks] = *reinterpret_cast<const pa_u4*>(src + 16 * ks);
+      };
+      auto gather_v = [&](uint32_t slot) {
+        vok = 0;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          const uint32_t s = (uint32_t)__shfl((int)slot, lr + TPR * h, kWave);
+          vok |= (uint32_t)(s != PA_NOSLOT) << h;
+          vv[h] = *reinterpret_cast<const pa_u4*>(vp + (int64_t)(s == PA_NOSLOT ? 0u : s) * row_elems +
+                                                  lc * 8);
+        }
+      };
+      int32_t page = page_of(0);
+      uint32_t slot = slot_of(0, page);
+      page = page_of(1);
+      gather_k(slot);
+      gather_v(slot);
+      for (int t = 0; t < nstep; ++t) {
+        slot = slot_of(t + 1, page);
+        page = page_of(t + 2);
+        pa_f16 s[1] = {};
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) s[0] = pa_mfma<FMT>(kk[ks], qa[ks], s[0]);
+        if (t + 1 < nstep) gather_k(slot);
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          const int r = lr + TPR * h;
+          *reinterpret_cast<pa_u4*>(v + r * RB + ((lc ^ pa_swz_v<D>(r)) << 4)) =
+              (vok >> h) & 1u ? vv[h] : (pa_u4){0, 0, 0, 0};
+        }
+        if (t + 1 < nstep) gather_v(slot);
+        const int k0 = t * PA_STEP + 32 * w;
+        if (k0 + 32 <= seen) pa_softmax<D, 1, false>(st, s, a.scale_log2, 0, 0, hi);
+        else pa_softmax<D, 1, true>(st, s, a.scale_log2, k0, lim, hi);
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        __builtin_amdgcn_wave_barrier();  // V written by the whole wave before it is read
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        pa_pv<D, FMT, 1>(st, s, v, va);
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        __builtin_amdgcn_wave_barrier();  // and read before it is written again
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+      }
+      // join of the four waves: weights 2^(m_w - m), O summed through LDS
+      st.l = pa_sum_halves(st.l);
+      float2* const sML = reinterpret_cast<float2*>(sSlot);  // [wave][row]
+      __syncthreads();  // the tiles' LDS is free
+      if (hi == 0) sML[w * PA_WROWS + l31] = make_float2(st.m, st.l);
+      float* const so = reinterpret_cast<float*>(sMem) + (w * PA_WROWS + l31) * (D + 4);
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<float4*>(so + 32 * db + 8 * e + 4 * hi) =
+              make_float4(st.o[db][4 * e], st.o[db][4 * e + 1], st.o[db][4 * e + 2], st.o[db][4 * e + 3]);
+      __syncthreads();
+      for (int e = tid; e < u.m * (D / 4); e += PA_NT) {
+        const int i = e / (D / 4), d = e % (D / 4) * 4;
+        float m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < PA_NW; ++k) m = fmaxf(m, sML[k * PA_WROWS + i].x);
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < PA_NW; ++k) {
+          const float2 ml = sML[k * PA_WROWS + i];
+          const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - m);
+          const float4 v4 = *reinterpret_cast<const float4*>(
+              reinterpret_cast<const float*>(sMem) + (k * PA_WROWS + i) * (D + 4) + d);
+          l += f * ml.y;
+          o.x += f * v4.x;
+          o.y += f * v4.y;
+          o.z += f * v4.z;
+          o.w += f * v4.w;
+        }
+        const int64_t qrow = pa_qrow(a, u, i);
+        if (u.direct) {
+          const float f = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+          o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+        } else if (d == 0) {
+          a.part_ml[(int64_t)u.part * a.tokens * a.hq + qrow] = make_float2(m, l);
+        }
+        pa_store4<D, FMT>(a, u, qrow, d, o);
+      }
+      __syncthreads();  // LDS is used again by the next unit
+    }
+    if (bad && a.error) *a.error = 1;
+  }
+}
+
+// Join of a query row's parts: out = sum_c w_c O_c, w_c = 2^(m_c - m) / sum 2^(m_c - m) l_c.
+// SL slices of D / 4 threads take every SL-th part; a workgroup has R rows.
+template <int D, int FMT, int SL, int R>
+__global__ void __launch_bounds__(D / 4 * SL * R) prefix_attn_join_kernel(PrefixAttnArgs a) {
+  constexpr int DL = D / 4;
+  __shared__ float4 sO[R][SL][DL];
+  __shared__ float sL[R][SL];
+  const int tid = threadIdx.x, d4 = tid % DL, sl = tid / DL % SL, rr = tid / (DL * SL);
+  const int64_t qrow = (int64_t)blockIdx.x * R + rr;
+  const bool in = qrow < a.tokens * a.hq;
+  const int64_t t = in ? qrow / a.hq : 0;
+  const int64_t b = pa_find(a.cu_q, a.batch, t);
+  const PaRow row = pa_row(a, b);
+  int np = 0, ns = 0;
+  if (in && row.ok && t >= row.t0 && t < row.t0 + row.nt) {
+    const PaChunks c{a.head[0], a.head[1]};
+    const PaGroup g = pa_group(a, pa_find(a.cu_group, a.groups, b));
+    np = pa_nchunk(pa_seg(a, g.nt, g.prefix), c);
+    ns = pa_nchunk(pa_seg(a, row.nt, max((int64_t)0, row.kv - row.prefix)), c);
+    if (row.prefix == 0 && ns == 1) ns = 0;  // written directly
+  }
+  const int64_t stride = a.tokens * a.hq;
+  const int n = np + ns, gap = a.parts / 2 - np;  // part i: i, or i + gap from np
+  float m = -INFINITY, l = 0.0f;
+  for (int i = 0; i < n; ++i) m = fmaxf(m, a.part_ml[(i + (i < np ? 0 : gap)) * stride + qrow].x);
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int i = sl; i < n; i += SL) {
+    const int64_t p = (i + (i < np ? 0 : gap)) * stride + qrow;
+    const float2 ml = a.part_ml[p];
+    const float4 v = *reinterpret_cast<const float4*>(a.part_o + p * D + d4 * 4);
+    const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - m);
+    l += f * ml.y;
+    o.x += f * v.x;
+    o.y += f * v.y;
+    o.z += f * v.z;
+    o.w += f * v.w;
+  }
+  sO[rr][sl][d4] = o;
+  if (d4 == 0) sL[rr][sl] = l;
+  __syncthreads();
+  if (n == 0 || sl != 0) return;
+#pragma unroll
+  for (int k = 1; k < SL; ++k) {
+    const float4 v = sO[rr][k][d4];
+    o.x += v.x;
+    o.y += v.y;
+    o.z += v.z;
+    o.w += v.w;
+    l += sL[rr][k];
+  }
+  const float f = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + qrow * D + d4 * 4) =
+      make_uint2(pa_pack<FMT>(o.x * f, o.y * f), pa_pack<FMT>(o.z * f, o.w * f));
+}
+
+// Parts per query row: half for the prefix, half for the row's own keys. As many as the
+// grid could fill from one row, in at most PA_ROOM bytes (but two).
+constexpr int64_t PA_ROOM = (int64_t)192 << 20;
+int prefix_attn_parts(int64_t tokens, int32_t hq, int32_t hkv, int32_t d) {
+  const int64_t one = tokens * hq * (d + 2) * 4;
+  const int64_t want = 2 * ((PA_GRID + hkv - 1) / hkv);
+  return (int)(std::max<int64_t>(1, std::min<int64_t>(want, PA_ROOM / std::max<int64_t>(1, one)) / 2) * 2);
+}
+
+template <int D, int FMT>
+static hipError_t launch_prefix_attn_t(const PrefixAttnArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((prefix_attn_kernel<D, FMT>), dim3(PA_GRID), dim3(PA_NT), 0, s, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const int64_t rows = a.tokens * a.hq;
+  constexpr int DL = D / 4;
+  if (rows <= 2048) {  // few rows, many parts: 8 slices a row
+    hipLaunchKernelGGL((prefix_attn_join_kernel<D, FMT, 8, 1>), dim3((unsigned)rows), dim3(DL * 8), 0,
+                       s, a);
+  } else {
+    constexpr int R = 256 / (DL * 2);
+    hipLaunchKernelGGL((prefix_attn_join_kernel<D, FMT, 2, R>), dim3((unsigned)((rows + R - 1) / R)),
+                       dim3(256), 0, s, a);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_prefix_attn(int dtype, int d, const PrefixAttnArgs& a, hipStream_t s) {
+  if (dtype == SDX_BF16)
+    return d == 64 ? launch_prefix_attn_t<64, SDX_BF16>(a, s) : launch_prefix_attn_t<128, SDX_BF16>(a, s);
+  return d == 64 ? launch_prefix_attn_t<64, SDX_F16>(a, s) : launch_prefix_attn_t<128, SDX_F16>(a, s);
+}
+
+}  // namespace sdx

@@ -449,6 +449,34 @@ size_t sdx_verify_attention_workspace(int64_t batch, int32_t max_q, int32_t num_
                                       int32_t num_kv_heads, int32_t block_size,
                                       int64_t max_blocks, int32_t chunk_tokens);
 
+/* ---- attention of rows that share a prefix: as sdx_verify_attention_paged, one layer, for a
+ * batch whose groups of rows hold a prefix's keys once. Groups are consecutive rows, cu_group
+ * [num_groups + 1] int64 from 0 to batch; the first prefix_len[g] (int64) keys of every row of
+ * group g are those of its first row, read through that row's block table once for all of the
+ * group's queries (a whole block of query rows at a time); keys from prefix_len[g] on are read
+ * through the row's own table. kv_len counts both. The prefix need not end with a page: of the
+ * page that holds its end, a row's own table gives the keys behind the end. sdx_build_block_tables
+ * lays such tables out. Query j of row b sees keys s <= kv_len[b] - q_b + j, the prefix's too.
+ * q / out: [num_tokens, num_q_heads, head_dim], bf16 or fp16 as the pools, 16-byte aligned;
+ * q_b = cu_q[b+1] - cu_q[b] of any size; head_dim 64 or 128; scale positive and finite. Softmax
+ * and sums in fp32, weights rounded to the type for the second product, output rounded to it.
+ * Rows, or groups with all their rows, whose lengths or offsets are out of range set *error
+ * (nullable) and leave their output as it was; tokens behind the last row too, without the
+ * error. Page ids outside the pool set *error and the output of the rows that read them is
+ * unspecified. Two kernels are queued; `workspace` (sdx_prefix_attention_workspace bytes, no
+ * initial contents) holds fp32 parts. A row's bits depend on the whole batch's lengths. No
+ * reference counterpart (the reference keeps a copy of every row's keys). */
+int sdx_prefix_attention_paged(const void* q, int dtype, int64_t num_tokens, int64_t batch,
+                               const int64_t* cu_q, int32_t num_q_heads, int32_t num_kv_heads,
+                               int32_t head_dim, const void* k_pool, const void* v_pool,
+                               int64_t num_blocks, int32_t block_size, const int32_t* block_table,
+                               int64_t max_blocks, const int64_t* kv_len, const int64_t* cu_group,
+                               const int64_t* prefix_len, int64_t num_groups, float scale,
+                               void* workspace, size_t workspace_bytes, void* out, int32_t* error,
+                               sdx_stream_t stream);
+size_t sdx_prefix_attention_workspace(int64_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads,
+                                      int32_t head_dim);
+
 #ifdef __cplusplus
 }
 #endif

@@ -74,13 +74,45 @@ def test_layout_statuses():
     assert append(layers=40000) == EUNSUP and append(T=1 << 40) == EUNSUP
 
 
+def test_prefix_attention_statuses():
+    from specdec import _lib
+    L = _lib.lib()
+
+    def call(T=3, B=2, hq=4, hkv=2, d=64, dtype=BF16, nb=8, bs=16, mb=4, G=1, scale=0.1, q=FAKE,
+             pool=FAKE, out=FAKE, ws=FAKE, nbytes=None):
+        need = L.sdx_prefix_attention_workspace(max(T, 1), max(hq, 1), max(hkv, 1), d)
+        return L.sdx_prefix_attention_paged(q, dtype, T, B, FAKE, hq, hkv, d, pool, FAKE, nb, bs, FAKE,
+                                            mb, FAKE, FAKE, FAKE, G, scale, ws,
+                                            need if nbytes is None else nbytes, out, None, None)
+
+    assert call(T=0) == OK
+    off = ctypes.c_void_p(4104)
+    for bad in (dict(T=-1), dict(B=-1), dict(B=0), dict(G=0), dict(hq=0), dict(hq=3), dict(hkv=0),
+                dict(bs=0), dict(mb=0), dict(nb=0), dict(scale=0.0), dict(scale=float("nan")),
+                dict(scale=float("inf")), dict(q=None), dict(out=None), dict(q=off), dict(pool=off),
+                dict(out=off)):
+        assert call(**bad) == EINVAL, bad
+    for bad in (dict(d=96), dict(d=256), dict(dtype=F32), dict(mb=1 << 28), dict(nb=1 << 29),
+                dict(T=1 << 24)):
+        assert call(**bad) == EUNSUP, bad
+    need = L.sdx_prefix_attention_workspace(3, 4, 2, 64)
+    assert call(nbytes=need - 1) == EWS and call(ws=None) == EWS and call(ws=off) == EWS
+    assert L.sdx_prefix_attention_workspace(0, 4, 2, 64) == 0
+    assert L.sdx_prefix_attention_workspace(3, 4, 3, 64) == 0
+    # two parts at least, and no more room than for two where queries are many
+    assert L.sdx_prefix_attention_workspace(1 << 16, 32, 8, 128) >= 2 * (1 << 21) * 130 * 4
+    assert L.sdx_prefix_attention_workspace(640, 32, 8, 128) <= 200 << 20
+
+
 def test_entry_points_refuse_cpu_tensors():
+    from specdec import attention as A
     from specdec import kvcache as K
     from specdec import sampling as S
     z = torch.zeros(2, dtype=torch.long)
     for call in (lambda: S.token_logprobs(torch.zeros(2, 8), z),
                  lambda: K.build_block_tables(z, z, 16, 2),
                  lambda: K.paged_slot_mapping(z.view(1, 2), z, z[:1], 16, 1),
+                 lambda: A.shared_prefix_attention_paged(*[z] * 8),
                  lambda: K.append_paged_slots(torch.zeros(1, 2, 1, 1, 8), torch.zeros(1, 2, 2, 8), z)):
         with pytest.raises(RuntimeError, match="ROCm device"):
             call()
