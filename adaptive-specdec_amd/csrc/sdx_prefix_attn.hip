@@ -27,6 +27,7 @@
 // A unit leaves (O, max, sum) in fp32, a second kernel joins them; a row without a prefix
 // whose keys fit one unit is written directly.
 #include <algorithm>
+#include <type_traits>
 
 #include "sdx_launch.hpp"
 
@@ -343,18 +344,20 @@ struct PaState {
   float m, l;
 };
 
-// Weights of NB x 32 scores s (keys t0 + 32 nb + 8 (i / 4) + 4 (l / 32) + i % 4 of the
-// chunk), in s. MASK: keys past the lane's lim weigh nothing.
-template <int D, int NB, bool MASK>
-__device__ __forceinline__ void pa_softmax(PaState<D>& st, pa_f16 (&s)[NB], float scale, int t0,
-                                           int lim, int hi) {
-  if constexpr (MASK) {
+// Scores of keys past the lane's lim: keys t0 + 32 nb + 8 (i / 4) + 4 (l / 32) + i % 4 of the
+// chunk in s[nb][i].
+template <int NB>
+__device__ __forceinline__ void pa_mask(pa_f16 (&s)[NB], int t0, int lim, int hi) {
+  const int left = lim - t0 - 4 * hi;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+  for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (t0 + 32 * nb + 8 * (i / 4) + 4 * hi + i % 4 > lim) s[nb][i] = -INFINITY;
-  }
+    for (int i = 0; i < 16; ++i)
+      if (32 * nb + 8 * (i / 4) + i % 4 > left) s[nb][i] = -INFINITY;
+}
+// Weights of NB x 32 scores, in s.
+template <int D, int NB>
+__device__ __forceinline__ void pa_softmax(PaState<D>& st, pa_f16 (&s)[NB], float scale) {
   float mx = s[0][0];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
@@ -372,15 +375,15 @@ __device__ __forceinline__ void pa_softmax(PaState<D>& st, pa_f16 (&s)[NB], floa
     st.m = mn;
   }
   const float off = st.m == -INFINITY ? 0.0f : -st.m;  // no key seen yet: all weights 0
-  float sum = 0.0f;
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       s[nb][i] = __builtin_amdgcn_exp2f(fmaf(s[nb][i], scale, off));
-      sum += s[nb][i];
+      sum[i % 4] += s[nb][i];
     }
-  st.l += sum;
+  st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 // 16-byte chunk c of row r of a tile in LDS lies in chunk c ^ swizzle(r): the operand reads
@@ -457,6 +460,10 @@ __device__ __forceinline__ int64_t pa_qrow(const PrefixAttnArgs& a, const PaUnit
   return (u.t0 + r / a.group) * a.hq + u.kvh * a.group + r % a.group;
 }
 
+// What is read in place of a key past the chunk, or without a page: its weight is 0, and its
+// V must not be NaN.
+__device__ const uint4 pa_zero_row[16] = {};
+
 template <int D, int FMT>
 __global__ void __launch_bounds__(PA_NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 prefix_attn_kernel(PrefixAttnArgs a) {
@@ -485,6 +492,7 @@ prefix_attn_kernel(PrefixAttnArgs a) {
     const int32_t* const table = a.block_table + u.table * a.max_blocks;
     const uint16_t* const kp = a.k_pool + u.kvh * D;
     const uint16_t* const vp = a.v_pool + u.kvh * D;
+    const uint16_t* const zero = reinterpret_cast<const uint16_t*>(pa_zero_row);
     const uint32_t pos0 = (uint32_t)u.key0;
     int bad = 0;
     PaState<D> st;
@@ -531,28 +539,24 @@ prefix_attn_kernel(PrefixAttnArgs a) {
         sSlot[(tile % PA_RING) * PA_TILE + lane] = s;
       };
       pa_u4 kk[H], vv[H];
-      uint32_t vok = 0;
       auto gather = [&](int tile) {
-        vok = 0;
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           const uint32_t s = sSlot[(tile % PA_RING) * PA_TILE + lr + TPR * h];
-          const int64_t off = (int64_t)(s == PA_NOSLOT ? 0u : s) * row_elems + lc * 8;
-          vok |= (uint32_t)(s != PA_NOSLOT) << h;
-          kk[h] = *reinterpret_cast<const pa_u4*>(kp + off);
-          vv[h] = *reinterpret_cast<const pa_u4*>(vp + off);
+          const int64_t off = (int64_t)s * row_elems + lc * 8;
+          kk[h] = *reinterpret_cast<const pa_u4*>(s == PA_NOSLOT ? zero : kp + off);
+          vv[h] = *reinterpret_cast<const pa_u4*>(s == PA_NOSLOT ? zero : vp + off);
         }
       };
-      auto stage = [&](int tile) {
-        uint8_t* const k = sMem + (tile & 1) * (2 * PA_TILE * RB);
-        uint8_t* const v = k + PA_TILE * RB;
+      static_assert(TPR % 16 == 0, "a pass's rows are swizzled alike");
+      const uint32_t kw = lr * RB + ((lc ^ pa_swz_k<D>(lr)) << 4);
+      const uint32_t vw = lr * RB + ((lc ^ pa_swz_v<D>(lr)) << 4);
+      auto stage = [&](auto buf) {
+        uint8_t* const k = sMem + buf * (2 * PA_TILE * RB);
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-          const int r = lr + TPR * h;
-          *reinterpret_cast<pa_u4*>(k + r * RB + ((lc ^ pa_swz_k<D>(r)) << 4)) = kk[h];
-          // keys past the chunk, or without a page, weigh 0: their V must not be NaN
-          *reinterpret_cast<pa_u4*>(v + r * RB + ((lc ^ pa_swz_v<D>(r)) << 4)) =
-              (vok >> h) & 1u ? vv[h] : (pa_u4){0, 0, 0, 0};
+          *reinterpret_cast<pa_u4*>(k + kw + TPR * h * RB) = kk[h];
+          *reinterpret_cast<pa_u4*>(k + vw + (PA_TILE + TPR * h) * RB) = vv[h];
         }
       };
       int32_t page = 0;
@@ -565,17 +569,19 @@ prefix_attn_kernel(PrefixAttnArgs a) {
         for (int i = 0; i < 3; ++i) put_slot(i, pg[i]);
       }
       __syncthreads();
+      typedef std::integral_constant<int, 0> even;
+      typedef std::integral_constant<int, 1> odd;
       gather(0);
-      stage(0);
+      stage(even());
       gather(1);
       __syncthreads();
-      for (int t = 0; t < ntile; ++t) {
+      auto tile = [&](int t, auto buf, auto next) {
         if (w == 0) {  // tile t + 3
           put_slot(t + 3, page);
           page = page_of(t + 4);
         }
         if (active) {
-          const uint8_t* const k = sMem + (t & 1) * (2 * PA_TILE * RB);
+          const uint8_t* const k = sMem + buf * (2 * PA_TILE * RB);
           pa_f16 s[2] = {};
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks)
@@ -583,15 +589,19 @@ prefix_attn_kernel(PrefixAttnArgs a) {
             for (int n = 0; n < 2; ++n)
               s[n] = pa_mfma<FMT>(*reinterpret_cast<const pa_u4*>(k + (ka ^ (ks << 5)) + n * 32 * RB),
                                   qa[ks], s[n]);
-          if ((t + 1) * PA_TILE <= seen) pa_softmax<D, 2, false>(st, s, a.scale_log2, 0, 0, hi);
-          else pa_softmax<D, 2, true>(st, s, a.scale_log2, t * PA_TILE, lim, hi);
+          if ((t + 1) * PA_TILE > seen) pa_mask<2>(s, t * PA_TILE, lim, hi);  // uniform
+          pa_softmax<D, 2>(st, s, a.scale_log2);
           pa_pv<D, FMT, 2>(st, s, k + PA_TILE * RB, va);
         }
-        if (t + 1 < ntile) {  // uniform
-          stage(t + 1);
-          if (t + 2 < ntile) gather(t + 2);
-        }
+        stage(next);  // past the last tile: rows of zeros
+        gather(t + 2);
         __syncthreads();
+      };
+      for (int t = 0;; t += 2) {
+        tile(t, even(), odd());
+        if (t + 1 >= ntile) break;
+        tile(t + 1, odd(), even());
+        if (t + 2 >= ntile) break;
       }
       st.l = pa_sum_halves(st.l);
       const int i = r0 + l31;
@@ -626,20 +636,17 @@ prefix_attn_kernel(PrefixAttnArgs a) {
         return s;
       };
       pa_u4 kk[D / 16], vv[H];
-      uint32_t vok = 0;
       auto gather_k = [&](uint32_t slot) {
-        const uint16_t* src = kp + (int64_t)(slot == PA_NOSLOT ? 0u : slot) * row_elems + 8 * hi;
+        const uint16_t* src = slot == PA_NOSLOT ? zero : kp + (int64_t)slot * row_elems + 8 * hi;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) kk[ks] = *reinterpret_cast<const pa_u4*>(src + 16 * ks);
       };
       auto gather_v = [&](uint32_t slot) {
-        vok = 0;
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           const uint32_t s = (uint32_t)__shfl((int)slot, lr + TPR * h, kWave);
-          vok |= (uint32_t)(s != PA_NOSLOT) << h;
-          vv[h] = *reinterpret_cast<const pa_u4*>(vp + (int64_t)(s == PA_NOSLOT ? 0u : s) * row_elems +
-                                                  lc * 8);
+          vv[h] = *reinterpret_cast<const pa_u4*>(s == PA_NOSLOT ? zero
+                                                                : vp + (int64_t)s * row_elems + lc * 8);
         }
       };
       int32_t page = page_of(0);
@@ -657,13 +664,12 @@ prefix_attn_kernel(PrefixAttnArgs a) {
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           const int r = lr + TPR * h;
-          *reinterpret_cast<pa_u4*>(v + r * RB + ((lc ^ pa_swz_v<D>(r)) << 4)) =
-              (vok >> h) & 1u ? vv[h] : (pa_u4){0, 0, 0, 0};
+          *reinterpret_cast<pa_u4*>(v + r * RB + ((lc ^ pa_swz_v<D>(r)) << 4)) = vv[h];
         }
         if (t + 1 < nstep) gather_v(slot);
         const int k0 = t * PA_STEP + 32 * w;
-        if (k0 + 32 <= seen) pa_softmax<D, 1, false>(st, s, a.scale_log2, 0, 0, hi);
-        else pa_softmax<D, 1, true>(st, s, a.scale_log2, k0, lim, hi);
+        if (k0 + 32 > seen) pa_mask<1>(s, k0, lim, hi);  // uniform
+        pa_softmax<D, 1>(st, s, a.scale_log2);
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
         __builtin_amdgcn_wave_barrier();  // V written by the whole wave before it is read
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
