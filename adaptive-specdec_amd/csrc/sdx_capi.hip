@@ -1201,14 +1201,34 @@ int sdx_verify_attention_paged(const void* q, int dtype, int64_t batch, const in
 }
 
 // ------------------------------------------------------------------ shared prefixes
-size_t sdx_prefix_attention_workspace(int64_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads,
-                                      int32_t head_dim) {
-  if (num_tokens < 1 || num_q_heads < 1 || num_kv_heads < 1 || num_q_heads % num_kv_heads != 0 ||
-      (head_dim != 64 && head_dim != 128))
+static size_t prefix_ws(Carve& c, int64_t tokens, int64_t batch, int64_t groups, int32_t hq,
+                        int32_t hkv, int32_t d, sdx::PrefixAttnArgs* a) {
+  a->parts = sdx::prefix_attn_parts(tokens, hq, hkv, d);
+  a->max_entries = sdx::prefix_attn_entries(tokens, batch, groups, hq / hkv, a->parts);
+  const size_t rows = (size_t)a->parts * tokens * hq;
+  a->head = c.take<int32_t>(256);
+  a->entries = c.take<sdx::PrefixAttnUnit>((size_t)a->max_entries);
+  a->token_parts = c.take<uint32_t>((size_t)tokens);
+  a->group_seg = c.take<int2>((size_t)groups);
+  a->part_ml = c.take<float2>(rows);
+  a->part_o = c.take<float>(rows * d);
+  return c.used;
+}
+
+// query rows index 32-bit tiles, a launch has less than 2^32 threads
+static bool prefix_fits(int64_t tokens, int64_t batch, int64_t groups, int32_t hq) {
+  return tokens <= ((int64_t)1 << 23) / hq && batch <= (1 << 22) && groups <= (1 << 22);
+}
+
+size_t sdx_prefix_attention_workspace(int64_t num_tokens, int64_t batch, int64_t num_groups,
+                                      int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim) {
+  if (num_tokens < 1 || batch < 1 || num_groups < 1 || num_q_heads < 1 || num_kv_heads < 1 ||
+      num_q_heads % num_kv_heads != 0 || (head_dim != 64 && head_dim != 128) ||
+      !prefix_fits(num_tokens, batch, num_groups, num_q_heads))
     return 0;
-  const size_t parts = sdx::prefix_attn_parts(num_tokens, num_q_heads, num_kv_heads, head_dim);
-  const size_t rows = parts * (size_t)num_tokens * num_q_heads;
-  return 256 + align256(rows * sizeof(float2)) + rows * head_dim * sizeof(float);
+  Carve c{nullptr};
+  sdx::PrefixAttnArgs a = {};
+  return prefix_ws(c, num_tokens, batch, num_groups, num_q_heads, num_kv_heads, head_dim, &a);
 }
 
 int sdx_prefix_attention_paged(const void* q, int dtype, int64_t num_tokens, int64_t batch,
@@ -1232,19 +1252,19 @@ int sdx_prefix_attention_paged(const void* q, int dtype, int64_t num_tokens, int
                 (long long)num_tokens);
   if (!q || !cu_q || !k_pool || !v_pool || !block_table || !kv_len || !cu_group || !prefix_len || !out)
     return fail(SDX_EINVAL, "sdx_prefix_attention_paged: null pointer");
-  if (max_blocks > 0x7FFFFFFF / block_size || num_blocks > (int64_t)0xFFFFFFFE / block_size)
-    return fail(SDX_EUNSUPPORTED, "sdx_prefix_attention_paged: rows of 2^31 or a pool of 2^32 - 1 "
-                                  "tokens or more");
-  // query rows index 32-bit tiles, the join's grid has less than 2^32 threads
-  if (num_tokens > ((int64_t)1 << 25) / num_q_heads || batch > (1 << 24) || num_groups > (1 << 24))
-    return fail(SDX_EUNSUPPORTED, "sdx_prefix_attention_paged: more than 2^25 query vectors or 2^24 rows");
+  if (max_blocks > (1 << 30) / block_size || num_blocks > (int64_t)0xFFFFFFFE / block_size)
+    return fail(SDX_EUNSUPPORTED, "sdx_prefix_attention_paged: rows of more than 2^30 or a pool of "
+                                  "2^32 - 1 tokens or more");
+  if (!prefix_fits(num_tokens, batch, num_groups, num_q_heads))
+    return fail(SDX_EUNSUPPORTED, "sdx_prefix_attention_paged: more than 2^23 query vectors or 2^22 rows");
   if (!aligned16(q) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out))
     return fail(SDX_EINVAL, "sdx_prefix_attention_paged: tensors must be 16-byte aligned");
-  const size_t need = sdx_prefix_attention_workspace(num_tokens, num_q_heads, num_kv_heads, head_dim);
+  Carve c{(uint8_t*)workspace};
+  sdx::PrefixAttnArgs a = {};
+  const size_t need = prefix_ws(c, num_tokens, batch, num_groups, num_q_heads, num_kv_heads, head_dim, &a);
   if (!workspace || !aligned16(workspace) || workspace_bytes < need)
     return fail(SDX_EWORKSPACE, "sdx_prefix_attention_paged: needs a 16-byte aligned workspace of %zu "
                                 "bytes (got %zu)", need, workspace_bytes);
-  sdx::PrefixAttnArgs a = {};
   a.q = (const uint16_t*)q; a.cu_q = cu_q;
   a.k_pool = (const uint16_t*)k_pool; a.v_pool = (const uint16_t*)v_pool;
   a.block_table = block_table; a.kv_len = kv_len;
@@ -1254,13 +1274,6 @@ int sdx_prefix_attention_paged(const void* q, int dtype, int64_t num_tokens, int
   a.hq = num_q_heads; a.hkv = num_kv_heads; a.group = num_q_heads / num_kv_heads; a.bs = block_size;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.out = (uint16_t*)out; a.error = error;
-  a.parts = sdx::prefix_attn_parts(num_tokens, num_q_heads, num_kv_heads, head_dim);
-  a.min_chunk = 2;
-  Carve c{(uint8_t*)workspace};
-  const size_t rows = (size_t)a.parts * num_tokens * num_q_heads;
-  a.head = c.take<int32_t>(2);
-  a.part_ml = c.take<float2>(rows);
-  a.part_o = c.take<float>(rows * head_dim);
   return hip_status(sdx::launch_prefix_attn(dtype, head_dim, a, (hipStream_t)stream), "prefix_attn");
 }
 

@@ -517,6 +517,13 @@ int logprob_parts(int64_t rows, int64_t V);  // workgroups per row
 hipError_t launch_logprob(int dtype, const LogprobArgs& a, hipStream_t s);
 
 // sdx_prefix_attn.hip: attention of groups of rows that share a prefix's keys
+constexpr int32_t PA_PART = 0xFFFFFF, PA_SHARED = 1 << 24, PA_GROUP = 1 << 25, PA_DIRECT = 1 << 26;
+struct PrefixAttnUnit {  // a tile of query rows against a chunk of keys
+  int32_t table, key0, n;  // row of the block table, first key, keys
+  int32_t t0, r0, m;       // the segment's first token, the tile's first query row, its rows
+  int32_t base;            // rows: the last key that the segment's first token sees
+  int32_t part;            // part index and the flags above
+};
 struct PrefixAttnArgs {
   const uint16_t* q;           // [tokens, hq, d] bf16 or fp16
   const int64_t* cu_q;         // [batch + 1] token offsets
@@ -531,13 +538,17 @@ struct PrefixAttnArgs {
   float scale_log2;            // softmax scale * log2(e)
   uint16_t* out;               // [tokens, hq, d]
   int32_t* error;
-  int32_t* head;               // [2] tiles per chunk (for the join)
+  int32_t* head;               // [256] the queues' heads, a line each; units of groups, of rows, masked
+  PrefixAttnUnit* entries;     // [max_entries] units but for their KV head
+  uint32_t* token_parts;       // [tokens] parts: the prefix's | the row's own << 16
+  int2* group_seg;             // [groups] the plan's sizes, then parts of each group
   float2* part_ml;             // [parts, tokens * hq] max and sum of each part
   float* part_o;               // [parts, tokens * hq, d]
+  int64_t max_entries;
   int32_t parts;               // the first half the prefix's, the second the rows' own
-  int32_t min_chunk;           // fewest 64-key tiles per chunk
 };
 int prefix_attn_parts(int64_t tokens, int32_t hq, int32_t hkv, int32_t d);
+int64_t prefix_attn_entries(int64_t tokens, int64_t batch, int64_t groups, int32_t group, int32_t parts);
 hipError_t launch_prefix_attn(int dtype, int d, const PrefixAttnArgs& a, hipStream_t s);
 
 }  // namespace sdx

@@ -21,11 +21,11 @@
 // its rows in LDS by the transposing 64-bit reads. The running maximum moves only when a
 // score passes it by 2^8 (weights up to 2^8 lose nothing), which spares rescaling O.
 //
-// Units are dealt to a fixed grid, each XCD a contiguous share of them, so that the units
-// of one chunk of keys read it from one L2. Every workgroup derives the units from the
-// lengths itself: chunk sizes from the total work, then offsets by a scan over segments.
-// A unit leaves (O, max, sum) in fp32, a second kernel joins them; a row without a prefix
-// whose keys fit one unit is written directly.
+// A plan kernel of one workgroup lists the units from the lengths. A fixed grid takes them
+// from eight queues, one for each XCD's share, so that the units of one chunk of keys read
+// it from one L2: the groups' long ones first, then the rows'. A unit leaves (O, max, sum)
+// in fp32, a third kernel joins them; a row without a prefix whose keys fit one unit is
+// written directly.
 #include <algorithm>
 #include <type_traits>
 
@@ -41,6 +41,8 @@ constexpr int PA_ROWS = 128;      // query rows per unit of the shared form
 constexpr int PA_WROWS = 32;      // query rows per wave
 constexpr int PA_GRID = 512;      // two workgroups on each of 256 CUs
 constexpr uint32_t PA_NOSLOT = 0xFFFFFFFFu;
+constexpr uint32_t PA_ASK = 0xFFFFFFFFu;
+constexpr int PA_QUEUE = 32;      // words between the queues' heads
 constexpr float PA_SLACK = 8.0f;  // log2 by which a weight may pass 1
 
 typedef short pa_s4 __attribute__((ext_vector_type(4)));
@@ -97,41 +99,45 @@ __device__ __forceinline__ int64_t pa_find(const int64_t* cu, int64_t n, int64_t
   return lo;
 }
 
+// the call's lengths and offsets, in memory or copied to LDS
+struct PaShape {
+  const int64_t *cu_q, *kv_len, *cu_group, *prefix_len;
+};
 struct PaGroup {
   int64_t first, rows, prefix;  // rows of the batch, and their shared keys (0 in a group of one)
   int64_t t0, nt;               // tokens
   bool ok;
 };
-__device__ __forceinline__ PaGroup pa_group(const PrefixAttnArgs& a, int64_t g) {
+__device__ __forceinline__ PaGroup pa_group(const PrefixAttnArgs& a, const PaShape& c, int64_t g) {
   PaGroup r;
-  const int64_t f = a.cu_group[g], e = a.cu_group[g + 1], p = a.prefix_len[g];
+  const int64_t f = c.cu_group[g], e = c.cu_group[g + 1], p = c.prefix_len[g];
   r.first = f;
   r.rows = e - f;
   r.ok = f >= 0 && e >= f && e <= a.batch && p >= 0 && p <= a.max_blocks * a.bs;
   r.prefix = r.ok && r.rows > 1 ? p : 0;
   r.t0 = r.nt = 0;
   if (r.ok) {
-    const int64_t t0 = a.cu_q[f], t1 = a.cu_q[e];
+    const int64_t t0 = c.cu_q[f], t1 = c.cu_q[e];
     r.ok = t0 >= 0 && t1 >= t0 && t1 <= a.tokens;
     if (r.ok) r.t0 = t0, r.nt = t1 - t0;
   }
   return r;
 }
 struct PaRow {
-  int64_t t0, nt, kv, prefix;
+  int64_t t0, nt, kv, prefix, group;
   bool ok;
 };
-__device__ __forceinline__ PaRow pa_row(const PrefixAttnArgs& a, int64_t b) {
+__device__ __forceinline__ PaRow pa_row(const PrefixAttnArgs& a, const PaShape& c, int64_t b) {
   PaRow r;
-  const int64_t g = pa_find(a.cu_group, a.groups, b);
-  const PaGroup gr = pa_group(a, g);
-  const int64_t t0 = a.cu_q[b], t1 = a.cu_q[b + 1];
-  r.kv = a.kv_len[b];
+  r.group = pa_find(c.cu_group, a.groups, b);
+  const PaGroup gr = pa_group(a, c, r.group);
+  const int64_t t0 = c.cu_q[b], t1 = c.cu_q[b + 1];
+  r.kv = c.kv_len[b];
   r.t0 = t0;
   r.nt = t1 - t0;
   r.prefix = gr.prefix;
-  r.ok = gr.ok && b >= gr.first && b < gr.first + gr.rows && t0 >= 0 && t1 >= t0 &&
-         t1 <= a.tokens && r.kv >= r.nt && r.kv <= a.max_blocks * a.bs;
+  r.ok = gr.ok && b >= gr.first && b < gr.first + gr.rows && t0 >= gr.t0 && t1 >= t0 &&
+         t1 <= gr.t0 + gr.nt && r.kv >= r.nt && r.kv <= a.max_blocks * a.bs;
   return r;
 }
 
@@ -145,192 +151,305 @@ __device__ __forceinline__ PaSeg pa_seg(const PrefixAttnArgs& a, int64_t nt, int
   const int64_t m = nt * a.group;
   s.shared = m > PA_WROWS;
   s.qt = keys > 0 ? (int32_t)((m + PA_ROWS - 1) / PA_ROWS) : 0;
-  s.kt = nt > 0 ? (int32_t)((keys + PA_TILE - 1) / PA_TILE) : 0;
+  s.kt = s.qt > 0 ? (int32_t)((keys + PA_TILE - 1) / PA_TILE) : 0;
   return s;
 }
 
-// Work of a 64-key tile, in units of one of the shared form.
-constexpr int PA_COST = 1, PA_COST_ALONE = 2;
-// Tiles per chunk of the two forms, for all segments of a call.
-struct PaChunks {
-  int32_t shared, alone;
-};
-__device__ __forceinline__ int32_t pa_chunk(const PaSeg& s, const PaChunks& c) {
-  return s.shared ? c.shared : c.alone;
-}
-__device__ __forceinline__ int32_t pa_nchunk(const PaSeg& s, const PaChunks& c) {
-  const int32_t n = pa_chunk(s, c);
-  return s.qt > 0 ? (s.kt + n - 1) / n : 0;
-}
+// ---- plan: one workgroup lists the units, resets the queues and notes the parts of every
+// token for the join. Work is counted in 64-key tiles of the shared form.
+constexpr int PL_NT = 512;
+constexpr int PL_CAND = 32;      // chunk sizes weighed for the groups
+constexpr int PA_ALONE = 2;      // a 64-key tile of the other form
+constexpr int PA_UNIT = 8;       // what a unit costs beside its tiles, the write of its part first
+constexpr int PL_OWN = 8;        // entries that a thread writes by itself
 
-// What a workgroup keeps of the batch: the units before each thread's run of segments.
-// Segments 0 .. G - 1 are the groups', G .. G + B - 1 the rows'.
-struct PaPlan {
-  PaChunks chunks;
-  int64_t run;             // segments per thread
-  int64_t units[2];        // in all: of groups, of rows
-  uint32_t before[2][PA_NT + 1];
-  uint64_t red[2][PA_NW + 1];
-  int32_t most;
-  int32_t masked;          // some token does not see its whole prefix
-};
-
-__device__ __forceinline__ PaSeg pa_segment(const PrefixAttnArgs& a, int64_t i, bool* ok,
-                                            bool* masked) {
-  *ok = true;
-  if (i < a.groups) {
-    const PaGroup g = pa_group(a, i);
-    *ok = g.ok;
-    return pa_seg(a, g.ok ? g.nt : 0, g.prefix);
-  }
-  const PaRow r = pa_row(a, i - a.groups);
-  *ok = r.ok;
-  if (!r.ok) return PaSeg{0, 0, false};
-  if (r.nt > 0 && r.kv - r.nt < r.prefix - 1) *masked = true;
-  return pa_seg(a, r.nt, max((int64_t)0, r.kv - r.prefix));
-}
-
-// exclusive scan over the workgroup's threads; total to every thread
-__device__ __forceinline__ uint32_t pa_scan(uint32_t v, uint32_t* wave_sum, uint32_t* total) {
+// exclusive scan over the workgroup's threads; *total to every thread
+__device__ __forceinline__ uint32_t pl_scan(uint32_t v, uint64_t* red, uint32_t* total) {
   const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
   const uint32_t inc = wave_incl_scan_u32(v, lane);
-  if (lane == kWave - 1) wave_sum[w] = inc;
+  __syncthreads();
+  if (lane == kWave - 1) red[w] = inc;
   __syncthreads();
   uint32_t ex = inc - v, t = 0;
 #pragma unroll
-  for (int i = 0; i < PA_NW; ++i) {
-    if (i < w) ex += wave_sum[i];
-    t += wave_sum[i];
+  for (int i = 0; i < PL_NT / kWave; ++i) {
+    if (i < w) ex += (uint32_t)red[i];
+    t += (uint32_t)red[i];
   }
   *total = t;
-  __syncthreads();
   return ex;
 }
-
-__device__ __forceinline__ void pa_plan(const PrefixAttnArgs& a, PaPlan& p, bool report) {
-  const int tid = threadIdx.x;
-  const int64_t n = a.groups + a.batch, run = (n + PA_NT - 1) / PA_NT;
-  if (tid == 0) p.most = 0, p.masked = 0;
-  __syncthreads();
-  uint64_t cost = 0;
-  int32_t most = 0;
-  bool masked = false, bad = false;
-  for (int64_t i = tid * run; i < min(n, (tid + 1) * run); ++i) {
-    bool ok;
-    const PaSeg s = pa_segment(a, i, &ok, &masked);
-    bad |= !ok;
-    cost += (uint64_t)s.qt * s.kt * (s.shared ? PA_COST : PA_COST_ALONE);
-    most = max(most, s.kt);
+// f(x, k) for k < n of every lane's x (words): a lane's first few by itself, the rest by the
+// wave. All lanes of the wave call it.
+template <int W, class F>
+__device__ __forceinline__ void pl_each(const int32_t (&x)[W], int32_t n, F f) {
+  for (int k = 0; k < min(n, PL_OWN); ++k) f(x, k);
+  uint64_t big = __ballot(n > PL_OWN);
+  while (big) {  // uniform
+    const int src = __ffsll((unsigned long long)big) - 1;
+    big &= big - 1;
+    int32_t y[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) y[i] = __shfl(x[i], src, kWave);
+    const int32_t m = __shfl(n, src, kWave);
+    for (int k = PL_OWN + (threadIdx.x & (kWave - 1)); k < m; k += kWave) f(y, k);
   }
-  if (tid == 0 && (a.cu_group[0] != 0 || a.cu_group[a.groups] != a.batch)) bad = true;
-  if (bad && report && a.error) *a.error = 1;
-  if (masked) p.masked = 1;
-  atomicMax(&p.most, most);
+}
+
+// tiles per chunk of a segment of kt tiles for chunks of about c tiles: equal chunks (whole
+// steps of 128 keys of the one form)
+__device__ __forceinline__ int32_t pl_chunk(int32_t kt, int32_t c, bool shared) {
+  const int32_t n = (kt + c - 1) / c, e = (kt + n - 1) / n;
+  return shared ? e : (e + 1) / 2 * 2;
+}
+
+__global__ void __launch_bounds__(PL_NT) prefix_attn_plan_kernel(PrefixAttnArgs a) {
+  __shared__ uint64_t red[PL_NT / kWave], sCost[PL_NT / kWave];
+  __shared__ uint32_t sMost[PL_NT / kWave][3];
+  __shared__ uint32_t sUnits[PL_CAND];
+  __shared__ int32_t sChunk;
+  __shared__ int64_t sQ[PL_NT + 1], sKv[PL_NT], sGroup[PL_NT + 1], sPrefix[PL_NT];
+  const int tid = threadIdx.x;
+  const int32_t half = a.parts / 2;
+  // one round of loads where the batch fits: everything after it reads LDS
+  PaShape c{a.cu_q, a.kv_len, a.cu_group, a.prefix_len};
+  const bool rows_fit = a.batch <= PL_NT, groups_fit = a.groups <= PL_NT;
+  if (rows_fit) {
+    c.cu_q = sQ;
+    c.kv_len = sKv;
+    sQ[tid] = a.cu_q[min((int64_t)tid, a.batch)];
+    if (tid == 0) sQ[PL_NT] = a.cu_q[a.batch];
+    sKv[tid] = a.kv_len[min((int64_t)tid, a.batch - 1)];
+  }
+  if (groups_fit) {
+    c.cu_group = sGroup;
+    c.prefix_len = sPrefix;
+    sGroup[tid] = a.cu_group[min((int64_t)tid, a.groups)];
+    if (tid == 0) sGroup[PL_NT] = a.cu_group[a.groups];
+    sPrefix[tid] = a.prefix_len[min((int64_t)tid, a.groups - 1)];
+  }
+  if (tid < 8) a.head[PA_QUEUE * tid] = PA_GRID / 8;
+  if (tid < PL_CAND) sUnits[tid] = 0;
+  for (int64_t t = tid; t < a.tokens; t += PL_NT) a.token_parts[t] = 0;
+  __syncthreads();
+  bool bad = tid == 0 && (c.cu_group[0] != 0 || c.cu_group[a.groups] != a.batch);
+  bool masked = false;
+
+  // sizes: of the groups, kept for the rest, and of the rows
+  uint64_t cost = 0;
+  uint32_t most = 0, most_row = 0, any_shared = 0;
+  for (int64_t g = tid; g < a.groups; g += PL_NT) {
+    const PaGroup r = pa_group(a, c, g);
+    const PaSeg s = pa_seg(a, r.nt, r.prefix);
+    bad |= !r.ok;
+    cost += (uint64_t)s.qt * s.kt * (s.shared ? 1 : PA_ALONE);
+    most = max(most, (uint32_t)s.kt);
+    any_shared |= s.kt > 0 && s.shared;
+    a.group_seg[g] = make_int2(s.shared ? s.qt : -s.qt, s.kt);
+  }
+  PaRow row0 = {};
+  for (int64_t b = tid; b < a.batch; b += PL_NT) {
+    const PaRow r = pa_row(a, c, b);
+    if (b == tid) row0 = r;
+    bad |= !r.ok;
+    if (!r.ok) continue;
+    const PaSeg s = pa_seg(a, r.nt, max((int64_t)0, r.kv - r.prefix));
+    masked |= r.nt > 0 && r.kv - r.nt < r.prefix - 1;
+    cost += (uint64_t)s.qt * s.kt * (s.shared ? 1 : PA_ALONE);
+    most_row = max(most_row, (uint32_t)s.kt);
+  }
   cost = wave_sum_u64(cost);
-  if ((tid & (kWave - 1)) == 0) p.red[0][tid / kWave] = cost;
+  most = wave_max_u32(most);
+  most_row = wave_max_u32(most_row);
+  any_shared = wave_max_u32(any_shared);
+  if ((tid & (kWave - 1)) == 0) {
+    sCost[tid / kWave] = cost;
+    sMost[tid / kWave][0] = most, sMost[tid / kWave][1] = most_row, sMost[tid / kWave][2] = any_shared;
+  }
   __syncthreads();
   cost = 0;
 #pragma unroll
-  for (int w = 0; w < PA_NW; ++w) cost += p.red[0][w];
-  // chunks of equal work that fill the grid, few enough for the parts there is room for
-  const int32_t half = a.parts / 2, least = (p.most + half - 1) / half;
-  const uint64_t each = (cost * a.hkv + PA_GRID - 1) / PA_GRID;
-  PaChunks c;
-  c.shared = (int32_t)min((uint64_t)0x3FFFFFFF, (each + PA_COST - 1) / PA_COST);
-  c.alone = (int32_t)min((uint64_t)0x3FFFFFFF, (each + PA_COST_ALONE - 1) / PA_COST_ALONE);
-  c.shared = max(max(c.shared, least), a.min_chunk);
-  c.alone = (max(max(c.alone, least), a.min_chunk) + 1) / 2 * 2;  // whole steps of 128 keys
-  uint32_t u[2] = {0, 0};
-  for (int64_t i = tid * run; i < min(n, (tid + 1) * run); ++i) {
-    bool ok;
-    const PaSeg s = pa_segment(a, i, &ok, &masked);
-    u[i >= a.groups] += (uint32_t)s.qt * (uint32_t)pa_nchunk(s, c) * (uint32_t)a.hkv;
+  for (int w = 0; w < PL_NT / kWave; ++w) {
+    cost += sCost[w];
+    most = max(most, sMost[w][0]);
+    most_row = max(most_row, sMost[w][1]);
+    any_shared = max(any_shared, sMost[w][2]);
   }
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    uint32_t total;
-    p.before[k][tid] = pa_scan(u[k], reinterpret_cast<uint32_t*>(p.red[1]), &total);
-    if (tid == 0) p.before[k][PA_NT] = total, p.units[k] = total;
+
+  // chunks of the groups: of the sizes most / 1, most / 2, ... the one whose units, dealt to
+  // the grid round by round, are done first
+  const int cand = tid % PL_CAND;
+  constexpr int lanes = PL_NT / PL_CAND;
+  // 1 .. 16, then to 224 in growing steps
+  auto cut = [](int c) { return c < 16 ? c + 1 : (16 + (c & 3) * 4) << ((c - 16) >> 2); };
+  auto size = [&](int c) { return max(2, (int)((most + cut(c) - 1) / cut(c))); };
+  {
+    const int32_t each = size(cand);
+    uint32_t n = 0;
+    for (int64_t g = tid / PL_CAND; g < a.groups; g += lanes) {
+      const int2 s = a.group_seg[g];
+      if (s.y <= 0) continue;
+      const int32_t k = pl_chunk(s.y, each, s.x > 0);
+      n += (uint32_t)abs(s.x) * ((s.y + k - 1) / k);
+    }
+    if (n) atomicAdd(&sUnits[cand], n * a.hkv);
   }
-  if (tid == 0) p.chunks = c, p.run = run;
   __syncthreads();
+  if (tid < kWave) {
+    uint32_t best = 0xFFFFFFFFu;
+    if (tid < PL_CAND && cut(tid) <= half) {
+      const uint32_t rounds = (sUnits[tid] + PA_GRID - 1) / PA_GRID;
+      const uint32_t w = any_shared ? 1 : PA_ALONE;
+      // in eighths of a tile: the rounds, and the join's read of the parts
+      const uint64_t t = (uint64_t)rounds * (size(tid) * w + PA_UNIT) * 8 + cut(tid);
+      best = (uint32_t)min(t, (uint64_t)0x3FFFFFF) << 5 | tid;
+    }
+    best = ~wave_max_u32(~best);
+    if (tid == 0) sChunk = size((int)(best & (PL_CAND - 1)));
+  }
+  __syncthreads();
+  const int32_t cg = sChunk;
+  // chunks of the rows: several per workgroup, which level out, but not below 8 tiles (of a
+  // part's cost) where the grid is full without
+  const uint64_t each = (cost * a.hkv + PA_GRID - 1) / PA_GRID;
+  auto row_chunk = [&](bool shared) {
+    const uint64_t e = each / (shared ? 1 : PA_ALONE);
+    uint64_t c = max(min(e, (uint64_t)8), e / 6);
+    c = max(max(c, (uint64_t)2), (uint64_t)(most_row + half - 1) / half);
+    return (int32_t)min(c, (uint64_t)0x3FFFFFFF);
+  };
+  const int32_t cr[2] = {row_chunk(false), row_chunk(true)};
+
+  // entries of the groups: the query tiles of a chunk follow each other
+  uint32_t base = 0;
+  for (int64_t g0 = 0; g0 < a.groups; g0 += PL_NT) {  // uniform
+    const int64_t g = g0 + tid;
+    int32_t x[7] = {};
+    uint32_t n = 0;
+    if (g < a.groups) {
+      const PaGroup r = pa_group(a, c, g);
+      const PaSeg s = pa_seg(a, r.nt, r.prefix);
+      if (s.qt > 0) {
+        const int32_t k = pl_chunk(s.kt, cg, s.shared);
+        x[0] = (int32_t)r.first, x[1] = (int32_t)r.prefix, x[2] = (int32_t)r.t0, x[3] = s.qt;
+        x[4] = k, x[5] = (int32_t)(r.nt * a.group), x[6] = s.shared;
+        n = (uint32_t)s.qt * ((s.kt + k - 1) / k);
+        a.group_seg[g].x = (s.kt + k - 1) / k;
+      } else {
+        a.group_seg[g].x = 0;
+      }
+    }
+    uint32_t total;
+    const uint32_t at = base + pl_scan(n, red, &total);
+    int32_t y[8];
+#pragma unroll
+    for (int i = 0; i < 7; ++i) y[i] = x[i];
+    y[7] = (int32_t)at;
+    base += total;
+    if (base > a.max_entries) break;  // uniform
+    pl_each(y, (int32_t)n, [&](const int32_t (&z)[8], int32_t k) {
+      const int32_t qt = k % z[3], ch = k / z[3];
+      PrefixAttnUnit u;
+      u.table = z[0];
+      u.key0 = ch * z[4] * PA_TILE;
+      u.n = min(z[4] * PA_TILE, z[1] - u.key0);
+      u.t0 = z[2];
+      u.r0 = qt * PA_ROWS;
+      u.m = min(PA_ROWS, z[5] - u.r0);
+      u.base = 0x7FFFFFFF;
+      u.part = ch | (z[6] ? PA_SHARED : 0) | PA_GROUP;
+      a.entries[z[7] + k] = u;
+    });
+  }
+  const uint32_t ngroup = base;
+  __syncthreads();  // group_seg holds the groups' parts
+  for (int64_t b0 = 0; b0 < a.batch && base <= a.max_entries; b0 += PL_NT) {  // uniform
+    const int64_t b = b0 + tid;
+    int32_t x[8] = {};
+    uint32_t n = 0;
+    int32_t nt = 0, info = 0;
+    if (b < a.batch) {
+      const PaRow r = b0 == 0 ? row0 : pa_row(a, c, b);
+      if (r.ok) {
+        const PaSeg s = pa_seg(a, r.nt, max((int64_t)0, r.kv - r.prefix));
+        int32_t ns = 0;
+        if (s.qt > 0) {
+          const int32_t k = pl_chunk(s.kt, cr[s.shared], s.shared);
+          ns = (s.kt + k - 1) / k;
+          x[0] = (int32_t)b, x[1] = (int32_t)r.prefix, x[2] = (int32_t)r.t0, x[3] = s.qt, x[4] = k;
+          x[5] = (int32_t)r.nt, x[6] = (int32_t)r.kv;
+          x[7] = s.shared | (r.prefix == 0 && ns == 1 ? 2 : 0);
+          n = (uint32_t)s.qt * ns;
+        }
+        const int32_t np = r.prefix > 0 ? a.group_seg[r.group].x : 0;
+        nt = (int32_t)r.nt;
+        info = np == 0 && ns == 1 ? 0 : np | ns << 16;  // one part is written directly
+      }
+    }
+    uint32_t total;
+    const uint32_t at = base + pl_scan(n, red, &total);
+    base += total;
+    if (base > a.max_entries) break;  // uniform
+    int32_t y[9];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = x[i];
+    y[8] = (int32_t)at;
+    pl_each(y, (int32_t)n, [&](const int32_t (&z)[9], int32_t k) {
+      const int32_t qt = k % z[3], ch = k / z[3];
+      PrefixAttnUnit u;
+      u.table = z[0];
+      u.key0 = z[1] + ch * z[4] * PA_TILE;
+      u.n = min(z[4] * PA_TILE, z[6] - u.key0);
+      u.t0 = z[2];
+      u.r0 = qt * PA_ROWS;
+      u.m = min(PA_ROWS, z[5] * a.group - u.r0);
+      u.base = z[6] - z[5];
+      u.part = (a.parts / 2 + ch) | (z[7] & 1 ? PA_SHARED : 0) | (z[7] & 2 ? PA_DIRECT : 0);
+      a.entries[z[8] + k] = u;
+    });
+    const int32_t v[2] = {nt > 0 ? (int32_t)c.cu_q[b] : 0, info};
+    pl_each(v, info ? nt : 0, [&](const int32_t (&z)[2], int32_t k) {
+      a.token_parts[z[0] + k] = (uint32_t)z[1];
+    });
+  }
+  if (base > a.max_entries) bad = true;  // rows that share tokens: offsets out of order
+  bad = __syncthreads_or(bad);
+  masked = __syncthreads_or(masked);
+  if (tid == 0) {
+    const bool none = base > a.max_entries;
+    a.head[1] = none ? 0 : (int32_t)(ngroup * a.hkv);
+    a.head[2] = none ? 0 : (int32_t)((base - ngroup) * a.hkv);
+    a.head[3] = masked;
+    if (bad && a.error) *a.error = 1;
+  }
+  if (base > a.max_entries)  // nothing was computed: nothing to join
+    for (int64_t t = tid; t < a.tokens; t += PL_NT) a.token_parts[t] = 0;
 }
 
 struct PaUnit {
-  int64_t table;       // row of the block table
-  int64_t key0;        // first key
-  int64_t t0;          // first token of the segment
-  int64_t base;        // rows: the last key that the segment's first token sees
-  int32_t n;           // keys
-  int32_t r0, m;       // first query row of the tile, rows in it
-  int32_t kvh, part;
+  int64_t table, key0, t0, base;
+  int32_t n, r0, m, kvh, part;
   bool shared, group, direct;
 };
-
-// Unit u of kind k (0 groups: query tiles of one chunk follow each other; 1 rows: KV heads).
-__device__ __forceinline__ PaUnit pa_unit(const PrefixAttnArgs& a, const PaPlan& p, int k, uint32_t u) {
-  // the thread whose run holds it: the last with before <= u
-  const int lane = threadIdx.x & (kWave - 1);
-  int t = -1;
-#pragma unroll
-  for (int w = 0; w < PA_NT / kWave; ++w) t += __popcll(__ballot(p.before[k][w * kWave + lane] <= u));
-  u -= p.before[k][t];
-  const int64_t n = a.groups + a.batch;
-  int64_t i = t * p.run;
-  const int64_t end = min(n, i + p.run);
-  PaSeg s;
-  uint32_t units = 0;
-  for (; i < end; ++i) {  // uniform
-    if ((i >= a.groups) != (k == 1)) continue;
-    bool ok, masked = false;
-    s = pa_segment(a, i, &ok, &masked);
-    units = (uint32_t)s.qt * (uint32_t)pa_nchunk(s, p.chunks) * (uint32_t)a.hkv;
-    if (u < units) break;
-    u -= units;
-  }
-  if (i >= end) {  // lengths that changed under the call
-    PaUnit none = {};
-    return none;
-  }
-  const uint32_t nch = (uint32_t)pa_nchunk(s, p.chunks);
+// Unit u: of the groups first (KV head slowest), then of the rows (KV head fastest).
+__device__ __forceinline__ PaUnit pa_unit(const PrefixAttnArgs& a, uint32_t u, uint32_t ng) {
+  uint32_t e;
   PaUnit r;
-  uint32_t qt, ch;
-  int64_t keys, nt;
-  r.group = k == 0;
-  if (k == 0) {
-    qt = u % s.qt;
-    ch = (u / s.qt) % nch;
-    r.kvh = u / s.qt / nch;
-    const PaGroup g = pa_group(a, i);
-    r.table = g.first;
-    r.key0 = 0;
-    keys = g.prefix;
-    r.t0 = g.t0;
-    nt = g.nt;
-    r.base = 0;
-    r.direct = false;
-    r.part = (int32_t)ch;
+  if (u < ng) {
+    const uint32_t entries = ng / (uint32_t)a.hkv;
+    e = u % entries;
+    r.kvh = (int32_t)(u / entries);
   } else {
-    r.kvh = u % a.hkv;
-    qt = (u / a.hkv) % s.qt;
-    ch = u / a.hkv / s.qt;
-    const int64_t b = i - a.groups;
-    const PaRow w = pa_row(a, b);
-    r.table = b;
-    r.key0 = w.prefix;
-    keys = w.kv - w.prefix;
-    r.t0 = w.t0;
-    nt = w.nt;
-    r.base = w.kv - w.nt;
-    r.direct = w.prefix == 0 && nch == 1;
-    r.part = a.parts / 2 + (int32_t)ch;
+    e = ng / (uint32_t)a.hkv + (u - ng) / (uint32_t)a.hkv;
+    r.kvh = (int32_t)((u - ng) % (uint32_t)a.hkv);
   }
-  r.shared = s.shared;
-  const int64_t c = (int64_t)pa_chunk(s, p.chunks) * PA_TILE;
-  r.n = (int32_t)min(c, keys - ch * c);
-  r.key0 += ch * c;
-  r.r0 = (int32_t)qt * PA_ROWS;
-  r.m = (int32_t)min((int64_t)PA_ROWS, nt * a.group - r.r0);
+  const PrefixAttnUnit x = a.entries[e];
+  r.table = x.table, r.key0 = x.key0, r.t0 = x.t0, r.base = x.base;
+  r.n = x.n, r.r0 = x.r0, r.m = x.m;
+  r.part = x.part & PA_PART;
+  r.shared = x.part & PA_SHARED;
+  r.group = x.part & PA_GROUP;
+  r.direct = x.part & PA_DIRECT;
   return r;
 }
 
@@ -471,24 +590,43 @@ prefix_attn_kernel(PrefixAttnArgs a) {
   constexpr int RB = 2 * D;            // bytes of a row
   __shared__ __align__(256) uint8_t sMem[PA_LDS];
   __shared__ uint32_t sSlot[PA_RING * PA_TILE];
-  __shared__ PaPlan sPlan;
+  __shared__ uint32_t sUnit;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), w = tid / kWave;
   const int hi = lane / 32, l31 = lane & 31;
-  pa_plan(a, sPlan, blockIdx.x == 0);
-  if (blockIdx.x == 0 && tid == 0) a.head[0] = sPlan.chunks.shared, a.head[1] = sPlan.chunks.alone;
   const int64_t row_elems = (int64_t)a.hkv * D;
   // addresses of the lane's operands in LDS tiles
   const uint32_t ka = l31 * RB + ((hi ^ pa_swz_k<D>(l31)) << 4);
   const int vr = 4 * hi + ((lane & 15) >> 2), vd = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
   const uint32_t va = vr * RB + (((vd >> 3) ^ pa_swz_v<D>(vr)) << 4) + (vd & 7) * 2;
-
-  // the XCD's share of both kinds of units
-  const int x = blockIdx.x % 8;
-  const uint32_t g0 = (uint32_t)(sPlan.units[0] * x / 8), ng = (uint32_t)(sPlan.units[0] * (x + 1) / 8) - g0;
-  const uint32_t b0 = (uint32_t)(sPlan.units[1] * x / 8), nb = (uint32_t)(sPlan.units[1] * (x + 1) / 8) - b0;
-  for (uint32_t at = blockIdx.x / 8; at < ng + nb; at += PA_GRID / 8) {  // uniform
-    const PaUnit u = at < ng ? pa_unit(a, sPlan, 0, g0 + at) : pa_unit(a, sPlan, 1, b0 + at - ng);
-    if (u.n <= 0 || u.m <= 0) continue;  // uniform
+  const bool masked = a.head[3];
+  // queue q: its eighth of the groups' units, then of the rows'. An XCD's workgroups have one
+  // of its queue each to begin with, then empty it, then the others'; queues that the first
+  // round empties are not asked (512 atomics to one line take as long as a small call)
+  const uint32_t ng = a.head[1], nr = a.head[2];
+  uint32_t at = blockIdx.x / 8;
+  for (int queue = 0; queue < 8;) {  // uniform
+    const uint32_t q = (blockIdx.x + queue) % 8;
+    const uint32_t g0 = (uint32_t)((uint64_t)ng * q / 8), g1 = (uint32_t)((uint64_t)ng * (q + 1) / 8);
+    const uint32_t b0 = (uint32_t)((uint64_t)nr * q / 8), b1 = (uint32_t)((uint64_t)nr * (q + 1) / 8);
+    const uint32_t n = g1 - g0 + b1 - b0;
+    if (at == PA_ASK) {
+      if (n <= PA_GRID / 8) {
+        ++queue;
+        continue;
+      }
+      if (tid == 0) sUnit = (uint32_t)__hip_atomic_fetch_add(a.head + PA_QUEUE * q, 1, __ATOMIC_RELAXED,
+                                                              __HIP_MEMORY_SCOPE_AGENT);
+      __syncthreads();
+      at = sUnit;
+      __syncthreads();
+    }
+    if (at >= n) {
+      ++queue;
+      at = PA_ASK;
+      continue;
+    }
+    const PaUnit u = pa_unit(a, at < g1 - g0 ? g0 + at : ng + b0 + at - (g1 - g0), ng);
+    at = PA_ASK;
     const int32_t* const table = a.block_table + u.table * a.max_blocks;
     const uint16_t* const kp = a.k_pool + u.kvh * D;
     const uint16_t* const vp = a.v_pool + u.kvh * D;
@@ -505,9 +643,9 @@ prefix_attn_kernel(PrefixAttnArgs a) {
     // the wave's rows: 32 w .. of the shared form, all of the other
     const int r0 = u.shared ? PA_WROWS * w : 0;
     const bool active = r0 < u.m;
-    const int lim = pa_lim(a, u, sPlan.masked, r0 + l31);
+    const int lim = pa_lim(a, u, masked, r0 + l31);
     // keys that every query row of the unit sees
-    const int seen = u.group ? (sPlan.masked ? 0 : u.n)
+    const int seen = u.group ? (masked ? 0 : u.n)
                              : (int)max((int64_t)0, min((int64_t)u.n, u.base + u.r0 / a.group + 1 - u.key0));
     pa_u4 qa[D / 16];
     {
@@ -724,57 +862,76 @@ prefix_attn_kernel(PrefixAttnArgs a) {
   }
 }
 
-// Join of a query row's parts: out = sum_c w_c O_c, w_c = 2^(m_c - m) / sum 2^(m_c - m) l_c.
-// SL slices of D / 4 threads take every SL-th part; a workgroup has R rows.
-template <int D, int FMT, int SL, int R>
-__global__ void __launch_bounds__(D / 4 * SL * R) prefix_attn_join_kernel(PrefixAttnArgs a) {
-  constexpr int DL = D / 4;
-  __shared__ float4 sO[R][SL][DL];
-  __shared__ float sL[R][SL];
-  const int tid = threadIdx.x, d4 = tid % DL, sl = tid / DL % SL, rr = tid / (DL * SL);
-  const int64_t qrow = (int64_t)blockIdx.x * R + rr;
-  const bool in = qrow < a.tokens * a.hq;
-  const int64_t t = in ? qrow / a.hq : 0;
-  const int64_t b = pa_find(a.cu_q, a.batch, t);
-  const PaRow row = pa_row(a, b);
-  int np = 0, ns = 0;
-  if (in && row.ok && t >= row.t0 && t < row.t0 + row.nt) {
-    const PaChunks c{a.head[0], a.head[1]};
-    const PaGroup g = pa_group(a, pa_find(a.cu_group, a.groups, b));
-    np = pa_nchunk(pa_seg(a, g.nt, g.prefix), c);
-    ns = pa_nchunk(pa_seg(a, row.nt, max((int64_t)0, row.kv - row.prefix)), c);
-    if (row.prefix == 0 && ns == 1) ns = 0;  // written directly
-  }
-  const int64_t stride = a.tokens * a.hq;
-  const int n = np + ns, gap = a.parts / 2 - np;  // part i: i, or i + gap from np
+// Join of a query row's parts: out = sum_c w_c O_c, w_c = 2^(m_c - m) / sum 2^(m_c - m) l_c. A
+// workgroup has HG heads of a token; 256 / (D / 4 HG) slices of D / 4 threads share a row's
+// parts, each with a running maximum of its own, and are joined in LDS.
+template <int D, int FMT, int HG>
+__global__ void __launch_bounds__(PA_NT) prefix_attn_join_kernel(PrefixAttnArgs a) {
+  constexpr int DL = D / 4, SL = PA_NT / DL / HG, UN = 4;
+  __shared__ float4 sO[SL][HG][DL];
+  __shared__ float2 sML[SL][HG];
+  const uint32_t blocks = (uint32_t)(a.hq + HG - 1) / HG;
+  const int64_t t = blockIdx.x / blocks;
+  const uint32_t info = a.token_parts[t];
+  if (info == 0) return;  // uniform
+  const int tid = threadIdx.x, d4 = tid % DL, hh = tid / DL % HG, sl = tid / DL / HG;
+  const int h = (int)(blockIdx.x % blocks) * HG + hh;
+  const int np = info & 0xFFFF, n = np + (info >> 16), gap = a.parts / 2 - np;
+  const int64_t stride = a.tokens * a.hq, qrow = t * a.hq + min(h, a.hq - 1);
   float m = -INFINITY, l = 0.0f;
-  for (int i = 0; i < n; ++i) m = fmaxf(m, a.part_ml[(i + (i < np ? 0 : gap)) * stride + qrow].x);
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-  for (int i = sl; i < n; i += SL) {
-    const int64_t p = (i + (i < np ? 0 : gap)) * stride + qrow;
-    const float2 ml = a.part_ml[p];
-    const float4 v = *reinterpret_cast<const float4*>(a.part_o + p * D + d4 * 4);
-    const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - m);
-    l += f * ml.y;
-    o.x += f * v.x;
-    o.y += f * v.y;
-    o.z += f * v.z;
-    o.w += f * v.w;
-  }
-  sO[rr][sl][d4] = o;
-  if (d4 == 0) sL[rr][sl] = l;
-  __syncthreads();
-  if (n == 0 || sl != 0) return;
+  for (int i0 = sl; i0 < n; i0 += SL * UN) {
+    float2 ml[UN];
+    float4 v[UN];
 #pragma unroll
-  for (int k = 1; k < SL; ++k) {
-    const float4 v = sO[rr][k][d4];
-    o.x += v.x;
-    o.y += v.y;
-    o.z += v.z;
-    o.w += v.w;
-    l += sL[rr][k];
+    for (int k = 0; k < UN; ++k) {  // part i lies at i, from np on at i + gap
+      const int i = min(i0 + k * SL, n - 1);
+      const int64_t p = (i + (i < np ? 0 : gap)) * stride + qrow;
+      ml[k] = a.part_ml[p];
+      v[k] = *reinterpret_cast<const float4*>(a.part_o + p * D + d4 * 4);
+    }
+    float mn = m;
+#pragma unroll
+    for (int k = 0; k < UN; ++k) mn = fmaxf(mn, ml[k].x);
+    const float s = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+    l *= s;
+    o = make_float4(o.x * s, o.y * s, o.z * s, o.w * s);
+    m = mn;
+#pragma unroll
+    for (int k = 0; k < UN; ++k) {
+      const float f = i0 + k * SL >= n || ml[k].x == -INFINITY ? 0.0f
+                                                              : __builtin_amdgcn_exp2f(ml[k].x - m);
+      l += f * ml[k].y;
+      o.x += f * v[k].x;
+      o.y += f * v[k].y;
+      o.z += f * v[k].z;
+      o.w += f * v[k].w;
+    }
   }
+  if constexpr (SL > 1) {
+    sO[sl][hh][d4] = o;
+    if (d4 == 0) sML[sl][hh] = make_float2(m, l);
+    __syncthreads();
+    if (sl > 0) return;
+    float mn = m;
+#pragma unroll
+    for (int k = 1; k < SL; ++k) mn = fmaxf(mn, sML[k][hh].x);
+    float s = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+    l *= s;
+    o = make_float4(o.x * s, o.y * s, o.z * s, o.w * s);
+#pragma unroll
+    for (int k = 1; k < SL; ++k) {
+      const float2 ml = sML[k][hh];
+      const float4 v = sO[k][hh][d4];
+      s = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
+      l += s * ml.y;
+      o.x += s * v.x;
+      o.y += s * v.y;
+      o.z += s * v.z;
+      o.w += s * v.w;
+    }
+  }
+  if (h >= a.hq) return;
   const float f = l > 0.0f || l != l ? 1.0f / l : 0.0f;
   *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + qrow * D + d4 * 4) =
       make_uint2(pa_pack<FMT>(o.x * f, o.y * f), pa_pack<FMT>(o.z * f, o.w * f));
@@ -785,25 +942,29 @@ __global__ void __launch_bounds__(D / 4 * SL * R) prefix_attn_join_kernel(Prefix
 constexpr int64_t PA_ROOM = (int64_t)192 << 20;
 int prefix_attn_parts(int64_t tokens, int32_t hq, int32_t hkv, int32_t d) {
   const int64_t one = tokens * hq * (d + 2) * 4;
-  const int64_t want = 2 * ((PA_GRID + hkv - 1) / hkv);
-  return (int)(std::max<int64_t>(1, std::min<int64_t>(want, PA_ROOM / std::max<int64_t>(1, one)) / 2) * 2);
+  const int64_t want = std::min<int64_t>(512, 2 * ((PA_GRID + hkv - 1) / hkv));
+  return (int)std::max<int64_t>(2, std::min<int64_t>(want, PA_ROOM / std::max<int64_t>(1, one)) / 2 * 2);
+}
+// A segment has a query tile of 128 rows for every 128 of its tokens' rows and one more.
+int64_t prefix_attn_entries(int64_t tokens, int64_t batch, int64_t groups, int32_t group, int32_t parts) {
+  return (2 * (tokens * group / PA_ROWS) + batch + groups) * (parts / 2);
 }
 
 template <int D, int FMT>
 static hipError_t launch_prefix_attn_t(const PrefixAttnArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((prefix_attn_kernel<D, FMT>), dim3(PA_GRID), dim3(PA_NT), 0, s, a);
+  hipLaunchKernelGGL(prefix_attn_plan_kernel, dim3(1), dim3(PL_NT), 0, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int64_t rows = a.tokens * a.hq;
-  constexpr int DL = D / 4;
-  if (rows <= 2048) {  // few rows, many parts: 8 slices a row
-    hipLaunchKernelGGL((prefix_attn_join_kernel<D, FMT, 8, 1>), dim3((unsigned)rows), dim3(DL * 8), 0,
-                       s, a);
-  } else {
-    constexpr int R = 256 / (DL * 2);
-    hipLaunchKernelGGL((prefix_attn_join_kernel<D, FMT, 2, R>), dim3((unsigned)((rows + R - 1) / R)),
-                       dim3(256), 0, s, a);
-  }
+  hipLaunchKernelGGL((prefix_attn_kernel<D, FMT>), dim3(PA_GRID), dim3(PA_NT), 0, s, a);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  // few query rows have many parts: a workgroup for each
+  if (a.tokens * a.hq <= 4096)
+    hipLaunchKernelGGL((prefix_attn_join_kernel<D, FMT, 1>), dim3((unsigned)(a.tokens * a.hq)),
+                       dim3(PA_NT), 0, s, a);
+  else
+    hipLaunchKernelGGL((prefix_attn_join_kernel<D, FMT, 8>),
+                       dim3((unsigned)(a.tokens * ((a.hq + 7) / 8))), dim3(PA_NT), 0, s, a);
   return hipGetLastError();
 }
 

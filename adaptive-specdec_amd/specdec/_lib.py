@@ -78,7 +78,7 @@ _SIGS = {
                                          I64, P, F, I32, P, SZ, P, P, P]),
     "sdx_prefix_attention_paged": (INT, [P, INT, I64, I64, P, I32, I32, I32, P, P, I64, I32, P,
                                          I64, P, P, P, I64, F, P, SZ, P, P, P]),
-    "sdx_prefix_attention_workspace": (SZ, [I64, I32, I32, I32]),
+    "sdx_prefix_attention_workspace": (SZ, [I64, I64, I64, I32, I32, I32]),
     "sdx_verify_attention_workspace": (SZ, [I64, I32, I32, I32, I32, I64, I32]),
 }
 

@@ -72,12 +72,13 @@ def verify_attention_paged(q, cu_q, k_pool, v_pool, block_table, kv_len, max_q, 
     return out
 
 
-def shared_attention_workspace(num_tokens, hq, hkv, head_dim, device="cuda"):
+def shared_attention_workspace(num_tokens, batch, num_groups, hq, hkv, head_dim, device="cuda"):
     """A workspace for shared_prefix_attention_paged at these sizes (uint8 device tensor)."""
-    need = _lib.lib().sdx_prefix_attention_workspace(int(num_tokens), hq, hkv, head_dim)
+    need = _lib.lib().sdx_prefix_attention_workspace(int(num_tokens), int(batch), int(num_groups), hq,
+                                                     hkv, head_dim)
     if need == 0:
-        raise ValueError("shared_attention_workspace: num_tokens and heads of at least 1, query "
-                         "heads a multiple of KV heads, head_dim 64 or 128")
+        raise ValueError("shared_attention_workspace: tokens, rows, groups and heads of at least 1, "
+                         "query heads a multiple of KV heads, head_dim 64 or 128")
     return torch.empty(need, dtype=torch.uint8, device=device)
 
 
@@ -141,8 +142,8 @@ def shared_prefix_attention_paged(q, cu_q, k_pool, v_pool, block_table, kv_len, 
     L = _lib.lib()
     with _lib.on_device(q):
         if workspace is None:
-            workspace = _lib.cached_workspace(L.sdx_prefix_attention_workspace(T, hq, hkv, d), q.device,
-                                              "prefix_attn")
+            workspace = _lib.cached_workspace(L.sdx_prefix_attention_workspace(T, B, G, hq, hkv, d),
+                                              q.device, "prefix_attn")
         rc = L.sdx_prefix_attention_paged(
             _lib.ptr(q), _lib.dtype_code(q), T, B, _lib.ptr(cu), hq, hkv, d, _lib.ptr(k_pool),
             _lib.ptr(v_pool), nb, bs, _lib.ptr(bt), bt.shape[1], _lib.ptr(kl), _lib.ptr(cg),

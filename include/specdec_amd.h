@@ -463,7 +463,7 @@ size_t sdx_verify_attention_workspace(int64_t batch, int32_t max_q, int32_t num_
  * Rows, or groups with all their rows, whose lengths or offsets are out of range set *error
  * (nullable) and leave their output as it was; tokens behind the last row too, without the
  * error. Page ids outside the pool set *error and the output of the rows that read them is
- * unspecified. Two kernels are queued; `workspace` (sdx_prefix_attention_workspace bytes, no
+ * unspecified. Three kernels are queued; `workspace` (sdx_prefix_attention_workspace bytes, no
  * initial contents) holds fp32 parts. A row's bits depend on the whole batch's lengths. No
  * reference counterpart (the reference keeps a copy of every row's keys). */
 int sdx_prefix_attention_paged(const void* q, int dtype, int64_t num_tokens, int64_t batch,
@@ -474,8 +474,8 @@ int sdx_prefix_attention_paged(const void* q, int dtype, int64_t num_tokens, int
                                const int64_t* prefix_len, int64_t num_groups, float scale,
                                void* workspace, size_t workspace_bytes, void* out, int32_t* error,
                                sdx_stream_t stream);
-size_t sdx_prefix_attention_workspace(int64_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads,
-                                      int32_t head_dim);
+size_t sdx_prefix_attention_workspace(int64_t num_tokens, int64_t batch, int64_t num_groups,
+                                      int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim);
 
 #ifdef __cplusplus
 }

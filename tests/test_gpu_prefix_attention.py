@@ -276,7 +276,7 @@ def test_arguments():
     with pytest.raises(RuntimeError, match="ROCm device"):
         bad(kv_len=c["kv_len"].cpu())
     with pytest.raises(ValueError):
-        shared_attention_workspace(3, 4, 3, 64)
+        shared_attention_workspace(3, 2, 1, 4, 3, 64)
     assert bad(q=c["q"][:0], cu_q=torch.zeros(3, dtype=torch.long, device=DEV)).shape == (0, 4, 64)
 
 
@@ -284,7 +284,7 @@ def test_strided_queries_and_given_workspace():
     c = make(12, [3], [90], [3, 40, 4], [1, 2, 9], 8, 2, 128)
     want = check(c)
     qkv = torch.cat([c["q"], c["q"][:, :4]], 1)
-    ws = shared_attention_workspace(12, 8, 2, 128)
+    ws = shared_attention_workspace(12, 3, 1, 8, 2, 128)
     got = shared_prefix_attention_paged(**dict(c, q=qkv[:, :8]), workspace=ws)
     assert torch.equal(got, want)
     ws.fill_(255)                       # no initial contents

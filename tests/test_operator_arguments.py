@@ -80,7 +80,8 @@ def test_prefix_attention_statuses():
 
     def call(T=3, B=2, hq=4, hkv=2, d=64, dtype=BF16, nb=8, bs=16, mb=4, G=1, scale=0.1, q=FAKE,
              pool=FAKE, out=FAKE, ws=FAKE, nbytes=None):
-        need = L.sdx_prefix_attention_workspace(max(T, 1), max(hq, 1), max(hkv, 1), d)
+        need = L.sdx_prefix_attention_workspace(max(T, 1), max(B, 1), max(G, 1), max(hq, 1),
+                                                max(hkv, 1), d)
         return L.sdx_prefix_attention_paged(q, dtype, T, B, FAKE, hq, hkv, d, pool, FAKE, nb, bs, FAKE,
                                             mb, FAKE, FAKE, FAKE, G, scale, ws,
                                             need if nbytes is None else nbytes, out, None, None)
@@ -95,13 +96,13 @@ def test_prefix_attention_statuses():
     for bad in (dict(d=96), dict(d=256), dict(dtype=F32), dict(mb=1 << 28), dict(nb=1 << 29),
                 dict(T=1 << 24)):
         assert call(**bad) == EUNSUP, bad
-    need = L.sdx_prefix_attention_workspace(3, 4, 2, 64)
+    need = L.sdx_prefix_attention_workspace(3, 2, 1, 4, 2, 64)
     assert call(nbytes=need - 1) == EWS and call(ws=None) == EWS and call(ws=off) == EWS
-    assert L.sdx_prefix_attention_workspace(0, 4, 2, 64) == 0
-    assert L.sdx_prefix_attention_workspace(3, 4, 3, 64) == 0
+    assert L.sdx_prefix_attention_workspace(0, 2, 1, 4, 2, 64) == 0
+    assert L.sdx_prefix_attention_workspace(3, 2, 1, 4, 3, 64) == 0
     # two parts at least, and no more room than for two where queries are many
-    assert L.sdx_prefix_attention_workspace(1 << 16, 32, 8, 128) >= 2 * (1 << 21) * 130 * 4
-    assert L.sdx_prefix_attention_workspace(640, 32, 8, 128) <= 200 << 20
+    assert L.sdx_prefix_attention_workspace(1 << 16, 9, 1, 32, 8, 128) >= 2 * (1 << 21) * 130 * 4
+    assert L.sdx_prefix_attention_workspace(640, 128, 1, 32, 8, 128) <= 200 << 20
 
 
 def test_entry_points_refuse_cpu_tensors():
