@@ -1206,7 +1206,7 @@ static size_t prefix_ws(Carve& c, int64_t tokens, int64_t batch, int64_t groups,
   a->parts = sdx::prefix_attn_parts(tokens, hq, hkv, d);
   a->max_entries = sdx::prefix_attn_entries(tokens, batch, groups, hq / hkv, a->parts);
   const size_t rows = (size_t)a->parts * tokens * hq;
-  a->head = c.take<int32_t>(256);
+  a->head = c.take<int32_t>(320);
   a->entries = c.take<sdx::PrefixAttnUnit>((size_t)a->max_entries);
   a->token_parts = c.take<uint32_t>((size_t)tokens);
   a->group_seg = c.take<int2>((size_t)groups);

@@ -538,7 +538,8 @@ struct PrefixAttnArgs {
   float scale_log2;            // softmax scale * log2(e)
   uint16_t* out;               // [tokens, hq, d]
   int32_t* error;
-  int32_t* head;               // [256] the queues' heads, a line each; units of groups, of rows, masked
+  int32_t* head;               // [320] the queues' heads, a line each; units of groups, of rows, masked;
+                               // a row of zeros
   PrefixAttnUnit* entries;     // [max_entries] units but for their KV head
   uint32_t* token_parts;       // [tokens] parts: the prefix's | the row's own << 16
   int2* group_seg;             // [groups] the plan's sizes, then parts of each group

@@ -43,6 +43,7 @@ constexpr int PA_GRID = 512;      // two workgroups on each of 256 CUs
 constexpr uint32_t PA_NOSLOT = 0xFFFFFFFFu;
 constexpr uint32_t PA_ASK = 0xFFFFFFFFu;
 constexpr int PA_QUEUE = 32;      // words between the queues' heads
+constexpr int PA_ZERO = 8 * PA_QUEUE;  // word of the head where a row of zeros lies
 constexpr float PA_SLACK = 8.0f;  // log2 by which a weight may pass 1
 
 typedef short pa_s4 __attribute__((ext_vector_type(4)));
@@ -229,6 +230,7 @@ __global__ void __launch_bounds__(PL_NT) prefix_attn_plan_kernel(PrefixAttnArgs 
     sPrefix[tid] = a.prefix_len[min((int64_t)tid, a.groups - 1)];
   }
   if (tid < 8) a.head[PA_QUEUE * tid] = PA_GRID / 8;
+  if (tid < 64) a.head[PA_ZERO + tid] = 0;
   if (tid < PL_CAND) sUnits[tid] = 0;
   for (int64_t t = tid; t < a.tokens; t += PL_NT) a.token_parts[t] = 0;
   __syncthreads();
@@ -513,27 +515,42 @@ __device__ __forceinline__ int pa_swz_k(int r) { return r & (D / 8 - 1); }
 template <int D>
 __device__ __forceinline__ int pa_swz_v(int r) { return D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3); }
 
-// O^T += V^T P^T for NB x 32 keys. va: the lane's byte address in V's first row block.
+// O^T += V^T P^T for NB x 32 keys. va: the lane's byte address in V's first row block. The
+// operands of four products are read ahead.
 template <int D, int FMT, int NB>
 __device__ __forceinline__ void pa_pv(PaState<D>& st, const pa_f16 (&s)[NB], const uint8_t* sV,
                                       uint32_t va) {
+  constexpr int DB = D / 32, N = NB * 2 * DB, AHEAD = 4;
+  pa_u4 x[AHEAD];
+  auto read = [&](int j) {  // product j: keys 16 (j / DB) .., dims 32 (j % DB) ..
+    const uint8_t* const at = sV + (va ^ ((j % DB) << 6)) + 16 * (j / DB) * 2 * D;
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    const u2 lo = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s4*)at));
+    const u2 up = __builtin_bit_cast(
+        u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s4*)(at + 8 * 2 * D)));
+    x[j % AHEAD] = (pa_u4){lo[0], lo[1], up[0], up[1]};
+  };
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
+  for (int j = 0; j < AHEAD; ++j) read(j);
+  pa_u4 p;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      pa_u4 p;
+  for (int j = 0; j < N; ++j) {
+    const int k = j / DB;
+    if (j % DB == 0) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) p[e] = pa_pack<FMT>(s[nb][8 * k + 2 * e], s[nb][8 * k + 2 * e + 1]);
-#pragma unroll
-      for (int db = 0; db < D / 32; ++db) {
-        const uint8_t* const at = sV + (va ^ (db << 6)) + (32 * nb + 16 * k) * 2 * D;
-        const pa_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s4*)at);
-        const pa_s4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s4*)(at + 8 * 2 * D));
-        typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-        const u2 x = __builtin_bit_cast(u2, lo), y = __builtin_bit_cast(u2, up);
-        st.o[db] = pa_mfma<FMT>((pa_u4){x[0], x[1], y[0], y[1]}, p, st.o[db]);
-      }
+      for (int e = 0; e < 4; ++e)
+        p[e] = pa_pack<FMT>(s[k / 2][8 * (k % 2) + 2 * e], s[k / 2][8 * (k % 2) + 2 * e + 1]);
     }
+    st.o[j % DB] = pa_mfma<FMT>(x[j % AHEAD], p, st.o[j % DB]);
+    if (j + AHEAD < N) read(j + AHEAD);
+  }
+  // reads (0x100) and products (0x008) in this order; the rest falls between them
+  __builtin_amdgcn_sched_group_barrier(0x100, 2 * AHEAD, 0);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if (j + AHEAD < N) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+  }
 }
 
 constexpr int PA_LDS_TILES = 2 * 2 * PA_TILE * 2 * 128;          // two tiles of K and V
@@ -579,10 +596,6 @@ __device__ __forceinline__ int64_t pa_qrow(const PrefixAttnArgs& a, const PaUnit
   return (u.t0 + r / a.group) * a.hq + u.kvh * a.group + r % a.group;
 }
 
-// What is read in place of a key past the chunk, or without a page: its weight is 0, and its
-// V must not be NaN.
-__device__ const uint4 pa_zero_row[16] = {};
-
 template <int D, int FMT>
 __global__ void __launch_bounds__(PA_NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 prefix_attn_kernel(PrefixAttnArgs a) {
@@ -593,7 +606,7 @@ prefix_attn_kernel(PrefixAttnArgs a) {
   __shared__ uint32_t sUnit;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), w = tid / kWave;
   const int hi = lane / 32, l31 = lane & 31;
-  const int64_t row_elems = (int64_t)a.hkv * D;
+  const uint32_t row_bytes = (uint32_t)a.hkv * RB;
   // addresses of the lane's operands in LDS tiles
   const uint32_t ka = l31 * RB + ((hi ^ pa_swz_k<D>(l31)) << 4);
   const int vr = 4 * hi + ((lane & 15) >> 2), vd = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
@@ -628,9 +641,11 @@ prefix_attn_kernel(PrefixAttnArgs a) {
     const PaUnit u = pa_unit(a, at < g1 - g0 ? g0 + at : ng + b0 + at - (g1 - g0), ng);
     at = PA_ASK;
     const int32_t* const table = a.block_table + u.table * a.max_blocks;
-    const uint16_t* const kp = a.k_pool + u.kvh * D;
-    const uint16_t* const vp = a.v_pool + u.kvh * D;
-    const uint16_t* const zero = reinterpret_cast<const uint16_t*>(pa_zero_row);
+    const uint8_t* const kp = reinterpret_cast<const uint8_t*>(a.k_pool + u.kvh * D);
+    const uint8_t* const vp = reinterpret_cast<const uint8_t*>(a.v_pool + u.kvh * D);
+    // read in place of a key past the chunk, or without a page: its weight is 0, and its V
+    // must not be NaN
+    const uint8_t* const zero = reinterpret_cast<const uint8_t*>(a.head + PA_ZERO);
     const uint32_t pos0 = (uint32_t)u.key0;
     int bad = 0;
     PaState<D> st;
@@ -681,9 +696,9 @@ prefix_attn_kernel(PrefixAttnArgs a) {
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           const uint32_t s = sSlot[(tile % PA_RING) * PA_TILE + lr + TPR * h];
-          const int64_t off = (int64_t)s * row_elems + lc * 8;
-          kk[h] = *reinterpret_cast<const pa_u4*>(s == PA_NOSLOT ? zero : kp + off);
-          vv[h] = *reinterpret_cast<const pa_u4*>(s == PA_NOSLOT ? zero : vp + off);
+          const uint64_t off = (uint64_t)s * row_bytes;
+          kk[h] = *reinterpret_cast<const pa_u4*>((s == PA_NOSLOT ? zero : kp + off) + lc * 16);
+          vv[h] = *reinterpret_cast<const pa_u4*>((s == PA_NOSLOT ? zero : vp + off) + lc * 16);
         }
       };
       static_assert(TPR % 16 == 0, "a pass's rows are swizzled alike");
@@ -721,17 +736,32 @@ prefix_attn_kernel(PrefixAttnArgs a) {
         if (active) {
           const uint8_t* const k = sMem + buf * (2 * PA_TILE * RB);
           pa_f16 s[2] = {};
-#pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks)
+          pa_u4 x[2][2];  // operands of a step, read a step ahead
+          auto read = [&](int ks) {
 #pragma unroll
             for (int n = 0; n < 2; ++n)
-              s[n] = pa_mfma<FMT>(*reinterpret_cast<const pa_u4*>(k + (ka ^ (ks << 5)) + n * 32 * RB),
-                                  qa[ks], s[n]);
+              x[ks & 1][n] = *reinterpret_cast<const pa_u4*>(k + (ka ^ (ks << 5)) + n * 32 * RB);
+          };
+          read(0);
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) {
+            if (ks + 1 < D / 16) read(ks + 1);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) s[n] = pa_mfma<FMT>(x[ks & 1][n], qa[ks], s[n]);
+          }
+          // in this order: two steps' reads, then a step's products and the reads after next
+          __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+            if (ks + 2 < D / 16) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+          }
           if ((t + 1) * PA_TILE > seen) pa_mask<2>(s, t * PA_TILE, lim, hi);  // uniform
           pa_softmax<D, 2>(st, s, a.scale_log2);
           pa_pv<D, FMT, 2>(st, s, k + PA_TILE * RB, va);
         }
         stage(next);  // past the last tile: rows of zeros
+        __builtin_amdgcn_sched_barrier(0);  // the registers are free before they are loaded
         gather(t + 2);
         __syncthreads();
       };
@@ -775,16 +805,16 @@ prefix_attn_kernel(PrefixAttnArgs a) {
       };
       pa_u4 kk[D / 16], vv[H];
       auto gather_k = [&](uint32_t slot) {
-        const uint16_t* src = slot == PA_NOSLOT ? zero : kp + (int64_t)slot * row_elems + 8 * hi;
+        const uint8_t* src = (slot == PA_NOSLOT ? zero : kp + (uint64_t)slot * row_bytes) + 16 * hi;
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) kk[ks] = *reinterpret_cast<const pa_u4*>(src + 16 * ks);
+        for (int ks = 0; ks < D / 16; ++ks) kk[ks] = *reinterpret_cast<const pa_u4*>(src + 32 * ks);
       };
       auto gather_v = [&](uint32_t slot) {
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           const uint32_t s = (uint32_t)__shfl((int)slot, lr + TPR * h, kWave);
-          vv[h] = *reinterpret_cast<const pa_u4*>(s == PA_NOSLOT ? zero
-                                                                : vp + (int64_t)s * row_elems + lc * 8);
+          vv[h] = *reinterpret_cast<const pa_u4*>(
+              (s == PA_NOSLOT ? zero : vp + (uint64_t)s * row_bytes) + lc * 16);
         }
       };
       int32_t page = page_of(0);
