@@ -507,13 +507,13 @@ __device__ __forceinline__ void pa_softmax(PaState<D>& st, pa_f16 (&s)[NB], floa
   st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
-// 16-byte chunk c of row r of a tile in LDS lies in chunk c ^ swizzle(r): the operand reads
-// of consecutive rows then fall into different banks. K rows are read 16 bytes a lane, 8
-// rows at a time; V rows 32 bytes, 4 rows at a time.
+// 16-byte chunk c of row r of a tile in LDS lies in chunk c ^ swizzle(r): the operand reads of
+// a phase then fall into different banks of the 64. K rows are read 16 bytes a lane, 16 rows
+// at a time; V rows 64 bytes of 4 rows at a time.
 template <int D>
 __device__ __forceinline__ int pa_swz_k(int r) { return r & (D / 8 - 1); }
 template <int D>
-__device__ __forceinline__ int pa_swz_v(int r) { return D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3); }
+__device__ __forceinline__ int pa_swz_v(int r) { return D == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); }
 
 // O^T += V^T P^T for NB x 32 keys. va: the lane's byte address in V's first row block. The
 // operands of four products are read ahead.
@@ -735,6 +735,7 @@ prefix_attn_kernel(PrefixAttnArgs a) {
         }
         if (active) {
           const uint8_t* const k = sMem + buf * (2 * PA_TILE * RB);
+          __builtin_amdgcn_s_setprio(1);
           pa_f16 s[2] = {};
           pa_u4 x[2][2];  // operands of a step, read a step ahead
           auto read = [&](int ks) {
@@ -756,9 +757,12 @@ prefix_attn_kernel(PrefixAttnArgs a) {
             __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
             if (ks + 2 < D / 16) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
           }
+          __builtin_amdgcn_s_setprio(0);
           if ((t + 1) * PA_TILE > seen) pa_mask<2>(s, t * PA_TILE, lim, hi);  // uniform
           pa_softmax<D, 2>(st, s, a.scale_log2);
+          __builtin_amdgcn_s_setprio(1);
           pa_pv<D, FMT, 2>(st, s, k + PA_TILE * RB, va);
+          __builtin_amdgcn_s_setprio(0);
         }
         stage(next);  // past the last tile: rows of zeros
         __builtin_amdgcn_sched_barrier(0);  // the registers are free before they are loaded
