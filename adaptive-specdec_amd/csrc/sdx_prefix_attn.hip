@@ -164,22 +164,6 @@ constexpr int PA_ALONE = 2;      // a 64-key tile of the other form
 constexpr int PA_UNIT = 8;       // what a unit costs beside its tiles, the write of its part first
 constexpr int PL_OWN = 8;        // entries that a thread writes by itself
 
-// exclusive scan over the workgroup's threads; *total to every thread
-__device__ __forceinline__ uint32_t pl_scan(uint32_t v, uint64_t* red, uint32_t* total) {
-  const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
-  const uint32_t inc = wave_incl_scan_u32(v, lane);
-  __syncthreads();
-  if (lane == kWave - 1) red[w] = inc;
-  __syncthreads();
-  uint32_t ex = inc - v, t = 0;
-#pragma unroll
-  for (int i = 0; i < PL_NT / kWave; ++i) {
-    if (i < w) ex += (uint32_t)red[i];
-    t += (uint32_t)red[i];
-  }
-  *total = t;
-  return ex;
-}
 // f(x, k) for k < n of every lane's x (words): a lane's first few by itself, the rest by the
 // wave. All lanes of the wave call it.
 template <int W, class F>
@@ -204,13 +188,22 @@ __device__ __forceinline__ int32_t pl_chunk(int32_t kt, int32_t c, bool shared) 
   return shared ? e : (e + 1) / 2 * 2;
 }
 
+// What the workgroup sums up over its threads, one wave's record after another in LDS.
+struct PlSum {
+  uint64_t cost;
+  uint32_t most, most_row, any_shared, flags;  // flags: 1 an error, 2 a token before the prefix's end
+};
+
+// The plan's steps are short and depend on each other, so its time is that of its rounds of
+// loads (one, where the batch fits LDS) and barriers (four). 4 rows 6 us, 128 rows 8.
 __global__ void __launch_bounds__(PL_NT) prefix_attn_plan_kernel(PrefixAttnArgs a) {
-  __shared__ uint64_t red[PL_NT / kWave], sCost[PL_NT / kWave];
-  __shared__ uint32_t sMost[PL_NT / kWave][3];
+  constexpr int NW = PL_NT / kWave;
+  __shared__ PlSum sSum[NW];
+  __shared__ uint64_t sScan[2][NW];
   __shared__ uint32_t sUnits[PL_CAND];
-  __shared__ int32_t sChunk;
   __shared__ int64_t sQ[PL_NT + 1], sKv[PL_NT], sGroup[PL_NT + 1], sPrefix[PL_NT];
-  const int tid = threadIdx.x;
+  __shared__ int2 sSeg[PL_NT];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wv = tid / kWave;
   const int32_t half = a.parts / 2;
   // one round of loads where the batch fits: everything after it reads LDS
   PaShape c{a.cu_q, a.kv_len, a.cu_group, a.prefix_len};
@@ -229,203 +222,234 @@ __global__ void __launch_bounds__(PL_NT) prefix_attn_plan_kernel(PrefixAttnArgs 
     if (tid == 0) sGroup[PL_NT] = a.cu_group[a.groups];
     sPrefix[tid] = a.prefix_len[min((int64_t)tid, a.groups - 1)];
   }
+  int2* const seg = groups_fit ? sSeg : a.group_seg;  // query tiles (< 0: the other form), key tiles
   if (tid < 8) a.head[PA_QUEUE * tid] = PA_GRID / 8;
   if (tid < 64) a.head[PA_ZERO + tid] = 0;
   if (tid < PL_CAND) sUnits[tid] = 0;
   for (int64_t t = tid; t < a.tokens; t += PL_NT) a.token_parts[t] = 0;
   __syncthreads();
-  bool bad = tid == 0 && (c.cu_group[0] != 0 || c.cu_group[a.groups] != a.batch);
-  bool masked = false;
 
-  // sizes: of the groups, kept for the rest, and of the rows
-  uint64_t cost = 0;
-  uint32_t most = 0, most_row = 0, any_shared = 0;
+  // sizes
+  PlSum sum = {};
+  if (tid == 0 && (c.cu_group[0] != 0 || c.cu_group[a.groups] != a.batch)) sum.flags = 1;
+  PaGroup group0 = {};
+  PaRow row0 = {};
   for (int64_t g = tid; g < a.groups; g += PL_NT) {
     const PaGroup r = pa_group(a, c, g);
+    if (g == tid) group0 = r;
     const PaSeg s = pa_seg(a, r.nt, r.prefix);
-    bad |= !r.ok;
-    cost += (uint64_t)s.qt * s.kt * (s.shared ? 1 : PA_ALONE);
-    most = max(most, (uint32_t)s.kt);
-    any_shared |= s.kt > 0 && s.shared;
-    a.group_seg[g] = make_int2(s.shared ? s.qt : -s.qt, s.kt);
+    if (!r.ok) sum.flags |= 1;
+    sum.cost += (uint64_t)s.qt * s.kt * (s.shared ? 1 : PA_ALONE);
+    sum.most = max(sum.most, (uint32_t)s.kt);
+    sum.any_shared |= s.kt > 0 && s.shared;
+    seg[g] = make_int2(s.shared ? s.qt : -s.qt, s.kt);
   }
-  PaRow row0 = {};
   for (int64_t b = tid; b < a.batch; b += PL_NT) {
     const PaRow r = pa_row(a, c, b);
     if (b == tid) row0 = r;
-    bad |= !r.ok;
-    if (!r.ok) continue;
+    if (!r.ok) {
+      sum.flags |= 1;
+      continue;
+    }
     const PaSeg s = pa_seg(a, r.nt, max((int64_t)0, r.kv - r.prefix));
-    masked |= r.nt > 0 && r.kv - r.nt < r.prefix - 1;
-    cost += (uint64_t)s.qt * s.kt * (s.shared ? 1 : PA_ALONE);
-    most_row = max(most_row, (uint32_t)s.kt);
+    if (r.nt > 0 && r.kv - r.nt < r.prefix - 1) sum.flags |= 2;
+    sum.cost += (uint64_t)s.qt * s.kt * (s.shared ? 1 : PA_ALONE);
+    sum.most_row = max(sum.most_row, (uint32_t)s.kt);
   }
-  cost = wave_sum_u64(cost);
-  most = wave_max_u32(most);
-  most_row = wave_max_u32(most_row);
-  any_shared = wave_max_u32(any_shared);
-  if ((tid & (kWave - 1)) == 0) {
-    sCost[tid / kWave] = cost;
-    sMost[tid / kWave][0] = most, sMost[tid / kWave][1] = most_row, sMost[tid / kWave][2] = any_shared;
-  }
+  sum.cost = wave_sum_u64(sum.cost);
+  sum.most = wave_max_u32(sum.most);
+  sum.most_row = wave_max_u32(sum.most_row);
+  sum.flags = (__any(sum.flags & 1) ? 1 : 0) | (__any(sum.flags & 2) ? 2 : 0);
+  sum.any_shared = __any(sum.any_shared);
+  if (lane == 0) sSum[wv] = sum;
   __syncthreads();
-  cost = 0;
+  sum = sSum[0];
 #pragma unroll
-  for (int w = 0; w < PL_NT / kWave; ++w) {
-    cost += sCost[w];
-    most = max(most, sMost[w][0]);
-    most_row = max(most_row, sMost[w][1]);
-    any_shared = max(any_shared, sMost[w][2]);
+  for (int w = 1; w < NW; ++w) {
+    sum.cost += sSum[w].cost;
+    sum.most = max(sum.most, sSum[w].most);
+    sum.most_row = max(sum.most_row, sSum[w].most_row);
+    sum.any_shared |= sSum[w].any_shared;
+    sum.flags |= sSum[w].flags;
   }
 
   // chunks of the groups: of the sizes most / 1, most / 2, ... the one whose units, dealt to
-  // the grid round by round, are done first
-  const int cand = tid % PL_CAND;
-  constexpr int lanes = PL_NT / PL_CAND;
+  // the grid round by round, are done first. A candidate for each pair of lanes; of many
+  // groups every wave takes some.
+  const int cand = lane % PL_CAND;
   // 1 .. 16, then to 224 in growing steps
-  auto cut = [](int c) { return c < 16 ? c + 1 : (16 + (c & 3) * 4) << ((c - 16) >> 2); };
-  auto size = [&](int c) { return max(2, (int)((most + cut(c) - 1) / cut(c))); };
+  auto cut = [](int i) { return i < 16 ? i + 1 : (16 + (i & 3) * 4) << ((i - 16) >> 2); };
+  auto size = [&](int i) { return max(2, (int)((sum.most + cut(i) - 1) / cut(i))); };
+  int32_t cg;
   {
-    const int32_t each = size(cand);
+    const int32_t mine = size(cand);
+    const bool few = a.groups <= 32;
     uint32_t n = 0;
-    for (int64_t g = tid / PL_CAND; g < a.groups; g += lanes) {
-      const int2 s = a.group_seg[g];
+    for (int64_t g = few ? lane / PL_CAND : tid / PL_CAND; g < a.groups; g += few ? 2 : PL_NT / PL_CAND) {
+      const int2 s = seg[g];
       if (s.y <= 0) continue;
-      const int32_t k = pl_chunk(s.y, each, s.x > 0);
+      const int32_t k = pl_chunk(s.y, mine, s.x > 0);
       n += (uint32_t)abs(s.x) * ((s.y + k - 1) / k);
     }
-    if (n) atomicAdd(&sUnits[cand], n * a.hkv);
-  }
-  __syncthreads();
-  if (tid < kWave) {
-    uint32_t best = 0xFFFFFFFFu;
-    if (tid < PL_CAND && cut(tid) <= half) {
-      const uint32_t rounds = (sUnits[tid] + PA_GRID - 1) / PA_GRID;
-      const uint32_t w = any_shared ? 1 : PA_ALONE;
-      // in eighths of a tile: the rounds, and the join's read of the parts
-      const uint64_t t = (uint64_t)rounds * (size(tid) * w + PA_UNIT) * 8 + cut(tid);
-      best = (uint32_t)min(t, (uint64_t)0x3FFFFFF) << 5 | tid;
+    n *= (uint32_t)a.hkv;
+    if (few) {
+      n += (uint32_t)__shfl_xor((int)n, 32, kWave);
+    } else {  // uniform
+      atomicAdd(&sUnits[cand], n);
+      __syncthreads();
+      n = sUnits[cand];
     }
+    const uint32_t rounds = (n + PA_GRID - 1) / PA_GRID, w = sum.any_shared ? 1 : PA_ALONE;
+    // in eighths of a tile: the rounds, and the join's read of the parts
+    const uint64_t t = (uint64_t)rounds * (mine * w + PA_UNIT) * 8 + cut(cand);
+    uint32_t best = cut(cand) <= half ? (uint32_t)min(t, (uint64_t)0x3FFFFFF) << 5 | cand : 0xFFFFFFFFu;
     best = ~wave_max_u32(~best);
-    if (tid == 0) sChunk = size((int)(best & (PL_CAND - 1)));
+    cg = size((int)(best & (PL_CAND - 1)));
   }
-  __syncthreads();
-  const int32_t cg = sChunk;
   // chunks of the rows: several per workgroup, which level out, but not below 8 tiles (of a
   // part's cost) where the grid is full without
-  const uint64_t each = (cost * a.hkv + PA_GRID - 1) / PA_GRID;
+  const uint64_t each = (sum.cost * a.hkv + PA_GRID - 1) / PA_GRID;
   auto row_chunk = [&](bool shared) {
     const uint64_t e = each / (shared ? 1 : PA_ALONE);
-    uint64_t c = max(min(e, (uint64_t)8), e / 6);
-    c = max(max(c, (uint64_t)2), (uint64_t)(most_row + half - 1) / half);
-    return (int32_t)min(c, (uint64_t)0x3FFFFFFF);
+    uint64_t k = max(min(e, (uint64_t)8), e / 6);
+    k = max(max(k, (uint64_t)2), (uint64_t)(sum.most_row + half - 1) / half);
+    return (int32_t)min(k, (uint64_t)0x3FFFFFFF);
   };
   const int32_t cr[2] = {row_chunk(false), row_chunk(true)};
 
-  // entries of the groups: the query tiles of a chunk follow each other
-  uint32_t base = 0;
-  for (int64_t g0 = 0; g0 < a.groups; g0 += PL_NT) {  // uniform
-    const int64_t g = g0 + tid;
-    int32_t x[7] = {};
-    uint32_t n = 0;
-    if (g < a.groups) {
-      const PaGroup r = pa_group(a, c, g);
-      const PaSeg s = pa_seg(a, r.nt, r.prefix);
-      if (s.qt > 0) {
-        const int32_t k = pl_chunk(s.kt, cg, s.shared);
-        x[0] = (int32_t)r.first, x[1] = (int32_t)r.prefix, x[2] = (int32_t)r.t0, x[3] = s.qt;
-        x[4] = k, x[5] = (int32_t)(r.nt * a.group), x[6] = s.shared;
-        n = (uint32_t)s.qt * ((s.kt + k - 1) / k);
-        a.group_seg[g].x = (s.kt + k - 1) / k;
-      } else {
-        a.group_seg[g].x = 0;
-      }
+  // entries: of the groups (the query tiles of a chunk follow each other), then of the rows
+  uint32_t ngroup = 0, nrow = 0;  // of the threads' items so far
+  auto group_item = [&](int64_t g, int32_t (&x)[8]) -> uint32_t {
+    if (g >= a.groups) return 0;
+    const PaGroup r = g == tid ? group0 : pa_group(a, c, g);
+    const PaSeg s = pa_seg(a, r.nt, r.prefix);
+    if (s.qt == 0) {
+      a.group_seg[g].x = 0;
+      return 0;
     }
-    uint32_t total;
-    const uint32_t at = base + pl_scan(n, red, &total);
-    int32_t y[8];
-#pragma unroll
-    for (int i = 0; i < 7; ++i) y[i] = x[i];
-    y[7] = (int32_t)at;
-    base += total;
-    if (base > a.max_entries) break;  // uniform
-    pl_each(y, (int32_t)n, [&](const int32_t (&z)[8], int32_t k) {
-      const int32_t qt = k % z[3], ch = k / z[3];
-      PrefixAttnUnit u;
-      u.table = z[0];
-      u.key0 = ch * z[4] * PA_TILE;
-      u.n = min(z[4] * PA_TILE, z[1] - u.key0);
-      u.t0 = z[2];
-      u.r0 = qt * PA_ROWS;
-      u.m = min(PA_ROWS, z[5] - u.r0);
-      u.base = 0x7FFFFFFF;
-      u.part = ch | (z[6] ? PA_SHARED : 0) | PA_GROUP;
-      a.entries[z[7] + k] = u;
-    });
-  }
-  const uint32_t ngroup = base;
-  __syncthreads();  // group_seg holds the groups' parts
-  for (int64_t b0 = 0; b0 < a.batch && base <= a.max_entries; b0 += PL_NT) {  // uniform
-    const int64_t b = b0 + tid;
-    int32_t x[8] = {};
-    uint32_t n = 0;
-    int32_t nt = 0, info = 0;
-    if (b < a.batch) {
-      const PaRow r = b0 == 0 ? row0 : pa_row(a, c, b);
-      if (r.ok) {
-        const PaSeg s = pa_seg(a, r.nt, max((int64_t)0, r.kv - r.prefix));
-        int32_t ns = 0;
-        if (s.qt > 0) {
-          const int32_t k = pl_chunk(s.kt, cr[s.shared], s.shared);
-          ns = (s.kt + k - 1) / k;
-          x[0] = (int32_t)b, x[1] = (int32_t)r.prefix, x[2] = (int32_t)r.t0, x[3] = s.qt, x[4] = k;
-          x[5] = (int32_t)r.nt, x[6] = (int32_t)r.kv;
-          x[7] = s.shared | (r.prefix == 0 && ns == 1 ? 2 : 0);
-          n = (uint32_t)s.qt * ns;
-        }
-        const int32_t np = r.prefix > 0 ? a.group_seg[r.group].x : 0;
-        nt = (int32_t)r.nt;
-        info = np == 0 && ns == 1 ? 0 : np | ns << 16;  // one part is written directly
-      }
+    const int32_t k = pl_chunk(s.kt, cg, s.shared), n = (s.kt + k - 1) / k;
+    x[0] = (int32_t)r.first, x[1] = (int32_t)r.prefix, x[2] = (int32_t)r.t0, x[3] = s.qt, x[4] = k;
+    x[5] = (int32_t)(r.nt * a.group), x[6] = s.shared;
+    a.group_seg[g].x = n;
+    return (uint32_t)s.qt * n;
+  };
+  int32_t row_t0 = 0, row_nt = 0, row_parts = 0;
+  auto row_item = [&](int64_t b, int32_t (&x)[9]) -> uint32_t {
+    row_nt = row_parts = 0;
+    if (b >= a.batch) return 0;
+    const PaRow r = b == tid ? row0 : pa_row(a, c, b);
+    if (!r.ok) return 0;
+    const PaSeg s = pa_seg(a, r.nt, max((int64_t)0, r.kv - r.prefix));
+    row_t0 = (int32_t)r.t0, row_nt = (int32_t)r.nt;
+    if (s.qt == 0) return 0;
+    const int32_t k = pl_chunk(s.kt, cr[s.shared], s.shared), n = (s.kt + k - 1) / k;
+    x[0] = (int32_t)b, x[1] = (int32_t)r.prefix, x[2] = (int32_t)r.t0, x[3] = s.qt, x[4] = k;
+    x[5] = (int32_t)r.nt, x[6] = (int32_t)r.kv, x[7] = s.shared | (r.prefix == 0 && n == 1 ? 2 : 0);
+    row_parts = n;
+    return (uint32_t)s.qt * n;
+  };
+  auto put_group = [&](const int32_t (&z)[8], int32_t k) {
+    const int32_t qt = k % z[3], ch = k / z[3];
+    PrefixAttnUnit u;
+    u.table = z[0];
+    u.key0 = ch * z[4] * PA_TILE;
+    u.n = min(z[4] * PA_TILE, z[1] - u.key0);
+    u.t0 = z[2];
+    u.r0 = qt * PA_ROWS;
+    u.m = min(PA_ROWS, z[5] - u.r0);
+    u.base = 0x7FFFFFFF;
+    u.part = ch | (z[6] ? PA_SHARED : 0) | PA_GROUP;
+    a.entries[z[7] + k] = u;
+  };
+  auto put_row = [&](const int32_t (&z)[9], int32_t k) {
+    const int32_t qt = k % z[3], ch = k / z[3];
+    PrefixAttnUnit u;
+    u.table = z[0];
+    u.key0 = z[1] + ch * z[4] * PA_TILE;
+    u.n = min(z[4] * PA_TILE, z[6] - u.key0);
+    u.t0 = z[2];
+    u.r0 = qt * PA_ROWS;
+    u.m = min(PA_ROWS, z[5] * a.group - u.r0);
+    u.base = z[6] - z[5];
+    u.part = (a.parts / 2 + ch) | (z[7] & 1 ? PA_SHARED : 0) | (z[7] & 2 ? PA_DIRECT : 0);
+    a.entries[z[8] + k] = u;
+  };
+  auto note_tokens = [&](int64_t b) {  // after the groups' parts are known
+    if (row_nt > 0) {
+      const PaRow& r = row0;
+      const int64_t g = b == tid ? r.group : pa_find(c.cu_group, a.groups, b);
+      const int64_t prefix = b == tid ? r.prefix : pa_group(a, c, g).prefix;
+      const int32_t np = prefix > 0 ? a.group_seg[g].x : 0;
+      row_parts = np == 0 && row_parts == 1 ? 0 : np | row_parts << 16;  // one part: written directly
     }
-    uint32_t total;
-    const uint32_t at = base + pl_scan(n, red, &total);
-    base += total;
-    if (base > a.max_entries) break;  // uniform
-    int32_t y[9];
+    const int32_t v[2] = {row_t0, row_parts};
+    pl_each(v, row_parts ? row_nt : 0,
+            [&](const int32_t (&z)[2], int32_t k) { a.token_parts[z[0] + k] = (uint32_t)z[1]; });
+  };
+  // one scan of both counts, for as many blocks of PL_NT items as the larger of them has
+  auto scan = [&](uint32_t x, uint32_t y, uint32_t* ex, uint32_t* ey, int par) {
+    const uint64_t v = (uint64_t)x | (uint64_t)y << 32, inc = wave_incl_scan_u64(v, lane);
+    if (lane == kWave - 1) sScan[par][wv] = inc;
+    __syncthreads();
+    uint64_t before = inc - v, total = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = x[i];
-    y[8] = (int32_t)at;
-    pl_each(y, (int32_t)n, [&](const int32_t (&z)[9], int32_t k) {
-      const int32_t qt = k % z[3], ch = k / z[3];
-      PrefixAttnUnit u;
-      u.table = z[0];
-      u.key0 = z[1] + ch * z[4] * PA_TILE;
-      u.n = min(z[4] * PA_TILE, z[6] - u.key0);
-      u.t0 = z[2];
-      u.r0 = qt * PA_ROWS;
-      u.m = min(PA_ROWS, z[5] * a.group - u.r0);
-      u.base = z[6] - z[5];
-      u.part = (a.parts / 2 + ch) | (z[7] & 1 ? PA_SHARED : 0) | (z[7] & 2 ? PA_DIRECT : 0);
-      a.entries[z[8] + k] = u;
-    });
-    const int32_t v[2] = {nt > 0 ? (int32_t)c.cu_q[b] : 0, info};
-    pl_each(v, info ? nt : 0, [&](const int32_t (&z)[2], int32_t k) {
-      a.token_parts[z[0] + k] = (uint32_t)z[1];
-    });
+    for (int w = 0; w < NW; ++w) {
+      if (w < wv) before += sScan[par][w];
+      total += sScan[par][w];
+    }
+    *ex = (uint32_t)before, *ey = (uint32_t)(before >> 32);
+    return total;
+  };
+  if (rows_fit && groups_fit) {
+    int32_t x[8] = {}, y[9] = {};
+    const uint32_t n = group_item(tid, x), m = row_item(tid, y);
+    uint32_t ex, ey;
+    const uint64_t total = scan(n, m, &ex, &ey, 0);
+    ngroup = (uint32_t)total, nrow = (uint32_t)(total >> 32);
+    if ((int64_t)ngroup + nrow <= a.max_entries) {  // uniform
+      x[7] = (int32_t)ex;
+      y[8] = (int32_t)(ngroup + ey);
+      pl_each(x, (int32_t)n, put_group);
+      pl_each(y, (int32_t)m, put_row);
+      note_tokens(tid);
+    }
+  } else {
+    int par = 0;
+    for (int64_t i = 0; i < a.groups; i += PL_NT, par ^= 1) {  // uniform
+      int32_t x[8] = {};
+      const uint32_t n = group_item(i + tid, x);
+      uint32_t ex, ey;
+      const uint32_t total = (uint32_t)scan(n, 0, &ex, &ey, par);
+      x[7] = (int32_t)(ngroup + ex);
+      ngroup += total;
+      if (ngroup > a.max_entries) break;
+      pl_each(x, (int32_t)n, put_group);
+    }
+    __syncthreads();  // group_seg holds the groups' parts
+    for (int64_t i = 0; i < a.batch && (int64_t)ngroup + nrow <= a.max_entries; i += PL_NT, par ^= 1) {
+      int32_t y[9] = {};
+      const uint32_t n = row_item(i + tid, y);
+      uint32_t ex, ey;
+      const uint32_t total = (uint32_t)scan(n, 0, &ex, &ey, par);
+      y[8] = (int32_t)(ngroup + nrow + ex);
+      nrow += total;
+      if ((int64_t)ngroup + nrow > a.max_entries) break;
+      pl_each(y, (int32_t)n, put_row);
+      note_tokens(i + tid);
+    }
   }
-  if (base > a.max_entries) bad = true;  // rows that share tokens: offsets out of order
-  bad = __syncthreads_or(bad);
-  masked = __syncthreads_or(masked);
+  // more entries than there is room for: rows that share tokens, offsets out of order
+  const bool none = (int64_t)ngroup + nrow > a.max_entries;
   if (tid == 0) {
-    const bool none = base > a.max_entries;
     a.head[1] = none ? 0 : (int32_t)(ngroup * a.hkv);
-    a.head[2] = none ? 0 : (int32_t)((base - ngroup) * a.hkv);
-    a.head[3] = masked;
-    if (bad && a.error) *a.error = 1;
+    a.head[2] = none ? 0 : (int32_t)(nrow * a.hkv);
+    a.head[3] = (sum.flags & 2) != 0;
+    if ((none || (sum.flags & 1)) && a.error) *a.error = 1;
   }
-  if (base > a.max_entries)  // nothing was computed: nothing to join
+  if (none) {  // uniform: nothing is computed, nothing is joined
+    __syncthreads();
     for (int64_t t = tid; t < a.tokens; t += PL_NT) a.token_parts[t] = 0;
+  }
 }
 
 struct PaUnit {

@@ -5,6 +5,7 @@ The library is built in-tree by `adaptive-specdec_amd/build.py` (or
 is not on a ROCm device, calls raise.
 """
 import ctypes
+import functools
 import os
 
 import torch
@@ -132,10 +133,14 @@ def require_gpu(*tensors):
                 f"{getattr(t, 'device', type(t))}")
 
 
-def same_device(first, *others):
-    """Every tensor on the first one's device."""
+def one_gpu(first, *others):
+    """Every tensor (None aside) on the ROCm device of the first."""
+    dev = first.get_device() if isinstance(first, torch.Tensor) else -1
+    if dev < 0:
+        require_gpu(first)
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != dev):
+            require_gpu(t)
             raise ValueError(f"tensors on several devices: {first.device} and {t.device}")
 
 
@@ -148,13 +153,20 @@ class _Here:
 
 
 _HERE = _Here()
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def on_device(t):
     """A context in which t's device is the current one (kernels launch on the current
     device, whatever stream they are given)."""
-    d = t.device.index
-    return _HERE if d is None or d == torch.cuda.current_device() else torch.cuda.device(d)
+    d = t.get_device()
+    return _HERE if d == _current_device() else torch.cuda.device(d)
+
+
+@functools.lru_cache(maxsize=4096)
+def workspace_bytes(query, *args):
+    """What the C ABI's workspace query of that name answers (a function of its arguments)."""
+    return getattr(lib(), query)(*args)
 
 
 def ptr(t):

@@ -98,10 +98,8 @@ def shared_prefix_attention_paged(q, cu_q, k_pool, v_pool, block_table, kv_len, 
     [1] device tensor) when given, and so do page ids outside the pool. `workspace` (uint8,
     `shared_attention_workspace`) holds fp32 parts; None: the stream's own, kept for its next
     calls."""
-    _lib.require_gpu(q, cu_q, k_pool, v_pool, block_table, kv_len, cu_group, prefix_len, out, error,
-                     workspace)
-    _lib.same_device(q, cu_q, k_pool, v_pool, block_table, kv_len, cu_group, prefix_len, out, error,
-                     workspace)
+    _lib.one_gpu(q, cu_q, k_pool, v_pool, block_table, kv_len, cu_group, prefix_len, out, error,
+                 workspace)
     if q.dtype not in (torch.bfloat16, torch.float16) or k_pool.dtype != q.dtype or \
             v_pool.dtype != q.dtype:
         raise TypeError("shared_prefix_attention_paged: q and pools all bf16 or all fp16")
@@ -139,12 +137,11 @@ def shared_prefix_attention_paged(q, cu_q, k_pool, v_pool, block_table, kv_len, 
     cg = _lib.as_dtype(cu_group, torch.int64)
     pl = _lib.as_dtype(prefix_len, torch.int64)
     bt = _lib.as_dtype(block_table, torch.int32)
-    L = _lib.lib()
     with _lib.on_device(q):
         if workspace is None:
-            workspace = _lib.cached_workspace(L.sdx_prefix_attention_workspace(T, B, G, hq, hkv, d),
-                                              q.device, "prefix_attn")
-        rc = L.sdx_prefix_attention_paged(
+            need = _lib.workspace_bytes("sdx_prefix_attention_workspace", T, B, G, hq, hkv, d)
+            workspace = _lib.cached_workspace(need, q.device, "prefix_attn")
+        rc = _lib.lib().sdx_prefix_attention_paged(
             _lib.ptr(q), _lib.dtype_code(q), T, B, _lib.ptr(cu), hq, hkv, d, _lib.ptr(k_pool),
             _lib.ptr(v_pool), nb, bs, _lib.ptr(bt), bt.shape[1], _lib.ptr(kl), _lib.ptr(cg),
             _lib.ptr(pl), G, scale, _lib.ptr(workspace), workspace.numel(), _lib.ptr(out),

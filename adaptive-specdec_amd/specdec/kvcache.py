@@ -327,10 +327,9 @@ class PagedKVCache:
         return flat[self.slots(b, length)]
 
 
-def _error_word(error, like):
+def _error_word(error):
     if error is not None and (error.dtype != torch.int32 or error.numel() < 1):
         raise TypeError("error must be an int32 device tensor of one element")
-    _lib.same_device(like, error)
 
 
 def build_block_tables(kv_len, free_blocks, block_size, max_blocks, cu_group=None, prefix_len=None,
@@ -346,9 +345,8 @@ def build_block_tables(kv_len, free_blocks, block_size, max_blocks, cu_group=Non
     free). All or nothing: lengths, groups or free pages that do not fit give a table of -1
     and used 0, and set `error` (an int32 [1] device tensor) when given.
     """
-    _lib.require_gpu(kv_len, free_blocks, cu_group, prefix_len, out, error)
-    _lib.same_device(kv_len, free_blocks, cu_group, prefix_len, out)
-    _error_word(error, kv_len)
+    _lib.one_gpu(kv_len, free_blocks, cu_group, prefix_len, out, error)
+    _error_word(error)
     block_size, max_blocks = int(block_size), int(max_blocks)
     if (cu_group is None) != (prefix_len is None):
         raise ValueError("cu_group and prefix_len go together")
@@ -390,9 +388,8 @@ def paged_slot_mapping(block_table, cu_q, kv_len, block_size, num_tokens, paddin
     padding (position 0, slot padding_slot_id), and so are those of a row whose length or
     pages are out of range, which set `error` (an int32 [1] device tensor) when given.
     """
-    _lib.require_gpu(block_table, cu_q, kv_len, error)
-    _lib.same_device(block_table, cu_q, kv_len)
-    _error_word(error, block_table)
+    _lib.one_gpu(block_table, cu_q, kv_len, error)
+    _error_word(error)
     bt = _lib.as_dtype(block_table, torch.int32)
     cu = _lib.as_dtype(cu_q, torch.int64)
     kl = _lib.as_dtype(kv_len, torch.int64)
@@ -416,9 +413,8 @@ def append_paged_slots(pool, staged, slots, error=None):
     pool [L, 2, num_blocks, block_size, row_elems] (contiguous; written in place). Negative
     slots are padding and skipped; slots past the pool are skipped and set `error` (an int32
     [1] device tensor) when given."""
-    _lib.require_gpu(pool, staged, slots, error)
-    _lib.same_device(pool, staged, slots)
-    _error_word(error, pool)
+    _lib.one_gpu(pool, staged, slots, error)
+    _error_word(error)
     if pool.dim() != 5 or pool.shape[1] != 2 or not pool.is_contiguous():
         raise ValueError("pool must be a contiguous [L, 2, num_blocks, block_size, row_elems]")
     L, _, nb, bs, re = pool.shape

@@ -158,8 +158,7 @@ def token_logprobs(logits, ids, temperature=1.0, top_n=0):
     lowest id first among equals (else None, None). temperature > 0: the greedy limit has no
     finite scores. Rows without a finite maximum, or with NaN, score NaN.
     """
-    _lib.require_gpu(logits, ids)
-    _lib.same_device(logits, ids)
+    _lib.one_gpu(logits, ids)
     lead, V = logits.shape[:-1], logits.shape[-1]
     if tuple(ids.shape) != tuple(lead) and tuple(ids.shape[:-1]) != tuple(lead):
         raise ValueError(f"ids must be {tuple(lead)} or {tuple(lead)} + (n,), got "
@@ -188,15 +187,13 @@ def token_logprobs(logits, ids, temperature=1.0, top_n=0):
         top_ids = torch.empty((*lead, top_n), dtype=torch.int64, device=dev)
     if rows == 0:
         return logp, entropy, top_logp, top_ids
-    L = _lib.lib()
     with _lib.on_device(x):
-        need = L.sdx_token_logprobs_workspace(rows, V, top_n)
+        need = _lib.workspace_bytes("sdx_token_logprobs_workspace", rows, V, top_n)
         ws = _lib.cached_workspace(need, dev, "logprobs") if need else None
-        rc = L.sdx_token_logprobs(_lib.ptr(x), _lib.dtype_code(x), rows, V,
-                                  x.stride(0) if rows > 1 else V, T, _lib.ptr(i), n, top_n,
-                                  _lib.ptr(logp), _lib.ptr(entropy), _lib.ptr(top_logp),
-                                  _lib.ptr(top_ids), _lib.ptr(ws), ws.numel() if need else 0,
-                                  _lib.stream_of(x))
+        rc = _lib.lib().sdx_token_logprobs(
+            _lib.ptr(x), _lib.dtype_code(x), rows, V, x.stride(0) if rows > 1 else V, T, _lib.ptr(i), n,
+            top_n, _lib.ptr(logp), _lib.ptr(entropy), _lib.ptr(top_logp), _lib.ptr(top_ids),
+            _lib.ptr(ws), ws.numel() if need else 0, _lib.stream_of(x))
     _lib.check(rc, "token_logprobs")
     return logp, entropy, top_logp, top_ids
 
