@@ -6,15 +6,18 @@
 //   log p(i) = d_i - ln z          entropy = ln z - w / z
 // One pass: every thread keeps (m, z, w) of what it has read, in base 2 and shifted to its
 // own running maximum (w of a sum shifted by s: 2^s (w + s z)), and joins with the others
-// at the end. Sums are fp32; no decision depends on them.
+// at the end. Sums are fp32; no decision depends on them. The shift is taken in x, before the
+// product with log2(e) / T: one operation an element more than x c - m c fused, but the
+// largest logit's term is exactly 1 and rows masked by their type's lowest value do not
+// overflow.
 //
 // Likeliest tokens, by (value, lowest id): a thread also keeps its largest value and the
-// first 16-byte vector that holds it, unique to the thread. Every one of the n best
-// elements lies in one of the n best threads by (largest value, first vector): an element
-// outside them is beaten by one element of each. So the n threads' vectors are read again
-// (1 / 12 of a row's part at n = 20), those elements collected that reach the n-th thread's
-// (value, vector), and sorted. Per element the list costs the maximum that the sums need
-// anyway.
+// first 16-byte vector that holds it, unique to the thread. Take the n-th best of any n or
+// more of these heads as an edge: n elements reach it, so no element below it is listed, and
+// a thread whose head is below it has none that is. The edge comes from 64 heads, the best
+// of four threads each (n-th of 64 in a wave); the few threads that reach it read their
+// vectors again, and what reaches it there, n elements and a few, is sorted. Per element the
+// list costs the maximum that the sums need anyway.
 //
 // Bound by the read of the logits. A row is split over workgroups where rows are few, and a
 // second kernel joins its parts.
@@ -53,31 +56,64 @@ __device__ __forceinline__ float lp_elem(const void* row, int64_t i) {
   else return decode16<FMT>(reinterpret_cast<const uint16_t*>(row)[i]);
 }
 
-// The 16-byte vector of elements first .. first + VEC - 1, which all lie in the row.
+// A row in 16-byte vectors from the boundary at or before its start: vector v holds elements
+// v VEC - off .. + VEC - 1. A part is vectors v0 .. v1 - 1.
+struct LpSpan {
+  const uint8_t* row;
+  int64_t V, v0, v1, safe;  // safe: a vector that lies in the row as a whole (-1: none)
+  int off;
+};
 template <int FMT>
-__device__ __forceinline__ void lp_load(const void* row, int64_t first, float (&x)[lp_vec<FMT>()]) {
-  if constexpr (FMT == SDX_F32) {
-    const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row) + first);
-    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-  } else {
-    const uint4 v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(row) + first);
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+__device__ __forceinline__ LpSpan lp_span(const LogprobArgs& a, int64_t r, int part) {
+  constexpr int VEC = lp_vec<FMT>(), ES = 16 / VEC;
+  LpSpan s;
+  s.row = reinterpret_cast<const uint8_t*>(a.logits) + r * a.ld * ES;
+  s.V = a.V;
+  s.off = (int)(((uintptr_t)s.row & 15u) / ES);
+  const int64_t n = (a.V + s.off + VEC - 1) / VEC;
+  s.v0 = n * part / a.parts;
+  s.v1 = n * (part + 1) / a.parts;
+  s.safe = s.off > 0 ? 1 : 0;
+  if ((s.safe + 1) * VEC - s.off > a.V) s.safe = -1;
+  return s;
+}
+template <int FMT>
+__device__ __forceinline__ bool lp_whole(const LpSpan& s, int64_t v) {
+  constexpr int VEC = lp_vec<FMT>();
+  return v < s.v1 && v * VEC >= s.off && (v + 1) * VEC - s.off <= s.V;
+}
+// Vector v, or another of the row where v is not whole: loads that no branch holds up.
+template <int FMT>
+__device__ __forceinline__ uint4 lp_load(const LpSpan& s, int64_t v) {
+  const int64_t w = lp_whole<FMT>(s, v) ? v : s.safe;
+  if (s.safe < 0) return make_uint4(0, 0, 0, 0);  // uniform
+  return *reinterpret_cast<const uint4*>(s.row - s.off * (16 / lp_vec<FMT>()) + w * 16);
+}
+template <int FMT>
+__device__ __forceinline__ void lp_elems_whole(uint4 raw, float (&x)[lp_vec<FMT>()]) {
+  const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (FMT == SDX_F32) {
+      x[i] = __uint_as_float(u[i]);
+    } else {
       x[2 * i] = decode16<FMT>(u[i] & 0xFFFFu);
       x[2 * i + 1] = decode16<FMT>(u[i] >> 16);
     }
   }
 }
-// The same where it may reach past [lo, hi): those elements are not read, and are -inf.
+// Its elements; those outside the part or the row are -inf, and not read.
 template <int FMT>
-__device__ __forceinline__ void lp_load_edge(const void* row, int64_t first, int64_t lo, int64_t hi,
-                                             float (&x)[lp_vec<FMT>()]) {
+__device__ __forceinline__ void lp_elems(const LpSpan& s, int64_t v, uint4 raw,
+                                         float (&x)[lp_vec<FMT>()]) {
   constexpr int VEC = lp_vec<FMT>();
-  if (first >= lo && first + VEC <= hi) return lp_load<FMT>(row, first, x);
+  lp_elems_whole<FMT>(raw, x);
+  if (lp_whole<FMT>(s, v)) return;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i)
-    x[i] = first + i >= lo && first + i < hi ? lp_elem<FMT>(row, first + i) : -INFINITY;
+  for (int i = 0; i < VEC; ++i) {
+    const int64_t id = v * VEC - s.off + i;
+    x[i] = v < s.v1 && id >= 0 && id < s.V ? lp_elem<FMT>(s.row, id) : -INFINITY;
+  }
 }
 
 // (m, z, w) moved to the larger maximum mn.
@@ -126,24 +162,42 @@ __device__ __forceinline__ int lp_pow2(int n) {
   return n <= 2 ? 2 : 1 << (32 - __clz(n - 1));
 }
 
-// A row's results from its sums and its sorted keys (value order << 32 | ~id).
+struct LpRow {  // a row's sums, and ln z
+  float m, z, w, lnz;
+};
+__device__ __forceinline__ LpRow lp_row(const LpPart& p) { return LpRow{p.m, p.z, p.w, logf(p.z)}; }
+// log p at logit x.
+__device__ __forceinline__ float lp_logp(const LogprobArgs& a, const LpRow& p, float x) {
+  return !(p.z > 0.0f) ? NAN : (x - p.m) / a.T - p.lnz;  // no finite maximum, or a NaN
+}
+// A row's results from its sums, by `lanes` threads from `tid` on.
 template <int FMT>
 __device__ __forceinline__ void lp_finish(const LogprobArgs& a, int64_t r, const void* row,
-                                          const LpPart& p, const uint64_t* keys) {
-  const float lnz = logf(p.z);
-  const bool none = !(p.z > 0.0f);  // no finite maximum, or a NaN
-  auto logp = [&](float x) { return none ? NAN : (x - p.m) / a.T - lnz; };
-  for (int i = threadIdx.x; i < a.n_ids; i += LP_NT) {
+                                          const LpRow& p, int tid, int lanes) {
+  for (int i = tid; i < a.n_ids; i += lanes) {
     const int64_t id = a.ids[r * a.n_ids + i];
-    a.logp[r * a.n_ids + i] =
-        id >= 0 && id < a.V ? logp(lp_elem<FMT>(row, id)) : (none ? NAN : -INFINITY);
+    const bool in = id >= 0 && id < a.V;
+    const float v = lp_logp(a, p, in ? lp_elem<FMT>(row, id) : 0.0f);
+    a.logp[r * a.n_ids + i] = in || v != v ? v : -INFINITY;
   }
-  if (threadIdx.x == 0) a.entropy[r] = none ? NAN : lnz - 0.6931471805599453f * (p.w / p.z);
-  for (int i = threadIdx.x; i < a.top_n; i += LP_NT) {
-    const uint32_t o = (uint32_t)(keys[i] >> 32);  // 0 and 1 only in a row with NaN
-    a.top_ids[r * a.top_n + i] = o == 0u ? -1 : (int64_t)(uint32_t)~(uint32_t)keys[i];
-    a.top_logp[r * a.top_n + i] = o <= 1u ? NAN : logp(lp_unord(o));
+  if (tid == 0) a.entropy[r] = !(p.z > 0.0f) ? NAN : p.lnz - 0.6931471805599453f * (p.w / p.z);
+}
+// Entry i of a row's list from its key (value order << 32 | ~id).
+__device__ __forceinline__ void lp_put(const LogprobArgs& a, int64_t r, int i, const LpRow& p,
+                                       uint64_t key) {
+  const uint32_t o = (uint32_t)(key >> 32);  // 0 and 1 only in a row with NaN
+  a.top_ids[r * a.top_n + i] = o == 0u ? -1 : (int64_t)(uint32_t)~(uint32_t)key;
+  a.top_logp[r * a.top_n + i] = o <= 1u ? NAN : lp_logp(a, p, lp_unord(o));
+}
+// The number of lanes whose key is greater than this lane's; keys differ, or are 0.
+__device__ __forceinline__ int lp_wave_rank(uint64_t key) {
+  int rank = 0;
+#pragma unroll 8
+  for (int t = 0; t < kWave; ++t) {
+    const uint64_t k = (uint64_t)rdlane((uint32_t)(key >> 32), t) << 32 | rdlane((uint32_t)key, t);
+    rank += k > key;
   }
+  return rank;
 }
 
 // Part blockIdx.x % parts of row blockIdx.x / parts: elements [lo, hi). One part: the results; several: the
@@ -154,46 +208,43 @@ __global__ void __launch_bounds__(LP_NT) logprob_kernel(LogprobArgs a) {
   __shared__ LpPart sPart[LP_NT / kWave];
   __shared__ uint64_t sKeys[TOP ? LP_CAP : 1];
   __shared__ uint64_t sHead[TOP ? LP_NT : 1];
-  __shared__ int sSel[TOP ? LP_NT : 1], sCount;
+  __shared__ int sSel[TOP ? LP_NT : 1], sCount, sNsel;
   const int tid = threadIdx.x;
   const int64_t r = blockIdx.x / (uint32_t)a.parts;
   const int part = (int)(blockIdx.x % (uint32_t)a.parts);
-  const void* const row = reinterpret_cast<const uint8_t*>(a.logits) +
-                          r * a.ld * (FMT == SDX_F32 ? 4 : 2);
-  // vectors of the row from the 16-byte boundary at or before it; this part's [v0, v1)
-  const int off = (int)(((uintptr_t)row & 15u) / (FMT == SDX_F32 ? 4 : 2));
-  const int64_t nvec = (a.V + off + VEC - 1) / VEC;
-  const int64_t v0 = nvec * part / a.parts, v1 = nvec * (part + 1) / a.parts;
-  const int64_t lo = max((int64_t)0, v0 * VEC - off), hi = min(a.V, v1 * VEC - off);
+  const LpSpan span = lp_span<FMT>(a, r, part);
+  const int64_t v0 = span.v0, v1 = span.v1;
   const float c = a.c;
 
   LpPart p{LP_LOWEST, 0.0f, 0.0f, 0.0f};
   uint32_t best = 0;  // order of the thread's largest value, and the vector it first came in
   uint32_t at = 0;
   for (int64_t vb = v0; vb < v1; vb += LP_NT * LP_UN) {  // uniform
-    float x[LP_UN][VEC];
-    if (vb > v0 && vb + LP_NT * LP_UN < v1) {  // whole vectors throughout
+    uint4 raw[LP_UN];
 #pragma unroll
-      for (int u = 0; u < LP_UN; ++u)
-        lp_load<FMT>(row, (vb + u * LP_NT + tid) * VEC - off, x[u]);
+    for (int u = 0; u < LP_UN; ++u) raw[u] = lp_load<FMT>(span, vb + u * LP_NT + tid);
+    float x[LP_UN][VEC];
+    if (vb > v0 && vb + LP_NT * LP_UN < v1) {  // uniform: all whole
+#pragma unroll
+      for (int u = 0; u < LP_UN; ++u) lp_elems_whole<FMT>(raw[u], x[u]);
     } else {
 #pragma unroll
-      for (int u = 0; u < LP_UN; ++u)
-        lp_load_edge<FMT>(row, (vb + u * LP_NT + tid) * VEC - off, lo, hi, x[u]);
+      for (int u = 0; u < LP_UN; ++u) lp_elems<FMT>(span, vb + u * LP_NT + tid, raw[u], x[u]);
     }
-    float mn = p.m;
+    float top = LP_LOWEST;
 #pragma unroll
     for (int u = 0; u < LP_UN; ++u) {
       float vm = x[u][0];
 #pragma unroll
       for (int i = 1; i < VEC; ++i) vm = fmaxf(vm, x[u][i]);
-      mn = fmaxf(mn, vm);
+      top = fmaxf(top, vm);
       if constexpr (TOP) {
         const int64_t v = vb + u * LP_NT + tid;
         const uint32_t o = lp_ord(vm);
         if (o > best && v < v1) best = o, at = (uint32_t)v;
       }
     }
+    const float mn = fmaxf(p.m, top);
     lp_shift(p.z, p.w, p.m, mn, c);
     p.m = mn;
 #pragma unroll
@@ -208,37 +259,60 @@ __global__ void __launch_bounds__(LP_NT) logprob_kernel(LogprobArgs a) {
   }
   lp_wave_join(p, c);
   if ((tid & (kWave - 1)) == 0) sPart[tid / kWave] = p;
-  if constexpr (TOP) sHead[tid] = ((uint64_t)best << 32) | (uint32_t)~at;
-  if (tid == 0) sCount = 0;
+  const uint64_t head = best ? (uint64_t)best << 32 | (uint32_t)~at : 0;
+  if constexpr (TOP) sHead[tid] = head;
+  if (tid == 0) sCount = 0, sNsel = 0;
   __syncthreads();
   p = sPart[0];
 #pragma unroll
   for (int w = 1; w < LP_NT / kWave; ++w) lp_join(p, sPart[w], c);
 
+  const LpRow row_sums = lp_row(p);
+  bool sorted = false;  // the list lies in sKeys in order
   if constexpr (TOP) {
-    // the top_n best threads by (value, first vector); threads without a vector have 0
-    const uint64_t mine = sHead[tid];
-    int rank = 0;
-    for (int t = 0; t < LP_NT; ++t) rank += sHead[t] > mine || (sHead[t] == mine && t < tid);
-    if (rank < a.top_n) sSel[rank] = tid;
-    __syncthreads();
-    const int nsel = min(a.top_n, LP_NT);
-    const uint64_t edge = sHead[sSel[nsel - 1]];
-    const uint32_t eo = (uint32_t)(edge >> 32), ev = ~(uint32_t)edge;
-    const int per = (int)((v1 - v0 + LP_NT - 1) / LP_NT);  // vectors of a thread
-    // `take` gets every element (key) of the selected threads that can be in the list
-    auto visit = [&](auto take) {
-      for (int i = tid; i < nsel * per; i += LP_NT) {
-        const int64_t v = v0 + (int64_t)(i / nsel) * LP_NT + sSel[i % nsel];
-        if (v >= v1) continue;
-        float y[VEC];
-        lp_load_edge<FMT>(row, v * VEC - off, lo, hi, y);
+    // every wave: the n-th best of 64 heads, of four threads each
+    uint64_t h = sHead[tid & (kWave - 1)];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const int64_t id = v * VEC - off + e;
-          const uint32_t o = lp_ord(y[e]);
-          if (id >= lo && id < hi && (o > eo || (o == eo && (eo == 0 || (uint32_t)v <= ev))))
-            take(((uint64_t)o << 32) | (uint32_t)~(uint32_t)id);
+    for (int w = 1; w < LP_NT / kWave; ++w) {
+      const uint64_t k = sHead[w * kWave + (tid & (kWave - 1))];
+      h = k > h ? k : h;
+    }
+    // lanes without a vector are last, and equal
+    const int rank = lp_wave_rank(h);
+    const uint64_t reach = __ballot(h > 0 && rank < a.top_n);
+    uint64_t edge = 0;  // fewer heads than n: everything is listed
+    if (__popcll(reach) >= a.top_n) {
+      const int at_n = __ffsll((unsigned long long)__ballot(rank == a.top_n - 1)) - 1;
+      edge = (uint64_t)rdlane((uint32_t)(h >> 32), at_n) << 32 | rdlane((uint32_t)h, at_n);
+    }
+    const uint32_t eo = (uint32_t)(edge >> 32), ev = ~(uint32_t)edge;
+    if (best && head >= edge) sSel[atomicAdd(&sNsel, 1)] = tid;
+    __syncthreads();
+    // take(key) for the elements of those threads that reach the edge: their vectors spread
+    // over the workgroup, several loads in flight
+    const uint32_t nsel = (uint32_t)sNsel, all = nsel * (uint32_t)((v1 - v0 + LP_NT - 1) / LP_NT);
+    auto visit = [&](auto take) {
+      for (uint32_t i0 = tid; i0 < all; i0 += LP_NT * LP_UN) {
+        int64_t v[LP_UN];
+        uint4 raw[LP_UN];
+#pragma unroll
+        for (int u = 0; u < LP_UN; ++u) {
+          const uint32_t i = i0 + u * LP_NT;
+          v[u] = i < all ? v0 + (int64_t)(i / nsel) * LP_NT + sSel[i % nsel] : v1;
+          raw[u] = lp_load<FMT>(span, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < LP_UN; ++u) {
+          float y[VEC];
+          lp_elems<FMT>(span, v[u], raw[u], y);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const int64_t id = v[u] * VEC - span.off + e;
+            const uint32_t o = lp_ord(y[e]);
+            if (o >= eo && (o > eo || edge == 0 || (uint32_t)v[u] <= ev) && v[u] < v1 && id >= 0 &&
+                id < a.V)
+              take((uint64_t)o << 32 | (uint32_t)~(uint32_t)id);
+          }
         }
       }
     };
@@ -248,11 +322,25 @@ __global__ void __launch_bounds__(LP_NT) logprob_kernel(LogprobArgs a) {
     });
     __syncthreads();
     const int n = sCount;
-    if (n <= LP_CAP) {
-      lp_sort(sKeys, n, lp_pow2(max(n, a.top_n)));
+    if (n <= kWave) {  // one wave ranks them
+      if (tid < kWave) {
+        const uint64_t k = tid < n ? sKeys[tid] : 0;
+        const int i = lp_wave_rank(k);
+        // the list is longer than a part with fewer elements: zeros follow
+        if (k > 0 && i < a.top_n) {
+          if (a.parts == 1) lp_put(a, r, i, row_sums, k);
+          else a.part_keys[(r * a.parts + part) * a.top_n + i] = k;
+        }
+        if (tid >= n && tid < a.top_n) {
+          if (a.parts == 1) lp_put(a, r, tid, row_sums, 0);
+          else a.part_keys[(r * a.parts + part) * a.top_n + tid] = 0;
+        }
+      }
+    } else if (n <= LP_CAP) {
+      lp_sort(sKeys, n, lp_pow2(n));
+      sorted = true;
     } else {  // many elements of few threads: the largest, then the largest below it, ...
       uint64_t last = ~0ull;
-      __syncthreads();
       for (int k = 0; k < a.top_n; ++k) {
         uint64_t b = 0;
         visit([&](uint64_t q) { b = q < last && q > b ? q : b; });
@@ -268,44 +356,65 @@ __global__ void __launch_bounds__(LP_NT) logprob_kernel(LogprobArgs a) {
         last = b;
         __syncthreads();
       }
+      sorted = true;
     }
+    if (sorted)
+      for (int i = tid; i < a.top_n; i += LP_NT) {
+        if (a.parts == 1) lp_put(a, r, i, row_sums, sKeys[i]);
+        else a.part_keys[(r * a.parts + part) * a.top_n + i] = sKeys[i];
+      }
   }
-  if (a.parts == 1) {
-    lp_finish<FMT>(a, r, row, p, sKeys);
-  } else {
-    const int64_t to = r * a.parts + part;
-    if (tid == 0) reinterpret_cast<LpPart*>(a.part)[to] = p;
-    if constexpr (TOP)
-      for (int i = tid; i < a.top_n; i += LP_NT) a.part_keys[to * a.top_n + i] = sKeys[i];
-  }
+  if (a.parts == 1) lp_finish<FMT>(a, r, span.row, row_sums, tid, LP_NT);
+  else if (tid == 0) reinterpret_cast<LpPart*>(a.part)[r * a.parts + part] = p;
 }
 
-// A workgroup per row joins its parts: the sums in a wave, the sorted lists by a sort of all.
+// A wave per row joins its parts: the sums across lanes, a lane a part, and the list by
+// taking the largest of the parts' first keys n times.
 template <int FMT>
 __global__ void __launch_bounds__(LP_NT) logprob_join_kernel(LogprobArgs a) {
-  __shared__ uint64_t sKeys[LP_MAX_PARTS * LP_MAX_TOP];
-  __shared__ LpPart sPart;
-  const int64_t r = blockIdx.x;
-  const int tid = threadIdx.x, n = a.parts * a.top_n;
-  for (int i = tid; i < n; i += LP_NT) sKeys[i] = a.part_keys[r * n + i];
-  if (tid < kWave) {
-    LpPart p{LP_LOWEST, 0.0f, 0.0f, 0.0f};
-    if (tid < a.parts) p = reinterpret_cast<const LpPart*>(a.part)[r * a.parts + tid];
-    lp_wave_join(p, a.c);
-    if (tid == 0) sPart = p;
-  }
-  __syncthreads();
-  if (a.top_n > 0) lp_sort(sKeys, n, lp_pow2(n));
+  __shared__ uint64_t sKeys[LP_NT / kWave][LP_MAX_PARTS * LP_MAX_TOP];
+  const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
+  const int64_t r = (int64_t)blockIdx.x * (LP_NT / kWave) + w;
+  if (r >= a.rows) return;
+  const int n = a.parts * a.top_n;
+  uint64_t* const keys = sKeys[w];
+  for (int i = lane; i < n; i += kWave) keys[i] = a.part_keys[r * n + i];
+  LpPart p{LP_LOWEST, 0.0f, 0.0f, 0.0f};
+  if (lane < a.parts) p = reinterpret_cast<const LpPart*>(a.part)[r * a.parts + lane];
+  lp_wave_join(p, a.c);
   const void* const row = reinterpret_cast<const uint8_t*>(a.logits) +
                           r * a.ld * (FMT == SDX_F32 ? 4 : 2);
-  lp_finish<FMT>(a, r, row, sPart, sKeys);
+  const LpRow sums = lp_row(p);
+  lp_finish<FMT>(a, r, row, sums, lane, kWave);
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_wave_barrier();  // the keys are in LDS
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  int at = lane * a.top_n, left = lane < a.parts ? a.top_n : 0;
+  uint64_t key = left > 0 ? keys[at] : 0, mine = 0;
+  for (int i = 0; i < a.top_n; ++i) {  // uniform
+    const uint32_t o = wave_max_u32((uint32_t)(key >> 32));
+    const uint32_t id = wave_max_u32((uint32_t)(key >> 32) == o ? (uint32_t)key : 0u);
+    const uint64_t best = (uint64_t)o << 32 | id;
+    if (lane == i) mine = best;
+    if (key == best && left > 0) {
+      ++at;
+      key = --left > 0 ? keys[at] : 0;
+    }
+  }
+  if (lane < a.top_n) lp_put(a, r, lane, sums, mine);
 }
 
-// Parts of a row: about LP_WGS workgroups in all, none of less than LP_LEAST elements.
-constexpr int64_t LP_WGS = 2048, LP_LEAST = 4096;
+// Parts of a row: the fewest that give the shortest rounds of workgroups on the chip, a part
+// counted by its elements and LP_OVER more for what follows them.
+constexpr int64_t LP_SLOTS = 2048, LP_LEAST = 2048, LP_OVER = 8192;
 int logprob_parts(int64_t rows, int64_t V) {
-  const int64_t want = (LP_WGS + rows - 1) / rows;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({want, V / LP_LEAST, LP_MAX_PARTS}));
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int p = 1; p <= LP_MAX_PARTS && (p == 1 || V / p >= LP_LEAST); ++p) {
+    const int64_t t = (rows * p + LP_SLOTS - 1) / LP_SLOTS * (V / p + LP_OVER);
+    if (t < least) least = t, best = p;
+  }
+  return best;
 }
 
 template <int FMT>
@@ -315,7 +424,9 @@ static hipError_t launch_logprob_t(const LogprobArgs& a, hipStream_t s) {
   else hipLaunchKernelGGL((logprob_kernel<FMT, false>), grid, dim3(LP_NT), 0, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.parts == 1) return e;
-  hipLaunchKernelGGL((logprob_join_kernel<FMT>), dim3((unsigned)a.rows), dim3(LP_NT), 0, s, a);
+  constexpr int R = LP_NT / kWave;
+  hipLaunchKernelGGL((logprob_join_kernel<FMT>), dim3((unsigned)((a.rows + R - 1) / R)), dim3(LP_NT), 0,
+                     s, a);
   return hipGetLastError();
 }
 
