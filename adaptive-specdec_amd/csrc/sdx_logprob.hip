@@ -15,7 +15,7 @@
 // first 16-byte vector that holds it, unique to the thread. Take the n-th best of any n or
 // more of these heads as an edge: n elements reach it, so no element below it is listed, and
 // a thread whose head is below it has none that is. The edge comes from 64 heads, the best
-// of four threads each (n-th of 64 in a wave); the few threads that reach it read their
+// of four threads each (by a wave, the largest n times); the few threads that reach it read their
 // vectors again, and what reaches it there, n elements and a few, is sorted. Per element the
 // list costs the maximum that the sums need anyway.
 //
@@ -56,41 +56,35 @@ __device__ __forceinline__ float lp_elem(const void* row, int64_t i) {
   else return decode16<FMT>(reinterpret_cast<const uint16_t*>(row)[i]);
 }
 
-// A row in 16-byte vectors from the boundary at or before its start: vector v holds elements
-// v VEC - off .. + VEC - 1. A part is vectors v0 .. v1 - 1.
+// A row as whole 16-byte vectors, from `head` elements after its start, and its edges: those
+// elements and the ones behind the last vector. A part is vectors v0 .. v1 - 1; part 0 has the
+// edges too.
 struct LpSpan {
   const uint8_t* row;
-  int64_t V, v0, v1, safe;  // safe: a vector that lies in the row as a whole (-1: none)
-  int off;
+  const uint8_t* vec;  // vector 0, on a 16-byte boundary
+  uint32_t V, head, edges, v0, v1;
 };
 template <int FMT>
 __device__ __forceinline__ LpSpan lp_span(const LogprobArgs& a, int64_t r, int part) {
   constexpr int VEC = lp_vec<FMT>(), ES = 16 / VEC;
   LpSpan s;
   s.row = reinterpret_cast<const uint8_t*>(a.logits) + r * a.ld * ES;
-  s.V = a.V;
-  s.off = (int)(((uintptr_t)s.row & 15u) / ES);
-  const int64_t n = (a.V + s.off + VEC - 1) / VEC;
-  s.v0 = n * part / a.parts;
-  s.v1 = n * (part + 1) / a.parts;
-  s.safe = s.off > 0 ? 1 : 0;
-  if ((s.safe + 1) * VEC - s.off > a.V) s.safe = -1;
+  s.V = (uint32_t)a.V;
+  s.head = min(s.V, (uint32_t)(-(uintptr_t)s.row & 15u) / ES);
+  s.vec = s.row + s.head * ES;
+  const uint32_t n = (s.V - s.head) / VEC;
+  s.v0 = (uint32_t)((uint64_t)n * part / a.parts);
+  s.v1 = (uint32_t)((uint64_t)n * (part + 1) / a.parts);
+  s.edges = part == 0 ? s.V - n * VEC : 0;
   return s;
 }
-template <int FMT>
-__device__ __forceinline__ bool lp_whole(const LpSpan& s, int64_t v) {
-  constexpr int VEC = lp_vec<FMT>();
-  return v < s.v1 && v * VEC >= s.off && (v + 1) * VEC - s.off <= s.V;
-}
-// Vector v, or another of the row where v is not whole: loads that no branch holds up.
-template <int FMT>
-__device__ __forceinline__ uint4 lp_load(const LpSpan& s, int64_t v) {
-  const int64_t w = lp_whole<FMT>(s, v) ? v : s.safe;
-  if (s.safe < 0) return make_uint4(0, 0, 0, 0);  // uniform
-  return *reinterpret_cast<const uint4*>(s.row - s.off * (16 / lp_vec<FMT>()) + w * 16);
+// Vector v, or another of the part behind its end: loads that no branch holds up. The part
+// has a vector.
+__device__ __forceinline__ uint4 lp_load(const LpSpan& s, uint32_t v) {
+  return *reinterpret_cast<const uint4*>(s.vec + (uint64_t)min(v, s.v1 - 1) * 16);
 }
 template <int FMT>
-__device__ __forceinline__ void lp_elems_whole(uint4 raw, float (&x)[lp_vec<FMT>()]) {
+__device__ __forceinline__ void lp_elems(uint4 raw, float (&x)[lp_vec<FMT>()]) {
   const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -102,18 +96,10 @@ __device__ __forceinline__ void lp_elems_whole(uint4 raw, float (&x)[lp_vec<FMT>
     }
   }
 }
-// Its elements; those outside the part or the row are -inf, and not read.
+// Id of edge e, and its element.
 template <int FMT>
-__device__ __forceinline__ void lp_elems(const LpSpan& s, int64_t v, uint4 raw,
-                                         float (&x)[lp_vec<FMT>()]) {
-  constexpr int VEC = lp_vec<FMT>();
-  lp_elems_whole<FMT>(raw, x);
-  if (lp_whole<FMT>(s, v)) return;
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    const int64_t id = v * VEC - s.off + i;
-    x[i] = v < s.v1 && id >= 0 && id < s.V ? lp_elem<FMT>(s.row, id) : -INFINITY;
-  }
+__device__ __forceinline__ uint32_t lp_edge_id(const LpSpan& s, uint32_t e) {
+  return e < s.head ? e : s.V - s.edges + e;
 }
 
 // (m, z, w) moved to the larger maximum mn.
@@ -189,15 +175,47 @@ __device__ __forceinline__ void lp_put(const LogprobArgs& a, int64_t r, int i, c
   a.top_ids[r * a.top_n + i] = o == 0u ? -1 : (int64_t)(uint32_t)~(uint32_t)key;
   a.top_logp[r * a.top_n + i] = o <= 1u ? NAN : lp_logp(a, p, lp_unord(o));
 }
-// The number of lanes whose key is greater than this lane's; keys differ, or are 0.
-__device__ __forceinline__ int lp_wave_rank(uint64_t key) {
+// The number of the first n of a wave's keys in LDS that are greater than `key`.
+__device__ __forceinline__ int lp_rank(const uint64_t* keys, int n, uint64_t key) {
   int rank = 0;
-#pragma unroll 8
-  for (int t = 0; t < kWave; ++t) {
-    const uint64_t k = (uint64_t)rdlane((uint32_t)(key >> 32), t) << 32 | rdlane((uint32_t)key, t);
-    rank += k > key;
+  for (int t = 0; t < n; t += 4) {  // uniform; the keys are padded with zeros
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rank += keys[t + i] > key;
   }
   return rank;
+}
+// Orders the writes and reads of a wave's own LDS.
+__device__ __forceinline__ void lp_wave_sync() {
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_wave_barrier();
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+// The n-th best of a wave's 64 heads (value order << 32 | ~vector; 0: none), or 0 where there
+// are fewer. s: 64 words of LDS.
+__device__ __forceinline__ uint64_t lp_wave_nth(uint64_t head, int n, uint32_t* s) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const uint32_t o = (uint32_t)(head >> 32);
+  s[lane] = o;
+  lp_wave_sync();
+  int above = 0;
+#pragma unroll
+  for (int t = 0; t < kWave; t += 4) {
+    const uint4 k = *reinterpret_cast<const uint4*>(s + t);
+    above += (k.x > o) + (k.y > o) + (k.z > o) + (k.w > o);
+  }
+  // the smallest value with fewer than n above it
+  const uint32_t nth = ~wave_max_u32(above < n ? ~o : 0u);
+  if (nth == 0) return 0;
+  const bool tied = o == nth;
+  uint32_t v = tied ? (uint32_t)head : 0u, last = wave_max_u32(v);
+  int left = n - (int)rdlane((uint32_t)above, __ffsll((unsigned long long)__ballot(tied)) - 1);
+  // the left-th first vector of the tied ones; all of them where they are no more
+  if (__popcll(__ballot(tied)) <= left) return (uint64_t)nth << 32 | ~wave_max_u32(tied ? ~v : 0u);
+  for (; left > 1; --left) {  // uniform
+    if (v == last) v = 0;  // vectors differ
+    last = wave_max_u32(v);
+  }
+  return (uint64_t)nth << 32 | last;
 }
 
 // Part blockIdx.x % parts of row blockIdx.x / parts: elements [lo, hi). One part: the results; several: the
@@ -206,30 +224,38 @@ template <int FMT, bool TOP>
 __global__ void __launch_bounds__(LP_NT) logprob_kernel(LogprobArgs a) {
   constexpr int VEC = lp_vec<FMT>();
   __shared__ LpPart sPart[LP_NT / kWave];
-  __shared__ uint64_t sKeys[TOP ? LP_CAP : 1];
-  __shared__ uint64_t sHead[TOP ? LP_NT : 1];
+  __shared__ __align__(16) uint64_t sKeys[TOP ? LP_CAP : 1];
+  __shared__ uint64_t sHead[TOP ? LP_NT : 1], sEdge;
   __shared__ int sSel[TOP ? LP_NT : 1], sCount, sNsel;
   const int tid = threadIdx.x;
   const int64_t r = blockIdx.x / (uint32_t)a.parts;
   const int part = (int)(blockIdx.x % (uint32_t)a.parts);
   const LpSpan span = lp_span<FMT>(a, r, part);
-  const int64_t v0 = span.v0, v1 = span.v1;
+  const uint32_t v0 = span.v0, v1 = span.v1;
   const float c = a.c;
 
   LpPart p{LP_LOWEST, 0.0f, 0.0f, 0.0f};
+  // a NaN or an infinite maximum reaches z; -inf adds nothing to either sum
+  auto add = [&](float x) {
+    const float d = (x - p.m) * c, e = __builtin_amdgcn_exp2f(d);
+    p.z += e;
+    p.w = fmaf(fmaxf(d, LP_FAR), e, p.w);
+  };
   uint32_t best = 0;  // order of the thread's largest value, and the vector it first came in
   uint32_t at = 0;
-  for (int64_t vb = v0; vb < v1; vb += LP_NT * LP_UN) {  // uniform
+  for (uint32_t vb = v0; vb < v1; vb += LP_NT * LP_UN) {  // uniform
     uint4 raw[LP_UN];
 #pragma unroll
-    for (int u = 0; u < LP_UN; ++u) raw[u] = lp_load<FMT>(span, vb + u * LP_NT + tid);
+    for (int u = 0; u < LP_UN; ++u) raw[u] = lp_load(span, vb + u * LP_NT + tid);
     float x[LP_UN][VEC];
-    if (vb > v0 && vb + LP_NT * LP_UN < v1) {  // uniform: all whole
 #pragma unroll
-      for (int u = 0; u < LP_UN; ++u) lp_elems_whole<FMT>(raw[u], x[u]);
-    } else {
+    for (int u = 0; u < LP_UN; ++u) lp_elems<FMT>(raw[u], x[u]);
+    if (vb + LP_NT * LP_UN > v1) {  // uniform: the last ones
 #pragma unroll
-      for (int u = 0; u < LP_UN; ++u) lp_elems<FMT>(span, vb + u * LP_NT + tid, raw[u], x[u]);
+      for (int u = 0; u < LP_UN; ++u)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (vb + u * LP_NT + tid >= v1) x[u][i] = -INFINITY;
     }
     float top = LP_LOWEST;
 #pragma unroll
@@ -239,9 +265,8 @@ __global__ void __launch_bounds__(LP_NT) logprob_kernel(LogprobArgs a) {
       for (int i = 1; i < VEC; ++i) vm = fmaxf(vm, x[u][i]);
       top = fmaxf(top, vm);
       if constexpr (TOP) {
-        const int64_t v = vb + u * LP_NT + tid;
-        const uint32_t o = lp_ord(vm);
-        if (o > best && v < v1) best = o, at = (uint32_t)v;
+        const uint32_t v = vb + u * LP_NT + tid, o = lp_ord(vm);
+        if (o > best && v < v1) best = o, at = v;
       }
     }
     const float mn = fmaxf(p.m, top);
@@ -250,12 +275,16 @@ __global__ void __launch_bounds__(LP_NT) logprob_kernel(LogprobArgs a) {
 #pragma unroll
     for (int u = 0; u < LP_UN; ++u)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        // a NaN or an infinite maximum reaches z; -inf adds nothing to either sum
-        const float d = (x[u][i] - mn) * c, e = __builtin_amdgcn_exp2f(d);
-        p.z += e;
-        p.w = fmaf(fmaxf(d, LP_FAR), e, p.w);
-      }
+      for (int i = 0; i < VEC; ++i) add(x[u][i]);
+  }
+  const bool has_edge = (uint32_t)tid < span.edges;
+  float edge_x = 0.0f;
+  if (has_edge) {
+    edge_x = lp_elem<FMT>(span.row, lp_edge_id<FMT>(span, tid));
+    const float mn = fmaxf(p.m, edge_x);
+    lp_shift(p.z, p.w, p.m, mn, c);
+    p.m = mn;
+    add(edge_x);
   }
   lp_wave_join(p, c);
   if ((tid & (kWave - 1)) == 0) sPart[tid / kWave] = p;
@@ -270,50 +299,53 @@ __global__ void __launch_bounds__(LP_NT) logprob_kernel(LogprobArgs a) {
   const LpRow row_sums = lp_row(p);
   bool sorted = false;  // the list lies in sKeys in order
   if constexpr (TOP) {
-    // every wave: the n-th best of 64 heads, of four threads each
-    uint64_t h = sHead[tid & (kWave - 1)];
+    if (tid < kWave) {
+      uint64_t h = head;
 #pragma unroll
-    for (int w = 1; w < LP_NT / kWave; ++w) {
-      const uint64_t k = sHead[w * kWave + (tid & (kWave - 1))];
-      h = k > h ? k : h;
+      for (int w = 1; w < LP_NT / kWave; ++w) {
+        const uint64_t k = sHead[w * kWave + tid];
+        h = k > h ? k : h;
+      }
+      // 0, fewer heads than n: everything is listed
+      h = lp_wave_nth(h, a.top_n, reinterpret_cast<uint32_t*>(sKeys));
+      if (tid == 0) sEdge = h;
     }
-    // lanes without a vector are last, and equal
-    const int rank = lp_wave_rank(h);
-    const uint64_t reach = __ballot(h > 0 && rank < a.top_n);
-    uint64_t edge = 0;  // fewer heads than n: everything is listed
-    if (__popcll(reach) >= a.top_n) {
-      const int at_n = __ffsll((unsigned long long)__ballot(rank == a.top_n - 1)) - 1;
-      edge = (uint64_t)rdlane((uint32_t)(h >> 32), at_n) << 32 | rdlane((uint32_t)h, at_n);
-    }
+    __syncthreads();
+    const uint64_t edge = sEdge;
     const uint32_t eo = (uint32_t)(edge >> 32), ev = ~(uint32_t)edge;
     if (best && head >= edge) sSel[atomicAdd(&sNsel, 1)] = tid;
     __syncthreads();
     // take(key) for the elements of those threads that reach the edge: their vectors spread
-    // over the workgroup, several loads in flight
-    const uint32_t nsel = (uint32_t)sNsel, all = nsel * (uint32_t)((v1 - v0 + LP_NT - 1) / LP_NT);
+    // over the workgroup, several loads in flight; and for the row's edges that do. Of equal
+    // values those behind the n-th head's vector are beaten by n heads.
+    constexpr int SL = 8;  // lanes a thread's vectors are spread over
+    const int nsel = sNsel;
+    const uint32_t per = (v1 - v0 + LP_NT - 1) / LP_NT;
     auto visit = [&](auto take) {
-      for (uint32_t i0 = tid; i0 < all; i0 += LP_NT * LP_UN) {
-        int64_t v[LP_UN];
-        uint4 raw[LP_UN];
+      for (int i0 = tid / SL; i0 < nsel; i0 += LP_NT / SL)
+        for (uint32_t j0 = tid % SL; j0 < per; j0 += SL * LP_UN) {
+          uint4 raw[LP_UN];
+          const uint32_t vs = v0 + j0 * LP_NT + sSel[i0];
 #pragma unroll
-        for (int u = 0; u < LP_UN; ++u) {
-          const uint32_t i = i0 + u * LP_NT;
-          v[u] = i < all ? v0 + (int64_t)(i / nsel) * LP_NT + sSel[i % nsel] : v1;
-          raw[u] = lp_load<FMT>(span, v[u]);
-        }
+          for (int u = 0; u < LP_UN; ++u) raw[u] = lp_load(span, vs + u * SL * LP_NT);
 #pragma unroll
-        for (int u = 0; u < LP_UN; ++u) {
-          float y[VEC];
-          lp_elems<FMT>(span, v[u], raw[u], y);
+          for (int u = 0; u < LP_UN; ++u) {
+            const uint32_t v = vs + u * SL * LP_NT;
+            float y[VEC];
+            lp_elems<FMT>(raw[u], y);
+            const uint32_t least = edge == 0 || v <= ev ? max(eo, 1u) : eo + 1;
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const int64_t id = v[u] * VEC - span.off + e;
-            const uint32_t o = lp_ord(y[e]);
-            if (o >= eo && (o > eo || edge == 0 || (uint32_t)v[u] <= ev) && v[u] < v1 && id >= 0 &&
-                id < a.V)
-              take((uint64_t)o << 32 | (uint32_t)~(uint32_t)id);
+            for (int e = 0; e < VEC; ++e) {
+              const uint32_t o = lp_ord(y[e]);
+              if (o >= least && v < v1)
+                take((uint64_t)o << 32 | (uint32_t)~(span.head + v * VEC + e));
+            }
           }
         }
+      if (has_edge) {
+        const uint32_t o = lp_ord(edge_x);
+        if (o >= (edge == 0 || (uint32_t)tid < span.head ? max(eo, 1u) : eo + 1))
+          take((uint64_t)o << 32 | (uint32_t)~lp_edge_id<FMT>(span, tid));
       }
     };
     visit([&](uint64_t k) {
@@ -325,7 +357,10 @@ __global__ void __launch_bounds__(LP_NT) logprob_kernel(LogprobArgs a) {
     if (n <= kWave) {  // one wave ranks them
       if (tid < kWave) {
         const uint64_t k = tid < n ? sKeys[tid] : 0;
-        const int i = lp_wave_rank(k);
+        lp_wave_sync();
+        if (tid >= n) sKeys[tid] = 0;
+        lp_wave_sync();
+        const int i = lp_rank(sKeys, n, k);
         // the list is longer than a part with fewer elements: zeros follow
         if (k > 0 && i < a.top_n) {
           if (a.parts == 1) lp_put(a, r, i, row_sums, k);
@@ -368,17 +403,16 @@ __global__ void __launch_bounds__(LP_NT) logprob_kernel(LogprobArgs a) {
   else if (tid == 0) reinterpret_cast<LpPart*>(a.part)[r * a.parts + part] = p;
 }
 
-// A wave per row joins its parts: the sums across lanes, a lane a part, and the list by
-// taking the largest of the parts' first keys n times.
+// A wave per row joins its parts: the sums across lanes, a lane a part, and the sorted lists.
+// Of p lists' j-th best, p j >= n, the smallest, or, of p >= n lists, the n-th best of their
+// first is reached by n keys: the few keys that reach it are ranked.
 template <int FMT>
-__global__ void __launch_bounds__(LP_NT) logprob_join_kernel(LogprobArgs a) {
-  __shared__ uint64_t sKeys[LP_NT / kWave][LP_MAX_PARTS * LP_MAX_TOP];
-  const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
-  const int64_t r = (int64_t)blockIdx.x * (LP_NT / kWave) + w;
-  if (r >= a.rows) return;
+__global__ void __launch_bounds__(kWave) logprob_join_kernel(LogprobArgs a) {
+  __shared__ __align__(16) uint64_t sKeys[LP_MAX_PARTS * LP_MAX_TOP], sList[kWave];
+  const int lane = threadIdx.x;
+  const int64_t r = blockIdx.x;
   const int n = a.parts * a.top_n;
-  uint64_t* const keys = sKeys[w];
-  for (int i = lane; i < n; i += kWave) keys[i] = a.part_keys[r * n + i];
+  for (int i = lane; i < n; i += kWave) sKeys[i] = a.part_keys[r * n + i];
   LpPart p{LP_LOWEST, 0.0f, 0.0f, 0.0f};
   if (lane < a.parts) p = reinterpret_cast<const LpPart*>(a.part)[r * a.parts + lane];
   lp_wave_join(p, a.c);
@@ -386,22 +420,51 @@ __global__ void __launch_bounds__(LP_NT) logprob_join_kernel(LogprobArgs a) {
                           r * a.ld * (FMT == SDX_F32 ? 4 : 2);
   const LpRow sums = lp_row(p);
   lp_finish<FMT>(a, r, row, sums, lane, kWave);
-  __atomic_signal_fence(__ATOMIC_SEQ_CST);
-  __builtin_amdgcn_wave_barrier();  // the keys are in LDS
-  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  if (a.top_n == 0) return;
+  lp_wave_sync();  // the keys are in LDS
+  const int depth = (a.top_n + a.parts - 1) / a.parts;
+  const uint64_t mine = lane < a.parts ? sKeys[lane * a.top_n + depth - 1] : 0;
+  uint64_t least;
+  if (depth == 1) {  // the n-th best first key: its value, ties included
+    least = lp_wave_nth(mine, a.top_n, reinterpret_cast<uint32_t*>(sList)) & ~0xFFFFFFFFull;
+  } else {
+    const uint32_t o = ~wave_max_u32(lane < a.parts ? ~(uint32_t)(mine >> 32) : 0u);
+    least = (uint64_t)o << 32;
+  }
+  lp_wave_sync();
+  int count = 0;
+  for (int i0 = 0; i0 < n; i0 += kWave) {  // uniform
+    const uint64_t k = i0 + lane < n ? sKeys[i0 + lane] : 0;
+    const uint64_t in = __ballot(k > 0 && k >= least);
+    const int at = count + __popcll(in & ((1ull << lane) - 1));
+    if (k > 0 && k >= least && at < kWave) sList[at] = k;
+    count += __popcll(in);
+  }
+  if (count <= kWave) {  // uniform
+    lp_wave_sync();
+    const uint64_t k = lane < count ? sList[lane] : 0;
+    lp_wave_sync();
+    if (lane >= count) sList[lane] = 0;
+    lp_wave_sync();
+    const int i = lp_rank(sList, count, k);
+    if (k > 0 && i < a.top_n) lp_put(a, r, i, sums, k);
+    if (lane >= count && lane < a.top_n) lp_put(a, r, lane, sums, 0);
+    return;
+  }
+  // many equal values: the largest of the lists' first keys, n times
   int at = lane * a.top_n, left = lane < a.parts ? a.top_n : 0;
-  uint64_t key = left > 0 ? keys[at] : 0, mine = 0;
+  uint64_t key = left > 0 ? sKeys[at] : 0, best = 0;
   for (int i = 0; i < a.top_n; ++i) {  // uniform
     const uint32_t o = wave_max_u32((uint32_t)(key >> 32));
     const uint32_t id = wave_max_u32((uint32_t)(key >> 32) == o ? (uint32_t)key : 0u);
-    const uint64_t best = (uint64_t)o << 32 | id;
-    if (lane == i) mine = best;
-    if (key == best && left > 0) {
+    const uint64_t top = (uint64_t)o << 32 | id;
+    if (lane == i) best = top;
+    if (key == top && left > 0) {
       ++at;
-      key = --left > 0 ? keys[at] : 0;
+      key = --left > 0 ? sKeys[at] : 0;
     }
   }
-  if (lane < a.top_n) lp_put(a, r, lane, sums, mine);
+  if (lane < a.top_n) lp_put(a, r, lane, sums, best);
 }
 
 // Parts of a row: the fewest that give the shortest rounds of workgroups on the chip, a part
@@ -424,9 +487,7 @@ static hipError_t launch_logprob_t(const LogprobArgs& a, hipStream_t s) {
   else hipLaunchKernelGGL((logprob_kernel<FMT, false>), grid, dim3(LP_NT), 0, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.parts == 1) return e;
-  constexpr int R = LP_NT / kWave;
-  hipLaunchKernelGGL((logprob_join_kernel<FMT>), dim3((unsigned)((a.rows + R - 1) / R)), dim3(LP_NT), 0,
-                     s, a);
+  hipLaunchKernelGGL((logprob_join_kernel<FMT>), dim3((unsigned)a.rows), dim3(kWave), 0, s, a);
   return hipGetLastError();
 }
 
