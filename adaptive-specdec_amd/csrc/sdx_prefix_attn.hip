@@ -160,7 +160,7 @@ __device__ __forceinline__ PaSeg pa_seg(const PrefixAttnArgs& a, int64_t nt, int
 // token for the join. Work is counted in 64-key tiles of the shared form.
 constexpr int PL_NT = 512;
 constexpr int PL_CAND = 32;      // chunk sizes weighed for the groups
-constexpr int PA_ALONE = 2;      // a 64-key tile of the other form
+constexpr int PA_ALONE = 1;      // a 64-key tile of the other form
 constexpr int PA_UNIT = 8;       // what a unit costs beside its tiles, the write of its part first
 constexpr int PL_OWN = 8;        // entries that a thread writes by itself
 
@@ -288,8 +288,7 @@ __global__ void __launch_bounds__(PL_NT) prefix_attn_plan_kernel(PrefixAttnArgs 
     for (int64_t g = few ? lane / PL_CAND : tid / PL_CAND; g < a.groups; g += few ? 2 : PL_NT / PL_CAND) {
       const int2 s = seg[g];
       if (s.y <= 0) continue;
-      const int32_t k = pl_chunk(s.y, mine, s.x > 0);
-      n += (uint32_t)abs(s.x) * ((s.y + k - 1) / k);
+      n += (uint32_t)abs(s.x) * ((s.y + mine - 1) / mine);
     }
     n *= (uint32_t)a.hkv;
     if (few) {
@@ -620,6 +619,11 @@ __device__ __forceinline__ int64_t pa_qrow(const PrefixAttnArgs& a, const PaUnit
   return (u.t0 + r / a.group) * a.hq + u.kvh * a.group + r % a.group;
 }
 
+__device__ __forceinline__ uint32_t pa_take(const PrefixAttnArgs& a, uint32_t q) {
+  return (uint32_t)__hip_atomic_fetch_add(a.head + PA_QUEUE * q, 1, __ATOMIC_RELAXED,
+                                          __HIP_MEMORY_SCOPE_AGENT);
+}
+
 template <int D, int FMT>
 __global__ void __launch_bounds__(PA_NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 prefix_attn_kernel(PrefixAttnArgs a) {
@@ -628,7 +632,10 @@ prefix_attn_kernel(PrefixAttnArgs a) {
   __shared__ __align__(256) uint8_t sMem[PA_LDS];
   __shared__ uint32_t sSlot[PA_RING * PA_TILE];
   __shared__ uint32_t sUnit;
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), w = tid / kWave;
+  // the wave's index and the unit are made scalar: what follows from them takes no vector
+  // registers, of which a wave of two per SIMD has 256
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int w = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int hi = lane / 32, l31 = lane & 31;
   const uint32_t row_bytes = (uint32_t)a.hkv * RB;
   // addresses of the lane's operands in LDS tiles
@@ -651,10 +658,9 @@ prefix_attn_kernel(PrefixAttnArgs a) {
         ++queue;
         continue;
       }
-      if (tid == 0) sUnit = (uint32_t)__hip_atomic_fetch_add(a.head + PA_QUEUE * q, 1, __ATOMIC_RELAXED,
-                                                              __HIP_MEMORY_SCOPE_AGENT);
+      if (tid == 0) sUnit = pa_take(a, q);
       __syncthreads();
-      at = sUnit;
+      at = __builtin_amdgcn_readfirstlane(sUnit);
       __syncthreads();
     }
     if (at >= n) {
@@ -1008,6 +1014,12 @@ int64_t prefix_attn_entries(int64_t tokens, int64_t batch, int64_t groups, int32
   return (2 * (tokens * group / PA_ROWS) + batch + groups) * (parts / 2);
 }
 
+template <int D, int FMT, int HG>
+static void launch_join(const PrefixAttnArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((prefix_attn_join_kernel<D, FMT, HG>),
+                     dim3((unsigned)(a.tokens * ((a.hq + HG - 1) / HG))), dim3(PA_NT), 0, s, a);
+}
+
 template <int D, int FMT>
 static hipError_t launch_prefix_attn_t(const PrefixAttnArgs& a, hipStream_t s) {
   hipLaunchKernelGGL(prefix_attn_plan_kernel, dim3(1), dim3(PL_NT), 0, s, a);
@@ -1016,13 +1028,11 @@ static hipError_t launch_prefix_attn_t(const PrefixAttnArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((prefix_attn_kernel<D, FMT>), dim3(PA_GRID), dim3(PA_NT), 0, s, a);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  // few query rows have many parts: a workgroup for each
-  if (a.tokens * a.hq <= 4096)
-    hipLaunchKernelGGL((prefix_attn_join_kernel<D, FMT, 1>), dim3((unsigned)(a.tokens * a.hq)),
-                       dim3(PA_NT), 0, s, a);
-  else
-    hipLaunchKernelGGL((prefix_attn_join_kernel<D, FMT, 8>),
-                       dim3((unsigned)(a.tokens * ((a.hq + 7) / 8))), dim3(PA_NT), 0, s, a);
+  // few query rows have many parts: slices of a workgroup share them
+  const int64_t rows = a.tokens * a.hq;
+  if (rows <= 2048) launch_join<D, FMT, 1>(a, s);
+  else if (rows <= 8192) launch_join<D, FMT, 2>(a, s);
+  else launch_join<D, FMT, 4>(a, s);
   return hipGetLastError();
 }
 

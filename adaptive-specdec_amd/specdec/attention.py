@@ -121,7 +121,7 @@ def shared_prefix_attention_paged(q, cu_q, k_pool, v_pool, block_table, kv_len, 
         raise ValueError(f"shared_prefix_attention_paged: {B} lengths need cu_q [{B + 1}] and "
                          f"block_table [{B}, max_blocks], {G} prefixes cu_group [{G + 1}]")
     if out is None:
-        out = torch.empty((T, hq, d), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError("shared_prefix_attention_paged: out must be contiguous, of q's shape and type")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
