@@ -706,8 +706,8 @@ prefix_attn_kernel(PrefixAttnArgs a) {
       constexpr int H = NC / 4, TPR = PA_NT / NC;  // passes, rows per pass
       const int ntile = (u.n + PA_TILE - 1) / PA_TILE;
       const int lr = tid / NC, lc = tid % NC;
-      // slots of the chunk's tiles, by the first wave: page ids are loaded a tile before
-      // they are needed here, four tiles before their keys
+      // slots of the chunk's tiles, four tiles at a time, one by each wave: page ids are loaded
+      // four tiles before they are needed here, eight before their keys
       auto page_of = [&](int tile) {
         const int t = tile * PA_TILE + lane;
         return t < u.n ? table[(pos0 + t) / (uint32_t)a.bs] : 0;
@@ -742,15 +742,8 @@ prefix_attn_kernel(PrefixAttnArgs a) {
           *reinterpret_cast<pa_u4*>(k + vw + (PA_TILE + TPR * h) * RB) = vv[h];
         }
       };
-      int32_t page = 0;
-      if (w == 0) {
-        int32_t pg[3];
-#pragma unroll
-        for (int i = 0; i < 3; ++i) pg[i] = page_of(i);
-        page = page_of(3);
-#pragma unroll
-        for (int i = 0; i < 3; ++i) put_slot(i, pg[i]);
-      }
+      put_slot(w, page_of(w));
+      int32_t page = page_of(4 + w);
       __syncthreads();
       typedef std::integral_constant<int, 0> even;
       typedef std::integral_constant<int, 1> odd;
@@ -759,9 +752,9 @@ prefix_attn_kernel(PrefixAttnArgs a) {
       gather(1);
       __syncthreads();
       auto tile = [&](int t, auto buf, auto next) {
-        if (w == 0) {  // tile t + 3
-          put_slot(t + 3, page);
-          page = page_of(t + 4);
+        if (buf == 0 && t % 4 == 0) {  // uniform
+          put_slot(t + 4 + w, page);
+          page = page_of(t + 8 + w);
         }
         if (active) {
           const uint8_t* const k = sMem + buf * (2 * PA_TILE * RB);
