@@ -576,6 +576,37 @@ __device__ __forceinline__ void pa_pv(PaState<D>& st, const pa_f16 (&s)[NB], con
   }
 }
 
+// V in tiles of which some query rows see a part: a weight of 0 times an infinity or a NaN would
+// be a NaN, so such elements are 0 for the products, and are added behind the last tile to the
+// rows that see their key. One comparison for the largest of a thread's elements costs 0 to 1%
+// of a call; one for each, or the sums in every tile, 3 to 9%.
+template <int FMT, int H>
+__device__ __forceinline__ bool pa_finite_only(pa_u4 (&v)[H]) {
+  typedef uint16_t h2 __attribute__((ext_vector_type(2)));
+  constexpr uint16_t E = FMT == SDX_BF16 ? 0x7F80u : 0x7C00u;
+  h2 mx = {0, 0};  // of the elements without their signs
+#pragma unroll
+  for (int h = 0; h < H; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      mx = __builtin_elementwise_max(mx, __builtin_bit_cast(h2, v[h][i] & 0x7FFF7FFFu));
+  const bool odd = max(mx.x, mx.y) >= E;
+  if (__any(odd)) {
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[h][i] &= ((v[h][i] & E) == E ? 0u : 0xFFFFu) | ((v[h][i] >> 16 & E) == E ? 0u : 0xFFFF0000u);
+  }
+  return odd;
+}
+template <int FMT>
+__device__ __forceinline__ float pa_odd(uint16_t x) {
+  if constexpr (FMT == SDX_BF16)
+    return __uint_as_float((uint32_t)x << 16);
+  else
+    return (float)__builtin_bit_cast(_Float16, x);
+}
 constexpr int PA_LDS_TILES = 2 * 2 * PA_TILE * 2 * 128;          // two tiles of K and V
 constexpr int PA_LDS_JOIN = PA_NW * PA_WROWS * (128 + 4) * 4;     // four waves' O
 constexpr int PA_LDS = PA_LDS_JOIN > PA_LDS_TILES ? PA_LDS_JOIN : PA_LDS_TILES;
@@ -586,6 +617,32 @@ __device__ __forceinline__ uint32_t pa_slot(const PrefixAttnArgs& a, int32_t pag
   return page >= 0 && page < a.num_blocks ? (uint32_t)page * (uint32_t)a.bs + pos % (uint32_t)a.bs
                                           : PA_NOSLOT;
 }
+// Those elements of keys from .. of the chunk; in the form with waves alone, of the wave's.
+template <int D, int FMT>
+__device__ __forceinline__ void pa_add_odd(PaState<D>& st, const PrefixAttnArgs& a, const PaUnit& u,
+                                           const int32_t* table, const uint8_t* vp, uint32_t row_bytes,
+                                           int from, int w, int lim, int hi) {
+  constexpr uint32_t E = FMT == SDX_BF16 ? 0x7F80u : 0x7C00u;
+#pragma nounroll
+  for (int t = from; t < u.n; ++t) {
+    if (!u.shared && t / 32 % PA_NW != w) continue;  // uniform, as all here but lim and hi
+    const uint32_t pos = (uint32_t)u.key0 + t, s = pa_slot(a, table[pos / (uint32_t)a.bs], pos);
+    if (s == PA_NOSLOT) continue;
+    const uint16_t* const row = reinterpret_cast<const uint16_t*>(vp + (uint64_t)s * row_bytes);
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const ushort4 x = *reinterpret_cast<const ushort4*>(row + 32 * db + 8 * e + 4 * hi);
+        const uint16_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (t <= lim && (y[i] & E) == E) st.o[db][4 * e + i] += pa_odd<FMT>(y[i]);
+        __builtin_amdgcn_sched_barrier(0);  // few registers, the speed of this is no concern
+      }
+  }
+}
+
 
 // lim of query row i of a unit: the last key it sees, of the chunk (-1: none)
 __device__ __forceinline__ int pa_lim(const PrefixAttnArgs& a, const PaUnit& u, bool masked, int i) {
@@ -632,6 +689,7 @@ prefix_attn_kernel(PrefixAttnArgs a) {
   __shared__ __align__(256) uint8_t sMem[PA_LDS];
   __shared__ uint32_t sSlot[PA_RING * PA_TILE];
   __shared__ uint32_t sUnit;
+  __shared__ int sOdd;
   // the wave's index and the unit are made scalar: what follows from them takes no vector
   // registers, of which a wave of two per SIMD has 256
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
@@ -678,6 +736,7 @@ prefix_attn_kernel(PrefixAttnArgs a) {
     const uint8_t* const zero = reinterpret_cast<const uint8_t*>(a.head + PA_ZERO);
     const uint32_t pos0 = (uint32_t)u.key0;
     int bad = 0;
+    bool found;  // uniform: V has elements that pa_add_odd adds
     PaState<D> st;
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
@@ -734,8 +793,9 @@ prefix_attn_kernel(PrefixAttnArgs a) {
       static_assert(TPR % 16 == 0, "a pass's rows are swizzled alike");
       const uint32_t kw = lr * RB + ((lc ^ pa_swz_k<D>(lr)) << 4);
       const uint32_t vw = lr * RB + ((lc ^ pa_swz_v<D>(lr)) << 4);
-      auto stage = [&](auto buf) {
+      auto stage = [&](auto buf, int tile) {
         uint8_t* const k = sMem + buf * (2 * PA_TILE * RB);
+        if ((tile + 1) * PA_TILE > seen && pa_finite_only<FMT, H>(vv)) sOdd = 1;
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           *reinterpret_cast<pa_u4*>(k + kw + TPR * h * RB) = kk[h];
@@ -744,11 +804,12 @@ prefix_attn_kernel(PrefixAttnArgs a) {
       };
       put_slot(w, page_of(w));
       int32_t page = page_of(4 + w);
+      if (tid == 0) sOdd = 0;
       __syncthreads();
       typedef std::integral_constant<int, 0> even;
       typedef std::integral_constant<int, 1> odd;
       gather(0);
-      stage(even());
+      stage(even(), 0);
       gather(1);
       __syncthreads();
       auto tile = [&](int t, auto buf, auto next) {
@@ -787,7 +848,7 @@ prefix_attn_kernel(PrefixAttnArgs a) {
           pa_pv<D, FMT, 2>(st, s, k + PA_TILE * RB, va);
           __builtin_amdgcn_s_setprio(0);
         }
-        stage(next);  // past the last tile: rows of zeros
+        stage(next, t + 1);  // past the last tile: rows of zeros
         __builtin_amdgcn_sched_barrier(0);  // the registers are free before they are loaded
         gather(t + 2);
         __syncthreads();
@@ -798,21 +859,7 @@ prefix_attn_kernel(PrefixAttnArgs a) {
         tile(t + 1, odd(), even());
         if (t + 2 >= ntile) break;
       }
-      st.l = pa_sum_halves(st.l);
-      const int i = r0 + l31;
-      if (active && i < u.m) {
-        const int64_t qrow = pa_qrow(a, u, i);
-        const float f = u.direct ? (st.l > 0.0f || st.l != st.l ? 1.0f / st.l : 0.0f) : 1.0f;
-#pragma unroll
-        for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            pa_store4<D, FMT>(a, u, qrow, 32 * db + 8 * e + 4 * hi,
-                              make_float4(st.o[db][4 * e] * f, st.o[db][4 * e + 1] * f,
-                                          st.o[db][4 * e + 2] * f, st.o[db][4 * e + 3] * f));
-        if (!u.direct && hi == 0)
-          a.part_ml[(int64_t)u.part * a.tokens * a.hq + qrow] = make_float2(st.m, st.l);
-      }
+      found = __builtin_amdgcn_readfirstlane(sOdd);
     } else {
       constexpr int H = NC / 2, TPR = kWave / NC;  // passes and rows per pass of a wave's V
       const int nstep = (u.n + PA_STEP - 1) / PA_STEP;
@@ -849,20 +896,22 @@ prefix_attn_kernel(PrefixAttnArgs a) {
       page = page_of(1);
       gather_k(slot);
       gather_v(slot);
+      bool any = false;
       for (int t = 0; t < nstep; ++t) {
+        const int k0 = t * PA_STEP + 32 * w;
         slot = slot_of(t + 1, page);
         page = page_of(t + 2);
         pa_f16 s[1] = {};
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) s[0] = pa_mfma<FMT>(kk[ks], qa[ks], s[0]);
         if (t + 1 < nstep) gather_k(slot);
+        if (k0 + 32 > seen) any |= pa_finite_only<FMT, H>(vv);  // uniform
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           const int r = lr + TPR * h;
           *reinterpret_cast<pa_u4*>(v + r * RB + ((lc ^ pa_swz_v<D>(r)) << 4)) = vv[h];
         }
         if (t + 1 < nstep) gather_v(slot);
-        const int k0 = t * PA_STEP + 32 * w;
         if (k0 + 32 > seen) pa_mask<1>(s, k0, lim, hi);  // uniform
         pa_softmax<D, 1>(st, s, a.scale_log2);
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
@@ -873,8 +922,29 @@ prefix_attn_kernel(PrefixAttnArgs a) {
         __builtin_amdgcn_wave_barrier();  // and read before it is written again
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
       }
+      found = __any(any);
+    }
+    if (found)
+      pa_add_odd<D, FMT>(st, a, u, table, vp, row_bytes,
+                         u.shared ? seen / PA_TILE * PA_TILE : seen / 32 * 32, w, lim, hi);
+    st.l = pa_sum_halves(st.l);
+    if (u.shared) {
+      const int i = r0 + l31;
+      if (active && i < u.m) {
+        const int64_t qrow = pa_qrow(a, u, i);
+        const float f = u.direct ? (st.l > 0.0f || st.l != st.l ? 1.0f / st.l : 0.0f) : 1.0f;
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            pa_store4<D, FMT>(a, u, qrow, 32 * db + 8 * e + 4 * hi,
+                              make_float4(st.o[db][4 * e] * f, st.o[db][4 * e + 1] * f,
+                                          st.o[db][4 * e + 2] * f, st.o[db][4 * e + 3] * f));
+        if (!u.direct && hi == 0)
+          a.part_ml[(int64_t)u.part * a.tokens * a.hq + qrow] = make_float2(st.m, st.l);
+      }
+    } else {
       // join of the four waves: weights 2^(m_w - m), O summed through LDS
-      st.l = pa_sum_halves(st.l);
       float2* const sML = reinterpret_cast<float2*>(sSlot);  // [wave][row]
       __syncthreads();  // the tiles' LDS is free
       if (hi == 0) sML[w * PA_WROWS + l31] = make_float2(st.m, st.l);
@@ -956,8 +1026,9 @@ __global__ void __launch_bounds__(PA_NT) prefix_attn_join_kernel(PrefixAttnArgs 
     m = mn;
 #pragma unroll
     for (int k = 0; k < UN; ++k) {
-      const float f = i0 + k * SL >= n || ml[k].x == -INFINITY ? 0.0f
-                                                              : __builtin_amdgcn_exp2f(ml[k].x - m);
+      const bool none = i0 + k * SL >= n || ml[k].x == -INFINITY;  // no part: not a 0 times its O
+      const float f = none ? 0.0f : __builtin_amdgcn_exp2f(ml[k].x - m);
+      if (none) v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       l += f * ml[k].y;
       o.x += f * v[k].x;
       o.y += f * v[k].y;

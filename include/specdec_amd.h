@@ -460,6 +460,7 @@ size_t sdx_verify_attention_workspace(int64_t batch, int32_t max_q, int32_t num_
  * q / out: [num_tokens, num_q_heads, head_dim], bf16 or fp16 as the pools, 16-byte aligned;
  * q_b = cu_q[b+1] - cu_q[b] of any size; head_dim 64 or 128; scale positive and finite. Softmax
  * and sums in fp32, weights rounded to the type for the second product, output rounded to it.
+ * Keys and values that a query does not see do not reach its output, whatever they hold.
  * Rows, or groups with all their rows, whose lengths or offsets are out of range set *error
  * (nullable) and leave their output as it was; tokens behind the last row too, without the
  * error. Page ids outside the pool set *error and the output of the rows that read them is

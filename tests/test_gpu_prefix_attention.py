@@ -173,6 +173,52 @@ def test_keys_that_no_query_sees():
             check(c)
 
 
+@pytest.mark.parametrize("dtype,heads,q", [
+    (torch.bfloat16, (32, 8, 128), [6, 3, 8, 1]),   # a wave's keys each
+    (torch.bfloat16, (16, 1, 128), [9, 70, 40, 3]),  # tiles that the waves share
+    (torch.float16, (8, 2, 64), [5, 8, 2, 7]),
+    (torch.float16, (8, 1, 64), [9, 80, 20, 30]),
+])
+def test_keys_that_some_queries_see(dtype, heads, q):
+    """NaN and infinities in K and V of one of a row's new tokens: the row's tokens before it
+    are as without them, it and those after it as the formula has it."""
+    for seed, prefix, kv in ((21, 100, None), (22, 200, [200, 150, 70, 260])):
+        own = [0, 150, 64, 7]
+        c = make(seed, [4], [prefix], own, q, *heads, dtype=dtype, kv=kv)
+        plain = shared_prefix_attention_paged(**c)
+        for b in range(4):
+            end, at = int(c["kv_len"][b]), q[b] // 2  # the at-th new token's position
+            pos = end - q[b] + at
+            page = int(c["block_table"][0 if pos < prefix else b, pos // 16])
+            rows = slice(int(c["cu_q"][b]), int(c["cu_q"][b]) + at)
+            for name, value, dims in (("v_pool", float("nan"), slice(3, 5)),
+                                      ("v_pool", float("inf"), slice(0, None)),
+                                      ("v_pool", -float("inf"), slice(17, 50)),
+                                      ("k_pool", float("nan"), slice(1, 2))):
+                d = dict(c, **{name: c[name].clone()})
+                d[name][page, pos % 16, dims] = value
+                got = shared_prefix_attention_paged(**d)
+                if name == "v_pool":
+                    assert torch.equal(got[rows], plain[rows])
+                else:  # other rows' scores move the running maximum's steps
+                    check(c, got=got, rows=torch.arange(rows.start, rows.stop, device=DEV))
+                if pos >= prefix and name == "v_pool":  # of this row alone
+                    keep = torch.ones(got.shape[0], dtype=torch.bool, device=DEV)
+                    keep[rows.stop:int(c["cu_q"][b + 1])] = False
+                    assert torch.equal(got[keep], plain[keep])
+                after = got[rows.stop:int(c["cu_q"][b + 1])].view(-1, heads[0], heads[2])
+                if name == "k_pool":  # the first KV head's scores
+                    assert after[:, :heads[0] // heads[1]].isnan().all()
+                else:  # the formula's value in the dims set, and finite values in the others
+                    want = torch.zeros(heads[1] * heads[2], dtype=dtype, device=DEV)
+                    want[dims] = value
+                    want = want.view(heads[1], heads[2]).repeat_interleave(heads[0] // heads[1], 0)
+                    odd = ~want.isfinite()
+                    assert after.isfinite().logical_not().equal(odd.expand_as(after))
+                    assert after[odd.expand_as(after)].nan_to_num(7, 8, 9).eq(
+                        want.nan_to_num(7, 8, 9)[odd].repeat(after.shape[0])).all()
+
+
 def test_extreme_scores():
     """Scores far apart (one key takes all), equal everywhere, and rising along the keys, so
     that the running maximum moves by more and by less than its slack."""
