@@ -159,27 +159,32 @@ def token_logprobs(logits, ids, temperature=1.0, top_n=0):
     finite scores. Rows without a finite maximum, or with NaN, score NaN.
     """
     _lib.one_gpu(logits, ids)
-    lead, V = logits.shape[:-1], logits.shape[-1]
-    if tuple(ids.shape) != tuple(lead) and tuple(ids.shape[:-1]) != tuple(lead):
-        raise ValueError(f"ids must be {tuple(lead)} or {tuple(lead)} + (n,), got "
-                         f"{tuple(ids.shape)}")
-    if ids.dtype.is_floating_point or ids.dtype is torch.bool:
+    shape, ishape = logits.shape, ids.shape
+    lead, V = shape[:-1], shape[-1]
+    n = 1
+    if ishape != lead:
+        if ishape[:-1] != lead or len(ishape) != len(shape):
+            raise ValueError(f"ids must be {tuple(lead)} or {tuple(lead)} + (n,), got {tuple(ishape)}")
+        n = ishape[-1]
+    if ids.dtype is not torch.int64 and (ids.dtype.is_floating_point or ids.dtype.is_complex or
+                                         ids.dtype is torch.bool):
         raise TypeError(f"ids must be whole numbers, got {ids.dtype}")
     T, top_n = float(temperature), int(top_n)
     if not 0.0 < T < float("inf"):
         raise ValueError(f"temperature must be positive and finite, got {temperature}")
     if not 0 <= top_n <= min(V, 64):
         raise ValueError(f"top_n must lie in [0, min(64, V = {V})], got {top_n}")
-    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
-    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+    x = logits if len(shape) == 2 else logits.reshape(-1, V)
+    if x.dtype not in _lib._DTYPE:
         x = x.float()
     rows = x.shape[0]
-    if x.stride(1) != 1 or (rows > 1 and x.stride(0) < V):
+    ld, unit = x.stride()
+    if unit != 1 or (rows > 1 and ld < V):
         x = x.contiguous()
+        ld = V
     dev = x.device
     i = _lib.as_dtype(ids, torch.int64)
-    n = 1 if ids.dim() == len(lead) else ids.shape[-1]
-    logp = torch.empty(ids.shape, dtype=torch.float32, device=dev)
+    logp = torch.empty(ishape, dtype=torch.float32, device=dev)
     entropy = torch.empty(lead, dtype=torch.float32, device=dev)
     top_logp = top_ids = None
     if top_n:
@@ -191,8 +196,8 @@ def token_logprobs(logits, ids, temperature=1.0, top_n=0):
         need = _lib.workspace_bytes("sdx_token_logprobs_workspace", rows, V, top_n)
         ws = _lib.cached_workspace(need, dev, "logprobs") if need else None
         rc = _lib.lib().sdx_token_logprobs(
-            _lib.ptr(x), _lib.dtype_code(x), rows, V, x.stride(0) if rows > 1 else V, T, _lib.ptr(i), n,
-            top_n, _lib.ptr(logp), _lib.ptr(entropy), _lib.ptr(top_logp), _lib.ptr(top_ids),
+            _lib.ptr(x), _lib.dtype_code(x), rows, V, ld if rows > 1 else V, T, _lib.ptr(i), n, top_n,
+            _lib.ptr(logp), _lib.ptr(entropy), _lib.ptr(top_logp), _lib.ptr(top_ids),
             _lib.ptr(ws), ws.numel() if need else 0, _lib.stream_of(x))
     _lib.check(rc, "token_logprobs")
     return logp, entropy, top_logp, top_ids
