@@ -517,7 +517,7 @@ int logprob_parts(int64_t rows, int64_t V);  // workgroups per row
 hipError_t launch_logprob(int dtype, const LogprobArgs& a, hipStream_t s);
 
 // sdx_prefix_attn.hip: attention of groups of rows that share a prefix's keys
-constexpr int32_t PA_PART = 0xFFFFFF, PA_SHARED = 1 << 24, PA_GROUP = 1 << 25, PA_DIRECT = 1 << 26;
+constexpr int32_t PA_PART = 0xFFFFFF, PA_GROUP = 1 << 24, PA_DIRECT = 1 << 25;
 struct PrefixAttnUnit {  // a tile of query rows against a chunk of keys
   int32_t table, key0, n;  // row of the block table, first key, keys
   int32_t t0, r0, m;       // the segment's first token, the tile's first query row, its rows
