@@ -64,6 +64,17 @@ def test_matches_oracle(dtype, rows, V, n, top_n, T):
     _check(x, ids, T, top_n)
 
 
+def test_row_offsets_past_32_bits():
+    """Rows further apart than 2^32 elements, split over workgroups and whole."""
+    V, ld = 20000, (1 << 32) + 24
+    buf = torch.empty(ld + V, dtype=torch.bfloat16, device=DEV)
+    x = buf.as_strided((2, V), (ld, 1))
+    x.copy_(_logits(2, V, 77, torch.bfloat16))
+    _check(x, torch.randint(0, V, (2, 2), device=DEV), 0.9, 20)
+    short = x[:, :300]
+    _check(short, torch.randint(0, 300, (2, 2), device=DEV), 0.9, 20)
+
+
 def test_many_rows_run_whole():
     """Rows enough that each is one workgroup's, beside the split of few rows above."""
     x = _logits(2300, 1000, 4, torch.bfloat16)

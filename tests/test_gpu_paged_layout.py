@@ -159,6 +159,21 @@ def test_far_positions_pass_32_bits():
     assert p.item() == 4500 * bs and s.item() == 3 * bs
 
 
+@pytest.mark.parametrize("bs,shift", [(1 << 30, 30), ((1 << 31) - 1, 31), (1 << 28, 28)])
+def test_block_tables_of_lengths_past_32_bits(bs, shift):
+    kv = np.array([7 * bs, 3 * bs + 5, 3 * bs + 6, 0, 1, (5 << shift) + 1])
+    cu, pre, free = np.array([0, 3, 3, 6]), np.array([3 * bs + 5, 0, 0]), np.arange(40, 0, -1)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    want, used, ok = OP.build_block_tables(kv, free, bs, 8, cu, pre)
+    t, u = build_block_tables(_dev(kv), torch.as_tensor(free.astype(np.int32), device=DEV), bs, 8,
+                              _dev(cu), _dev(pre), error=err)
+    assert ok and np.array_equal(t.cpu().numpy(), want) and u.item() == used and err.item() == 0
+    kv[4] = 8 * bs + 1  # a page more than the table has
+    t, u = build_block_tables(_dev(kv), torch.as_tensor(free.astype(np.int32), device=DEV), bs, 8,
+                              _dev(cu), _dev(pre), error=err)
+    assert (t == -1).all() and u.item() == 0 and err.item() == 1
+
+
 @pytest.mark.parametrize("L,T,hkv,d,dtype", [
     (1, 1, 1, 64, torch.bfloat16), (3, 5, 2, 64, torch.float16), (2, 257, 8, 128, torch.bfloat16),
     (64, 33, 8, 128, torch.bfloat16), (2, 100, 1, 40, torch.float16), (1, 70, 3, 28, torch.float32),

@@ -290,6 +290,30 @@ def test_pool_offsets_past_32_bits():
     check(c)
 
 
+def test_a_long_prompt_in_one_call():
+    """33,000 new tokens of a group's first row and none of the others': 132,000 query rows of
+    a KV head; some of them checked."""
+    T, hq, hkv, d = 33000, 8, 2, 64
+    c = make(31, [3], [T], [0, 0, 0], [T, 0, 0], hq, hkv, d, kv=[T, T, T], dtype=torch.float16)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = shared_prefix_attention_paged(**c, error=err)
+    assert err.item() == 0 and torch.isfinite(got).all()
+    pos = torch.arange(T, device=DEV)
+    page = c["block_table"][0, pos // 16].long()
+    k, v = (c[n][page, pos % 16].double().view(T, hkv, d) for n in ("k_pool", "v_pool"))
+    for t in (0, 1, 63, 64, 127, 128, 5000, 16383, 16384, 32767, 32768, T - 1):
+        x = c["q"][t].double().view(hkv, hq // hkv, d)
+        kt = k[:t + 1].permute(1, 2, 0).contiguous()
+        vt = v[:t + 1].permute(1, 0, 2).contiguous()
+        w = torch.softmax(torch.matmul(x, kt) / math.sqrt(d), -1)
+        S = float(torch.matmul(x.abs(), kt.abs()).max()) / math.sqrt(d)
+        want, A = torch.matmul(w, vt), torch.matmul(w, vt.abs())
+        u = 2.0 ** -11
+        e = 2.0 ** -24 * (4 * (d + 8) * S + T / 32 + 256)
+        off = (got[t].double().view_as(want) - want).abs() - (u * want.abs() + (u + e) * A * (1 + u))
+        assert off.max().item() <= 0, (t, off.max().item())
+
+
 def test_arguments():
     c = make(1, [2], [20], [3, 4], [1, 2], 4, 2, 64)
 
