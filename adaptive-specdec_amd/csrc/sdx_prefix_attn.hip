@@ -169,6 +169,7 @@ __device__ __forceinline__ PaSeg pa_seg(const PrefixAttnArgs& a, int64_t nt, int
 constexpr int PL_NT = 512;
 constexpr int PL_CAND = 32;      // chunk sizes weighed for the groups
 constexpr int PA_UNIT = 8;       // what a unit costs beside its tiles, the write of its part first
+                                 // (4 or 16: within 3% of it)
 constexpr int PL_OWN = 8;        // entries that a thread writes by itself
 
 // f(x, k) for k < n of every lane's x (words): a lane's first few by itself, the rest by the
