@@ -29,8 +29,8 @@
 // written directly.
 //
 // Measured, 32 query heads on 8 KV heads of 128, bf16, whole calls: a prefix of 16,384 under
-// 128 rows of up to 9 tokens with up to 1,024 own keys 267 us, 695 TFLOP/s; 64 rows behind 4,096
-// keys 73; 4 rows of one token behind 2,000 keys 19.4 (plan 7 to 8, units 8, join 4); keys of
+// 128 rows of up to 9 tokens with up to 1,024 own keys 261 us, 710 TFLOP/s; 64 rows behind 4,096
+// keys 70; 4 rows of one token behind 2,000 keys 20 (plan 6 to 8, units 8, join 4); keys of
 // 8,192 a row without a prefix 5.1 TB/s. A tile takes 3,900 clocks of the two
 // workgroups of a CU: QK 680, mask and softmax 910, PV 800, what is left the staging and its
 // waits; 64 matrix instructions a SIMD are 2,048 of them, so the exponentials and the staging
@@ -202,7 +202,7 @@ struct PlSum {
 };
 
 // The plan's steps are short and depend on each other, so its time is that of its rounds of
-// loads (one, where the batch fits LDS) and barriers (four). 4 rows 7 to 8 us, 128 rows 9 to 10,
+// loads (one, where the batch fits LDS) and barriers (four). 4 rows 6 to 8 us, 128 rows 9 to 10,
 // of them 2 the launch's own.
 __global__ void __launch_bounds__(PL_NT) prefix_attn_plan_kernel(PrefixAttnArgs a) {
   constexpr int NW = PL_NT / kWave;
