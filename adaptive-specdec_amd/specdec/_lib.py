@@ -7,6 +7,8 @@ is not on a ROCm device, calls raise.
 import ctypes
 import functools
 import os
+import threading
+import weakref
 
 import torch
 
@@ -208,28 +210,46 @@ def workspace(nbytes, device, prepare=True):
     return ws
 
 
-_WS_CACHE = {}
+class _Kept(dict):
+    """(device index, stream, kind) -> the workspace that a thread keeps for them."""
+    __hash__ = object.__hash__
+
+
+class _ThreadCache(threading.local):
+    def __init__(self):  # once per thread
+        self.kept = _Kept()
+        with _caches_lock:
+            _caches.add(self.kept)
+
+
+_caches = weakref.WeakSet()  # those of the threads that live
+_caches_lock = threading.Lock()
+_cache = _ThreadCache()
 # entry points whose workspace must be prepared (they keep arrival counters or
 # per-row state in it); the others use theirs as plain scratch
 _PREPARED_KINDS = {"verify", "draft", "greedy"}
 
 
 def cached_workspace(nbytes, device, kind):
-    """The current stream's reusable workspace for entry points of one `kind`,
-    grown when too small. Calls queued on one stream run in order, so they may
-    share it; each stream has its own. Kinds never share memory: the verify
-    workspaces keep their header (magic word and zeroed counters) at fixed
-    offsets that other entry points would overwrite. Under graph capture a new
-    workspace is allocated (from the graph's pool) and not kept."""
+    """The calling thread's reusable workspace on the current stream for entry
+    points of one `kind`, grown when too small and dropped with the thread. Calls
+    that one thread queues on one stream run in order, so they may share it; each
+    stream has its own, and so has each thread: a call queues several kernels that
+    hand data over in the workspace, and ctypes lets other threads run meanwhile,
+    so those of two threads' calls may lie in turn on the stream. Kinds never share
+    memory: the verify workspaces keep their header (magic word and zeroed counters)
+    at fixed offsets that other entry points would overwrite. Under graph capture a
+    new workspace is allocated (from the graph's pool) and not kept."""
     dev = device if isinstance(device, torch.device) else torch.device(device)
     prepare = kind in _PREPARED_KINDS
     if torch.cuda.is_current_stream_capturing():
         return workspace(nbytes, dev, prepare)
     key = (dev.index, _stream(dev), kind)
-    ws = _WS_CACHE.get(key)
+    kept = _cache.kept
+    ws = kept.get(key)
     if ws is None or ws.numel() < int(nbytes):
         ws = workspace(nbytes, dev, prepare)
-        _WS_CACHE[key] = ws
+        kept[key] = ws
     return ws
 
 
@@ -241,7 +261,11 @@ def prepare(ws):
 
 
 def reset_workspaces():
-    """Prepare every cached workspace of the prepared kinds again (see `prepare`)."""
-    for (_, _, kind), ws in _WS_CACHE.items():
-        if kind in _PREPARED_KINDS:
-            prepare(ws)
+    """Prepare every cached workspace of the prepared kinds, of all threads, again
+    (see `prepare`)."""
+    with _caches_lock:
+        caches = list(_caches)
+    for kept in caches:
+        for (_, _, kind), ws in list(kept.items()):
+            if kind in _PREPARED_KINDS:
+                prepare(ws)

@@ -8,7 +8,10 @@
  *   - returns 0 on success or a negative SDX_E* status, with a message
  *     retrievable from sdx_last_error() (thread-local);
  *   - never allocates: scratch comes from a caller workspace sized by the
- *     matching *_workspace() query.
+ *     matching *_workspace() query. A call may queue several kernels that hand data
+ *     over in it, so a workspace serves one call at a time: calls that one thread
+ *     queues on one stream may share it; calls of several host threads, on one stream
+ *     too, or on several streams may not.
  * Token ids are int64 (torch's index type); block tables are int32. All
  * tensors are row-major; a row stride ("ld") is given in elements.
  *
