@@ -19,8 +19,10 @@
 // query l % 32, so maxima and sums stay in the lane (one exchange with lane l ^ 32), and
 // the weights, rounded to 16 bits, are the second operand of O^T = V^T P^T as they lie:
 // its 16 keys are contracted in the order in which the scores hold them. V is read from
-// its rows in LDS by the transposing 64-bit reads. The running maximum moves only when a
-// score passes it by 2^8 (weights up to 2^8 lose nothing), which spares rescaling O.
+// its rows in LDS by the transposing 64-bit reads. The rounding of the weights is the second
+// product's price: matrix instructions take 16-bit operands, two halves of each weight would double
+// them. The running maximum moves only when a score passes it by 2^8 (weights up to 2^8 lose
+// nothing), which spares rescaling O.
 //
 // A plan kernel of one workgroup lists the units from the lengths. A fixed grid takes them
 // from eight queues, one for each XCD's share, so that the units of one chunk of keys read
@@ -54,7 +56,13 @@ constexpr uint32_t PA_NOSLOT = 0xFFFFFFFFu;
 constexpr uint32_t PA_ASK = 0xFFFFFFFFu;
 constexpr int PA_QUEUE = 32;      // words between the queues' heads
 constexpr int PA_ZERO = 8 * PA_QUEUE;  // word of the head where a row of zeros lies
-constexpr float PA_SLACK = 8.0f;  // log2 by which a weight may pass 1
+constexpr float PA_SLACK = 8.0f;  // log2 by which a weight may pass its step of the maximum
+// log2 of the weight that such a step gives the largest score. An fp16 weight below 2^-14 is rounded
+// to a multiple of 2^-24, which adds up over many keys far below the largest: n keys lose up to
+// n 2^-25 of the output with 1 as the largest weight, eight half steps of the type at 131,072, and
+// n 2^-32 with 2^7 (2^15 with the slack, below the type's 65,504). bf16 has fp32's exponents.
+template <int FMT>
+constexpr float pa_lift() { return FMT == SDX_F16 ? 7.0f : 0.0f; }
 
 typedef short pa_s4 __attribute__((ext_vector_type(4)));
 typedef uint32_t pa_u4 __attribute__((ext_vector_type(4)));
@@ -529,17 +537,19 @@ __device__ __forceinline__ void pa_mask(pa_f16 (&s)[NB], int t0, int lim, int hi
     for (int i = 0; i < 16; ++i)
       if (32 * nb + 8 * (i / 4) + i % 4 > left) s[nb][i] = -INFINITY;
 }
-// Weights of NB x 32 scores, in s.
-template <int D, int NB>
+// Weights of NB x 32 scores, in s. st.m is the largest score in log2 so far, less the lift and up to
+// the slack, which is tested with the weights' own argument: none passes 2^(lift + slack).
+template <int D, int FMT, int NB>
 __device__ __forceinline__ void pa_softmax(PaState<D>& st, pa_f16 (&s)[NB], float scale) {
   float mx = s[0][0];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[nb][i]);
-  mx = pa_max_halves(mx) * scale;
-  if (__any(mx > st.m + PA_SLACK)) {
-    const float mn = fmaxf(st.m, mx);
+  constexpr float LIFT = pa_lift<FMT>();
+  mx = pa_max_halves(mx);
+  if (__any(fmaf(mx, scale, -st.m) > LIFT + PA_SLACK)) {
+    const float mn = fmaxf(st.m, mx * scale - LIFT);
     const float alpha = st.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.m - mn);
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
@@ -866,7 +876,7 @@ prefix_attn_kernel(PrefixAttnArgs a) {
         }
         __builtin_amdgcn_s_setprio(0);
         if ((t + 1) * PA_TILE > seen) pa_mask<2>(s, t * PA_TILE, lim, hi);  // uniform
-        pa_softmax<D, 2>(st, s, a.scale_log2);
+        pa_softmax<D, FMT, 2>(st, s, a.scale_log2);
         __builtin_amdgcn_s_setprio(1);
         pa_pv<D, FMT, 2>(st, s, k + PA_TILE * RB, va);
         __builtin_amdgcn_s_setprio(0);
