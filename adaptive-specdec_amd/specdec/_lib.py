@@ -228,6 +228,10 @@ _cache = _ThreadCache()
 # entry points whose workspace must be prepared (they keep arrival counters or
 # per-row state in it); the others use theirs as plain scratch
 _PREPARED_KINDS = {"verify", "draft", "greedy"}
+# scratch beyond this is returned to torch's allocator after its call instead of kept: the
+# attention over shared prefixes takes two fp32 outputs at least, 1.1 GB for 33,000 tokens of
+# 32 heads of 128
+KEEP_BYTES = 512 << 20
 
 
 def cached_workspace(nbytes, device, kind):
@@ -239,10 +243,11 @@ def cached_workspace(nbytes, device, kind):
     so those of two threads' calls may lie in turn on the stream. Kinds never share
     memory: the verify workspaces keep their header (magic word and zeroed counters)
     at fixed offsets that other entry points would overwrite. Under graph capture a
-    new workspace is allocated (from the graph's pool) and not kept."""
+    new workspace is allocated (from the graph's pool) and not kept, and so is scratch
+    of more than KEEP_BYTES."""
     dev = device if isinstance(device, torch.device) else torch.device(device)
     prepare = kind in _PREPARED_KINDS
-    if torch.cuda.is_current_stream_capturing():
+    if (nbytes > KEEP_BYTES and not prepare) or torch.cuda.is_current_stream_capturing():
         return workspace(nbytes, dev, prepare)
     key = (dev.index, _stream(dev), kind)
     kept = _cache.kept

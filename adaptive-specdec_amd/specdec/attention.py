@@ -97,7 +97,8 @@ def shared_prefix_attention_paged(q, cu_q, k_pool, v_pool, block_table, kv_len, 
     [T, Hq, d] of q's type. Rows or groups out of range are skipped and set `error` (an int32
     [1] device tensor) when given, and so do page ids outside the pool. `workspace` (uint8,
     `shared_attention_workspace`) holds fp32 parts and serves one call at a time; None: the
-    calling thread's own for the current stream, kept for its next calls."""
+    calling thread's own for the current stream, kept for its next calls up to 512 MiB. Its size is
+    8 T Hq (d + 2) bytes at least (1.1 GB for 33,000 tokens of 32 heads of 128)."""
     _lib.one_gpu(q, cu_q, k_pool, v_pool, block_table, kv_len, cu_group, prefix_len, out, error,
                  workspace)
     if q.dtype not in (torch.bfloat16, torch.float16) or k_pool.dtype != q.dtype or \

@@ -91,3 +91,19 @@ def test_reset_reaches_every_thread(fake):
     t.join()
     assert {mine.data_ptr(), other[0].data_ptr()} <= set(fake)
     assert _lib.cached_workspace(64, "cuda:0", "sample").data_ptr() not in fake
+
+
+def test_large_scratch_is_not_kept(fake):
+    """One call over very many tokens does not hold its gigabytes for the thread's life, nor drop
+    the workspace of the ordinary calls; prepared kinds, which a call would have to prepare
+    again, are kept at any size."""
+    at = _lib.KEEP_BYTES
+    small = _lib.cached_workspace(1 << 20, "cuda:0", "prefix_attn")
+    large = weakref.ref(_lib.cached_workspace(at + 1, "cuda:0", "prefix_attn"))
+    gc.collect()
+    assert large() is None
+    assert _lib.cached_workspace(1 << 20, "cuda:0", "prefix_attn") is small
+    whole = _lib.cached_workspace(at, "cuda:0", "prefix_attn")
+    assert _lib.cached_workspace(1 << 20, "cuda:0", "prefix_attn") is whole
+    held = _lib.cached_workspace(at + 1, "cuda:0", "verify")
+    assert _lib.cached_workspace(at + 1, "cuda:0", "verify") is held
