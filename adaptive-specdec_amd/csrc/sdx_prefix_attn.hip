@@ -997,9 +997,11 @@ int prefix_attn_parts(int64_t tokens, int32_t hq, int32_t hkv, int32_t d) {
   const int64_t want = std::min<int64_t>(512, 2 * ((PA_GRID + hkv - 1) / hkv));
   return (int)std::max<int64_t>(2, std::min<int64_t>(want, PA_ROOM / std::max<int64_t>(1, one)) / 2 * 2);
 }
-// A segment has a query tile of 128 rows for every 128 of its tokens' rows and one more.
+// A segment that has tokens has a query tile of 128 rows for every 128 of its tokens' rows and one
+// more; rows and groups without tokens, which may be most of them, have none.
 int64_t prefix_attn_entries(int64_t tokens, int64_t batch, int64_t groups, int32_t group, int32_t parts) {
-  return (2 * (tokens * group / PA_ROWS) + batch + groups) * (parts / 2);
+  return (2 * (tokens * group / PA_ROWS) + std::min(batch, tokens) + std::min(groups, tokens)) *
+         (parts / 2);
 }
 
 template <int D, int FMT, int HG>
