@@ -1240,7 +1240,8 @@ int sdx_prefix_attention_paged(const void* q, int dtype, int64_t num_tokens, int
                                void* workspace, size_t workspace_bytes, void* out, int32_t* error,
                                sdx_stream_t stream) {
   if (num_tokens < 0 || batch < 0 || num_groups < 0 || num_q_heads < 1 || num_kv_heads < 1 ||
-      block_size < 1 || max_blocks < 1 || num_blocks < 1 || !(scale > 0.0f) || !(scale < INFINITY))
+      block_size < 1 || max_blocks < 1 || num_blocks < 1 || !(scale > 0.0f) ||
+      !(scale * 1.4426950408889634f < INFINITY))
     return fail(SDX_EINVAL, "sdx_prefix_attention_paged: bad arguments");
   if (num_q_heads % num_kv_heads != 0)
     return fail(SDX_EINVAL, "sdx_prefix_attention_paged: query heads must be a multiple of KV heads");

@@ -461,7 +461,7 @@ size_t sdx_verify_attention_workspace(int64_t batch, int32_t max_q, int32_t num_
  * page that holds its end, a row's own table gives the keys behind the end. sdx_build_block_tables
  * lays such tables out. Query j of row b sees keys s <= kv_len[b] - q_b + j, the prefix's too.
  * q / out: [num_tokens, num_q_heads, head_dim], bf16 or fp16 as the pools, 16-byte aligned;
- * q_b = cu_q[b+1] - cu_q[b] of any size; head_dim 64 or 128; scale positive and finite. Softmax
+ * q_b = cu_q[b+1] - cu_q[b] of any size; head_dim 64 or 128; scale positive, scale log2(e) finite. Softmax
  * and sums in fp32, weights rounded to the type for the second product, output rounded to it.
  * Keys and values that a query does not see do not reach its output, whatever they hold.
  * Rows, or groups with all their rows, whose lengths or offsets are out of range set *error

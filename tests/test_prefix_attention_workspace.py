@@ -43,3 +43,19 @@ def test_room_for_every_list_of_units():
         parts = max(2, min(512, 2 * -(-512 // hkv), (192 << 20) // one) // 2 * 2)
         need = 32 * tiles * (parts // 2) + parts * one
         assert L.sdx_prefix_attention_workspace(T, rows, len(groups), hq, hkv, d) >= need
+
+
+def test_scales_that_overflow_in_base_two_are_refused():
+    """The kernels multiply by scale log2(e) in fp32: infinite from 2.4e38 on, and 0 times it is no
+    score."""
+    L = _lib()
+
+    def call(scale):
+        need = L.sdx_prefix_attention_workspace(3, 2, 1, 4, 2, 64)
+        # no workspace: a scale that is taken ends there
+        return L.sdx_prefix_attention_paged(FAKE, 1, 3, 2, FAKE, 4, 2, 64, FAKE, FAKE, 8, 16, FAKE, 4,
+                                            FAKE, FAKE, FAKE, 1, scale, None, need, FAKE, None, None)
+
+    assert call(2.3e38) == -4 and call(0.125) == -4
+    for bad in (2.4e38, 3.4e38, float("inf"), float("nan"), 0.0, -1.0):
+        assert call(bad) == -1, bad
