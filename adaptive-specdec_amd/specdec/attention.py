@@ -116,6 +116,8 @@ def shared_prefix_attention_paged(q, cu_q, k_pool, v_pool, block_table, kv_len, 
         raise ValueError("shared_prefix_attention_paged: pools must be contiguous")
     if error is not None and error.dtype != torch.int32:
         raise TypeError("shared_prefix_attention_paged: error must be int32")
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("shared_prefix_attention_paged: workspace must be contiguous")
     B, G = kv_len.numel(), prefix_len.numel()
     if cu_q.numel() != B + 1 or cu_group.numel() != G + 1 or block_table.dim() != 2 or \
             block_table.shape[0] != B:

@@ -59,3 +59,19 @@ def test_scales_that_overflow_in_base_two_are_refused():
     assert call(2.3e38) == -4 and call(0.125) == -4
     for bad in (2.4e38, 3.4e38, float("inf"), float("nan"), 0.0, -1.0):
         assert call(bad) == -1, bad
+
+
+def test_workspaces_that_are_not_whole_are_refused(monkeypatch):
+    """A view whose elements do not lie one after another covers fewer bytes than it counts."""
+    import torch
+
+    from specdec import attention as A
+    from specdec import _lib as B
+    monkeypatch.setattr(B, "one_gpu", lambda *t: None)
+    z = torch.zeros
+    args = (z((3, 4, 64), dtype=torch.half), z(3).long(), z((8, 16, 128), dtype=torch.half),
+            z((8, 16, 128), dtype=torch.half), z((2, 4), dtype=torch.int32), z(2).long(), z(2).long(),
+            z(1).long())
+    for ws in (z(1, dtype=torch.uint8).expand(1 << 30), z(1 << 20, dtype=torch.uint8)[::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            A.shared_prefix_attention_paged(*args, workspace=ws)
