@@ -953,7 +953,7 @@ __global__ void __launch_bounds__(PA_NT) prefix_attn_join_kernel(PrefixAttnArgs 
       const bool none = i0 + k * SL >= n || ml[k].x == -INFINITY;  // no part: not a 0 times its O
       const float f = none ? 0.0f : __builtin_amdgcn_exp2f(ml[k].x - m);
       if (none) v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      l += f * ml[k].y;
+      l += f * ml[k].y;  // 0 times the NaN sum of a part whose scores are all NaN is NaN, and so is out
       o.x += f * v[k].x;
       o.y += f * v[k].y;
       o.z += f * v[k].z;

@@ -132,7 +132,7 @@ int sdx_gather_prob(const float* probs, int64_t rows, int64_t vocab, int64_t ld,
  *                           lowest id first among equal ones (-0 == +0), with their ln softmax
  * all fp32, ids int64. fp32 sums. A row whose logits are all -inf, or that holds a +inf or
  * NaN, has NaN log probabilities and entropy; its list orders the values all the same, NaN
- * last (id -1 where a row with NaN leaves none). top_n up to 64 and at most vocab;
+ * last, the lowest id first among NaN too. top_n up to 64 and at most vocab;
  * temperature positive and finite. Rows split over workgroups keep their parts in the
  * workspace (16-byte aligned, no initial contents; 0 bytes where rows are many). One kernel,
  * or two. What to_probs + gather_prob (sampling.py:34-67,93-95) would be composed for. */
@@ -464,6 +464,8 @@ size_t sdx_verify_attention_workspace(int64_t batch, int32_t max_q, int32_t num_
  * q_b = cu_q[b+1] - cu_q[b] of any size; head_dim 64 or 128; scale positive, scale log2(e) finite. Softmax
  * and sums in fp32, weights rounded to the type for the second product, output rounded to it.
  * Keys and values that a query does not see do not reach its output, whatever they hold.
+ * A NaN among the scores that a query sees makes its output NaN; where all of them are -inf
+ * it is 0, as sdx_verify_attention_paged has it.
  * Rows, or groups with all their rows, whose lengths or offsets are out of range set *error
  * (nullable) and leave their output as it was; tokens behind the last row too, without the
  * error. Page ids outside the pool set *error and the output of the rows that read them is
