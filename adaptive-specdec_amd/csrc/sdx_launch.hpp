@@ -475,6 +475,7 @@ struct BlockTableArgs {
   int32_t* table;               // [batch, max_blocks]
   int64_t* used;                // [1] pages handed out, or null
   int32_t* error;
+  int64_t rows;                 // of a workgroup (set by the launch)
 };
 hipError_t launch_block_tables(const BlockTableArgs& a, hipStream_t s);
 struct PagedSlotArgs {

@@ -43,16 +43,18 @@ __device__ __forceinline__ void pg_find(const int64_t* cu, int64_t n, int64_t st
   }
 }
 
-// ---- block tables. A workgroup fills the columns [PG_COLS y, PG_COLS (y + 1)) of row x.
-// Where its own pages start in the free list is a sum over the rows before it, and whether
-// anything is handed out depends on all rows: every workgroup adds up the rows itself (8
-// bytes each, from the L2), which saves the launch of a scan. Bound by latency: a row's
-// length, its group's first row's length and the free list are three dependent loads, PG_UN
-// rows of them in flight per thread; the offsets and prefixes lie in LDS
-// up to 1,024 groups. In a graph: 32 rows of 4 groups 4.1 us (4.7 with a row at a time), 789
-// rows of 128 groups with tables of 3 MB 10.4 (12.7).
+// ---- block tables. A workgroup fills the columns [PG_COLS y, PG_COLS (y + 1)) of a few
+// consecutive rows, one up to PG_GRID rows. Where their own pages start in the free list is a
+// sum over the rows before them, and whether anything is handed out depends on all rows: every
+// workgroup adds up the rows itself (8 bytes each, from the L2), which saves the launch of a
+// scan. Bound by latency: a row's length, its group's first row's length and the free list are
+// three dependent loads, PG_UN rows of them in flight per thread, and the adding up grows with
+// the rows; the offsets and prefixes lie in LDS up to 1,024 groups. In a graph, rows in
+// groups of 6 to 8 with tables of 44 columns: 32 rows 4.2 us, 786 9.8 (10.4 with tables of 3 MB),
+// 4,096 50 (83 with a workgroup for every row), 131,072 2,050 (92,000), 2^20 21,500.
 constexpr int PG_COLS = 4096;
 constexpr int PG_UN = 4;
+constexpr int PG_GRID = 2048;  // workgroups that the chip holds at once: more would add up again
 
 // I: uint32_t where the table's lengths fit 32 bits (a short division; a length or a prefix
 // that does not makes its row, or its group's first, bad, and that leaves every table empty),
@@ -83,13 +85,14 @@ __device__ __forceinline__ PgRow pg_row(const BlockTableArgs& a, int64_t b, int6
   return r;
 }
 
-template <typename I>
+// MANY: several rows a workgroup; the code for it costs a single one's 0.2 us of 4.
+template <typename I, bool MANY>
 __global__ void __launch_bounds__(PG_NT) block_tables_kernel(BlockTableArgs a) {
   constexpr int NW = PG_NT / kWave;
   __shared__ int64_t sCu[PG_LDS + 1], sPrefix[PG_LDS];
   __shared__ uint64_t sSum[NW][3];
   const int tid = threadIdx.x;
-  const int64_t row = blockIdx.x;
+  const int64_t row = MANY ? (int64_t)blockIdx.x * a.rows : blockIdx.x;
   const bool grouped = a.cu_group;
   const int64_t step = grouped ? pg_step(a.groups) : 1;
   int bad = 0;
@@ -165,20 +168,37 @@ __global__ void __launch_bounds__(PG_NT) block_tables_kernel(BlockTableArgs a) {
     if (a.used) *a.used = bad ? 0 : total;
     if (bad && a.error) *a.error = 1;
   }
-  int32_t* const out = a.table + row * a.max_blocks;
   const int64_t end = min(a.max_blocks, ((int64_t)blockIdx.y + 1) * PG_COLS);
-  for (int64_t c0 = (int64_t)blockIdx.y * PG_COLS + tid; c0 < end; c0 += PG_UN * PG_NT) {
-    int32_t v[PG_UN];
+  for (int64_t r = row;;) {  // uniform
+    int32_t* const out = a.table + r * a.max_blocks;
+    for (int64_t c0 = (int64_t)blockIdx.y * PG_COLS + tid; c0 < end; c0 += PG_UN * PG_NT) {
+      int32_t v[PG_UN];
 #pragma unroll
-    for (int i = 0; i < PG_UN; ++i) {
-      const int64_t c = c0 + i * PG_NT;
-      v[i] = -1;
-      if (!bad && c < me.need)  // the first row's own pages start at its column 0
-        v[i] = a.free_blocks[c < me.shared ? before_first + c : before + c - me.shared];
+      for (int i = 0; i < PG_UN; ++i) {
+        const int64_t c = c0 + i * PG_NT;
+        v[i] = -1;
+        if (!bad && c < me.need)  // the first row's own pages start at its column 0
+          v[i] = a.free_blocks[c < me.shared ? before_first + c : before + c - me.shared];
+      }
+#pragma unroll
+      for (int i = 0; i < PG_UN; ++i)
+        if (c0 + i * PG_NT < end) out[c0 + i * PG_NT] = v[i];
     }
-#pragma unroll
-    for (int i = 0; i < PG_UN; ++i)
-      if (c0 + i * PG_NT < end) out[c0 + i * PG_NT] = v[i];
+    if (!MANY || ++r == min(row + a.rows, a.batch)) break;
+    // the next row: behind this one's pages; its group's first row is this group's, or itself
+    before += me.need - me.shared;
+    int64_t f = 0, ge = 0, p = 0, kf = 0;
+    if (grouped) {
+      const int64_t x[1] = {r};
+      int64_t g[1];
+      pg_find<1>(a.cu_group, a.groups, step, sCu, x, g);
+      f = step == 1 ? sCu[g[0]] : a.cu_group[g[0]];
+      ge = step == 1 ? sCu[g[0] + 1] : a.cu_group[g[0] + 1];
+      p = step == 1 ? sPrefix[g[0]] : a.prefix_len[g[0]];
+      kf = a.kv_len[max((int64_t)0, min(f, a.batch - 1))];
+    }
+    me = pg_row<I>(a, r, a.kv_len[r], f, ge, p, kf);
+    if (me.first == r) before_first = before;
   }
 }
 
@@ -251,12 +271,17 @@ __global__ void __launch_bounds__(PG_NT) append_slots_kernel(AppendSlotArgs a) {
 }
 
 // ---------------------------------------------------------------- launches
-hipError_t launch_block_tables(const BlockTableArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)a.batch, (unsigned)((a.max_blocks + PG_COLS - 1) / PG_COLS));
-  if ((a.max_blocks + 1) * a.bs <= 0xFFFFFFFFll)
-    hipLaunchKernelGGL((block_tables_kernel<uint32_t>), grid, dim3(PG_NT), 0, s, a);
+hipError_t launch_block_tables(const BlockTableArgs& b, hipStream_t s) {
+  BlockTableArgs a = b;
+  a.rows = (a.batch + PG_GRID - 1) / PG_GRID;
+  const dim3 grid((unsigned)((a.batch + a.rows - 1) / a.rows),
+                  (unsigned)((a.max_blocks + PG_COLS - 1) / PG_COLS));
+  if ((a.max_blocks + 1) * a.bs > 0xFFFFFFFFll)
+    hipLaunchKernelGGL((block_tables_kernel<uint64_t, true>), grid, dim3(PG_NT), 0, s, a);
+  else if (a.rows > 1)
+    hipLaunchKernelGGL((block_tables_kernel<uint32_t, true>), grid, dim3(PG_NT), 0, s, a);
   else
-    hipLaunchKernelGGL((block_tables_kernel<uint64_t>), grid, dim3(PG_NT), 0, s, a);
+    hipLaunchKernelGGL((block_tables_kernel<uint32_t, false>), grid, dim3(PG_NT), 0, s, a);
   return hipGetLastError();
 }
 
