@@ -19,9 +19,11 @@
 // vectors again, and what reaches it there, n elements and a few, is sorted. Per element the
 // list costs the maximum that the sums need anyway.
 //
-// Bound by the read of the logits: 576 x 151,936 bf16 with 20 alternatives 52 us, 3.4 TB/s (a
-// sum over 1 GiB reads at 4.0). A row is split over workgroups where rows are few, and a
-// second kernel joins its parts: 5 x 50,257 fp32 6.5 us and 4.6, the launches' latency.
+// Bound by the read of the logits and of the list's second look: 576 x 151,936 bf16 without a list
+// 41 us and 175 MB fetched, 4.3 TB/s; with 20 alternatives 52 us (fp16 53, 288 rows of fp32 52) and
+// 263 MB, 5.1 TB/s, since 16-byte vectors of a few threads lie in half of the row's lines; 1 to 5
+// alternatives 47. A row is split over workgroups where rows are few, and a second kernel joins
+// its parts: 5 x 50,257 fp32 6.5 us and 4.6, the launches' latency.
 #include <algorithm>
 
 #include "sdx_launch.hpp"

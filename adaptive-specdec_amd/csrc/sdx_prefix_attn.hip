@@ -13,8 +13,8 @@
 // Few rows leave waves without any: such units are bound by the read of the keys, full ones by
 // the matrix instructions and the exponentials. (A form for up to 32 rows, in which every wave
 // held them all and took 32 keys of each 128 by itself, was measured beside it: 8 rows behind
-// 65,536 keys 79.7 us, now 71.7; 128 rows of 8,192 keys each 426, now 414; 4 rows behind 2,000
-// keys 21.8 and 21.9; 2 rows of one KV head behind 12,000 keys 23.3, now 25.3.)
+// 65,536 keys 79.7 us, now 71.0; 128 rows of up to 8,192 own keys, 2.08 GB, 426, now 414; 4 rows
+// behind 2,000 keys 21.8 and 21.9; 2 rows of one KV head behind 12,000 keys 23.3, now 24.5.)
 // S^T = K Q^T with v_mfma_f32_32x32x16: lane l then holds 16 keys' scores of
 // query l % 32, so maxima and sums stay in the lane (one exchange with lane l ^ 32), and
 // the weights, rounded to 16 bits, are the second operand of O^T = V^T P^T as they lie:
@@ -32,8 +32,12 @@
 //
 // Measured, 32 query heads on 8 KV heads of 128, bf16, whole calls: a prefix of 16,384 under
 // 128 rows of up to 9 tokens with up to 1,024 own keys 261 us, 710 TFLOP/s; 64 rows behind 4,096
-// keys 70; 4 rows of one token behind 2,000 keys 20 (plan 6 to 8, units 8, join 4); keys of
-// 8,192 a row without a prefix 5.1 TB/s. A tile takes 3,900 clocks of the two
+// keys 70; 4 rows of one token behind 2,000 keys 20 (plan 6 to 8, units 8, join 4); 128 rows of up
+// to 8,192 own keys behind a prefix of 16, 2.08 GB, 414, 5.0 TB/s, with one token each 5.8. A unit's
+// keys do not stop where its query tile's view does: a prompt of 16,384 tokens takes 4.92 ms, 447
+// TFLOP/s of the products that its mask leaves, about half of those done; and one row inside its
+// prefix has the tiles of all groups masked (64 rows' step of 72 us beside a prompt of 4,096 tokens
+// of 340: 392 us, 440 where that row shares the prompt). A tile takes 3,900 clocks of the two
 // workgroups of a CU: QK 680, mask and softmax 910, PV 800, what is left the staging and its
 // waits; 64 matrix instructions a SIMD are 2,048 of them, so the exponentials and the staging
 // bound it. Tried: PV of the tile before among the exponentials (spills, 246 -> 283 us without
@@ -618,8 +622,9 @@ __device__ __forceinline__ void pa_pv(PaState<D>& st, const pa_f16 (&s)[NB], con
 
 // V in tiles of which some query rows see a part: a weight of 0 times an infinity or a NaN would
 // be a NaN, so such elements are 0 for the products, and are added behind the last tile to the
-// rows that see their key. One comparison for the largest of a thread's elements costs 0 to 1%
-// of a call; one for each, or the sums in every tile, 3 to 9%.
+// rows that see their key. One comparison for the largest of a thread's elements costs nothing that
+// shows (128 rows of up to 8,192 own keys 414 us with and without, 64 rows 70.9 and 70.8; 0.8 and
+// 1.4% when it came in); one for each, or the sums in every tile, 3 to 9%.
 template <int FMT, int H>
 __device__ __forceinline__ bool pa_finite_only(pa_u4 (&v)[H]) {
   typedef uint16_t h2 __attribute__((ext_vector_type(2)));
@@ -992,6 +997,8 @@ __global__ void __launch_bounds__(PA_NT) prefix_attn_join_kernel(PrefixAttnArgs 
 // Parts per query row: half for the prefix, half for the row's own keys. As many as the
 // grid could fill from one row, in at most PA_ROOM bytes (but two).
 constexpr int64_t PA_ROOM = (int64_t)192 << 20;
+// That keeps two outputs in fp32 also where every row is written directly: 1.1 GB for 32,768 tokens
+// of 32 heads of 128.
 int prefix_attn_parts(int64_t tokens, int32_t hq, int32_t hkv, int32_t d) {
   const int64_t one = tokens * hq * (d + 2) * 4;
   const int64_t want = std::min<int64_t>(512, 2 * ((PA_GRID + hkv - 1) / hkv));
