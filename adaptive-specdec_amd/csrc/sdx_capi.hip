@@ -4,6 +4,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
 #include <mutex>
 
 #include <cstdlib>
@@ -1090,6 +1091,148 @@ int sdx_append_slots(void* pool, int64_t layer_stride, int64_t side_stride, cons
   sdx::AppendSlotArgs a{(uint8_t*)pool, (const uint8_t*)staged, slots, layer_stride * es,
                         side_stride * es, row_elems * es, num_tokens, num_slots, layers, error};
   return hip_status(sdx::launch_append_slots(a, (hipStream_t)stream), "append_slots");
+}
+
+// ------------------------------------------------------------------ trees of drafted tokens
+int sdx_tree_layout(const int32_t* parents, int64_t batch, const int64_t* cu_q, const int64_t* kv_len,
+                    int32_t max_nodes, const int32_t* block_table, int64_t max_blocks,
+                    int32_t block_size, int64_t num_tokens, int64_t padding_slot, int64_t* mask,
+                    int64_t* positions, int64_t* slots, int32_t* error, sdx_stream_t stream) {
+  if (!cu_q || !kv_len || batch < 0 || num_tokens < 0 || max_nodes < 1 ||
+      (num_tokens > 0 && (!parents || !mask || !positions)) || (!block_table != !slots && num_tokens > 0) ||
+      (block_table && (max_blocks < 1 || block_size < 1)))
+    return fail(SDX_EINVAL, "sdx_tree_layout: bad arguments");
+  if (max_nodes > sdx::TREE_MAX_NODES)
+    return fail(SDX_EUNSUPPORTED, "sdx_tree_layout: more than %d nodes in a row", sdx::TREE_MAX_NODES);
+  if (batch > (1 << 23) || max_blocks > ((int64_t)1 << 31) || num_tokens > ((int64_t)1 << 31))
+    return fail(SDX_EUNSUPPORTED, "sdx_tree_layout: more than 2^23 rows, 2^31 blocks or tokens");
+  if (num_tokens == 0) return SDX_OK;
+  if (batch == 0)
+    return fail(SDX_EINVAL, "sdx_tree_layout: %lld nodes of no row", (long long)num_tokens);
+  sdx::TreeLayoutArgs a{parents, cu_q, kv_len, block_table, batch, num_tokens,
+                        block_table ? max_blocks : (int64_t)1 << 62, block_table ? block_size : 1,
+                        padding_slot, (max_nodes + 63) / 64, mask, positions, slots, error};
+  return hip_status(sdx::launch_tree_layout(a, (hipStream_t)stream), "tree_layout");
+}
+
+int sdx_tree_accept(const int64_t* tokens, const int32_t* parents, const int64_t* choice, int64_t batch,
+                    const int64_t* cu_q, int64_t num_tokens, const uint8_t* active, int64_t max_path,
+                    int64_t* path, int64_t* keep, int64_t* y, int32_t* error, sdx_stream_t stream) {
+  if (!cu_q || batch < 0 || num_tokens < 0 || max_path < 1 || (batch > 0 && (!path || !keep || !y)) ||
+      (num_tokens > 0 && (!tokens || !parents || !choice)))
+    return fail(SDX_EINVAL, "sdx_tree_accept: bad arguments");
+  if (batch > (1 << 23) || max_path > sdx::TREE_MAX_NODES)
+    return fail(SDX_EUNSUPPORTED, "sdx_tree_accept: more than 2^23 rows or paths of more than %d nodes",
+                sdx::TREE_MAX_NODES);
+  if (batch == 0) return SDX_OK;
+  sdx::TreeAcceptArgs a{tokens, parents, choice, cu_q, active, batch, num_tokens, max_path,
+                        path, keep, y, error};
+  return hip_status(sdx::launch_tree_accept(a, (hipStream_t)stream), "tree_accept");
+}
+
+// ------------------------------------------------------------------ pages of the cache
+// pool arguments that compact and copy share
+static int pool_args(const char* who, const void* pool, int64_t layer_stride, int64_t side_stride, int dtype,
+                     int32_t layers, int64_t row_elems, int64_t num_blocks, int32_t block_size) {
+  if (!pool || !dtype_ok(dtype) || layers < 1 || row_elems < 1 || num_blocks < 1 || block_size < 1)
+    return fail(SDX_EINVAL, "%s: bad arguments", who);
+  const int64_t es = (int64_t)dsize(dtype);
+  if ((row_elems * es) % 16 != 0 || !aligned16(pool) || (layer_stride * es) % 16 != 0 ||
+      (side_stride * es) % 16 != 0)
+    return fail(SDX_EINVAL, "%s: rows and strides must be 16-byte multiples", who);
+  if (layers > 32767 || row_elems > ((int64_t)1 << 30) || row_elems * es > ((int64_t)1 << 31) / block_size)
+    return fail(SDX_EUNSUPPORTED, "%s: more than 32767 layers or pages of more than 2^31 bytes", who);
+  return SDX_OK;
+}
+
+int sdx_compact_paged(void* pool, int64_t layer_stride, int64_t side_stride, int dtype, int32_t layers,
+                      int64_t row_elems, int64_t num_blocks, int32_t block_size,
+                      const int32_t* block_table, int64_t batch, int64_t max_blocks,
+                      const int64_t* kv_start, const int64_t* path, int64_t max_path,
+                      const int64_t* keep, int32_t* error, sdx_stream_t stream) {
+  const int rc = pool_args("sdx_compact_paged", pool, layer_stride, side_stride, dtype, layers, row_elems,
+                           num_blocks, block_size);
+  if (rc != SDX_OK) return rc;
+  if (batch < 0 || max_blocks < 1 || max_path < 1 ||
+      (batch > 0 && (!block_table || !kv_start || !path || !keep)))
+    return fail(SDX_EINVAL, "sdx_compact_paged: bad arguments");
+  if (batch > (1 << 23) || max_blocks > ((int64_t)1 << 31) || max_path > sdx::TREE_MAX_NODES)
+    return fail(SDX_EUNSUPPORTED, "sdx_compact_paged: more than 2^23 rows, 2^31 blocks or paths of more "
+                                  "than %d tokens", sdx::TREE_MAX_NODES);
+  if (batch == 0) return SDX_OK;
+  const int64_t es = (int64_t)dsize(dtype);
+  sdx::CompactArgs a{(uint8_t*)pool, layer_stride * es, side_stride * es, row_elems * es, num_blocks,
+                     block_table, kv_start, path, keep, batch, max_blocks, block_size, max_path,
+                     layers, error};
+  return hip_status(sdx::launch_compact_paged(a, (hipStream_t)stream), "compact_paged");
+}
+
+static bool free_fits(int64_t batch, int64_t max_blocks, int64_t num_blocks) {
+  return batch >= 0 && max_blocks >= 1 && num_blocks >= 1 && num_blocks <= ((int64_t)1 << 30) &&
+         batch <= ((int64_t)1 << 31) / max_blocks;
+}
+size_t sdx_free_pages_workspace(int64_t batch, int64_t max_blocks, int64_t num_blocks) {
+  if (!free_fits(batch, max_blocks, num_blocks)) return 0;
+  return (size_t)sdx::free_pages_parts(batch * max_blocks) * ((num_blocks + 31) / 32) * sizeof(uint32_t);
+}
+int sdx_free_pages(const int32_t* block_table, int64_t batch, int64_t max_blocks, const int64_t* kv_len,
+                   int32_t block_size, int64_t num_blocks, int32_t* free_blocks, int64_t* num_free,
+                   void* workspace, size_t workspace_bytes, int32_t* error, sdx_stream_t stream) {
+  if (batch < 0 || max_blocks < 1 || block_size < 1 || num_blocks < 1 || !free_blocks || !num_free ||
+      (batch > 0 && !block_table))
+    return fail(SDX_EINVAL, "sdx_free_pages: bad arguments");
+  if (!free_fits(batch, max_blocks, num_blocks))
+    return fail(SDX_EUNSUPPORTED, "sdx_free_pages: more than 2^30 pages or 2^31 table entries");
+  const size_t need = sdx_free_pages_workspace(batch, max_blocks, num_blocks);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < need)
+    return fail(SDX_EWORKSPACE, "sdx_free_pages: needs a 16-byte aligned workspace of %zu bytes (got %zu)",
+                need, workspace_bytes);
+  sdx::FreePagesArgs a{block_table, kv_len, batch, max_blocks, block_size, num_blocks,
+                       sdx::free_pages_parts(batch * max_blocks), (num_blocks + 31) / 32,
+                       (uint32_t*)workspace, free_blocks, num_free, error};
+  return hip_status(sdx::launch_free_pages(a, (hipStream_t)stream), "free_pages");
+}
+
+size_t sdx_fork_block_tables_workspace(int64_t batch) {
+  return batch < 0 || batch > (1 << 23) ? 0 : (size_t)std::max<int64_t>(batch, 1) * sizeof(int32_t);
+}
+int sdx_fork_block_tables(const int32_t* block_table, int64_t old_batch, int64_t max_blocks,
+                          const int64_t* kv_len, const int64_t* parent, const int64_t* room,
+                          int64_t batch, int32_t block_size, const int32_t* free_blocks,
+                          int64_t max_free, const int64_t* num_free, int32_t* out, int32_t* copies,
+                          int64_t* used, void* workspace, size_t workspace_bytes, int32_t* error,
+                          sdx_stream_t stream) {
+  if (old_batch < 0 || batch < 0 || max_blocks < 1 || block_size < 1 || max_free < 0 ||
+      (old_batch > 0 && (!block_table || !kv_len)) || (max_free > 0 && !free_blocks) ||
+      (batch > 0 && (!parent || !room || !out || !copies || !used)))
+    return fail(SDX_EINVAL, "sdx_fork_block_tables: bad arguments");
+  if (batch > (1 << 23) || max_blocks > (1 << 27))
+    return fail(SDX_EUNSUPPORTED, "sdx_fork_block_tables: more than 2^23 rows or 2^27 blocks");
+  if (batch == 0) return SDX_OK;
+  if (out == block_table)
+    return fail(SDX_EINVAL, "sdx_fork_block_tables: the new tables may not lie over the old ones");
+  const size_t need = sdx_fork_block_tables_workspace(batch);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < need)
+    return fail(SDX_EWORKSPACE, "sdx_fork_block_tables: needs a 16-byte aligned workspace of %zu bytes "
+                                "(got %zu)", need, workspace_bytes);
+  sdx::ForkArgs a{block_table, kv_len, parent, room, free_blocks, num_free, old_batch, batch, max_blocks,
+                  block_size, max_free, (int32_t*)workspace, out, copies, used, error};
+  return hip_status(sdx::launch_fork_tables(a, (hipStream_t)stream), "fork_tables");
+}
+
+int sdx_copy_pages(void* pool, int64_t layer_stride, int64_t side_stride, int dtype, int32_t layers,
+                   int64_t row_elems, int64_t num_blocks, int32_t block_size, const int32_t* copies,
+                   int64_t n, int32_t* error, sdx_stream_t stream) {
+  const int rc = pool_args("sdx_copy_pages", pool, layer_stride, side_stride, dtype, layers, row_elems,
+                           num_blocks, block_size);
+  if (rc != SDX_OK) return rc;
+  if (n < 0 || (n > 0 && !copies)) return fail(SDX_EINVAL, "sdx_copy_pages: bad arguments");
+  if (n > (1 << 23)) return fail(SDX_EUNSUPPORTED, "sdx_copy_pages: more than 2^23 copies");
+  if (n == 0) return SDX_OK;
+  const int64_t es = (int64_t)dsize(dtype);
+  sdx::CopyPagesArgs a{(uint8_t*)pool, layer_stride * es, side_stride * es, row_elems * es, num_blocks,
+                       block_size, copies, n, layers, error};
+  return hip_status(sdx::launch_copy_pages(a, (hipStream_t)stream), "copy_pages");
 }
 
 // ------------------------------------------------------------------ verify attention

@@ -553,4 +553,85 @@ int prefix_attn_parts(int64_t tokens, int32_t hq, int32_t hkv, int32_t d);
 int64_t prefix_attn_entries(int64_t tokens, int64_t batch, int64_t groups, int32_t group, int32_t parts);
 hipError_t launch_prefix_attn(int dtype, int d, const PrefixAttnArgs& a, hipStream_t s);
 
+// sdx_tree.hip: trees of drafted tokens
+constexpr int TREE_MAX_NODES = 512;  // of a row
+struct TreeLayoutArgs {
+  const int32_t* parents;       // [tokens] index in the row, below the node's own; -1: a root
+  const int64_t* cu_q;          // [batch + 1] node offsets
+  const int64_t* kv_len;        // [batch] keys per row, the nodes included
+  const int32_t* table;         // [batch, max_blocks], or null: no slots
+  int64_t batch, tokens, max_blocks, bs, padding_slot;
+  int32_t words;                // 64-bit words of a node's mask
+  int64_t* mask;                // [tokens, words]
+  int64_t* positions;           // [tokens]
+  int64_t* slots;               // [tokens], or null
+  int32_t* error;
+};
+hipError_t launch_tree_layout(const TreeLayoutArgs& a, hipStream_t s);
+struct TreeAcceptArgs {
+  const int64_t* token_ids;     // [tokens] the nodes' tokens
+  const int32_t* parents;
+  const int64_t* choice;        // [tokens] the target's token behind each node
+  const int64_t* cu_q;
+  const uint8_t* active;        // [batch] or null
+  int64_t batch, tokens, max_path;
+  int64_t* path;                // [batch, max_path]
+  int64_t* keep;                // [batch]
+  int64_t* y;
+  int32_t* error;
+};
+hipError_t launch_tree_accept(const TreeAcceptArgs& a, hipStream_t s);
+
+// sdx_pages.hip
+struct CompactArgs {
+  uint8_t* pool;                // (layer, side) at layer * layer_bytes + side * side_bytes
+  int64_t layer_bytes, side_bytes, row_bytes, num_blocks;
+  const int32_t* table;         // [batch, max_blocks]
+  const int64_t* start;         // [batch] position of the row's first node
+  const int64_t* path;          // [batch, max_path] ascending nodes
+  const int64_t* keep;          // [batch]
+  int64_t batch, max_blocks, bs, max_path;
+  int32_t layers;
+  int32_t* error;
+};
+hipError_t launch_compact_paged(const CompactArgs& a, hipStream_t s);
+constexpr int FREE_RANGE = 1 << 18;  // pages whose bits fit a workgroup's LDS
+struct FreePagesArgs {
+  const int32_t* table;         // [batch, max_blocks]
+  const int64_t* kv_len;        // [batch], or null: every page >= 0 is held
+  int64_t batch, max_blocks, bs, num_blocks;
+  int32_t parts;
+  int64_t words;                // of 32 pages
+  uint32_t* bits;               // [parts, words]
+  int32_t* free_blocks;         // [num_blocks]
+  int64_t* num_free;
+  int32_t* error;
+};
+int free_pages_parts(int64_t entries);
+hipError_t launch_free_pages(const FreePagesArgs& a, hipStream_t s);
+struct ForkArgs {
+  const int32_t* table;         // [old_batch, max_blocks]
+  const int64_t* kv_len;        // [old_batch]
+  const int64_t* parent;        // [batch] old row, or -1
+  const int64_t* room;          // [batch] tokens that the new row's pages hold
+  const int32_t* free_blocks;   // [max_free], of which num_free (null: all)
+  const int64_t* num_free;
+  int64_t old_batch, batch, max_blocks, bs, max_free;
+  int32_t* own;                 // [batch] pages taken, and flags
+  int32_t* out;                 // [batch, max_blocks]
+  int32_t* copies;              // [3, batch]
+  int64_t* used;
+  int32_t* error;
+};
+hipError_t launch_fork_tables(const ForkArgs& a, hipStream_t s);
+struct CopyPagesArgs {
+  uint8_t* pool;
+  int64_t layer_bytes, side_bytes, row_bytes, num_blocks, bs;
+  const int32_t* copies;        // [3, n] page, page, tokens
+  int64_t n;
+  int32_t layers;
+  int32_t* error;
+};
+hipError_t launch_copy_pages(const CopyPagesArgs& a, hipStream_t s);
+
 }  // namespace sdx

@@ -1,0 +1,336 @@
+// Pages of the paged cache after a step: the accepted nodes of a tree moved together behind
+// their row, rows that go on from other rows, the pages that no row holds, and copies of pages.
+// Nothing is counted up and down between calls: a page is free when no table holds it. The pool
+// is the one of the paged append (vllm_draft_spec/proposer.py:18-22); without a counterpart in
+// the reference, which leaves tables to a host-side manager and drafts chains.
+#include <algorithm>
+
+#include "sdx_launch.hpp"
+
+namespace sdx {
+
+constexpr int PGS_NT = 256;
+constexpr int PGS_UN = 4;
+
+__device__ __forceinline__ uint8_t* pgs_side(uint8_t* pool, int64_t layer_bytes, int64_t side_bytes,
+                                             int64_t ls) {
+  return pool + ls / 2 * layer_bytes + ls % 2 * side_bytes;
+}
+
+// ---- compact: row b's tokens start + path[i] to start + i for i < keep, ascending. A thread
+// moves a 16-byte column of them: path ascends from 0 or more, so path[i] >= i and no token is
+// overwritten before the same thread has read it. A workgroup does CP_LS (layer, side) pairs of
+// a row; the slots are worked out once and lie in LDS, and tokens that stay are left out.
+constexpr int CP_PATH = TREE_MAX_NODES;
+constexpr int CP_LS = 8;
+
+__global__ void __launch_bounds__(PGS_NT) compact_paged_kernel(CompactArgs a) {
+  __shared__ int64_t sFrom[CP_PATH], sTo[CP_PATH];
+  __shared__ int sN;
+  const int tid = threadIdx.x;
+  const int64_t b = blockIdx.x;
+  const int64_t keep = a.keep[b], start = a.start[b];
+  const int64_t* const path = a.path + b * a.max_path;
+  const int32_t* const table = a.table + b * a.max_blocks;
+  int bad = keep < 0 || keep > a.max_path || start < 0 || start > a.max_blocks * a.bs;
+  if (!bad && keep == 0) return;  // uniform
+  int stay = 0;  // (the row's first tokens stay: path ascends)
+  if (!bad) {
+    auto slot = [&](int64_t pos) -> int64_t {
+      if (pos >= a.max_blocks * a.bs) return -1;
+      const int64_t page = table[pos / a.bs];
+      return page < 0 || page >= a.num_blocks ? -1 : page * a.bs + pos % a.bs;
+    };
+    for (int64_t i = tid; i < keep; i += PGS_NT) {
+      const int64_t p = path[i], before = i > 0 ? path[i - 1] : -1;
+      bad |= p <= before || p > a.max_blocks * a.bs;
+      if (bad) break;
+      const int64_t from = slot(start + p), to = slot(start + i);
+      bad |= from < 0 || to < 0;
+      sFrom[i] = from * a.row_bytes;
+      sTo[i] = to * a.row_bytes;
+      stay += p == i;
+    }
+  }
+  if (tid == 0) sN = 0;
+  if (__syncthreads_or(bad)) {
+    if (tid == 0 && a.error) *a.error = 1;
+    return;
+  }
+  if (stay) atomicAdd(&sN, stay);
+  __syncthreads();
+  const int i0 = sN;
+  const uint32_t upr = (uint32_t)(a.row_bytes / 16);
+  const int ls0 = (int)blockIdx.y * CP_LS, sides = min(CP_LS, 2 * a.layers - ls0);
+  for (uint32_t u = tid; u < sides * upr; u += PGS_NT) {
+    const uint32_t ls = u / upr;
+    uint8_t* const at = pgs_side(a.pool, a.layer_bytes, a.side_bytes, ls0 + ls) + (int64_t)(u - ls * upr) * 16;
+    for (int64_t i = i0; i < keep; i += PGS_UN) {
+      uint4 v[PGS_UN];
+#pragma unroll
+      for (int k = 0; k < PGS_UN; ++k)
+        if (i + k < keep) v[k] = *reinterpret_cast<const uint4*>(at + sFrom[i + k]);
+#pragma unroll
+      for (int k = 0; k < PGS_UN; ++k)
+        if (i + k < keep) *reinterpret_cast<uint4*>(at + sTo[i + k]) = v[k];
+    }
+  }
+}
+
+// ---- the pages that no table holds. FP_RANGE pages' bits fit a workgroup's LDS; `parts`
+// workgroups go through a share of the tables each and leave their bits, the second kernel
+// joins them and lists the pages whose bit is clear, by ascending id.
+constexpr int FP_NT = 512;
+constexpr int FP_SEG = 8192;  // pages that a workgroup of the second kernel lists
+
+__global__ void __launch_bounds__(FP_NT) free_pages_mark_kernel(FreePagesArgs a) {
+  __shared__ uint32_t sBits[FREE_RANGE / 32];
+  const int tid = threadIdx.x;
+  const int64_t base = (int64_t)blockIdx.x * FREE_RANGE;
+  const int words = (int)((min((int64_t)FREE_RANGE, a.num_blocks - base) + 31) / 32);
+  for (int w = tid; w < words; w += FP_NT) sBits[w] = 0;
+  __syncthreads();
+  const uint32_t n = (uint32_t)(a.batch * a.max_blocks), each = (n + a.parts - 1) / a.parts;
+  const uint32_t e0 = min(n, blockIdx.y * each), e1 = min(n, e0 + each), mb = (uint32_t)a.max_blocks;
+  int bad = 0;
+  for (uint32_t e = e0 + tid; e < e1; e += FP_NT) {
+    const int32_t page = a.table[e];
+    bool held = page >= 0;
+    if (a.kv_len) {
+      const uint32_t b = e / mb;
+      const int64_t kv = a.kv_len[b];
+      held = (int64_t)(e - b * mb) * a.bs < kv;
+      bad |= kv < 0 || kv > a.max_blocks * a.bs;
+    }
+    if (!held) continue;
+    const int64_t x = (int64_t)page - base;
+    if (page < 0 || page >= a.num_blocks) bad = 1;
+    else if (x >= 0 && x < FREE_RANGE) atomicOr(&sBits[x / 32], 1u << (x % 32));
+  }
+  if (bad && a.error) *a.error = 1;
+  __syncthreads();
+  uint32_t* const out = a.bits + (int64_t)blockIdx.y * a.words + base / 32;
+  for (int w = tid; w < words; w += FP_NT) out[w] = sBits[w];
+}
+
+__global__ void __launch_bounds__(FP_NT) free_pages_list_kernel(FreePagesArgs a) {
+  constexpr int SW = FP_SEG / 32, NW = FP_NT / kWave;
+  static_assert(SW <= FP_NT, "a word per thread");
+  __shared__ uint32_t sFree[SW], sAt[SW], sWave[NW];
+  __shared__ uint64_t sSum[NW][2];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wv = tid / kWave;
+  const int64_t w0 = (int64_t)blockIdx.x * SW;
+  // free pages of word w
+  auto word = [&](int64_t w) {
+    uint32_t held = 0;
+    for (int p = 0; p < a.parts; ++p) held |= a.bits[p * a.words + w];
+    const int64_t left = a.num_blocks - w * 32;
+    return ~held & (left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1u);
+  };
+  uint64_t before = 0, total = 0;
+  for (int64_t w = tid; w < a.words; w += FP_NT) {
+    const uint32_t n = (uint32_t)__popc(word(w));
+    total += n;
+    if (w < w0) before += n;
+  }
+  const uint32_t mine = tid < SW && w0 + tid < a.words ? word(w0 + tid) : 0u;
+  const uint32_t n = (uint32_t)__popc(mine);
+  const uint32_t inc = wave_incl_scan_u32(n, lane);
+  total = wave_sum_u64(total);
+  before = wave_sum_u64(before);
+  if (lane == kWave - 1) {
+    sWave[wv] = inc;
+    sSum[wv][0] = total, sSum[wv][1] = before;
+  }
+  __syncthreads();
+  uint32_t at = inc - n;
+  total = before = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    if (w < wv) at += sWave[w];
+    total += sSum[w][0], before += sSum[w][1];
+  }
+  if (tid < SW) sFree[tid] = mine, sAt[tid] = at;
+  __syncthreads();
+  if (blockIdx.x == 0 && tid == 0) *a.num_free = (int64_t)total;
+  const int64_t end = min(a.num_blocks, (w0 + SW) * 32);
+  for (int64_t x = w0 * 32 + tid; x < end; x += FP_NT) {
+    const int i = (int)(x - w0 * 32);
+    const uint32_t bits = sFree[i / 32], bit = 1u << (i % 32);
+    if (bits & bit) a.free_blocks[before + sAt[i / 32] + __popc(bits & (bit - 1))] = (int32_t)x;
+    if (x >= (int64_t)total) a.free_blocks[x] = -1;
+  }
+}
+
+// ---- tables of rows that go on from others. Row i goes on from row p = parent[i] of the old
+// table: it shares p's whole pages; p's last page, filled in part, goes to one row alone, the
+// first that goes on in it while none holds it whole, and the others get copies.
+struct FkRow {
+  int64_t p, len, whole, part;  // parent (-1: none), its tokens, whole pages, tokens behind them
+  bool ok;
+};
+__device__ __forceinline__ FkRow fk_row(const ForkArgs& a, int64_t i) {
+  FkRow r{a.parent[i], 0, 0, 0, true};
+  if (r.p < 0) {
+    r.ok = r.p == -1;
+    return r;
+  }
+  if (r.p >= a.old_batch) {
+    r.ok = false;
+    return r;
+  }
+  r.len = a.kv_len[r.p];
+  r.ok = r.len >= 0 && r.len <= a.max_blocks * a.bs;
+  if (r.ok) {
+    r.whole = r.len / a.bs;
+    r.part = r.len - r.whole * a.bs;
+  }
+  return r;
+}
+
+// a wave per new row: its own pages in own[i], and whether it copies its first
+constexpr int32_t FK_COPY = 1 << 30, FK_BAD = (int32_t)0x80000000;
+__global__ void __launch_bounds__(PGS_NT) fork_rows_kernel(ForkArgs a) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const int64_t i = (int64_t)blockIdx.x * (PGS_NT / kWave) + threadIdx.x / kWave;
+  if (i >= a.batch) return;  // uniform per wave
+  const FkRow r = fk_row(a, i);
+  const int64_t room = a.room[i];
+  bool ok = r.ok && room >= r.len && room <= a.max_blocks * a.bs;
+  bool copy = false;
+  if (ok && r.part > 0) {  // uniform
+    const int32_t page = a.table[r.p * a.max_blocks + r.whole];
+    ok = page >= 0;
+    int other = 0;
+    for (int64_t j = lane; ok && j < a.batch; j += kWave) {
+      const FkRow o = fk_row(a, j);
+      const bool holds = j != i && o.ok && o.p >= 0 &&
+                         (o.whole > r.whole || (o.whole == r.whole && o.part > 0 && j < i));
+      other |= holds && a.table[o.p * a.max_blocks + r.whole] == page;
+    }
+    copy = __any(other);
+  }
+  int hole = 0;
+  for (int64_t c = lane; ok && c < r.whole; c += kWave) hole |= a.table[r.p * a.max_blocks + c] < 0;
+  ok = ok && !__any(hole);
+  if (lane == 0) {
+    const int64_t kept = r.whole + (r.part > 0 && !copy), need = ok ? (room + a.bs - 1) / a.bs : 0;
+    a.own[i] = ok ? (int32_t)(need - kept) | (copy ? FK_COPY : 0) : FK_BAD;
+  }
+}
+
+__global__ void __launch_bounds__(PGS_NT) fork_tables_kernel(ForkArgs a) {
+  constexpr int NW = PGS_NT / kWave;
+  __shared__ uint64_t sSum[NW][2];
+  const int tid = threadIdx.x;
+  const int64_t i = blockIdx.x;
+  uint64_t total = 0, before = 0;
+  int bad = 0;
+  for (int64_t j = tid; j < a.batch; j += PGS_NT) {
+    const int32_t x = a.own[j];
+    bad |= x < 0;
+    const uint64_t n = (uint32_t)x & (FK_COPY - 1);
+    total += n;
+    if (j < i) before += n;
+  }
+  total = wave_sum_u64(total);
+  before = wave_sum_u64(before);
+  if ((tid & (kWave - 1)) == 0) sSum[tid / kWave][0] = total, sSum[tid / kWave][1] = before;
+  bad = __syncthreads_or(bad);
+  total = before = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) total += sSum[w][0], before += sSum[w][1];
+  const int64_t have = a.num_free ? min(*a.num_free, a.max_free) : a.max_free;
+  bad |= (int64_t)total > have;
+  const FkRow r = fk_row(a, i);
+  const int32_t x = a.own[i];
+  const bool copy = x & FK_COPY;
+  const int64_t kept = r.whole + (r.part > 0 && !copy), end = kept + (x & (FK_COPY - 1));
+  if (tid == 0) {
+    if (i == 0) {
+      *a.used = bad ? 0 : (int64_t)total;
+      if (bad && a.error) *a.error = 1;
+    }
+    const bool c = !bad && copy;
+    a.copies[i] = c ? a.table[r.p * a.max_blocks + r.whole] : -1;
+    a.copies[a.batch + i] = c ? a.free_blocks[before] : -1;
+    a.copies[2 * a.batch + i] = c ? (int32_t)r.part : 0;
+  }
+  int32_t* const out = a.out + i * a.max_blocks;
+  for (int64_t c = tid; c < a.max_blocks; c += PGS_NT) {
+    int32_t v = -1;
+    if (!bad && c < end) v = c < kept ? a.table[r.p * a.max_blocks + c] : a.free_blocks[before + c - kept];
+    out[c] = v;
+  }
+}
+
+// ---- copies of pages: entry e's first tokens[e] tokens from page to page, in every layer and
+// side. They lie one behind another on both sides.
+constexpr int CY_LS = 8;
+__global__ void __launch_bounds__(PGS_NT) copy_pages_kernel(CopyPagesArgs a) {
+  const int64_t e = blockIdx.x;
+  const int32_t from = a.copies[e], to = a.copies[a.n + e], tokens = a.copies[2 * a.n + e];
+  if (from < 0 || to < 0 || tokens == 0) return;  // uniform
+  if (from >= a.num_blocks || to >= a.num_blocks || tokens < 0 || tokens > a.bs) {
+    if (threadIdx.x == 0 && a.error) *a.error = 1;
+    return;
+  }
+  const int64_t page = a.bs * a.row_bytes;
+  const uint32_t upr = (uint32_t)(tokens * (a.row_bytes / 16));
+  const int ls0 = (int)blockIdx.y * CY_LS, sides = min(CY_LS, 2 * a.layers - ls0);
+  for (uint32_t u0 = threadIdx.x; u0 < sides * upr; u0 += PGS_NT * PGS_UN) {
+    uint4 v[PGS_UN];
+    uint8_t* dst[PGS_UN];
+#pragma unroll
+    for (int k = 0; k < PGS_UN; ++k) {
+      const uint32_t u = u0 + k * PGS_NT;
+      dst[k] = nullptr;
+      if (u >= sides * upr) continue;
+      const uint32_t ls = u / upr;
+      uint8_t* const at = pgs_side(a.pool, a.layer_bytes, a.side_bytes, ls0 + ls) + (int64_t)(u - ls * upr) * 16;
+      v[k] = *reinterpret_cast<const uint4*>(at + from * page);
+      dst[k] = at + to * page;
+    }
+#pragma unroll
+    for (int k = 0; k < PGS_UN; ++k)
+      if (dst[k]) *reinterpret_cast<uint4*>(dst[k]) = v[k];
+  }
+}
+
+// ---------------------------------------------------------------- launches
+hipError_t launch_compact_paged(const CompactArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)a.batch, (unsigned)((2 * a.layers + CP_LS - 1) / CP_LS));
+  hipLaunchKernelGGL(compact_paged_kernel, grid, dim3(PGS_NT), 0, s, a);
+  return hipGetLastError();
+}
+
+int free_pages_parts(int64_t entries) {  // a workgroup for every 4,096 entries
+  return (int)std::max<int64_t>(1, std::min<int64_t>(64, entries / 4096));
+}
+
+hipError_t launch_free_pages(const FreePagesArgs& a, hipStream_t s) {
+  const unsigned ranges = (unsigned)((a.num_blocks + FREE_RANGE - 1) / FREE_RANGE);
+  hipLaunchKernelGGL(free_pages_mark_kernel, dim3(ranges, (unsigned)a.parts), dim3(FP_NT), 0, s, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(free_pages_list_kernel, dim3((unsigned)((a.num_blocks + FP_SEG - 1) / FP_SEG)),
+                     dim3(FP_NT), 0, s, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_fork_tables(const ForkArgs& a, hipStream_t s) {
+  constexpr int rows = PGS_NT / kWave;
+  hipLaunchKernelGGL(fork_rows_kernel, dim3((unsigned)((a.batch + rows - 1) / rows)), dim3(PGS_NT), 0, s, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(fork_tables_kernel, dim3((unsigned)a.batch), dim3(PGS_NT), 0, s, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_copy_pages(const CopyPagesArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)a.n, (unsigned)((2 * a.layers + CY_LS - 1) / CY_LS));
+  hipLaunchKernelGGL(copy_pages_kernel, grid, dim3(PGS_NT), 0, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace sdx

@@ -77,6 +77,14 @@ _SIGS = {
     "sdx_build_block_tables": (INT, [P, I64, P, I64, I32, I64, P, P, I64, P, P, P, P]),
     "sdx_paged_slot_mapping": (INT, [P, I64, I64, P, P, I32, I64, I64, P, P, P, P]),
     "sdx_append_slots": (INT, [P, I64, I64, P, INT, I32, I64, I64, I64, P, P, P]),
+    "sdx_tree_layout": (INT, [P, I64, P, P, I32, P, I64, I32, I64, I64, P, P, P, P, P]),
+    "sdx_tree_accept": (INT, [P, P, P, I64, P, I64, P, I64, P, P, P, P, P]),
+    "sdx_compact_paged": (INT, [P, I64, I64, INT, I32, I64, I64, I32, P, I64, I64, P, P, I64, P, P, P]),
+    "sdx_free_pages": (INT, [P, I64, I64, P, I32, I64, P, P, P, SZ, P, P]),
+    "sdx_free_pages_workspace": (SZ, [I64, I64, I64]),
+    "sdx_fork_block_tables": (INT, [P, I64, I64, P, P, P, I64, I32, P, I64, P, P, P, P, P, SZ, P, P]),
+    "sdx_fork_block_tables_workspace": (SZ, [I64]),
+    "sdx_copy_pages": (INT, [P, I64, I64, INT, I32, I64, I64, I32, P, I64, P, P]),
     "sdx_verify_attention_paged": (INT, [P, INT, I64, P, I32, I32, I32, I32, P, P, I64, I32, P,
                                          I64, P, F, I32, P, SZ, P, P, P]),
     "sdx_prefix_attention_paged": (INT, [P, INT, I64, I64, P, I32, I32, I32, P, P, I64, I32, P,

@@ -17,6 +17,10 @@ and rolls back by per-row counts without touching K/V bytes.
 pages that the rows of a group share; `paged_slot_mapping` gives the positions
 and slots of a step's packed new tokens (the slot formula of `proposer.py:295-314`
 at a different count per row); `append_paged_slots` writes their K/V there.
+
+After a step, `compact_paged` moves the accepted nodes of a tree together; `fork_block_tables`
+lays out rows that go on from others, sharing their whole pages, with the page copies that
+`copy_pages` makes; `free_page_list` gives the pages that no row holds any more.
 """
 import torch
 
@@ -28,7 +32,7 @@ except Exception:  # pragma: no cover - transformers absent
     _HFCache, _HFLayer = object, object
 
 __all__ = ["RaggedCache", "PagedKVCache", "build_block_tables", "paged_slot_mapping",
-           "append_paged_slots"]
+           "append_paged_slots", "compact_paged", "free_page_list", "fork_block_tables", "copy_pages"]
 
 
 class _RaggedLayer(_HFLayer):
@@ -306,6 +310,13 @@ class PagedKVCache:
                                        _lib.stream_of(self.lengths))
         _lib.check(rc, "PagedKVCache.commit")
 
+    def compact(self, path, keep):
+        """Keep a tree's accepted nodes (path [B, P], keep [B] of `specdec.tree.tree_accept`), which
+        were appended from lengths[b] on: moves them together (`compact_paged`) and adds keep to the
+        lengths."""
+        compact_paged(self.pool, self.block_table, self.lengths, path, keep, error=self.error)
+        self.lengths += keep
+
     def rollback(self, n):
         """lengths -= n (device [B] int64); all-or-nothing, `error` set if any row
         would go negative (`kvcache.py:174-190`)."""
@@ -431,3 +442,149 @@ def append_paged_slots(pool, staged, slots, error=None):
             _lib.ptr(pool), 2 * side, side, _lib.ptr(st), _lib.dtype_code(pool), L, T, re, nb * bs,
             _lib.ptr(sl), _lib.ptr(error), _lib.stream_of(pool))
     _lib.check(rc, "append_paged_slots")
+
+
+def _pool_shape(pool):
+    if pool.dim() != 5 or pool.shape[1] != 2 or not pool.is_contiguous():
+        raise ValueError("pool must be a contiguous [L, 2, num_blocks, block_size, row_elems]")
+    L, _, nb, bs, re = pool.shape
+    return L, nb, bs, re, nb * bs * re
+
+
+def _table(block_table, what="block_table"):
+    if block_table.dim() != 2:
+        raise ValueError(f"{what} must be [B, max_blocks], got {tuple(block_table.shape)}")
+    return _lib.as_dtype(block_table, torch.int32)
+
+
+def compact_paged(pool, block_table, kv_start, path, keep, error=None):
+    """Move the K/V of a tree's accepted nodes together, in every layer and side of pool [L, 2,
+    num_blocks, block_size, row_elems] (contiguous; in place).
+
+    Row b's token at position kv_start[b] + path[b, i] goes to kv_start[b] + i for i < keep[b]
+    (kv_start, keep [B], path [B, P] int64, P at most 512, ascending in every row as
+    `specdec.tree.tree_accept` gives it). Rows whose path, lengths or pages are out of range are
+    left as they are and set `error` (an int32 [1] device tensor) when given. Rows must not share
+    the pages behind kv_start.
+    """
+    _lib.one_gpu(pool, block_table, kv_start, path, keep, error)
+    _error_word(error)
+    L, nb, bs, re, side = _pool_shape(pool)
+    bt = _table(block_table)
+    B = bt.shape[0]
+    if path.dim() != 2 or path.shape[0] != B or kv_start.numel() != B or keep.numel() != B:
+        raise ValueError(f"block_table of {B} rows needs kv_start [{B}], path [{B}, P] and keep [{B}], got "
+                         f"{kv_start.numel()}, {tuple(path.shape)} and {keep.numel()}")
+    st, pt, kp = (_lib.as_dtype(t, torch.int64) for t in (kv_start, path, keep))
+    if B == 0 or pt.shape[1] == 0:
+        return
+    with _lib.on_device(pool):
+        rc = _lib.lib().sdx_compact_paged(
+            _lib.ptr(pool), 2 * side, side, _lib.dtype_code(pool), L, re, nb, bs, _lib.ptr(bt), B,
+            bt.shape[1], _lib.ptr(st), _lib.ptr(pt), pt.shape[1], _lib.ptr(kp), _lib.ptr(error),
+            _lib.stream_of(pool))
+    _lib.check(rc, "compact_paged")
+
+
+def free_page_list(block_table, num_blocks, kv_len=None, block_size=None, error=None):
+    """The pages that no row holds, on the device.
+
+    Row b of block_table [B, max_blocks] int32 holds the pages of its kv_len[b] (int64) tokens of
+    block_size each, or without kv_len every entry that is not negative; any number of rows may
+    hold a page. Returns (free_blocks [num_blocks] int32, ids ascending and -1 behind the last;
+    num_free [1] int64). Held pages outside [0, num_blocks) and lengths out of range set `error`
+    (an int32 [1] device tensor) when given.
+    """
+    _lib.one_gpu(block_table, kv_len, error)
+    _error_word(error)
+    bt, num_blocks = _table(block_table), int(num_blocks)
+    if (kv_len is None) != (block_size is None):
+        raise ValueError("kv_len and block_size go together")
+    B, mb = bt.shape
+    kl = None
+    if kv_len is not None:
+        kl = _lib.as_dtype(kv_len, torch.int64)
+        if kl.numel() != B:
+            raise ValueError(f"kv_len must be [{B}], got {kl.numel()}")
+    if num_blocks < 1:
+        raise ValueError(f"num_blocks must be positive, got {num_blocks}")
+    free = torch.empty(num_blocks, dtype=torch.int32, device=bt.device)
+    num = torch.empty(1, dtype=torch.int64, device=bt.device)
+    with _lib.on_device(bt):
+        need = _lib.workspace_bytes("sdx_free_pages_workspace", B, max(mb, 1), num_blocks)
+        ws = _lib.cached_workspace(need, bt.device, "free_pages")
+        rc = _lib.lib().sdx_free_pages(
+            _lib.ptr(bt), B if mb else 0, max(mb, 1), _lib.ptr(kl), 1 if block_size is None else
+            int(block_size), num_blocks, _lib.ptr(free), _lib.ptr(num), _lib.ptr(ws), ws.numel(),
+            _lib.ptr(error), _lib.stream_of(bt))
+    _lib.check(rc, "free_page_list")
+    return free, num
+
+
+def fork_block_tables(block_table, kv_len, parent, room, free_blocks, block_size, num_free=None,
+                      out=None, error=None):
+    """Block tables of rows that go on from others, on the device: answers that branch, beams that
+    are reordered, rows that end or need more pages.
+
+    New row i goes on from row parent[i] (int64 [N]; -1: an empty row) of block_table [B,
+    max_blocks] int32 with its kv_len (int64 [B]) tokens, and gets pages for room[i] (int64 [N], no
+    less) tokens. It shares the old row's whole pages; a last page filled in part goes to the first
+    new row that goes on in it, unless another holds it whole, and the others get a new page and
+    an entry in copies. New pages are free_blocks (int32) in order, the first num_free (int64 [1] on
+    the device; None: all) of them, as `free_page_list` gives both. Returns (table [N, max_blocks] int32,
+    -1 behind a row's last page; copies [3, N] int32 for `copy_pages`; used [1] int64, the pages
+    taken). All or nothing: parents, lengths, pages or free pages that do not fit give a table of
+    -1, no copies and used 0, and set `error` (an int32 [1] device tensor) when given.
+    """
+    _lib.one_gpu(block_table, kv_len, parent, room, free_blocks, num_free, out, error)
+    _error_word(error)
+    bt = _table(block_table)
+    B, mb = bt.shape
+    kl, pa, ro = (_lib.as_dtype(t, torch.int64) for t in (kv_len, parent, room))
+    fb = _lib.as_dtype(free_blocks, torch.int32)
+    nf = None if num_free is None else _lib.as_dtype(num_free, torch.int64)
+    N = pa.numel()
+    if kl.numel() != B or ro.numel() != N or (nf is not None and nf.numel() != 1):
+        raise ValueError(f"block_table of {B} rows needs kv_len [{B}], {N} parents room [{N}] and num_free "
+                         f"[1], got {kl.numel()} and {ro.numel()}")
+    if out is None:
+        out = torch.empty((N, mb), dtype=torch.int32, device=bt.device)
+    elif out.dtype != torch.int32 or tuple(out.shape) != (N, mb) or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous int32 [{N}, {mb}]")
+    a0, b0 = out.data_ptr(), bt.data_ptr()
+    if a0 < b0 + bt.numel() * 4 and b0 < a0 + out.numel() * 4:
+        raise ValueError("out may not lie over block_table: rows read each other's entries")
+    copies = torch.empty((3, N), dtype=torch.int32, device=bt.device)
+    if N == 0:
+        return out, copies, torch.zeros(1, dtype=torch.int64, device=bt.device)
+    used = torch.empty(1, dtype=torch.int64, device=bt.device)
+    with _lib.on_device(bt):
+        need = _lib.workspace_bytes("sdx_fork_block_tables_workspace", N)
+        ws = _lib.cached_workspace(need, bt.device, "fork_tables")
+        rc = _lib.lib().sdx_fork_block_tables(
+            _lib.ptr(bt), B, mb, _lib.ptr(kl), _lib.ptr(pa), _lib.ptr(ro), N, int(block_size),
+            _lib.ptr(fb), fb.numel(), _lib.ptr(nf), _lib.ptr(out), _lib.ptr(copies), _lib.ptr(used),
+            _lib.ptr(ws), ws.numel(), _lib.ptr(error), _lib.stream_of(bt))
+    _lib.check(rc, "fork_block_tables")
+    return out, copies, used
+
+
+def copy_pages(pool, copies, error=None):
+    """Copy pages in every layer and side of pool [L, 2, num_blocks, block_size, row_elems]
+    (contiguous; in place): the first copies[2, e] tokens of page copies[0, e] to page copies[1, e]
+    (copies [3, N] int32, as `fork_block_tables` gives it). Entries with a negative page are skipped;
+    those out of range too, and set `error` (an int32 [1] device tensor) when given. A page that is the
+    target of two entries, or of one and the source of another, holds a mix."""
+    _lib.one_gpu(pool, copies, error)
+    _error_word(error)
+    L, nb, bs, re, side = _pool_shape(pool)
+    if copies.dim() != 2 or copies.shape[0] != 3:
+        raise ValueError(f"copies must be [3, N], got {tuple(copies.shape)}")
+    c = _lib.as_dtype(copies, torch.int32)
+    if c.shape[1] == 0:
+        return
+    with _lib.on_device(pool):
+        rc = _lib.lib().sdx_copy_pages(
+            _lib.ptr(pool), 2 * side, side, _lib.dtype_code(pool), L, re, nb, bs, _lib.ptr(c),
+            c.shape[1], _lib.ptr(error), _lib.stream_of(pool))
+    _lib.check(rc, "copy_pages")

@@ -415,6 +415,98 @@ int sdx_append_slots(void* pool, int64_t layer_stride, int64_t side_stride, cons
                      int64_t num_slots, const int64_t* slots, int32_t* error,
                      sdx_stream_t stream);
 
+/* ---- trees of drafted tokens ---------------------------------------------- */
+
+/* A tree drafts several continuations of a row at once. Row b's nodes are cu_q[b] .. cu_q[b+1] - 1
+ * of num_tokens packed ones (cu_q int64 [batch + 1] from 0), parents before their children:
+ * parents[t] int32 is the index in the row of t's parent, below t's own, or -1 for a root (a node
+ * that continues the row's cache itself; the row's pending token is one). The nodes' K/V lie in the
+ * cache in the order of the nodes, the last of the row's kv_len[b] keys: node i at position
+ * kv_len[b] - n_b + i of the cache.
+ *
+ * sdx_tree_layout writes for each node mask [num_tokens, ceil(max_nodes / 64)] int64, bit j % 64 of
+ * word j / 64 set where node j of the row is the node itself or an ancestor; positions (int64) =
+ * kv_len[b] - n_b + its depth, the position that its embedding or rotation goes by; and with a
+ * block_table [batch, max_blocks] int32 slots (int64) = the cache row that its K/V are appended to
+ * (both or neither null). Rows have up to max_nodes nodes, rounded up to a multiple of 64, 512 at
+ * most. The nodes of a row whose parents, lengths or offsets are out of range, and a slot whose page
+ * is negative, become padding (mask 0, position 0, slot padding_slot) and set *error (nullable);
+ * tokens behind the last row are padding without it. One kernel. No reference counterpart (the
+ * reference drafts chains). */
+int sdx_tree_layout(const int32_t* parents, int64_t batch, const int64_t* cu_q, const int64_t* kv_len,
+                    int32_t max_nodes, const int32_t* block_table, int64_t max_blocks,
+                    int32_t block_size, int64_t num_tokens, int64_t padding_slot, int64_t* mask,
+                    int64_t* positions, int64_t* slots, int32_t* error, sdx_stream_t stream);
+
+/* The walk of the accepted nodes: from node 0 of the row (its pending token) to the lowest child
+ * whose token is choice at the node, and on, as far as there is one and max_path (512 at most)
+ * allows. tokens, choice int64 [num_tokens]: the nodes' tokens, and the target's next token behind
+ * each node (its argmax, or a draw from its distribution: what comes out is then distributed as
+ * the target's own draws). path [batch, max_path] int64 = the nodes of the walk, -1 behind them;
+ * keep [batch] int64 = how many (at least 1); y [batch] int64 = choice at the last of them, which
+ * no kept node holds: the row's next pending token. A negative choice ends the walk with y -1.
+ * Rows without nodes, rows that are not active (uint8 [batch], nullable) and rows whose offsets are
+ * out of range keep 0 and have y -1; the last set *error (nullable). */
+int sdx_tree_accept(const int64_t* tokens, const int32_t* parents, const int64_t* choice, int64_t batch,
+                    const int64_t* cu_q, int64_t num_tokens, const uint8_t* active, int64_t max_path,
+                    int64_t* path, int64_t* keep, int64_t* y, int32_t* error, sdx_stream_t stream);
+
+/* ---- pages of the cache after a step ---------------------------------------- */
+
+/* Moves the K/V of a tree's accepted nodes together, in every layer and side of the pool (strides,
+ * element types and 16-byte rules as sdx_kv_append_paged): row b's token at position
+ * kv_start[b] + path[b, i] goes to kv_start[b] + i, for i < keep[b]. path [batch, max_path] int64
+ * (512 at most) ascends strictly from 0 or more, as sdx_tree_accept writes it; what lies behind
+ * keep[b] is not read. kv_start, keep int64 [batch]. A row whose path, lengths or pages are out of
+ * range is left as it is, all of it, and sets *error (nullable). Rows must not share the pages that
+ * are written. One kernel, in place. */
+int sdx_compact_paged(void* pool, int64_t layer_stride, int64_t side_stride, int dtype, int32_t layers,
+                      int64_t row_elems, int64_t num_blocks, int32_t block_size,
+                      const int32_t* block_table, int64_t batch, int64_t max_blocks,
+                      const int64_t* kv_start, const int64_t* path, int64_t max_path,
+                      const int64_t* keep, int32_t* error, sdx_stream_t stream);
+
+/* The pages that no row holds: free_blocks [num_blocks] int32 = their ids ascending, -1 behind the
+ * last; *num_free (int64) how many. Row b of block_table [batch, max_blocks] int32 holds the pages of
+ * its kv_len[b] (int64) tokens, ceil(kv_len[b] / block_size) entries, or without kv_len every entry
+ * that is not negative. Pages outside [0, num_blocks) among those, and lengths out of range, set
+ * *error (nullable). Any number of rows may hold a page: nothing is counted between calls, a row's
+ * pages are given back by leaving it out. Two kernels; `workspace` as the query says, 16-byte aligned,
+ * no initial contents. Up to 2^30 pages and 2^31 entries. */
+int sdx_free_pages(const int32_t* block_table, int64_t batch, int64_t max_blocks, const int64_t* kv_len,
+                   int32_t block_size, int64_t num_blocks, int32_t* free_blocks, int64_t* num_free,
+                   void* workspace, size_t workspace_bytes, int32_t* error, sdx_stream_t stream);
+size_t sdx_free_pages_workspace(int64_t batch, int64_t max_blocks, int64_t num_blocks);
+
+/* Block tables of rows that go on from others (answers that branch, beams that are reordered, rows
+ * that end or grow). Row i of the new tables out [batch, max_blocks] int32 goes on from row
+ * parent[i] (int64; -1: from none, an empty row) of block_table [old_batch, max_blocks] with its
+ * kv_len (int64 [old_batch]) tokens, and has pages for room[i] (int64) tokens, no less than those. It
+ * shares the old row's whole pages. A last page that is filled in part goes to the first new row that
+ * goes on in it, unless another new row holds it whole; every other takes a new page and an entry
+ * of copies [3, batch] int32: the page, the new page and the tokens to copy (-1, -1, 0: none), as
+ * sdx_copy_pages takes them. New pages come from free_blocks [max_free] int32, row after row, in order, the
+ * first *num_free (device int64; null: max_free) of them; *used (int64) = how many. out is written
+ * whole, -1 behind a row's last page, and may not lie over block_table. All or nothing: where a parent, a
+ * length, a page of an old row or the free pages are out of range, out and copies are -1 (tokens 0), *used 0
+ * and *error (nullable) 1. Two kernels; `workspace` as the query says. The time of a row's look at the
+ * others grows with the rows. Up to 2^23 rows and 2^27 columns. */
+int sdx_fork_block_tables(const int32_t* block_table, int64_t old_batch, int64_t max_blocks,
+                          const int64_t* kv_len, const int64_t* parent, const int64_t* room,
+                          int64_t batch, int32_t block_size, const int32_t* free_blocks,
+                          int64_t max_free, const int64_t* num_free, int32_t* out, int32_t* copies,
+                          int64_t* used, void* workspace, size_t workspace_bytes, int32_t* error,
+                          sdx_stream_t stream);
+size_t sdx_fork_block_tables_workspace(int64_t batch);
+
+/* Copies copies[2, e] tokens from the start of page copies[0, e] to page copies[1, e], in every layer
+ * and side of the pool, for e < n (copies int32 [3, n]); entries with a negative page are skipped, those with
+ * a page outside the pool or more tokens than a page has too, and those set *error (nullable). No page
+ * may be the target of two entries, or of one and the source of another: it would hold a mix. */
+int sdx_copy_pages(void* pool, int64_t layer_stride, int64_t side_stride, int dtype, int32_t layers,
+                   int64_t row_elems, int64_t num_blocks, int32_t block_size, const int32_t* copies,
+                   int64_t n, int32_t* error, sdx_stream_t stream);
+
 /* ---- verify attention: the target's multi-query attention of one verify
  * forward (bench/bench_engine.py:170-174 -> specdec/engine.py:273-275 through
  * HF SDPA with the mask of specdec/kvcache.py:138-162), one layer.

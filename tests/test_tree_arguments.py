@@ -1,0 +1,124 @@
+"""CPU checks of the refusals of the trees' and pages' entry points: the C ones return their status
+before anything is launched (the pointers are never dereferenced), the Python ones refuse CPU
+tensors; the oracles on cases worked by hand."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import tree as OT
+
+OK, EINVAL, EUNSUP, EWS = 0, -1, -2, -4
+F32, BF16 = 0, 1
+FAKE = ctypes.c_void_p(4096)
+OFF = ctypes.c_void_p(4104)
+
+
+def test_tree_statuses():
+    from specdec import _lib
+    L = _lib.lib()
+
+    def layout(B=2, nodes=26, table=FAKE, mb=4, bs=16, T=9, slots=FAKE, parents=FAKE, mask=FAKE):
+        return L.sdx_tree_layout(parents, B, FAKE, FAKE, nodes, table, mb, bs, T, -1, mask, FAKE, slots, None,
+                                 None)
+
+    assert layout(T=0) == OK
+    for bad in (dict(B=-1), dict(B=0), dict(nodes=0), dict(mb=0), dict(bs=0), dict(T=-1), dict(parents=None),
+                dict(mask=None), dict(slots=None), dict(table=None)):
+        assert layout(**bad) == EINVAL, bad
+    for bad in (dict(nodes=513), dict(B=1 << 24), dict(mb=1 << 32), dict(T=1 << 32)):
+        assert layout(**bad) == EUNSUP, bad
+
+    def accept(B=2, T=9, P=4, tokens=FAKE, path=FAKE):
+        return L.sdx_tree_accept(tokens, FAKE, FAKE, B, FAKE, T, None, P, path, FAKE, FAKE, None, None)
+
+    assert accept(B=0) == OK
+    for bad in (dict(B=-1), dict(T=-1), dict(P=0), dict(tokens=None), dict(path=None)):
+        assert accept(**bad) == EINVAL, bad
+    assert accept(P=513) == EUNSUP and accept(B=1 << 24) == EUNSUP
+
+
+def test_page_statuses():
+    from specdec import _lib
+    L = _lib.lib()
+
+    def compact(pool=FAKE, dtype=BF16, layers=2, re=64, nb=8, bs=16, table=FAKE, B=2, mb=4, P=4, stride=4096):
+        return L.sdx_compact_paged(pool, 2 * stride, stride, dtype, layers, re, nb, bs, table, B, mb, FAKE,
+                                   FAKE, P, FAKE, None, None)
+
+    def copy(pool=FAKE, dtype=BF16, layers=2, re=64, nb=8, bs=16, n=3, copies=FAKE, stride=4096):
+        return L.sdx_copy_pages(pool, 2 * stride, stride, dtype, layers, re, nb, bs, copies, n, None, None)
+
+    assert compact(B=0) == OK and copy(n=0) == OK
+    shared = (dict(pool=None), dict(dtype=5), dict(layers=0), dict(re=0), dict(re=4), dict(nb=0), dict(bs=0),
+              dict(pool=OFF), dict(stride=4100))
+    for bad in shared + (dict(table=None), dict(B=-1), dict(mb=0), dict(P=0)):
+        assert compact(**bad) == EINVAL, bad
+    for bad in shared + (dict(copies=None), dict(n=-1)):
+        assert copy(**bad) == EINVAL, bad
+    for bad in (dict(layers=40000), dict(re=1 << 30), dict(P=513), dict(B=1 << 24)):
+        assert compact(**bad) == EUNSUP, bad
+    assert copy(n=1 << 24) == EUNSUP and copy(re=1 << 30) == EUNSUP
+
+    def free(table=FAKE, B=2, mb=4, bs=16, nb=100, out=FAKE, ws=FAKE, nbytes=None):
+        need = L.sdx_free_pages_workspace(B, mb, nb)
+        return L.sdx_free_pages(table, B, mb, FAKE, bs, nb, out, FAKE, ws, need if nbytes is None else nbytes,
+                                None, None)
+
+    for bad in (dict(table=None), dict(B=-1), dict(mb=0), dict(bs=0), dict(nb=0), dict(out=None)):
+        assert free(**bad) == EINVAL, bad
+    assert free(nb=1 << 31) == EUNSUP and free(B=1 << 20, mb=1 << 20) == EUNSUP
+    assert L.sdx_free_pages_workspace(2, 4, 100) >= 16
+    assert free(nbytes=3) == EWS and free(ws=None) == EWS and free(ws=OFF) == EWS
+
+    def fork(table=FAKE, B=2, mb=4, N=3, bs=16, fb=FAKE, nf=8, out=ctypes.c_void_p(8192), copies=FAKE, ws=FAKE,
+             nbytes=None):
+        need = L.sdx_fork_block_tables_workspace(N)
+        return L.sdx_fork_block_tables(table, B, mb, FAKE, FAKE, FAKE, N, bs, fb, nf, None, out, copies, FAKE,
+                                       ws, need if nbytes is None else nbytes, None, None)
+
+    assert fork(N=0) == OK
+    for bad in (dict(table=None), dict(B=-1), dict(N=-1), dict(mb=0), dict(bs=0), dict(fb=None), dict(nf=-1),
+                dict(out=None), dict(copies=None), dict(out=FAKE)):
+        assert fork(**bad) == EINVAL, bad
+    assert fork(N=1 << 24) == EUNSUP and fork(mb=1 << 28) == EUNSUP
+    assert fork(nbytes=3) == EWS and fork(ws=None) == EWS
+
+
+def test_entry_points_refuse_cpu_tensors():
+    from specdec import kvcache as K
+    from specdec import tree as R
+    z, i = torch.zeros(2, dtype=torch.long), torch.zeros(2, dtype=torch.int32)
+    pool = torch.zeros(1, 2, 1, 1, 8)
+    for call in (lambda: R.tree_layout(i, z, z[:1]),
+                 lambda: R.tree_accept(z, i, z, z, 4),
+                 lambda: K.compact_paged(pool, i.view(1, 2), z[:1], z.view(1, 2), z[:1]),
+                 lambda: K.free_page_list(i.view(1, 2), 4),
+                 lambda: K.fork_block_tables(i.view(1, 2), z[:1], z, z, i, 16),
+                 lambda: K.copy_pages(pool, torch.zeros(3, 1, dtype=torch.int32))):
+        with pytest.raises(RuntimeError, match="ROCm device"):
+            call()
+
+
+def test_oracles_by_hand():
+    #      0          two children of the root, one of which has a child; a row of one node
+    #     / \.
+    #    1   2 - 3
+    parents, cu = [-1, 0, 0, 2, -1], [0, 4, 5]
+    table = np.array([[3, 1], [0, 2]])
+    sees, pos, slots, ok = OT.tree_layout(parents, cu, [18, 1], table, 16, 1, 6)
+    assert ok and sees == [{0}, {0, 1}, {0, 2}, {0, 2, 3}, {0}, set()]
+    assert pos.tolist() == [14, 15, 15, 16, 0, 0]
+    assert slots.tolist() == [3 * 16 + 14, 3 * 16 + 15, 16, 17, 0, -1]
+    path, keep, y = OT.tree_accept([9, 5, 7, 8, 4], parents, [7, 1, 8, 6, 2], cu, 4)
+    assert path.tolist() == [[0, 2, 3, -1], [0, -1, -1, -1]]
+    assert keep.tolist() == [3, 1] and y.tolist() == [6, 2]
+    pool = torch.arange(4 * 16.).view(1, 1, 4, 16, 1).expand(1, 2, 4, 16, 1).clone()
+    assert OT.compact(pool, table, [14, 0], path, keep)
+    assert pool[0, 0, 3, 14:, 0].tolist() == [62.0, 16.0] and pool[0, 0, 1, :2, 0].tolist() == [17.0, 17.0]
+    assert OT.free_pages(np.array([[1, 5], [1, -1]]), 6, [20, 3], 16) == ([0, 2, 3, 4], True)
+    # row 0 branches in two and row 1 ends: the branch takes a copy of 4 tokens of page 5
+    out, copies, used, ok = OT.fork(np.array([[1, 5], [2, -1]]), [20, 3], [0, 0, -1], [21, 32, 0], [7, 8], 16)
+    assert ok and used == 1 and out.tolist() == [[1, 5], [1, 7], [-1, -1]]
+    assert copies.tolist() == [[-1, 5, -1], [-1, 7, -1], [0, 4, 0]]
