@@ -956,6 +956,46 @@ int sdx_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t voca
   return hip_status(sdx::launch_logprob(dtype, a, (hipStream_t)stream), "logprob");
 }
 
+// ------------------------------------------------------------------ penalties
+int sdx_penalize_logits(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, void* out,
+                        int64_t out_ld, int64_t batch, const int64_t* cu_rows, const int64_t* history,
+                        int64_t history_ld, int64_t max_history, const int64_t* history_len,
+                        const int64_t* prompt_len, const float* repetition, const float* frequency,
+                        const float* presence, const int64_t* bias_ids, const float* bias,
+                        int32_t num_biases, const int32_t* allowed, int64_t allowed_ld,
+                        const int64_t* node_tokens, const int64_t* tree_mask, int32_t mask_words,
+                        int32_t* error, sdx_stream_t stream) {
+  if (rows < 0 || vocab < 1 || ld < vocab || out_ld < vocab || batch < 0 || !dtype_ok(dtype) ||
+      num_biases < 0 || max_history < 0 || mask_words < 0)
+    return fail(SDX_EINVAL, "sdx_penalize_logits: bad arguments");
+  if (rows == 0) return SDX_OK;
+  if (!logits || !out || (history && (!history_len || history_ld < max_history)) ||
+      (num_biases > 0 && (!bias_ids || !bias)) || (allowed && allowed_ld < (vocab + 31) / 32) ||
+      (tree_mask && (!node_tokens || mask_words < 1)) || batch == 0 || (!cu_rows && batch != rows))
+    return fail(SDX_EINVAL, "sdx_penalize_logits: bad arguments");
+  const size_t es = dsize(dtype);
+  if ((uintptr_t)logits % es || (uintptr_t)out % es)
+    return fail(SDX_EINVAL, "sdx_penalize_logits: logits and out must be aligned to their elements");
+  const char *l0 = (const char*)logits, *o0 = (const char*)out;
+  const size_t lb = ((size_t)(rows - 1) * ld + vocab) * es, ob = ((size_t)(rows - 1) * out_ld + vocab) * es;
+  if (l0 < o0 + ob && o0 < l0 + lb && !(l0 == o0 && ld == out_ld))
+    return fail(SDX_EINVAL, "sdx_penalize_logits: out may be the logits themselves or lie apart from them");
+  if (num_biases > sdx::PN_MAX_BIAS || (history && max_history > sdx::PN_HISTORY) || vocab > ((int64_t)1 << 30) ||
+      rows > ((int64_t)1 << 21))
+    return fail(SDX_EUNSUPPORTED, "sdx_penalize_logits: more than %d bias entries or %lld history tokens in a "
+                                  "row, 2^30 tokens or 2^21 rows", sdx::PN_MAX_BIAS, (long long)sdx::PN_HISTORY);
+  sdx::PenalizeArgs a = {};
+  a.logits = logits; a.out = out; a.rows = rows; a.V = vocab; a.ld = ld; a.out_ld = out_ld; a.batch = batch;
+  a.cu_rows = cu_rows; a.history = history; a.history_ld = history_ld; a.max_history = max_history;
+  a.history_len = history_len; a.prompt_len = prompt_len;
+  a.repetition = repetition; a.frequency = frequency; a.presence = presence;
+  a.bias_ids = bias_ids; a.bias = bias; a.biases = num_biases;
+  a.allowed = (const uint32_t*)allowed; a.allowed_ld = allowed_ld;
+  a.node_tokens = node_tokens; a.tree_mask = tree_mask; a.mask_words = mask_words; a.error = error;
+  a.vec = aligned16(logits) && aligned16(out) && (rows == 1 || (ld * es % 16 == 0 && out_ld * es % 16 == 0));
+  return hip_status(sdx::launch_penalize(dtype, a, (hipStream_t)stream), "penalize");
+}
+
 // ------------------------------------------------------------------ proposer
 int sdx_argmax(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld,
                int64_t* ids, sdx_stream_t stream) {

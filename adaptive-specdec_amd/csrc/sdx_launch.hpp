@@ -634,4 +634,32 @@ struct CopyPagesArgs {
 };
 hipError_t launch_copy_pages(const CopyPagesArgs& a, hipStream_t s);
 
+
+// sdx_penalty.hip
+constexpr int PN_MAX_BIAS = 1024;              // entries of a row
+constexpr int64_t PN_HISTORY = (1 << 20) - 1;  // tokens of a row's history
+struct PenalizeArgs {
+  const void* logits;           // [rows, ld]
+  void* out;                    // [rows, out_ld]
+  int64_t rows, V, ld, out_ld, batch;
+  const int64_t* cu_rows;       // [batch + 1] offsets of the rows' positions, or null: one each
+  const int64_t* history;       // [batch, history_ld], or null
+  int64_t history_ld, max_history;
+  const int64_t* history_len;   // [batch]
+  const int64_t* prompt_len;    // [batch] or null: 0
+  const float *repetition, *frequency, *presence;  // [batch] or null
+  const int64_t* bias_ids;      // [batch, biases]
+  const float* bias;
+  int32_t biases;
+  const uint32_t* allowed;      // [rows, allowed_ld] bits, or null
+  int64_t allowed_ld;
+  const int64_t* node_tokens;   // [rows] or null
+  const int64_t* tree_mask;     // [rows, mask_words], or null: chains
+  int32_t mask_words;
+  int32_t* error;
+  int64_t rows_each;            // of a workgroup (set by the launch)
+  bool vec;                     // rows of both start at multiples of 16 bytes
+};
+hipError_t launch_penalize(int dtype, const PenalizeArgs& a, hipStream_t s);
+
 }  // namespace sdx

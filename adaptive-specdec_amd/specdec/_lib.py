@@ -77,6 +77,8 @@ _SIGS = {
     "sdx_build_block_tables": (INT, [P, I64, P, I64, I32, I64, P, P, I64, P, P, P, P]),
     "sdx_paged_slot_mapping": (INT, [P, I64, I64, P, P, I32, I64, I64, P, P, P, P]),
     "sdx_append_slots": (INT, [P, I64, I64, P, INT, I32, I64, I64, I64, P, P, P]),
+    "sdx_penalize_logits": (INT, [P, INT, I64, I64, I64, P, I64, I64, P, P, I64, I64, P, P, P, P, P, P, P,
+                                  I32, P, I64, P, P, I32, P, P]),
     "sdx_tree_layout": (INT, [P, I64, P, P, I32, P, I64, I32, I64, I64, P, P, P, P, P]),
     "sdx_tree_accept": (INT, [P, P, P, I64, P, I64, P, I64, P, P, P, P, P]),
     "sdx_compact_paged": (INT, [P, I64, I64, INT, I32, I64, I64, I32, P, I64, I64, P, P, I64, P, P, P]),

@@ -27,6 +27,7 @@ import torch
 from . import _lib
 
 __all__ = ["to_probs", "sample_from_probs", "residual_probs", "gather_prob", "token_logprobs",
+           "penalize_logits",
            "rejection_sample", "rejection_sample_ragged", "Verifier", "draft_step"]
 
 # per-row flags of the verify calls (the SDX_FLAG_* bits of the C ABI)
@@ -201,6 +202,118 @@ def token_logprobs(logits, ids, temperature=1.0, top_n=0):
             _lib.ptr(ws), ws.numel() if need else 0, _lib.stream_of(x))
     _lib.check(rc, "token_logprobs")
     return logp, entropy, top_logp, top_ids
+
+
+def _rows_of(name, t, rows, cols, dtype):
+    """A [rows, cols] tensor of `dtype` as the kernels read it: (tensor, row stride)."""
+    if t.dim() != 2 or t.shape[0] != rows or (cols is not None and t.shape[1] != cols):
+        raise ValueError(f"{name} must be [{rows}, {'...' if cols is None else cols}], got {tuple(t.shape)}")
+    if t.dtype is not dtype:
+        t = t.to(dtype)
+    if t.shape[1] and (t.stride(1) != 1 or (rows > 1 and t.stride(0) < t.shape[1])):
+        t = t.contiguous()
+    return t, t.stride(0) if rows > 1 else t.shape[1]
+
+
+def _per_row(name, t, batch):
+    if t is None:
+        return None
+    if t.numel() != batch:
+        raise ValueError(f"{name} must be [{batch}], got {tuple(t.shape)}")
+    return _lib.as_dtype(t, torch.float32)
+
+
+def penalize_logits(logits, history=None, history_len=None, cu_rows=None, *, prompt_len=None,
+                    repetition=None, frequency=None, presence=None, bias_ids=None, bias=None,
+                    allowed=None, node_tokens=None, tree_mask=None, out=None, error=None):
+    """Penalties for repeated tokens, biases and grammar masks, before `to_probs` or an argmax.
+
+    logits [R, V] (fp32/bf16/fp16, any row stride and alignment). Batch row b's positions are the rows
+    cu_rows[b] .. cu_rows[b+1] - 1 (int64 [B+1]; None: one each, B = R). In fp32, rounded once:
+
+        x = l > 0 ? l / repetition[b] : l * repetition[b]   of tokens in the history or on the path
+        x -= frequency[b] * c, then x -= presence[b]        of tokens written c > 0 times
+        x += bias[b, e]                                     of token bias_ids[b, e], entry by entry
+        x = -inf                                            where the grammar refuses the token
+
+    history [B, H] int64, of which history_len [B] tokens count and the first prompt_len [B] (None: 0) are the
+    prompt (repetition alone goes by those); it ends before the step's first position. node_tokens [R]: the
+    positions' own input tokens, which count as written for every position that sees them: by tree_mask
+    [R, words] int64 (`specdec.tree.tree_layout`), or without it for itself and the later ones of its batch row
+    (a chain). repetition, frequency, presence fp32 [B]; bias_ids int64 and bias fp32 [B, n], n at most 1,024,
+    an id outside [0, V) for none; allowed int32 [R, ceil(V / 32) or more], bit v % 32 of word v / 32 set
+    where token v may follow. Any of them None: left out. Returns out (of logits' shape and type; given, it may
+    be logits itself, else apart from them). Rows behind cu_rows[B], and those of a batch row whose lengths
+    are out of range, are copied as they are; the latter set `error` (an int32 [1] device tensor) when given.
+    """
+    _lib.one_gpu(logits, history, history_len, cu_rows, prompt_len, repetition, frequency, presence,
+                 bias_ids, bias, allowed, node_tokens, tree_mask, out, error)
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [rows, V], got {tuple(logits.shape)}")
+    dt = _lib.dtype_code(logits)
+    for name, t in (("history", history), ("bias_ids", bias_ids), ("node_tokens", node_tokens),
+                    ("tree_mask", tree_mask), ("allowed", allowed)):
+        if t is not None and (t.dtype.is_floating_point or t.dtype.is_complex or t.dtype is torch.bool):
+            raise TypeError(f"{name} must be whole numbers, got {t.dtype}")
+    if error is not None and (error.dtype != torch.int32 or error.numel() < 1):
+        raise TypeError("error must be an int32 device tensor of one element")
+    R, V = logits.shape
+    B = R if cu_rows is None else cu_rows.numel() - 1
+    if B < 0 or (B == 0 and R > 0):
+        raise ValueError(f"{R} rows of no batch row")
+    x, ld = _rows_of("logits", logits, R, V, logits.dtype)
+    if out is None:
+        out = torch.empty((R, V), dtype=x.dtype, device=x.device)
+    elif out.dtype != logits.dtype or out.shape != logits.shape or (V > 1 and out.stride(1) != 1) or \
+            (R > 1 and out.stride(0) < V):
+        raise ValueError("out must be of logits' shape and type, its rows contiguous")
+    if (history is None) != (history_len is None) or (bias_ids is None) != (bias is None):
+        raise ValueError("history and history_len, bias_ids and bias go together")
+    if tree_mask is not None and node_tokens is None:
+        raise ValueError("tree_mask says which node_tokens a position sees: give those too")
+    hist, hist_ld, hl, pl = None, 0, None, None
+    if history is not None:
+        hist, hist_ld = _rows_of("history", history, B, None, torch.int64)
+        hl = _lib.as_dtype(history_len, torch.int64)
+        pl = None if prompt_len is None else _lib.as_dtype(prompt_len, torch.int64)
+        if hl.numel() != B or (pl is not None and pl.numel() != B):
+            raise ValueError(f"history_len and prompt_len must be [{B}]")
+    rep, freq, pres = (_per_row(n, t, B) for n, t in (("repetition", repetition), ("frequency", frequency),
+                                                      ("presence", presence)))
+    bi = bv = None
+    if bias_ids is not None:
+        if bias_ids.dim() != 2 or bias_ids.shape[0] != B or bias.shape != bias_ids.shape:
+            raise ValueError(f"bias_ids and bias must be [{B}, n], got {tuple(bias_ids.shape)} and "
+                             f"{tuple(bias.shape)}")
+        bi, bv = _lib.as_dtype(bias_ids, torch.int64), _lib.as_dtype(bias, torch.float32)
+    al, al_ld = None, 0
+    if allowed is not None:
+        if allowed.dim() == 2 and allowed.shape[1] < (V + 31) // 32:
+            raise ValueError(f"allowed must have {(V + 31) // 32} words a row, got {allowed.shape[1]}")
+        if allowed.dtype is not torch.int32:
+            raise TypeError(f"allowed must be int32 words, got {allowed.dtype}")
+        al, al_ld = _rows_of("allowed", allowed, R, None, torch.int32)
+    tk = tm = None
+    if node_tokens is not None:
+        if node_tokens.numel() != R:
+            raise ValueError(f"node_tokens must be [{R}], got {tuple(node_tokens.shape)}")
+        tk = _lib.as_dtype(node_tokens, torch.int64)
+    if tree_mask is not None:
+        if tree_mask.dim() != 2 or tree_mask.shape[0] != R or tree_mask.dtype is not torch.int64:
+            raise ValueError(f"tree_mask must be int64 [{R}, words], got {tuple(tree_mask.shape)}")
+        tm = tree_mask.contiguous()
+    if R == 0 or V == 0:
+        return out
+    with _lib.on_device(x):
+        rc = _lib.lib().sdx_penalize_logits(
+            _lib.ptr(x), dt, R, V, ld, _lib.ptr(out), out.stride(0) if R > 1 else V, B,
+            None if cu_rows is None else _lib.ptr(_lib.as_dtype(cu_rows, torch.int64)),
+            _lib.ptr(hist), hist_ld, 0 if hist is None else hist.shape[1], _lib.ptr(hl), _lib.ptr(pl),
+            _lib.ptr(rep), _lib.ptr(freq), _lib.ptr(pres), _lib.ptr(bi), _lib.ptr(bv),
+            0 if bi is None else bi.shape[1], _lib.ptr(al), al_ld, _lib.ptr(tk), _lib.ptr(tm),
+            0 if tm is None else tm.shape[1], _lib.ptr(error), _lib.stream_of(x))
+    _lib.check(rc, "penalize_logits")
+    return out
 
 
 def rejection_sample(target_logits, draft_logits, draft_ids, u_accept, u_final, *,

@@ -332,6 +332,36 @@ int sdx_slot_mapping(const int32_t* block_table, int64_t rows, int64_t max_block
                      int64_t padding_slot, int64_t* clamped_positions, int64_t* slots,
                      sdx_stream_t stream);
 
+/* ---- penalties, biases and grammar masks on logits, before the transforms of specdec/sampling.py:34-67.
+ * logits [rows, ld] -> out [rows, out_ld] of the same type (SDX_F32, SDX_BF16, SDX_F16; any
+ * alignment of rows), out = logits for in place, else apart from them. Batch row b's positions are the
+ * rows cu_rows[b] .. cu_rows[b+1] - 1 (int64 [batch + 1]; null: one each, batch = rows). For a logit l of
+ * token v, in fp32 and rounded once:
+ *   x = l > 0 ? l / repetition[b] : l * repetition[b]  where v is in the history or on the path
+ *   x -= frequency[b] * c, then x -= presence[b]       where v was written c > 0 times
+ *   x += bias[b, e]                                    for every e with bias_ids[b, e] = v, in order
+ *   x = -inf                                           where bit v % 32 of allowed[row, v / 32] is clear
+ * The history is history[b, 0 .. history_len[b]) (int64 [batch, history_ld], of max_history columns), its
+ * first prompt_len[b] (nullable: 0) tokens the prompt, which repetition alone goes by; the others are
+ * written, and so are the tokens of the position's path: node_tokens [rows] int64 of the batch row's
+ * nodes (nullable: none) where tree_mask [rows, mask_words] int64 has their bit (as sdx_tree_layout writes
+ * it; null: the row's nodes up to the position's own), itself included. The history ends before the
+ * step's first node. repetition, frequency and presence are fp32 [batch], nullable (1, 0, 0); bias_ids
+ * int64 and bias fp32 [batch, num_biases], ids outside the vocabulary for none; history null for none; allowed
+ * int32 [rows, allowed_ld], nullable. Ids outside [0, vocab) count nowhere. Logits that nothing concerns keep
+ * their bits; a row whose every token is refused is -inf throughout. Rows of no batch row, and those of a batch row
+ * whose lengths or offsets are out of range, are copied as they are; the latter set *error (nullable). One
+ * kernel. Up to 1,024 bias entries, 2^20 - 1 history tokens, 512 nodes in a row (with node_tokens). No
+ * reference counterpart. */
+int sdx_penalize_logits(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, void* out,
+                        int64_t out_ld, int64_t batch, const int64_t* cu_rows, const int64_t* history,
+                        int64_t history_ld, int64_t max_history, const int64_t* history_len,
+                        const int64_t* prompt_len, const float* repetition, const float* frequency,
+                        const float* presence, const int64_t* bias_ids, const float* bias,
+                        int32_t num_biases, const int32_t* allowed, int64_t allowed_ld,
+                        const int64_t* node_tokens, const int64_t* tree_mask, int32_t mask_words,
+                        int32_t* error, sdx_stream_t stream);
+
 /* ---- KV cache: specdec/kvcache.py ---------------------------------------- */
 
 /* RaggedCache.advance (kvcache.py:165-168): lengths[b] += q. */

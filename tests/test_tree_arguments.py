@@ -122,3 +122,43 @@ def test_oracles_by_hand():
     out, copies, used, ok = OT.fork(np.array([[1, 5], [2, -1]]), [20, 3], [0, 0, -1], [21, 32, 0], [7, 8], 16)
     assert ok and used == 1 and out.tolist() == [[1, 5], [1, 7], [-1, -1]]
     assert copies.tolist() == [[-1, 5, -1], [-1, 7, -1], [0, 4, 0]]
+
+
+def test_penalty_statuses():
+    from specdec import _lib
+    L = _lib.lib()
+    far = ctypes.c_void_p(1 << 30)
+
+    def call(logits=FAKE, dtype=BF16, R=4, V=100, ld=100, out=far, old=100, B=2, cu=FAKE, hist=FAKE, hld=50, H=50,
+             hlen=FAKE, bi=FAKE, nb=3, al=FAKE, ald=4, tok=FAKE, mask=FAKE, words=1):
+        return L.sdx_penalize_logits(logits, dtype, R, V, ld, out, old, B, cu, hist, hld, H, hlen, None, None, None,
+                                     None, bi, FAKE, nb, al, ald, tok, mask, words, None, None)
+
+    assert call(R=0) == OK
+    for bad in (dict(logits=None), dict(out=None), dict(dtype=4), dict(R=-1), dict(V=0), dict(ld=99), dict(old=99),
+                dict(B=-1), dict(B=0), dict(cu=None), dict(hlen=None), dict(hld=49), dict(bi=None), dict(nb=-1),
+                dict(ald=3), dict(tok=None), dict(words=0), dict(words=-1), dict(logits=ctypes.c_void_p(4097)),
+                dict(out=ctypes.c_void_p(4098)), dict(out=ctypes.c_void_p(4096), old=101)):
+        assert call(**bad) == EINVAL, bad
+    for bad in (dict(nb=1025), dict(H=1 << 20, hld=1 << 20), dict(R=(1 << 21) + 1, cu=FAKE),
+                dict(V=(1 << 30) + 1, ld=1 << 31, old=1 << 31, ald=1 << 30, R=1)):
+        assert call(**{"out": ctypes.c_void_p(1 << 50), **bad}) == EUNSUP, bad
+
+
+def test_penalties_refuse_cpu_tensors():
+    from specdec import sampling as S
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        S.penalize_logits(torch.zeros(2, 8))
+
+
+def test_penalty_oracle_by_hand():
+    from oracle import penalties as PN
+    x = np.array([[2.0, -2.0, 1.0, 0.5], [2.0, -2.0, 1.0, 0.5]])
+    out, _, touched = PN.penalize(x, np.array([[0, 1, 1, 3]]), [3], [0, 2], prompt_len=[1], repetition=[2.0],
+                                  frequency=[0.25], presence=[1.0], bias_ids=np.array([[2, 2, 9]]),
+                                  bias=np.array([[1.0, 0.5, 7.0]]), node_tokens=[0, 3],
+                                  allowed=np.array([[15], [13]], dtype=np.int32))
+    # row 0 saw 0 (prompt and path), 1 twice; row 1 token 3 too, and may not go on with 1
+    assert out[0].tolist() == [1.0 - 0.25 - 1.0, -4.0 - 0.5 - 1.0, 2.5, 0.5]
+    assert out[1].tolist() == [-0.25, -np.inf, 2.5, 0.25 - 0.25 - 1.0]
+    assert touched.tolist() == [[True, True, True, False], [True] * 4]
