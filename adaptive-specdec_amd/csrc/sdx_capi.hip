@@ -1461,4 +1461,69 @@ int sdx_prefix_attention_paged(const void* q, int dtype, int64_t num_tokens, int
   return hip_status(sdx::launch_prefix_attn(dtype, head_dim, a, (hipStream_t)stream), "prefix_attn");
 }
 
+// ------------------------------------------------------------------ attention of trees
+static size_t tree_attn_ws(Carve& c, int64_t tokens, int64_t batch, int32_t hq, int32_t hkv, int32_t d,
+                           sdx::TreeAttnArgs* a) {
+  a->head = c.take<uint32_t>(64);
+  a->max_items = sdx::tree_attn_items(tokens, batch, hkv, hq / hkv);
+  a->items = c.take<sdx::TreeAttnItem>((size_t)a->max_items);
+  a->part_ml = c.take<float2>((size_t)2 * sdx::TREE_ATTN_GRID * 128);
+  a->part_o = c.take<float>((size_t)2 * sdx::TREE_ATTN_GRID * 128 * d);
+  return c.used;
+}
+
+size_t sdx_tree_attention_workspace(int64_t num_tokens, int64_t batch, int32_t num_q_heads,
+                                    int32_t num_kv_heads, int32_t head_dim) {
+  if (num_tokens < 1 || batch < 1 || num_q_heads < 1 || num_kv_heads < 1 ||
+      num_q_heads % num_kv_heads != 0 || (head_dim != 64 && head_dim != 128) ||
+      !prefix_fits(num_tokens, batch, 1, num_q_heads))
+    return 0;
+  Carve c{nullptr};
+  sdx::TreeAttnArgs a = {};
+  return tree_attn_ws(c, num_tokens, batch, num_q_heads, num_kv_heads, head_dim, &a);
+}
+
+int sdx_tree_attention_paged(const void* q, int dtype, int64_t num_tokens, int64_t batch,
+                             const int64_t* cu_q, int32_t num_q_heads, int32_t num_kv_heads,
+                             int32_t head_dim, const void* k_pool, const void* v_pool,
+                             int64_t num_blocks, int32_t block_size, const int32_t* block_table,
+                             int64_t max_blocks, const int64_t* kv_len, const int64_t* tree_mask,
+                             int32_t mask_words, float scale, void* workspace, size_t workspace_bytes,
+                             void* out, int32_t* error, sdx_stream_t stream) {
+  if (num_tokens < 0 || batch < 0 || num_q_heads < 1 || num_kv_heads < 1 || block_size < 1 ||
+      max_blocks < 1 || num_blocks < 1 || mask_words < 1 || !(scale > 0.0f) ||
+      !(scale * 1.4426950408889634f < INFINITY))
+    return fail(SDX_EINVAL, "sdx_tree_attention_paged: bad arguments");
+  if (num_q_heads % num_kv_heads != 0)
+    return fail(SDX_EINVAL, "sdx_tree_attention_paged: query heads must be a multiple of KV heads");
+  if ((dtype != SDX_BF16 && dtype != SDX_F16) || (head_dim != 64 && head_dim != 128))
+    return fail(SDX_EUNSUPPORTED, "sdx_tree_attention_paged: bf16 or fp16 with head_dim 64 or 128");
+  if (num_tokens == 0) return SDX_OK;
+  if (batch == 0)
+    return fail(SDX_EINVAL, "sdx_tree_attention_paged: %lld nodes of no row", (long long)num_tokens);
+  if (!q || !cu_q || !k_pool || !v_pool || !block_table || !kv_len || !tree_mask || !out)
+    return fail(SDX_EINVAL, "sdx_tree_attention_paged: null pointer");
+  if (max_blocks > (1 << 30) / block_size || num_blocks > (int64_t)0xFFFFFFFE / block_size)
+    return fail(SDX_EUNSUPPORTED, "sdx_tree_attention_paged: rows of more than 2^30 or a pool of 2^32 - 1 "
+                                  "tokens or more");
+  if (!prefix_fits(num_tokens, batch, 1, num_q_heads))
+    return fail(SDX_EUNSUPPORTED, "sdx_tree_attention_paged: more than 2^23 query vectors or 2^22 rows");
+  if (!aligned16(q) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out))
+    return fail(SDX_EINVAL, "sdx_tree_attention_paged: tensors must be 16-byte aligned");
+  Carve c{(uint8_t*)workspace};
+  sdx::TreeAttnArgs a = {};
+  const size_t need = tree_attn_ws(c, num_tokens, batch, num_q_heads, num_kv_heads, head_dim, &a);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < need)
+    return fail(SDX_EWORKSPACE, "sdx_tree_attention_paged: needs a 16-byte aligned workspace of %zu bytes "
+                                "(got %zu)", need, workspace_bytes);
+  a.q = (const uint16_t*)q; a.cu_q = cu_q;
+  a.k_pool = (const uint16_t*)k_pool; a.v_pool = (const uint16_t*)v_pool;
+  a.block_table = block_table; a.kv_len = kv_len; a.mask = tree_mask; a.words = mask_words;
+  a.batch = batch; a.tokens = num_tokens; a.max_blocks = max_blocks; a.num_blocks = num_blocks;
+  a.hq = num_q_heads; a.hkv = num_kv_heads; a.group = num_q_heads / num_kv_heads; a.bs = block_size;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = (uint16_t*)out; a.error = error;
+  return hip_status(sdx::launch_tree_attn(dtype, head_dim, a, (hipStream_t)stream), "tree_attn");
+}
+
 }  // extern "C"

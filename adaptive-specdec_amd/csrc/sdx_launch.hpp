@@ -635,6 +635,34 @@ struct CopyPagesArgs {
 hipError_t launch_copy_pages(const CopyPagesArgs& a, hipStream_t s);
 
 
+// sdx_tree_attn.hip
+constexpr int TREE_ATTN_GRID = 512;  // workgroups
+struct TreeAttnItem {  // 128 query rows of a row, and the workgroups that have its keys
+  int32_t t0, kvh, r0, m;      // the row's first token, KV head, first query row, query rows
+  int32_t first, parts, pad[2];
+};
+struct TreeAttnArgs {
+  const uint16_t* q;           // [tokens, hq, d] bf16 or fp16
+  const int64_t* cu_q;         // [batch + 1] node offsets
+  const uint16_t* k_pool;      // [num_blocks, bs, hkv * d]
+  const uint16_t* v_pool;
+  const int32_t* block_table;  // [batch, max_blocks]
+  const int64_t* kv_len;       // [batch] keys per row, the nodes included
+  const int64_t* mask;         // [tokens, words]
+  int64_t batch, tokens, max_blocks, num_blocks;
+  int32_t hq, hkv, group, bs, words;
+  float scale_log2;            // softmax scale * log2(e)
+  uint16_t* out;               // [tokens, hq, d]
+  int32_t* error;
+  uint32_t* head;              // [64] the items
+  TreeAttnItem* items;         // [max_items]
+  int64_t max_items;
+  float2* part_ml;             // [2 TREE_ATTN_GRID, 128] max and sum of each part's query rows
+  float* part_o;               // [2 TREE_ATTN_GRID, 128, d]
+};
+int64_t tree_attn_items(int64_t tokens, int64_t batch, int32_t hkv, int32_t group);
+hipError_t launch_tree_attn(int dtype, int d, const TreeAttnArgs& a, hipStream_t s);
+
 // sdx_penalty.hip
 constexpr int PN_MAX_BIAS = 1024;              // entries of a row
 constexpr int64_t PN_HISTORY = (1 << 20) - 1;  // tokens of a row's history

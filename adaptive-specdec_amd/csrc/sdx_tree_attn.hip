@@ -1,0 +1,531 @@
+// Attention of trees of drafted tokens over the paged cache, one layer: the verify attention of
+// sdx_attn.hip (bench/bench_engine.py:170-174, the mask of specdec/kvcache.py:138-162) where a
+// row's new tokens are the nodes of a tree. Node i of row b sees the row's cache, the
+// kv_len - n keys in front of its nodes, and the nodes that its mask has a bit for:
+//
+//   out_i = sum_s p_s v_s / sum_s p_s,  p_s = 2^(scale log2(e) q_i k_s - m)
+//
+// An item is a tile of 128 query rows (nodes x the query heads of a KV head) of a row against
+// all of its keys, in tiles of 64 that never hold cache and nodes both: cache tiles are bare but
+// for the last one's end, a node tile takes one 64-bit word of each query row's mask. The items'
+// tiles lie one behind another on a line, TA_COST more in front of each for what an item costs
+// beside them, and every workgroup takes an equal stretch of it: no plan kernel, no queue, no
+// counter, and the work is even whatever the rows' lengths are. Each workgroup works out the
+// line from the lengths by itself (8 bytes a row, a scan). A stretch's first and last item may
+// be parts, so there is room for two parts a workgroup, which leave (O, max, sum) in fp32 for a
+// second kernel to join; whole items are written directly.
+#include <algorithm>
+#include <type_traits>
+
+#include "sdx_attn_tile.hpp"
+
+namespace sdx {
+
+constexpr int TA_GRID = TREE_ATTN_GRID;  // two workgroups on each of 256 CUs
+constexpr uint32_t TA_COST = 2;          // tiles that an item costs beside its own
+constexpr uint32_t TA_LEAST = 2;         // tiles of a stretch, at least
+
+struct TaRow {
+  int64_t t0, ctx;      // first node's token; keys in front of the nodes
+  int32_t n, ct, kt;    // nodes; tiles of the cache, and with the nodes'
+  int32_t qt;           // tiles of query rows
+  bool ok;
+  __device__ __forceinline__ uint64_t len() const { return (uint64_t)kt + TA_COST; }
+};
+__device__ __forceinline__ TaRow ta_row(const TreeAttnArgs& a, int64_t b) {
+  TaRow r;
+  const int64_t t1 = a.cu_q[b + 1], kv = a.kv_len[b];
+  r.t0 = a.cu_q[b];
+  const int64_t n = t1 - r.t0;
+  r.ok = r.t0 >= 0 && n >= 0 && t1 <= a.tokens && n <= min(a.words * 64, TREE_MAX_NODES) && kv >= n &&
+         kv <= a.max_blocks * a.bs;
+  r.n = r.ok ? (int32_t)n : 0;
+  r.ctx = kv - n;
+  r.ct = r.ok ? (int32_t)((r.ctx + PA_TILE - 1) / PA_TILE) : 0;
+  r.kt = r.ct + (r.n + PA_TILE - 1) / PA_TILE;
+  r.qt = (r.n * a.group + PA_ROWS - 1) / PA_ROWS;
+  return r;
+}
+__device__ __forceinline__ uint32_t ta_items(const TreeAttnArgs& a, const TaRow& r) {
+  return (uint32_t)(r.qt * a.hkv);
+}
+
+struct TaScan {
+  uint64_t line, lines;    // before this thread's, of all
+  uint64_t item, items;
+};
+// sums over the workgroup's threads, in their order
+__device__ __forceinline__ TaScan ta_scan(uint64_t line, uint64_t items, uint64_t* sLine, uint64_t* sItem) {
+  constexpr int NW = PA_NT / kWave;
+  const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave;
+  const uint64_t li = wave_incl_scan_u64(line, lane);
+  const uint64_t ii = wave_incl_scan_u64(items, lane);
+  if (lane == kWave - 1) sLine[wv] = li, sItem[wv] = ii;
+  __syncthreads();
+  TaScan r{li - line, 0, ii - items, 0};
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    if (w < wv) r.line += sLine[w], r.item += sItem[w];
+    r.lines += sLine[w], r.items += sItem[w];
+  }
+  __syncthreads();
+  return r;
+}
+
+// S^T = K Q^T for a tile's 64 keys. ka: the lane's byte address in K's first row block.
+template <int D, int FMT>
+__device__ __forceinline__ void ta_qk(pa_f16 (&s)[2], const pa_u4 (&qa)[D / 16], const uint8_t* k, uint32_t ka) {
+  constexpr int RB = 2 * D;
+  pa_u4 x[2][2];  // operands of a step, read a step ahead
+  auto read = [&](int ks) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+      x[ks & 1][n] = *reinterpret_cast<const pa_u4*>(k + (ka ^ (ks << 5)) + n * 32 * RB);
+  };
+  read(0);
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) {
+    if (ks + 1 < D / 16) read(ks + 1);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) s[n] = pa_mfma<FMT>(x[ks & 1][n], qa[ks], s[n]);
+  }
+  // in this order: two steps' reads, then a step's products and the reads after next
+  __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+    if (ks + 2 < D / 16) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+  }
+}
+
+// Scores of keys without their bit in m: key 32 nb + 8 (i / 4) + 4 hi + i % 4 in s[nb][i].
+__device__ __forceinline__ void ta_mask(pa_f16 (&s)[2], uint64_t m, int hi) {
+#pragma unroll
+  for (int nb = 0; nb < 2; ++nb) {
+    const uint32_t w = (uint32_t)(m >> (32 * nb)) >> (4 * hi);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (!((w >> (8 * (i / 4) + i % 4)) & 1)) s[nb][i] = -INFINITY;
+  }
+}
+
+// bits of the n nodes from 64 k on
+__device__ __forceinline__ uint64_t ta_valid(int n, int k) {
+  const int left = n - 64 * k;
+  return left >= 64 ? ~0ull : (1ull << left) - 1;
+}
+
+// a stretch of an item
+struct TaUnit {
+  int64_t b, t0, ctx;
+  int32_t n, ct, kvh, r0, m;  // r0, m: first query row, query rows
+  int32_t lo, hi;             // tiles
+  int32_t part;               // -1: whole, written directly
+};
+// token of query row i of the unit
+__device__ __forceinline__ int64_t ta_token(const TreeAttnArgs& a, const TaUnit& u, int i) {
+  return u.t0 + (uint32_t)(u.r0 + i) / (uint32_t)a.group;
+}
+__device__ __forceinline__ int64_t ta_qrow(const TreeAttnArgs& a, const TaUnit& u, int i) {
+  const uint32_t r = u.r0 + i, j = r / (uint32_t)a.group;
+  return (u.t0 + j) * a.hq + u.kvh * a.group + (r - j * a.group);
+}
+// the word of query row i's mask for nodes 64 k ..
+__device__ __forceinline__ uint64_t ta_word(const TreeAttnArgs& a, const TaUnit& u, int i, int k) {
+  return i < u.m ? (uint64_t)a.mask[ta_token(a, u, i) * a.words + k] & ta_valid(u.n, k) : 0ull;
+}
+
+// V of nodes that some query rows do not see: infinities and NaN of theirs are 0 for the
+// products (pa_finite_only) and are added here to the rows that see their node.
+template <int D, int FMT>
+__device__ __forceinline__ void ta_add_odd(PaState<D>& st, const TreeAttnArgs& a, const TaUnit& u,
+                                           const int32_t* table, const uint8_t* vp, uint32_t row_bytes, int i,
+                                           int hi) {
+  constexpr uint32_t E = FMT == SDX_BF16 ? 0x7F80u : 0x7C00u;
+#pragma nounroll
+  for (int t = (max(u.lo, u.ct) - u.ct) * PA_TILE; t < min(u.n, (u.hi - u.ct) * PA_TILE); ++t) {
+    const uint64_t w = ta_word(a, u, i, t / 64);
+    const uint32_t pos = (uint32_t)u.ctx + t;
+    const int32_t page = table[pos / (uint32_t)a.bs];
+    if (page < 0 || page >= a.num_blocks) continue;
+    const uint32_t s = (uint32_t)page * (uint32_t)a.bs + pos % (uint32_t)a.bs;
+    const uint16_t* const row = reinterpret_cast<const uint16_t*>(vp + (uint64_t)s * row_bytes);
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const ushort4 x = *reinterpret_cast<const ushort4*>(row + 32 * db + 8 * e + 4 * hi);
+        const uint16_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (((w >> (t % 64)) & 1) && (y[k] & E) == E) st.o[db][4 * e + k] += pa_odd<FMT>(y[k]);
+        __builtin_amdgcn_sched_barrier(0);  // few registers, the speed of this is no concern
+      }
+  }
+}
+
+template <int D, int FMT>
+__global__ void __launch_bounds__(PA_NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
+tree_attn_kernel(TreeAttnArgs a) {
+  constexpr int NC = D / 8;            // 16-byte chunks of a row
+  constexpr int RB = 2 * D;            // bytes of a row
+  __shared__ __align__(256) uint8_t sMem[2 * 2 * PA_TILE * RB];  // two tiles of K and V
+  __shared__ uint32_t sSlot[PA_RING * PA_TILE];
+  __shared__ uint64_t sLine[PA_NT / kWave], sItem[PA_NT / kWave], sAt[2];
+  __shared__ int sOdd;  // V of the unit has elements that ta_add_odd adds
+  // the wave's index and the unit are made scalar: what follows from them takes no vector
+  // registers, of which a wave of two per SIMD has 256
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int w = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int hi = lane / 32, l31 = lane & 31;
+  const uint32_t row_bytes = (uint32_t)a.hkv * RB;
+  // addresses of the lane's operands in LDS tiles
+  const uint32_t ka = l31 * RB + ((hi ^ pa_swz_k<D>(l31)) << 4);
+  const int vr = 4 * hi + ((lane & 15) >> 2), vd = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  const uint32_t va = vr * RB + (((vd >> 3) ^ pa_swz_v<D>(vr)) << 4) + (vd & 7) * 2;
+
+  // the line: its length, this workgroup's stretch, the row that the stretch starts in.
+  // Neighbours on the line share an XCD (workgroup index % 8), whose L2 their keys go through.
+  const uint32_t wg = blockIdx.x % 8 * (TA_GRID / 8) + blockIdx.x / 8;
+  uint64_t total, step, pos = 0, from = 0;  // from: where row b starts
+  uint32_t item0 = 0;
+  int64_t b = 0;
+  {
+    const bool one = a.batch <= PA_NT;
+    uint64_t line = 0, items = 0;
+    int bad = 0;
+    for (int64_t i = tid; i < a.batch; i += PA_NT) {
+      const TaRow r = ta_row(a, i);
+      bad |= !r.ok;
+      const uint32_t n = ta_items(a, r);
+      line += n * r.len();
+      items += n;
+    }
+    TaScan sc = ta_scan(line, items, sLine, sItem);
+    const bool over = sc.items > (uint64_t)a.max_items;  // rows that share nodes: offsets out of order
+    if ((bad || over) && a.error && blockIdx.x == 0) *a.error = 1;
+    if (blockIdx.x == 0 && tid == 0) a.head[0] = over ? 0u : (uint32_t)sc.items;
+    total = over ? 0 : sc.lines;
+    step = max((total + TA_GRID - 1) / TA_GRID, (uint64_t)TA_LEAST);
+    pos = wg * step;
+    if (pos >= total) return;  // uniform
+    uint64_t at = 0, it = 0;
+    for (int64_t b0 = 0;; b0 += PA_NT) {  // uniform; ends where the line holds pos
+      if (!one) {
+        const TaRow r = b0 + tid < a.batch ? ta_row(a, b0 + tid) : TaRow{};
+        items = b0 + tid < a.batch ? ta_items(a, r) : 0;
+        line = items ? items * r.len() : 0;
+        sc = ta_scan(line, items, sLine, sItem);
+      }
+      if (at + sc.line <= pos && pos < at + sc.line + line) {
+        sAt[0] = at + sc.line;
+        sAt[1] = (uint64_t)(b0 + tid) << 32 | (it + sc.item);
+      }
+      at += sc.lines, it += sc.items;
+      if (pos < at) break;
+    }
+    __syncthreads();
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)sAt[0]);
+    const uint32_t up = __builtin_amdgcn_readfirstlane((uint32_t)(sAt[0] >> 32));
+    from = (uint64_t)up << 32 | lo;
+    item0 = __builtin_amdgcn_readfirstlane((uint32_t)sAt[1]);
+    b = __builtin_amdgcn_readfirstlane((uint32_t)(sAt[1] >> 32));
+  }
+  const uint64_t end = min(total, pos + step);
+
+  TaRow row = ta_row(a, b);
+  while (pos < end) {  // uniform: the items of the stretch
+    const uint64_t len = row.len();
+    const uint32_t item = (uint32_t)((pos - from) / len);
+    const uint64_t p = from + item * len, e = min(end, p + len);
+    const uint32_t first = (uint32_t)((p + TA_COST) / step), last = (uint32_t)((p + len - 1) / step);
+    TaUnit u;
+    u.b = b, u.t0 = row.t0, u.ctx = row.ctx;
+    u.n = row.n, u.ct = row.ct;
+    u.kvh = item / row.qt;
+    u.r0 = (int32_t)(item - u.kvh * row.qt) * PA_ROWS;
+    u.m = min(PA_ROWS, row.n * a.group - u.r0);
+    u.lo = (int32_t)(max(pos - p, (uint64_t)TA_COST) - TA_COST);
+    u.hi = (int32_t)(max(e - p, (uint64_t)TA_COST) - TA_COST);
+    u.part = first == last ? -1 : (int32_t)(2 * wg + (wg == first));
+    if (wg == first && u.lo < u.hi && tid == 0)
+      a.items[item0 + item] = TreeAttnItem{(int32_t)u.t0, u.kvh, u.r0, u.m, (int32_t)first,
+                                           (int32_t)(last - first + 1), 0, 0};
+    pos = e;
+    const uint64_t row_end = from + (uint64_t)row.qt * a.hkv * len;
+    if (u.lo < u.hi) {
+      const int32_t* const table = a.block_table + u.b * a.max_blocks;
+      const uint8_t* const kp = reinterpret_cast<const uint8_t*>(a.k_pool + u.kvh * D);
+      const uint8_t* const vp = reinterpret_cast<const uint8_t*>(a.v_pool + u.kvh * D);
+      int bad = 0;
+      PaState<D> st;
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st.o[db][i] = 0.0f;
+      st.m = -INFINITY;
+      st.l = 0.0f;
+      const int r0 = PA_WROWS * w;  // the wave's rows
+      const bool active = r0 < u.m;
+      pa_u4 qa[D / 16];
+      {
+        const uint16_t* src = a.q + (r0 + l31 < u.m ? ta_qrow(a, u, r0 + l31) * D : 0);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          qa[ks] = *reinterpret_cast<const pa_u4*>(src + 16 * ks + 8 * hi);
+          if (r0 + l31 >= u.m) qa[ks] = (pa_u4){0, 0, 0, 0};
+        }
+      }
+      uint64_t word = u.hi > u.ct ? ta_word(a, u, r0 + l31, max(u.lo, u.ct) - u.ct) : 0;
+
+      constexpr int H = NC / 4, TPR = PA_NT / NC;  // passes, rows per pass
+      const int ntile = u.hi - u.lo;
+      const int lr = tid / NC, lc = tid % NC;
+      // slots of the unit's tiles, four tiles at a time, one by each wave: page ids are loaded
+      // four tiles before they are needed here, eight before their keys
+      auto key = [&](int tile) -> int64_t {  // position of the lane's key of a tile, -1: none
+        const int t = u.lo + tile;
+        if (t >= u.hi) return -1;
+        const int64_t x = t < u.ct ? (int64_t)t * PA_TILE + lane : (int64_t)(t - u.ct) * PA_TILE + lane;
+        if (t < u.ct) return x < u.ctx ? x : -1;
+        return x < u.n ? u.ctx + x : -1;
+      };
+      auto page_of = [&](int tile) {
+        const int64_t x = key(tile);
+        return x >= 0 ? table[(uint32_t)x / (uint32_t)a.bs] : 0;
+      };
+      auto put_slot = [&](int tile, int32_t page) {
+        const int64_t x = key(tile);
+        uint32_t s = PA_NOSLOT;
+        if (x >= 0) {
+          if (page >= 0 && page < a.num_blocks) s = (uint32_t)page * (uint32_t)a.bs + (uint32_t)x % (uint32_t)a.bs;
+          bad |= s == PA_NOSLOT;
+        }
+        sSlot[(tile % PA_RING) * PA_TILE + lane] = s;
+      };
+      pa_u4 kk[H], vv[H];
+      uint32_t none;  // passes whose key is none: their V is 0 for the products, their K never seen
+      auto gather = [&](int tile) {
+        none = 0;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          const uint32_t s = sSlot[(tile % PA_RING) * PA_TILE + lr + TPR * h];
+          const uint64_t off = (uint64_t)(s == PA_NOSLOT ? 0u : s) * row_bytes;
+          none |= (s == PA_NOSLOT ? 1u : 0u) << h;
+          kk[h] = *reinterpret_cast<const pa_u4*>(kp + off + lc * 16);
+          vv[h] = *reinterpret_cast<const pa_u4*>(vp + off + lc * 16);
+        }
+      };
+      static_assert(TPR % 16 == 0, "a pass's rows are swizzled alike");
+      const uint32_t kw = lr * RB + ((lc ^ pa_swz_k<D>(lr)) << 4);
+      const uint32_t vw = lr * RB + ((lc ^ pa_swz_v<D>(lr)) << 4);
+      auto stage = [&](auto buf, int tile) {
+        uint8_t* const k = sMem + buf * (2 * PA_TILE * RB);
+        if ((u.lo + tile + 1) * (int64_t)PA_TILE > u.ctx) {  // uniform: the cache's last tile, the nodes'
+#pragma unroll
+          for (int h = 0; h < H; ++h)
+            if ((none >> h) & 1) vv[h] = (pa_u4){0, 0, 0, 0};
+          if (u.lo + tile >= u.ct && pa_finite_only<FMT, H>(vv)) sOdd = 1;
+        }
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          *reinterpret_cast<pa_u4*>(k + kw + TPR * h * RB) = kk[h];
+          *reinterpret_cast<pa_u4*>(k + vw + (PA_TILE + TPR * h) * RB) = vv[h];
+        }
+      };
+      __syncthreads();  // the unit before is done with LDS
+      put_slot(w, page_of(w));
+      int32_t page = page_of(4 + w);
+      if (tid == 0) sOdd = 0;
+      __syncthreads();
+      typedef std::integral_constant<int, 0> even;
+      typedef std::integral_constant<int, 1> odd;
+      gather(0);
+      stage(even(), 0);
+      gather(1);
+      __syncthreads();
+      auto tile = [&](int t, auto buf, auto next) {
+        if (buf == 0 && t % 4 == 0) {  // uniform
+          put_slot(t + 4 + w, page);
+          page = page_of(t + 8 + w);
+        }
+        if (active) {
+          const uint8_t* const k = sMem + buf * (2 * PA_TILE * RB);
+          __builtin_amdgcn_s_setprio(1);
+          pa_f16 s[2] = {};
+          ta_qk<D, FMT>(s, qa, k, ka);
+          __builtin_amdgcn_s_setprio(0);
+          const int g = u.lo + t;
+          if ((g + 1) * (int64_t)PA_TILE > u.ctx) {  // uniform
+            if (g < u.ct) {
+              ta_mask(s, (1ull << (u.ctx - (int64_t)g * PA_TILE)) - 1, hi);
+            } else {
+              ta_mask(s, word, hi);
+              if (g + 1 < u.hi) word = ta_word(a, u, r0 + l31, g + 1 - u.ct);
+            }
+          }
+          pa_softmax<D, FMT, 2>(st, s, a.scale_log2);
+          __builtin_amdgcn_s_setprio(1);
+          pa_pv<D, FMT, 2>(st, s, k + PA_TILE * RB, va);
+          __builtin_amdgcn_s_setprio(0);
+        }
+        stage(next, t + 1);
+        __builtin_amdgcn_sched_barrier(0);  // the registers are free before they are loaded
+        gather(t + 2);
+        __syncthreads();
+      };
+      for (int t = 0;; t += 2) {
+        tile(t, even(), odd());
+        if (t + 1 >= ntile) break;
+        tile(t + 1, odd(), even());
+        if (t + 2 >= ntile) break;
+      }
+      if (__builtin_amdgcn_readfirstlane(sOdd))
+        ta_add_odd<D, FMT>(st, a, u, table, vp, row_bytes, r0 + l31, hi);
+      st.l = pa_sum_halves(st.l);
+      const int i = r0 + l31;
+      if (active && i < u.m) {
+        if (u.part < 0) {
+          const float f = st.l > 0.0f || st.l != st.l ? 1.0f / st.l : 0.0f;
+          uint16_t* const to = a.out + ta_qrow(a, u, i) * D + 4 * hi;
+#pragma unroll
+          for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+            for (int e4 = 0; e4 < 4; ++e4)
+              *reinterpret_cast<uint2*>(to + 32 * db + 8 * e4) =
+                  make_uint2(pa_pack<FMT>(st.o[db][4 * e4] * f, st.o[db][4 * e4 + 1] * f),
+                             pa_pack<FMT>(st.o[db][4 * e4 + 2] * f, st.o[db][4 * e4 + 3] * f));
+        } else {
+          float* const to = a.part_o + ((int64_t)u.part * PA_ROWS + i) * D + 4 * hi;
+#pragma unroll
+          for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+            for (int e4 = 0; e4 < 4; ++e4)
+              *reinterpret_cast<float4*>(to + 32 * db + 8 * e4) = make_float4(
+                  st.o[db][4 * e4], st.o[db][4 * e4 + 1], st.o[db][4 * e4 + 2], st.o[db][4 * e4 + 3]);
+          if (hi == 0) a.part_ml[(int64_t)u.part * PA_ROWS + i] = make_float2(st.m, st.l);
+        }
+      }
+      if (bad && a.error) *a.error = 1;
+    }
+    if (pos == row_end) {  // the next row that has nodes
+      from = pos;
+      item0 += ta_items(a, row);
+      while (++b < a.batch) {
+        row = ta_row(a, b);
+        if (row.n > 0) break;
+      }
+    }
+  }
+}
+
+// Join of the items that are split: out = sum_c w_c O_c, w_c = 2^(m_c - m) / sum 2^(m_c - m) l_c.
+// A workgroup has RB query rows of an item at a time; 256 / (D / 4 RB) slices of D / 4 threads
+// share a row's parts, each with a running maximum of its own, and are joined in LDS.
+template <int D, int FMT, int RB>
+__global__ void __launch_bounds__(PA_NT) tree_attn_join_kernel(TreeAttnArgs a) {
+  constexpr int DL = D / 4, SL = PA_NT / DL / RB, UN = 4;
+  __shared__ float4 sO[SL][RB][DL];
+  __shared__ float2 sML[SL][RB];
+  if (blockIdx.x >= a.head[0]) return;  // uniform
+  const TreeAttnItem x = a.items[blockIdx.x];
+  if (x.parts < 2) return;  // uniform: written directly
+  const int tid = threadIdx.x, d4 = tid % DL, rr = tid / DL % RB, sl = tid / DL / RB;
+  for (int i0 = blockIdx.y * RB; i0 < x.m; i0 += gridDim.y * RB) {  // uniform
+    const int i = min(i0 + rr, x.m - 1);
+    float m = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int c0 = sl; c0 < x.parts; c0 += SL * UN) {
+      float2 ml[UN];
+      float4 v[UN];
+#pragma unroll
+      for (int k = 0; k < UN; ++k) {
+        const int c = min(c0 + k * SL, x.parts - 1);
+        const int64_t p = (int64_t)(2 * (x.first + c) + (c == 0)) * PA_ROWS + i;
+        ml[k] = a.part_ml[p];
+        v[k] = *reinterpret_cast<const float4*>(a.part_o + p * D + d4 * 4);
+      }
+      float mn = m;
+#pragma unroll
+      for (int k = 0; k < UN; ++k) mn = fmaxf(mn, ml[k].x);
+      const float s = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+      l *= s;
+      o = make_float4(o.x * s, o.y * s, o.z * s, o.w * s);
+      m = mn;
+#pragma unroll
+      for (int k = 0; k < UN; ++k) {
+        const bool none = c0 + k * SL >= x.parts || ml[k].x == -INFINITY;  // not a 0 times its O
+        const float f = none ? 0.0f : __builtin_amdgcn_exp2f(ml[k].x - m);
+        if (none) v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        l += f * ml[k].y;  // 0 times the NaN sum of a part whose scores are all NaN is NaN, and so is out
+        o.x += f * v[k].x;
+        o.y += f * v[k].y;
+        o.z += f * v[k].z;
+        o.w += f * v[k].w;
+      }
+    }
+    if constexpr (SL > 1) {
+      __syncthreads();
+      sO[sl][rr][d4] = o;
+      if (d4 == 0) sML[sl][rr] = make_float2(m, l);
+      __syncthreads();
+      if (sl == 0) {
+        float mn = m;
+#pragma unroll
+        for (int k = 1; k < SL; ++k) mn = fmaxf(mn, sML[k][rr].x);
+        float s = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+        l *= s;
+        o = make_float4(o.x * s, o.y * s, o.z * s, o.w * s);
+#pragma unroll
+        for (int k = 1; k < SL; ++k) {
+          const float2 ml = sML[k][rr];
+          const float4 v = sO[k][rr][d4];
+          s = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
+          l += s * ml.y;
+          o.x += s * v.x;
+          o.y += s * v.y;
+          o.z += s * v.z;
+          o.w += s * v.w;
+        }
+      }
+    }
+    if (sl == 0 && i0 + rr < x.m) {
+      const float f = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+      const uint32_t r = x.r0 + i, j = r / (uint32_t)a.group;
+      const int64_t qrow = (int64_t)(x.t0 + j) * a.hq + x.kvh * a.group + (r - j * a.group);
+      *reinterpret_cast<uint2*>(a.out + qrow * D + d4 * 4) =
+          make_uint2(pa_pack<FMT>(o.x * f, o.y * f), pa_pack<FMT>(o.z * f, o.w * f));
+    }
+  }
+}
+
+// items of a call: tiles of 128 query rows, of every row that has nodes
+int64_t tree_attn_items(int64_t tokens, int64_t batch, int32_t hkv, int32_t group) {
+  return hkv * (tokens * group / PA_ROWS + std::min(batch, tokens));
+}
+
+template <int D, int FMT, int RB>
+static void launch_join(const TreeAttnArgs& a, int64_t items, hipStream_t s) {
+  const unsigned blocks = items >= 256 ? 8 : PA_ROWS / RB;
+  hipLaunchKernelGGL((tree_attn_join_kernel<D, FMT, RB>), dim3((unsigned)items, blocks), dim3(PA_NT), 0, s, a);
+}
+
+template <int D, int FMT>
+static hipError_t launch_tree_attn_t(const TreeAttnArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((tree_attn_kernel<D, FMT>), dim3(TA_GRID), dim3(PA_NT), 0, s, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const int64_t items = a.max_items;
+  if (items <= 16) launch_join<D, FMT, 1>(a, items, s);
+  else if (items <= 64) launch_join<D, FMT, 2>(a, items, s);
+  else launch_join<D, FMT, 4>(a, items, s);
+  return hipGetLastError();
+}
+
+hipError_t launch_tree_attn(int dtype, int d, const TreeAttnArgs& a, hipStream_t s) {
+  if (dtype == SDX_BF16)
+    return d == 64 ? launch_tree_attn_t<64, SDX_BF16>(a, s) : launch_tree_attn_t<128, SDX_BF16>(a, s);
+  return d == 64 ? launch_tree_attn_t<64, SDX_F16>(a, s) : launch_tree_attn_t<128, SDX_F16>(a, s);
+}
+
+}  // namespace sdx

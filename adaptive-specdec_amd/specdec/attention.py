@@ -1,7 +1,8 @@
 """Verify attention over the paged KV cache (one layer), on MFMA.
 
 `verify_attention_paged` reads every row's keys; `shared_prefix_attention_paged`
-reads the keys that a group's rows share once for all of them.
+reads the keys that a group's rows share once for all of them; `tree_attention_paged` is for
+rows whose new tokens are a tree (`specdec.tree`).
 
 The attention of the target's verify forward: every batch row's k_b + 1 new
 positions against the row's cached keys, under the mask of
@@ -18,7 +19,7 @@ import torch
 from . import _lib
 
 __all__ = ["verify_attention_paged", "attention_workspace", "shared_prefix_attention_paged",
-           "shared_attention_workspace"]
+           "shared_attention_workspace", "tree_attention_paged", "tree_attention_workspace"]
 
 
 def attention_workspace(B, max_q, hq, hkv, block_size, max_blocks, chunk_tokens=0,
@@ -150,4 +151,80 @@ def shared_prefix_attention_paged(q, cu_q, k_pool, v_pool, block_table, kv_len, 
             _lib.ptr(pl), G, scale, _lib.ptr(workspace), workspace.numel(), _lib.ptr(out),
             _lib.ptr(error), _lib.stream_of(q))
     _lib.check(rc, "shared_prefix_attention_paged")
+    return out
+
+
+def tree_attention_workspace(num_tokens, batch, hq, hkv, head_dim, device="cuda"):
+    """A workspace for tree_attention_paged at these sizes (uint8 device tensor)."""
+    need = _lib.lib().sdx_tree_attention_workspace(int(num_tokens), int(batch), hq, hkv, head_dim)
+    if need == 0:
+        raise ValueError("tree_attention_workspace: nodes, rows and heads of at least 1, query heads a "
+                         "multiple of KV heads, head_dim 64 or 128")
+    return torch.empty(need, dtype=torch.uint8, device=device)
+
+
+def tree_attention_paged(q, cu_q, k_pool, v_pool, block_table, kv_len, tree_mask, scale=None, out=None,
+                         error=None, workspace=None):
+    """`verify_attention_paged` for rows whose new tokens are the nodes of a tree.
+
+    q [T, Hq, d] bf16 or fp16 (head dim d of 64 or 128), row b's n_b nodes at cu_q[b] ..
+    cu_q[b+1] - 1 (cu_q [B+1] int64); k_pool / v_pool [num_blocks, block_size, Hkv * d] of q's
+    type; block_table [B, max_blocks] int32; kv_len [B] int64, keys per row, the nodes, which are
+    its last, included; tree_mask [T, words] int64 of `specdec.tree.tree_layout` (n_b up to 64
+    words and 512). Node i sees the kv_len[b] - n_b keys in front of the nodes and every node
+    j whose bit j % 64 of word j / 64 is set. Returns out [T, Hq, d] of q's type, 0 for a node that
+    sees nothing. Rows out of range are skipped and set `error` (an int32 [1] device tensor) when given, and so do
+    page ids outside the pool. `workspace` (uint8, `tree_attention_workspace`) holds fp32 parts and serves one
+    call at a time; None: the calling thread's own for the current stream, kept for its next calls."""
+    _lib.one_gpu(q, cu_q, k_pool, v_pool, block_table, kv_len, tree_mask, out, error, workspace)
+    if q.dtype not in (torch.bfloat16, torch.float16) or k_pool.dtype != q.dtype or \
+            v_pool.dtype != q.dtype:
+        raise TypeError("tree_attention_paged: q and pools all bf16 or all fp16")
+    if q.dim() != 3 or k_pool.dim() != 3 or k_pool.shape != v_pool.shape:
+        raise ValueError("tree_attention_paged: q [T, Hq, d], k_pool / v_pool [num_blocks, bs, Hkv*d]")
+    T, hq, d = q.shape
+    nb, bs, re = k_pool.shape
+    hkv = re // d
+    if re % d or hkv < 1 or hq % hkv:
+        raise ValueError(f"tree_attention_paged: {hq} query heads of {d} over rows of {re}")
+    if not (k_pool.is_contiguous() and v_pool.is_contiguous()):
+        raise ValueError("tree_attention_paged: pools must be contiguous")
+    if error is not None and (error.dtype != torch.int32 or error.numel() < 1):
+        raise TypeError("tree_attention_paged: error must be an int32 device tensor of one element")
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("tree_attention_paged: workspace must be contiguous")
+    B = kv_len.numel()
+    if cu_q.numel() != B + 1 or block_table.dim() != 2 or block_table.shape[0] != B:
+        raise ValueError(f"tree_attention_paged: {B} lengths need cu_q [{B + 1}] and block_table [{B}, "
+                         f"max_blocks]")
+    if tree_mask.dtype != torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != T or \
+            tree_mask.shape[1] < 1:
+        raise ValueError(f"tree_attention_paged: tree_mask must be int64 [{T}, words], got "
+                         f"{tree_mask.dtype} {tuple(tree_mask.shape)}")
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError("tree_attention_paged: out must be contiguous, of q's shape and type")
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError("tree_attention_paged: scale must be positive and finite")
+    if T == 0:
+        return out
+    q = q.contiguous()
+    if q.data_ptr() % 16:
+        q = q.clone()
+    cu = _lib.as_dtype(cu_q, torch.int64)
+    kl = _lib.as_dtype(kv_len, torch.int64)
+    bt = _lib.as_dtype(block_table, torch.int32)
+    tm = tree_mask.contiguous()
+    with _lib.on_device(q):
+        if workspace is None:
+            need = _lib.workspace_bytes("sdx_tree_attention_workspace", T, B, hq, hkv, d)
+            workspace = _lib.cached_workspace(need, q.device, "tree_attn")
+        rc = _lib.lib().sdx_tree_attention_paged(
+            _lib.ptr(q), _lib.dtype_code(q), T, B, _lib.ptr(cu), hq, hkv, d, _lib.ptr(k_pool),
+            _lib.ptr(v_pool), nb, bs, _lib.ptr(bt), bt.shape[1], _lib.ptr(kl), _lib.ptr(tm), tm.shape[1],
+            scale, _lib.ptr(workspace), workspace.numel(), _lib.ptr(out), _lib.ptr(error),
+            _lib.stream_of(q))
+    _lib.check(rc, "tree_attention_paged")
     return out

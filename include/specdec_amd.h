@@ -606,6 +606,30 @@ int sdx_prefix_attention_paged(const void* q, int dtype, int64_t num_tokens, int
 size_t sdx_prefix_attention_workspace(int64_t num_tokens, int64_t batch, int64_t num_groups,
                                       int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim);
 
+/* ---- attention of trees of drafted tokens: as sdx_verify_attention_paged, one layer, where row b's
+ * n_b = cu_q[b+1] - cu_q[b] new tokens are the nodes of a tree (sdx_tree_layout), appended as the last
+ * of its kv_len[b] keys in the order of the nodes. Node i sees the kv_len[b] - n_b keys in front of
+ * the nodes and every node j whose bit j % 64 of word j / 64 of its tree_mask [num_tokens, mask_words]
+ * int64 is set; bits from n_b on are not looked at. q / out: [num_tokens, num_q_heads, head_dim], bf16
+ * or fp16 as the pools, 16-byte aligned; n_b up to 64 mask_words and 512; head_dim 64 or 128; scale
+ * positive, scale log2(e) finite. Softmax and sums in fp32, weights rounded to the type for the second
+ * product, output rounded to it. Keys and values that a node does not see do not reach its output,
+ * whatever they hold. A NaN among the scores that a node sees makes its output NaN; where all of them
+ * are -inf, or it sees none, it is 0. Rows whose lengths or offsets are out of range set *error
+ * (nullable) and leave their output as it was; tokens behind the last row too, without the error. Page
+ * ids outside the pool set *error and the output of the rows that read them is unspecified. Two kernels
+ * are queued; `workspace` (sdx_tree_attention_workspace bytes, no initial contents) holds fp32 parts.
+ * A row's bits depend on the whole batch's lengths. No reference counterpart. */
+int sdx_tree_attention_paged(const void* q, int dtype, int64_t num_tokens, int64_t batch,
+                             const int64_t* cu_q, int32_t num_q_heads, int32_t num_kv_heads,
+                             int32_t head_dim, const void* k_pool, const void* v_pool,
+                             int64_t num_blocks, int32_t block_size, const int32_t* block_table,
+                             int64_t max_blocks, const int64_t* kv_len, const int64_t* tree_mask,
+                             int32_t mask_words, float scale, void* workspace, size_t workspace_bytes,
+                             void* out, int32_t* error, sdx_stream_t stream);
+size_t sdx_tree_attention_workspace(int64_t num_tokens, int64_t batch, int32_t num_q_heads,
+                                    int32_t num_kv_heads, int32_t head_dim);
+
 #ifdef __cplusplus
 }
 #endif

@@ -162,3 +162,30 @@ def test_penalty_oracle_by_hand():
     assert out[0].tolist() == [1.0 - 0.25 - 1.0, -4.0 - 0.5 - 1.0, 2.5, 0.5]
     assert out[1].tolist() == [-0.25, -np.inf, 2.5, 0.25 - 0.25 - 1.0]
     assert touched.tolist() == [[True, True, True, False], [True] * 4]
+
+
+def test_tree_attention_statuses():
+    from specdec import _lib
+    L = _lib.lib()
+
+    def call(T=3, B=2, hq=4, hkv=2, d=64, dtype=BF16, nb=8, bs=16, mb=4, words=1, scale=0.1, q=FAKE, pool=FAKE,
+             mask=FAKE, out=FAKE, ws=FAKE, nbytes=None):
+        need = L.sdx_tree_attention_workspace(max(T, 1), max(B, 1), max(hq, 1), max(hkv, 1), d)
+        return L.sdx_tree_attention_paged(q, dtype, T, B, FAKE, hq, hkv, d, pool, FAKE, nb, bs, FAKE, mb, FAKE,
+                                          mask, words, scale, ws, need if nbytes is None else nbytes, out, None,
+                                          None)
+
+    assert call(T=0) == OK
+    for bad in (dict(T=-1), dict(B=-1), dict(B=0), dict(hq=0), dict(hq=3), dict(hkv=0), dict(bs=0), dict(mb=0),
+                dict(nb=0), dict(words=0), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf")),
+                dict(scale=3e38), dict(q=None), dict(mask=None), dict(out=None), dict(q=OFF), dict(pool=OFF),
+                dict(out=OFF)):
+        assert call(**bad) == EINVAL, bad
+    for bad in (dict(d=96), dict(d=256), dict(dtype=F32), dict(mb=1 << 28), dict(nb=1 << 29), dict(T=1 << 24)):
+        assert call(**bad) == EUNSUP, bad
+    need = L.sdx_tree_attention_workspace(3, 2, 4, 2, 64)
+    assert call(nbytes=need - 1) == EWS and call(ws=None) == EWS and call(ws=OFF) == EWS
+    assert L.sdx_tree_attention_workspace(0, 2, 4, 2, 64) == 0
+    assert L.sdx_tree_attention_workspace(3, 2, 4, 3, 64) == 0
+    # two parts a workgroup, however many nodes there are
+    assert L.sdx_tree_attention_workspace(1 << 16, 2048, 32, 8, 128) <= 80 << 20
