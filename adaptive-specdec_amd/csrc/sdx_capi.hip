@@ -981,9 +981,9 @@ int sdx_penalize_logits(const void* logits, int dtype, int64_t rows, int64_t voc
   if (l0 < o0 + ob && o0 < l0 + lb && !(l0 == o0 && ld == out_ld))
     return fail(SDX_EINVAL, "sdx_penalize_logits: out may be the logits themselves or lie apart from them");
   if (num_biases > sdx::PN_MAX_BIAS || (history && max_history > sdx::PN_HISTORY) || vocab > ((int64_t)1 << 30) ||
-      rows > ((int64_t)1 << 21))
+      rows > ((int64_t)1 << 21) || rows * (vocab / 2048 + 2) > 0xFFFFFFFFll)
     return fail(SDX_EUNSUPPORTED, "sdx_penalize_logits: more than %d bias entries or %lld history tokens in a "
-                                  "row, 2^30 tokens or 2^21 rows", sdx::PN_MAX_BIAS, (long long)sdx::PN_HISTORY);
+                                  "row, 2^30 tokens, 2^21 rows or 2^43 logits", sdx::PN_MAX_BIAS, (long long)sdx::PN_HISTORY);
   sdx::PenalizeArgs a = {};
   a.logits = logits; a.out = out; a.rows = rows; a.V = vocab; a.ld = ld; a.out_ld = out_ld; a.batch = batch;
   a.cu_rows = cu_rows; a.history = history; a.history_ld = history_ld; a.max_history = max_history;
@@ -992,7 +992,7 @@ int sdx_penalize_logits(const void* logits, int dtype, int64_t rows, int64_t voc
   a.bias_ids = bias_ids; a.bias = bias; a.biases = num_biases;
   a.allowed = (const uint32_t*)allowed; a.allowed_ld = allowed_ld;
   a.node_tokens = node_tokens; a.tree_mask = tree_mask; a.mask_words = mask_words; a.error = error;
-  a.vec = aligned16(logits) && aligned16(out) && (rows == 1 || (ld * es % 16 == 0 && out_ld * es % 16 == 0));
+  a.vec = ((uintptr_t)logits - (uintptr_t)out) % 16 == 0 && (rows == 1 || (ld - out_ld) * (int64_t)es % 16 == 0);
   return hip_status(sdx::launch_penalize(dtype, a, (hipStream_t)stream), "penalize");
 }
 

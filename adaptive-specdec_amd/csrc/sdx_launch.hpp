@@ -665,7 +665,7 @@ hipError_t launch_tree_attn(int dtype, int d, const TreeAttnArgs& a, hipStream_t
 
 // sdx_penalty.hip
 constexpr int PN_MAX_BIAS = 1024;              // entries of a row
-constexpr int64_t PN_HISTORY = (1 << 20) - 1;  // tokens of a row's history
+constexpr int64_t PN_HISTORY = 1000000;        // tokens of a row's history
 struct PenalizeArgs {
   const void* logits;           // [rows, ld]
   void* out;                    // [rows, out_ld]
@@ -685,8 +685,8 @@ struct PenalizeArgs {
   const int64_t* tree_mask;     // [rows, mask_words], or null: chains
   int32_t mask_words;
   int32_t* error;
-  int64_t rows_each;            // of a workgroup (set by the launch)
-  bool vec;                     // rows of both start at multiples of 16 bytes
+  uint32_t each, more;          // units of a workgroup; workgroups that have one more (set by the launch)
+  bool vec;                     // rows of both lie alike to multiples of 16 bytes
 };
 hipError_t launch_penalize(int dtype, const PenalizeArgs& a, hipStream_t s);
 

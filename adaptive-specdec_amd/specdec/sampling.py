@@ -233,7 +233,7 @@ def penalize_logits(logits, history=None, history_len=None, cu_rows=None, *, pro
 
         x = l > 0 ? l / repetition[b] : l * repetition[b]   of tokens in the history or on the path
         x -= frequency[b] * c, then x -= presence[b]        of tokens written c > 0 times
-        x += bias[b, e]                                     of token bias_ids[b, e], entry by entry
+        x += b                                              the sum, in order, of bias[b, e] of token bias_ids[b, e]
         x = -inf                                            where the grammar refuses the token
 
     history [B, H] int64, of which history_len [B] tokens count and the first prompt_len [B] (None: 0) are the

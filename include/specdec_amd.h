@@ -339,7 +339,7 @@ int sdx_slot_mapping(const int32_t* block_table, int64_t rows, int64_t max_block
  * token v, in fp32 and rounded once:
  *   x = l > 0 ? l / repetition[b] : l * repetition[b]  where v is in the history or on the path
  *   x -= frequency[b] * c, then x -= presence[b]       where v was written c > 0 times
- *   x += bias[b, e]                                    for every e with bias_ids[b, e] = v, in order
+ *   x += b                                             the sum, in order, of bias[b, e] with bias_ids[b, e] = v
  *   x = -inf                                           where bit v % 32 of allowed[row, v / 32] is clear
  * The history is history[b, 0 .. history_len[b]) (int64 [batch, history_ld], of max_history columns), its
  * first prompt_len[b] (nullable: 0) tokens the prompt, which repetition alone goes by; the others are
@@ -351,7 +351,7 @@ int sdx_slot_mapping(const int32_t* block_table, int64_t rows, int64_t max_block
  * int32 [rows, allowed_ld], nullable. Ids outside [0, vocab) count nowhere. Logits that nothing concerns keep
  * their bits; a row whose every token is refused is -inf throughout. Rows of no batch row, and those of a batch row
  * whose lengths or offsets are out of range, are copied as they are; the latter set *error (nullable). One
- * kernel. Up to 1,024 bias entries, 2^20 - 1 history tokens, 512 nodes in a row (with node_tokens). No
+ * kernel. Up to 1,024 bias entries, a million history tokens, 512 nodes in a row (with node_tokens). No
  * reference counterpart. */
 int sdx_penalize_logits(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, void* out,
                         int64_t out_ld, int64_t batch, const int64_t* cu_rows, const int64_t* history,
