@@ -126,11 +126,11 @@ template <int D>
 __device__ __forceinline__ int pa_swz_v(int r) { return D == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); }
 
 // O^T += V^T P^T for NB x 32 keys. va: the lane's byte address in V's first row block. The
-// operands of four products are read ahead.
-template <int D, int FMT, int NB>
+// operands of AHEAD products are read ahead.
+template <int D, int FMT, int NB, int AHEAD = 4>
 __device__ __forceinline__ void pa_pv(PaState<D>& st, const pa_f16 (&s)[NB], const uint8_t* sV,
                                       uint32_t va) {
-  constexpr int DB = D / 32, N = NB * 2 * DB, AHEAD = 4;
+  constexpr int DB = D / 32, N = NB * 2 * DB;
   pa_u4 x[AHEAD];
   auto read = [&](int j) {  // product j: keys 16 (j / DB) .., dims 32 (j % DB) ..
     const uint8_t* const at = sV + (va ^ ((j % DB) << 6)) + 16 * (j / DB) * 2 * D;

@@ -1467,8 +1467,8 @@ static size_t tree_attn_ws(Carve& c, int64_t tokens, int64_t batch, int32_t hq, 
   a->head = c.take<uint32_t>(64);
   a->max_items = sdx::tree_attn_items(tokens, batch, hkv, hq / hkv);
   a->items = c.take<sdx::TreeAttnItem>((size_t)a->max_items);
-  a->part_ml = c.take<float2>((size_t)2 * sdx::TREE_ATTN_GRID * 128);
-  a->part_o = c.take<float>((size_t)2 * sdx::TREE_ATTN_GRID * 128 * d);
+  a->part_ml = c.take<float2>((size_t)2 * sdx::TREE_ATTN_GRID * sdx::TREE_ATTN_ROWS);
+  a->part_o = c.take<float>((size_t)2 * sdx::TREE_ATTN_GRID * sdx::TREE_ATTN_ROWS * d);
   return c.used;
 }
 

@@ -636,8 +636,9 @@ hipError_t launch_copy_pages(const CopyPagesArgs& a, hipStream_t s);
 
 
 // sdx_tree_attn.hip
-constexpr int TREE_ATTN_GRID = 512;  // workgroups
-struct TreeAttnItem {  // 128 query rows of a row, and the workgroups that have its keys
+constexpr int TREE_ATTN_GRID = 256;  // workgroups
+constexpr int TREE_ATTN_ROWS = 256;  // query rows of an item
+struct TreeAttnItem {  // query rows of a row, and the workgroups that have its keys
   int32_t t0, kvh, r0, m;      // the row's first token, KV head, first query row, query rows
   int32_t first, parts, pad[2];
 };
@@ -657,8 +658,8 @@ struct TreeAttnArgs {
   uint32_t* head;              // [64] the items
   TreeAttnItem* items;         // [max_items]
   int64_t max_items;
-  float2* part_ml;             // [2 TREE_ATTN_GRID, 128] max and sum of each part's query rows
-  float* part_o;               // [2 TREE_ATTN_GRID, 128, d]
+  float2* part_ml;             // [2 TREE_ATTN_GRID, TREE_ATTN_ROWS] max and sum of each part's query rows
+  float* part_o;               // [2 TREE_ATTN_GRID, TREE_ATTN_ROWS, d]
 };
 int64_t tree_attn_items(int64_t tokens, int64_t batch, int32_t hkv, int32_t group);
 hipError_t launch_tree_attn(int dtype, int d, const TreeAttnArgs& a, hipStream_t s);

@@ -26,12 +26,9 @@
 
 namespace sdx {
 
-#ifndef PN_S
-#define PN_S 8192
-#define PN_WGS 1024
-#define PN_THR 256
-#endif
-constexpr int PN_NT = PN_THR;
+constexpr int PN_NT = 256;
+constexpr int PN_S = 8192;    // tokens of a slice of 16-bit logits
+constexpr int PN_WGS = 1024;  // workgroups that the chip holds at once, by their LDS
 constexpr int PN_UN = 8;   // history tokens in flight per thread
 // a token's word: seen in the history, 1 + the index of its bias, times written
 constexpr uint32_t PN_SEEN = 0x80000000u, PN_COUNT = (1u << 20) - 1;

@@ -5,7 +5,7 @@
 //
 //   out_i = sum_s p_s v_s / sum_s p_s,  p_s = 2^(scale log2(e) q_i k_s - m)
 //
-// An item is a tile of 128 query rows (nodes x the query heads of a KV head) of a row against
+// An item is a tile of 256 query rows (nodes x the query heads of a KV head) of a row against
 // all of its keys, in tiles of 64 that never hold cache and nodes both: cache tiles are bare but
 // for the last one's end, a node tile takes one 64-bit word of each query row's mask. The items'
 // tiles lie one behind another on a line, TA_COST more in front of each for what an item costs
@@ -21,33 +21,43 @@
 
 namespace sdx {
 
-constexpr int TA_GRID = TREE_ATTN_GRID;  // two workgroups on each of 256 CUs
-constexpr uint32_t TA_COST = 2;          // tiles that an item costs beside its own
+constexpr int TA_GRID = TREE_ATTN_GRID;  // a workgroup on each of 256 CUs
+constexpr int TA_NT = 512;               // two waves per SIMD
+constexpr int TA_NW = TA_NT / kWave;
+constexpr int TA_ROWS = TREE_ATTN_ROWS;  // query rows of an item, 32 per wave
+constexpr int TA_RING = 2 * TA_NW;       // tiles of slots
+static_assert(TA_ROWS == TA_NW * PA_WROWS, "every wave has rows of a full item");
+constexpr uint32_t TA_COST = 4;          // tiles that an item costs beside its own
 constexpr uint32_t TA_LEAST = 2;         // tiles of a stretch, at least
 
 struct TaRow {
-  int64_t t0, ctx;      // first node's token; keys in front of the nodes
+  int32_t t0, ctx;      // first node's token; keys in front of the nodes
   int32_t n, ct, kt;    // nodes; tiles of the cache, and with the nodes'
   int32_t qt;           // tiles of query rows
   bool ok;
-  __device__ __forceinline__ uint64_t len() const { return (uint64_t)kt + TA_COST; }
+  __device__ __forceinline__ uint32_t len() const { return (uint32_t)kt + TA_COST; }
 };
 __device__ __forceinline__ TaRow ta_row(const TreeAttnArgs& a, int64_t b) {
   TaRow r;
-  const int64_t t1 = a.cu_q[b + 1], kv = a.kv_len[b];
-  r.t0 = a.cu_q[b];
-  const int64_t n = t1 - r.t0;
-  r.ok = r.t0 >= 0 && n >= 0 && t1 <= a.tokens && n <= min(a.words * 64, TREE_MAX_NODES) && kv >= n &&
-         kv <= a.max_blocks * a.bs;
+  const int64_t t0 = a.cu_q[b], t1 = a.cu_q[b + 1], kv = a.kv_len[b], n = t1 - t0;
+  r.ok = t0 >= 0 && n >= 0 && t1 <= a.tokens && n <= min(a.words * 64, TREE_MAX_NODES) && kv >= n &&
+         kv <= a.max_blocks * a.bs;  // 2^30 keys, 2^23 tokens at most
+  r.t0 = (int32_t)t0;
   r.n = r.ok ? (int32_t)n : 0;
-  r.ctx = kv - n;
-  r.ct = r.ok ? (int32_t)((r.ctx + PA_TILE - 1) / PA_TILE) : 0;
+  r.ctx = r.ok ? (int32_t)(kv - n) : 0;
+  r.ct = (r.ctx + PA_TILE - 1) / PA_TILE;
   r.kt = r.ct + (r.n + PA_TILE - 1) / PA_TILE;
-  r.qt = (r.n * a.group + PA_ROWS - 1) / PA_ROWS;
+  r.qt = (r.n * a.group + TA_ROWS - 1) / TA_ROWS;
   return r;
 }
 __device__ __forceinline__ uint32_t ta_items(const TreeAttnArgs& a, const TaRow& r) {
   return (uint32_t)(r.qt * a.hkv);
+}
+
+// a value that is the same in all lanes, as a scalar
+__device__ __forceinline__ uint64_t ta_uniform(uint64_t x) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32 |
+         (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)x);
 }
 
 struct TaScan {
@@ -56,7 +66,6 @@ struct TaScan {
 };
 // sums over the workgroup's threads, in their order
 __device__ __forceinline__ TaScan ta_scan(uint64_t line, uint64_t items, uint64_t* sLine, uint64_t* sItem) {
-  constexpr int NW = PA_NT / kWave;
   const int lane = threadIdx.x & (kWave - 1), wv = threadIdx.x / kWave;
   const uint64_t li = wave_incl_scan_u64(line, lane);
   const uint64_t ii = wave_incl_scan_u64(items, lane);
@@ -64,37 +73,39 @@ __device__ __forceinline__ TaScan ta_scan(uint64_t line, uint64_t items, uint64_
   __syncthreads();
   TaScan r{li - line, 0, ii - items, 0};
 #pragma unroll
-  for (int w = 0; w < NW; ++w) {
+  for (int w = 0; w < TA_NW; ++w) {
     if (w < wv) r.line += sLine[w], r.item += sItem[w];
     r.lines += sLine[w], r.items += sItem[w];
   }
   __syncthreads();
+  r.lines = ta_uniform(r.lines), r.items = ta_uniform(r.items);
   return r;
 }
 
 // S^T = K Q^T for a tile's 64 keys. ka: the lane's byte address in K's first row block.
 template <int D, int FMT>
 __device__ __forceinline__ void ta_qk(pa_f16 (&s)[2], const pa_u4 (&qa)[D / 16], const uint8_t* k, uint32_t ka) {
-  constexpr int RB = 2 * D;
-  pa_u4 x[2][2];  // operands of a step, read a step ahead
+  constexpr int RB = 2 * D, N = D / 16, AHEAD = 2;
+  pa_u4 x[AHEAD][2];  // operands of the steps to come
   auto read = [&](int ks) {
 #pragma unroll
     for (int n = 0; n < 2; ++n)
-      x[ks & 1][n] = *reinterpret_cast<const pa_u4*>(k + (ka ^ (ks << 5)) + n * 32 * RB);
+      x[ks % AHEAD][n] = *reinterpret_cast<const pa_u4*>(k + (ka ^ (ks << 5)) + n * 32 * RB);
   };
-  read(0);
 #pragma unroll
-  for (int ks = 0; ks < D / 16; ++ks) {
-    if (ks + 1 < D / 16) read(ks + 1);
+  for (int ks = 0; ks < AHEAD; ++ks) read(ks);
 #pragma unroll
-    for (int n = 0; n < 2; ++n) s[n] = pa_mfma<FMT>(x[ks & 1][n], qa[ks], s[n]);
+  for (int ks = 0; ks < N; ++ks) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) s[n] = pa_mfma<FMT>(x[ks % AHEAD][n], qa[ks], s[n]);
+    if (ks + AHEAD < N) read(ks + AHEAD);
   }
-  // in this order: two steps' reads, then a step's products and the reads after next
-  __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+  // in this order: the first reads, then a step's products and the reads that follow them
+  __builtin_amdgcn_sched_group_barrier(0x100, 2 * AHEAD, 0);
 #pragma unroll
-  for (int ks = 0; ks < D / 16; ++ks) {
+  for (int ks = 0; ks < N; ++ks) {
     __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-    if (ks + 2 < D / 16) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    if (ks + AHEAD < N) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
   }
 }
 
@@ -117,18 +128,18 @@ __device__ __forceinline__ uint64_t ta_valid(int n, int k) {
 
 // a stretch of an item
 struct TaUnit {
-  int64_t b, t0, ctx;
+  int32_t t0, ctx;
   int32_t n, ct, kvh, r0, m;  // r0, m: first query row, query rows
   int32_t lo, hi;             // tiles
   int32_t part;               // -1: whole, written directly
 };
 // token of query row i of the unit
 __device__ __forceinline__ int64_t ta_token(const TreeAttnArgs& a, const TaUnit& u, int i) {
-  return u.t0 + (uint32_t)(u.r0 + i) / (uint32_t)a.group;
+  return u.t0 + (int32_t)((uint32_t)(u.r0 + i) / (uint32_t)a.group);
 }
 __device__ __forceinline__ int64_t ta_qrow(const TreeAttnArgs& a, const TaUnit& u, int i) {
   const uint32_t r = u.r0 + i, j = r / (uint32_t)a.group;
-  return (u.t0 + j) * a.hq + u.kvh * a.group + (r - j * a.group);
+  return (int64_t)(u.t0 + j) * a.hq + u.kvh * a.group + (r - j * a.group);
 }
 // the word of query row i's mask for nodes 64 k ..
 __device__ __forceinline__ uint64_t ta_word(const TreeAttnArgs& a, const TaUnit& u, int i, int k) {
@@ -164,14 +175,23 @@ __device__ __forceinline__ void ta_add_odd(PaState<D>& st, const TreeAttnArgs& a
   }
 }
 
+// 16 bytes of each lane from its own address to the 1 KB at LDS byte `to`, lane after lane, without
+// a register in between. The compiler does not count it: ta_wait waits for it.
+__device__ __forceinline__ void ta_load_lds(const uint8_t* from, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+}
+__device__ __forceinline__ void ta_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 template <int D, int FMT>
-__global__ void __launch_bounds__(PA_NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ void __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 tree_attn_kernel(TreeAttnArgs a) {
   constexpr int NC = D / 8;            // 16-byte chunks of a row
   constexpr int RB = 2 * D;            // bytes of a row
-  __shared__ __align__(256) uint8_t sMem[2 * 2 * PA_TILE * RB];  // two tiles of K and V
-  __shared__ uint32_t sSlot[PA_RING * PA_TILE];
-  __shared__ uint64_t sLine[PA_NT / kWave], sItem[PA_NT / kWave], sAt[2];
+  constexpr uint32_t KB = PA_TILE * RB, TB = 2 * KB;  // bytes of a tile's K, of its K and V
+  constexpr int NB = D == 128 ? 4 : 8, PT = NB / 2;   // tiles in LDS, half of them in use
+  __shared__ __align__(1024) uint8_t sMem[NB * TB];
+  __shared__ uint32_t sSlot[TA_RING * PA_TILE];
+  __shared__ uint64_t sLine[TA_NW], sItem[TA_NW], sAt[2];
   __shared__ int sOdd;  // V of the unit has elements that ta_add_odd adds
   // the wave's index and the unit are made scalar: what follows from them takes no vector
   // registers, of which a wave of two per SIMD has 256
@@ -184,37 +204,40 @@ tree_attn_kernel(TreeAttnArgs a) {
   const int vr = 4 * hi + ((lane & 15) >> 2), vd = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
   const uint32_t va = vr * RB + (((vd >> 3) ^ pa_swz_v<D>(vr)) << 4) + (vd & 7) * 2;
 
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)sMem;
+
   // the line: its length, this workgroup's stretch, the row that the stretch starts in.
   // Neighbours on the line share an XCD (workgroup index % 8), whose L2 their keys go through.
   const uint32_t wg = blockIdx.x % 8 * (TA_GRID / 8) + blockIdx.x / 8;
-  uint64_t total, step, pos = 0, from = 0;  // from: where row b starts
+  uint32_t total, step, pos = 0, from = 0;  // from: where row b starts
   uint32_t item0 = 0;
   int64_t b = 0;
   {
-    const bool one = a.batch <= PA_NT;
+    const bool one = a.batch <= TA_NT;
     uint64_t line = 0, items = 0;
     int bad = 0;
-    for (int64_t i = tid; i < a.batch; i += PA_NT) {
+    for (int64_t i = tid; i < a.batch; i += TA_NT) {
       const TaRow r = ta_row(a, i);
       bad |= !r.ok;
       const uint32_t n = ta_items(a, r);
-      line += n * r.len();
+      line += (uint64_t)n * r.len();
       items += n;
     }
     TaScan sc = ta_scan(line, items, sLine, sItem);
-    const bool over = sc.items > (uint64_t)a.max_items;  // rows that share nodes: offsets out of order
+    // rows that share nodes (offsets out of order); a line of 2^32 tiles takes half a minute
+    const bool over = sc.items > (uint64_t)a.max_items || sc.lines >> 32;
     if ((bad || over) && a.error && blockIdx.x == 0) *a.error = 1;
     if (blockIdx.x == 0 && tid == 0) a.head[0] = over ? 0u : (uint32_t)sc.items;
-    total = over ? 0 : sc.lines;
-    step = max((total + TA_GRID - 1) / TA_GRID, (uint64_t)TA_LEAST);
+    total = over ? 0 : (uint32_t)sc.lines;
+    step = max(total / TA_GRID + (total % TA_GRID > 0), TA_LEAST);
     pos = wg * step;
-    if (pos >= total) return;  // uniform
+    if ((uint64_t)wg * step >= total) return;  // uniform
     uint64_t at = 0, it = 0;
-    for (int64_t b0 = 0;; b0 += PA_NT) {  // uniform; ends where the line holds pos
+    for (int64_t b0 = 0;; b0 += TA_NT) {  // uniform; ends where the line holds pos
       if (!one) {
         const TaRow r = b0 + tid < a.batch ? ta_row(a, b0 + tid) : TaRow{};
         items = b0 + tid < a.batch ? ta_items(a, r) : 0;
-        line = items ? items * r.len() : 0;
+        line = items ? items * (uint64_t)r.len() : 0;
         sc = ta_scan(line, items, sLine, sItem);
       }
       if (at + sc.line <= pos && pos < at + sc.line + line) {
@@ -225,36 +248,34 @@ tree_attn_kernel(TreeAttnArgs a) {
       if (pos < at) break;
     }
     __syncthreads();
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)sAt[0]);
-    const uint32_t up = __builtin_amdgcn_readfirstlane((uint32_t)(sAt[0] >> 32));
-    from = (uint64_t)up << 32 | lo;
-    item0 = __builtin_amdgcn_readfirstlane((uint32_t)sAt[1]);
-    b = __builtin_amdgcn_readfirstlane((uint32_t)(sAt[1] >> 32));
+    from = (uint32_t)ta_uniform(sAt[0]);
+    const uint64_t x = ta_uniform(sAt[1]);
+    item0 = (uint32_t)x;
+    b = (int64_t)(x >> 32);
   }
-  const uint64_t end = min(total, pos + step);
+  const uint32_t end = min((uint64_t)total, (uint64_t)pos + step);
 
   TaRow row = ta_row(a, b);
   while (pos < end) {  // uniform: the items of the stretch
-    const uint64_t len = row.len();
-    const uint32_t item = (uint32_t)((pos - from) / len);
-    const uint64_t p = from + item * len, e = min(end, p + len);
-    const uint32_t first = (uint32_t)((p + TA_COST) / step), last = (uint32_t)((p + len - 1) / step);
+    const uint32_t len = row.len(), item = (pos - from) / len;
+    const uint32_t p = from + item * len, e = min(end, p + len);
+    const uint32_t first = (p + TA_COST) / step, last = (p + len - 1) / step;
     TaUnit u;
-    u.b = b, u.t0 = row.t0, u.ctx = row.ctx;
+    u.t0 = row.t0, u.ctx = row.ctx;
     u.n = row.n, u.ct = row.ct;
     u.kvh = item / row.qt;
-    u.r0 = (int32_t)(item - u.kvh * row.qt) * PA_ROWS;
-    u.m = min(PA_ROWS, row.n * a.group - u.r0);
-    u.lo = (int32_t)(max(pos - p, (uint64_t)TA_COST) - TA_COST);
-    u.hi = (int32_t)(max(e - p, (uint64_t)TA_COST) - TA_COST);
+    u.r0 = (int32_t)(item - u.kvh * row.qt) * TA_ROWS;
+    u.m = min(TA_ROWS, row.n * a.group - u.r0);
+    u.lo = (int32_t)(max(pos - p, TA_COST) - TA_COST);
+    u.hi = (int32_t)(max(e - p, TA_COST) - TA_COST);
     u.part = first == last ? -1 : (int32_t)(2 * wg + (wg == first));
     if (wg == first && u.lo < u.hi && tid == 0)
       a.items[item0 + item] = TreeAttnItem{(int32_t)u.t0, u.kvh, u.r0, u.m, (int32_t)first,
                                            (int32_t)(last - first + 1), 0, 0};
     pos = e;
-    const uint64_t row_end = from + (uint64_t)row.qt * a.hkv * len;
+    const uint32_t row_end = from + ta_items(a, row) * len;
     if (u.lo < u.hi) {
-      const int32_t* const table = a.block_table + u.b * a.max_blocks;
+      const int32_t* const table = a.block_table + b * a.max_blocks;
       const uint8_t* const kp = reinterpret_cast<const uint8_t*>(a.k_pool + u.kvh * D);
       const uint8_t* const vp = reinterpret_cast<const uint8_t*>(a.v_pool + u.kvh * D);
       int bad = 0;
@@ -277,108 +298,115 @@ tree_attn_kernel(TreeAttnArgs a) {
         }
       }
       uint64_t word = u.hi > u.ct ? ta_word(a, u, r0 + l31, max(u.lo, u.ct) - u.ct) : 0;
-
-      constexpr int H = NC / 4, TPR = PA_NT / NC;  // passes, rows per pass
       const int ntile = u.hi - u.lo;
-      const int lr = tid / NC, lc = tid % NC;
-      // slots of the unit's tiles, four tiles at a time, one by each wave: page ids are loaded
-      // four tiles before they are needed here, eight before their keys
-      auto key = [&](int tile) -> int64_t {  // position of the lane's key of a tile, -1: none
+      // slots of the unit's tiles, eight tiles at a time, one by each wave: page ids are loaded
+      // eight tiles before they are needed here
+      auto key = [&](int tile) -> int32_t {  // position of the lane's key of a tile, -1: none
         const int t = u.lo + tile;
         if (t >= u.hi) return -1;
-        const int64_t x = t < u.ct ? (int64_t)t * PA_TILE + lane : (int64_t)(t - u.ct) * PA_TILE + lane;
+        const int x = (t < u.ct ? t : t - u.ct) * PA_TILE + lane;
         if (t < u.ct) return x < u.ctx ? x : -1;
         return x < u.n ? u.ctx + x : -1;
       };
       auto page_of = [&](int tile) {
-        const int64_t x = key(tile);
+        const int32_t x = key(tile);
         return x >= 0 ? table[(uint32_t)x / (uint32_t)a.bs] : 0;
       };
       auto put_slot = [&](int tile, int32_t page) {
-        const int64_t x = key(tile);
+        const int32_t x = key(tile);
         uint32_t s = PA_NOSLOT;
         if (x >= 0) {
           if (page >= 0 && page < a.num_blocks) s = (uint32_t)page * (uint32_t)a.bs + (uint32_t)x % (uint32_t)a.bs;
           bad |= s == PA_NOSLOT;
         }
-        sSlot[(tile % PA_RING) * PA_TILE + lane] = s;
+        sSlot[(tile % TA_RING) * PA_TILE + lane] = s;
       };
-      pa_u4 kk[H], vv[H];
-      uint32_t none;  // passes whose key is none: their V is 0 for the products, their K never seen
-      auto gather = [&](int tile) {
-        none = 0;
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-          const uint32_t s = sSlot[(tile % PA_RING) * PA_TILE + lr + TPR * h];
-          const uint64_t off = (uint64_t)(s == PA_NOSLOT ? 0u : s) * row_bytes;
-          none |= (s == PA_NOSLOT ? 1u : 0u) << h;
-          kk[h] = *reinterpret_cast<const pa_u4*>(kp + off + lc * 16);
-          vv[h] = *reinterpret_cast<const pa_u4*>(vp + off + lc * 16);
-        }
+      // Tile t lies in LDS part t % NB. A wave's load fills 1 KB of it, RW rows; 16-byte chunk c of row
+      // r lies in chunk c ^ swizzle(r), so the lanes ask for their chunks in that order. A key that is
+      // none takes row 0 of the pool: its K is never seen, its V is 0 by `clean`.
+      constexpr int RW = 1024 / RB, PW = PA_TILE / RW / TA_NW;  // loads of a wave for K, and for V
+      const int lr = lane / NC, lc = lane % NC;
+      auto slot = [&](int tile, int h) { return sSlot[(tile % TA_RING) * PA_TILE + (w * PW + h) * RW + lr]; };
+      auto load = [&](int tile, int h, uint32_t sl) {
+        const uint32_t at = lds0 + (uint32_t)(tile % NB) * TB + (w * PW + h) * 1024;
+        const int r = (w * PW + h) * RW + lr;
+        const uint64_t off = (uint64_t)(sl == PA_NOSLOT ? 0u : sl) * row_bytes;
+        ta_load_lds(kp + off + ((lc ^ pa_swz_k<D>(r)) << 4), at);
+        ta_load_lds(vp + off + ((lc ^ pa_swz_v<D>(r)) << 4), at + KB);
       };
-      static_assert(TPR % 16 == 0, "a pass's rows are swizzled alike");
-      const uint32_t kw = lr * RB + ((lc ^ pa_swz_k<D>(lr)) << 4);
-      const uint32_t vw = lr * RB + ((lc ^ pa_swz_v<D>(lr)) << 4);
-      auto stage = [&](auto buf, int tile) {
-        uint8_t* const k = sMem + buf * (2 * PA_TILE * RB);
-        if ((u.lo + tile + 1) * (int64_t)PA_TILE > u.ctx) {  // uniform: the cache's last tile, the nodes'
+      // V of the cache's last tile and of the nodes': rows of no key are 0, and so are elements that
+      // ta_add_odd adds
+      auto clean = [&](int tile) {
+        const int g = u.lo + tile, last = g < u.ct ? u.ctx - g * PA_TILE : u.n - (g - u.ct) * PA_TILE;
+        uint8_t* const v = sMem + (tile % NB) * TB + KB;
 #pragma unroll
-          for (int h = 0; h < H; ++h)
-            if ((none >> h) & 1) vv[h] = (pa_u4){0, 0, 0, 0};
-          if (u.lo + tile >= u.ct && pa_finite_only<FMT, H>(vv)) sOdd = 1;
-        }
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-          *reinterpret_cast<pa_u4*>(k + kw + TPR * h * RB) = kk[h];
-          *reinterpret_cast<pa_u4*>(k + vw + (PA_TILE + TPR * h) * RB) = vv[h];
+        for (int h = 0; h < PA_TILE * NC / TA_NT; ++h) {
+          const int c = tid + h * TA_NT;
+          pa_u4 x[1] = {*reinterpret_cast<const pa_u4*>(v + c * 16)};
+          if (c / NC >= last) x[0] = (pa_u4){0, 0, 0, 0};
+          if (g >= u.ct && pa_finite_only<FMT, 1>(x)) sOdd = 1;
+          *reinterpret_cast<pa_u4*>(v + c * 16) = x[0];
         }
       };
       __syncthreads();  // the unit before is done with LDS
       put_slot(w, page_of(w));
-      int32_t page = page_of(4 + w);
+      int32_t page = page_of(TA_NW + w);
       if (tid == 0) sOdd = 0;
       __syncthreads();
-      typedef std::integral_constant<int, 0> even;
-      typedef std::integral_constant<int, 1> odd;
-      gather(0);
-      stage(even(), 0);
-      gather(1);
-      __syncthreads();
-      auto tile = [&](int t, auto buf, auto next) {
-        if (buf == 0 && t % 4 == 0) {  // uniform
-          put_slot(t + 4 + w, page);
-          page = page_of(t + 8 + w);
+      // PT tiles between two barriers, half of LDS. The loads of the other half lie between the
+      // products and the exponentials of these: all at once they hold every wave up for a fifth of
+      // the time, since a CU takes in 64 bytes a clock
+      for (int t = 0; t < min(PT, ntile); ++t)
+#pragma unroll
+        for (int h = 0; h < PW; ++h) load(t, h, slot(t, h));
+#pragma nounroll
+      for (int t0 = 0; t0 < ntile; t0 += PT) {  // uniform
+        ta_wait();        // this wave's part of the tiles is there
+        __syncthreads();  // the tiles are whole, and nobody reads those before any more
+        if (t0 % TA_NW == 0) {
+          put_slot(t0 + TA_NW + w, page);
+          page = page_of(t0 + 2 * TA_NW + w);
         }
-        if (active) {
-          const uint8_t* const k = sMem + buf * (2 * PA_TILE * RB);
+        const int t1 = min(t0 + PT, ntile);
+        if ((u.lo + t1) * PA_TILE > u.ctx) {
+          for (int t = t0; t < t1; ++t)
+            if ((u.lo + t + 1) * PA_TILE > u.ctx) clean(t);
+          __syncthreads();
+        }
+#pragma nounroll
+        for (int t = t0; t < t1; ++t) {
+          const uint32_t at = (uint32_t)(t % NB) * TB;
+          const bool more = t + PT < ntile;
+          uint32_t sl[PW];
+#pragma unroll
+          for (int h = 0; h < PW; ++h) sl[h] = slot(t + PT, h);
+          if (!active) {
+#pragma unroll
+            for (int h = 0; h < PW; ++h)
+              if (more) load(t + PT, h, sl[h]);
+            continue;
+          }
           __builtin_amdgcn_s_setprio(1);
           pa_f16 s[2] = {};
-          ta_qk<D, FMT>(s, qa, k, ka);
+          ta_qk<D, FMT>(s, qa, sMem, ka + at);
           __builtin_amdgcn_s_setprio(0);
+          if (more) load(t + PT, 0, sl[0]);
           const int g = u.lo + t;
-          if ((g + 1) * (int64_t)PA_TILE > u.ctx) {  // uniform
+          if ((g + 1) * PA_TILE > u.ctx) {
             if (g < u.ct) {
-              ta_mask(s, (1ull << (u.ctx - (int64_t)g * PA_TILE)) - 1, hi);
+              ta_mask(s, (1ull << (u.ctx - g * PA_TILE)) - 1, hi);
             } else {
               ta_mask(s, word, hi);
               if (g + 1 < u.hi) word = ta_word(a, u, r0 + l31, g + 1 - u.ct);
             }
           }
           pa_softmax<D, FMT, 2>(st, s, a.scale_log2);
+          if constexpr (PW > 1)
+            if (more) load(t + PT, 1, sl[1]);
           __builtin_amdgcn_s_setprio(1);
-          pa_pv<D, FMT, 2>(st, s, k + PA_TILE * RB, va);
+          pa_pv<D, FMT, 2>(st, s, sMem, va + at + KB);
           __builtin_amdgcn_s_setprio(0);
         }
-        stage(next, t + 1);
-        __builtin_amdgcn_sched_barrier(0);  // the registers are free before they are loaded
-        gather(t + 2);
-        __syncthreads();
-      };
-      for (int t = 0;; t += 2) {
-        tile(t, even(), odd());
-        if (t + 1 >= ntile) break;
-        tile(t + 1, odd(), even());
-        if (t + 2 >= ntile) break;
       }
       if (__builtin_amdgcn_readfirstlane(sOdd))
         ta_add_odd<D, FMT>(st, a, u, table, vp, row_bytes, r0 + l31, hi);
@@ -396,14 +424,14 @@ tree_attn_kernel(TreeAttnArgs a) {
                   make_uint2(pa_pack<FMT>(st.o[db][4 * e4] * f, st.o[db][4 * e4 + 1] * f),
                              pa_pack<FMT>(st.o[db][4 * e4 + 2] * f, st.o[db][4 * e4 + 3] * f));
         } else {
-          float* const to = a.part_o + ((int64_t)u.part * PA_ROWS + i) * D + 4 * hi;
+          float* const to = a.part_o + ((int64_t)u.part * TA_ROWS + i) * D + 4 * hi;
 #pragma unroll
           for (int db = 0; db < D / 32; ++db)
 #pragma unroll
             for (int e4 = 0; e4 < 4; ++e4)
               *reinterpret_cast<float4*>(to + 32 * db + 8 * e4) = make_float4(
                   st.o[db][4 * e4], st.o[db][4 * e4 + 1], st.o[db][4 * e4 + 2], st.o[db][4 * e4 + 3]);
-          if (hi == 0) a.part_ml[(int64_t)u.part * PA_ROWS + i] = make_float2(st.m, st.l);
+          if (hi == 0) a.part_ml[(int64_t)u.part * TA_ROWS + i] = make_float2(st.m, st.l);
         }
       }
       if (bad && a.error) *a.error = 1;
@@ -424,7 +452,7 @@ tree_attn_kernel(TreeAttnArgs a) {
 // share a row's parts, each with a running maximum of its own, and are joined in LDS.
 template <int D, int FMT, int RB>
 __global__ void __launch_bounds__(PA_NT) tree_attn_join_kernel(TreeAttnArgs a) {
-  constexpr int DL = D / 4, SL = PA_NT / DL / RB, UN = 4;
+  constexpr int DL = D / 4, SL = PA_NT / DL / RB, UN = SL > 1 ? 4 : 2;
   __shared__ float4 sO[SL][RB][DL];
   __shared__ float2 sML[SL][RB];
   if (blockIdx.x >= a.head[0]) return;  // uniform
@@ -441,7 +469,7 @@ __global__ void __launch_bounds__(PA_NT) tree_attn_join_kernel(TreeAttnArgs a) {
 #pragma unroll
       for (int k = 0; k < UN; ++k) {
         const int c = min(c0 + k * SL, x.parts - 1);
-        const int64_t p = (int64_t)(2 * (x.first + c) + (c == 0)) * PA_ROWS + i;
+        const int64_t p = (int64_t)(2 * (x.first + c) + (c == 0)) * TA_ROWS + i;
         ml[k] = a.part_ml[p];
         v[k] = *reinterpret_cast<const float4*>(a.part_o + p * D + d4 * 4);
       }
@@ -499,26 +527,27 @@ __global__ void __launch_bounds__(PA_NT) tree_attn_join_kernel(TreeAttnArgs a) {
   }
 }
 
-// items of a call: tiles of 128 query rows, of every row that has nodes
+// items of a call: tiles of 256 query rows, of every row that has nodes
 int64_t tree_attn_items(int64_t tokens, int64_t batch, int32_t hkv, int32_t group) {
-  return hkv * (tokens * group / PA_ROWS + std::min(batch, tokens));
+  return hkv * (tokens * group / TA_ROWS + std::min(batch, tokens));
 }
 
 template <int D, int FMT, int RB>
 static void launch_join(const TreeAttnArgs& a, int64_t items, hipStream_t s) {
-  const unsigned blocks = items >= 256 ? 8 : PA_ROWS / RB;
+  const unsigned blocks = RB >= 8 ? TA_ROWS / RB / 2 : TA_ROWS / RB;
   hipLaunchKernelGGL((tree_attn_join_kernel<D, FMT, RB>), dim3((unsigned)items, blocks), dim3(PA_NT), 0, s, a);
 }
 
 template <int D, int FMT>
 static hipError_t launch_tree_attn_t(const TreeAttnArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((tree_attn_kernel<D, FMT>), dim3(TA_GRID), dim3(PA_NT), 0, s, a);
+  hipLaunchKernelGGL((tree_attn_kernel<D, FMT>), dim3(TA_GRID), dim3(TA_NT), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int64_t items = a.max_items;
+  // few items have many parts: slices of a workgroup share them
   if (items <= 16) launch_join<D, FMT, 1>(a, items, s);
   else if (items <= 64) launch_join<D, FMT, 2>(a, items, s);
-  else launch_join<D, FMT, 4>(a, items, s);
+  else launch_join<D, FMT, PA_NT / (D / 4)>(a, items, s);
   return hipGetLastError();
 }
 
