@@ -16,6 +16,19 @@ namespace sdx {
 
 constexpr int kWave = 64;
 
+// Stores of what this kernel does not read again, past the XCD's L2: those that stay dirty there
+// are written back when the kernel ends, which its successor waits for (the K/V moved by a
+// compaction, 69 MB: 23.7 us, 14.7 with these).
+__device__ __forceinline__ void store_nt(void* p, uint4 v) {
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  __builtin_nontemporal_store(__builtin_bit_cast(u4, v), reinterpret_cast<u4*>(p));
+}
+__device__ __forceinline__ void store_nt(void* p, float4 v) { store_nt(p, __builtin_bit_cast(uint4, v)); }
+__device__ __forceinline__ void store_nt(void* p, uint2 v) {
+  typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+  __builtin_nontemporal_store(__builtin_bit_cast(u2, v), reinterpret_cast<u2*>(p));
+}
+
 // ---------------------------------------------------------------- 16-bit keys
 // bf16 and fp16 are sign-magnitude: flipping all bits of negatives and the
 // sign bit of positives gives an unsigned key whose order is the value order

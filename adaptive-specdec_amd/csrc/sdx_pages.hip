@@ -17,18 +17,32 @@ __device__ __forceinline__ uint8_t* pgs_side(uint8_t* pool, int64_t layer_bytes,
   return pool + ls / 2 * layer_bytes + ls % 2 * side_bytes;
 }
 
+// Work on n items in every (layer, side): groups of LS sides go to the XCDs in turn (workgroup % 8),
+// so that an XCD's translations are those of its own sides. The workgroup's item, and its first side.
+__device__ __forceinline__ int64_t pgs_item(int64_t n, int LS, int& ls0) {
+  const uint32_t k = blockIdx.x / 8, g = k / (uint32_t)n;
+  ls0 = (int)(g * 8 + blockIdx.x % 8) * LS;
+  return k - g * (uint32_t)n;
+}
+static dim3 pgs_grid(int64_t n, int32_t layers, int LS) {
+  const int64_t groups = (2 * layers + LS - 1) / LS;
+  return dim3((unsigned)(n * ((groups + 7) / 8 * 8)));
+}
+
 // ---- compact: row b's tokens start + path[i] to start + i for i < keep, ascending. A thread
 // moves a 16-byte column of them: path ascends from 0 or more, so path[i] >= i and no token is
 // overwritten before the same thread has read it. A workgroup does CP_LS (layer, side) pairs of
 // a row; the slots are worked out once and lie in LDS, and tokens that stay are left out.
 constexpr int CP_PATH = TREE_MAX_NODES;
-constexpr int CP_LS = 8;
+constexpr int CP_LS = 2;
 
 __global__ void __launch_bounds__(PGS_NT) compact_paged_kernel(CompactArgs a) {
   __shared__ int64_t sFrom[CP_PATH], sTo[CP_PATH];
   __shared__ int sN;
   const int tid = threadIdx.x;
-  const int64_t b = blockIdx.x;
+  int ls0;
+  const int64_t b = pgs_item(a.batch, CP_LS, ls0);
+  if (ls0 >= 2 * a.layers) return;  // uniform
   const int64_t keep = a.keep[b], start = a.start[b];
   const int64_t* const path = a.path + b * a.max_path;
   const int32_t* const table = a.table + b * a.max_blocks;
@@ -61,7 +75,7 @@ __global__ void __launch_bounds__(PGS_NT) compact_paged_kernel(CompactArgs a) {
   __syncthreads();
   const int i0 = sN;
   const uint32_t upr = (uint32_t)(a.row_bytes / 16);
-  const int ls0 = (int)blockIdx.y * CP_LS, sides = min(CP_LS, 2 * a.layers - ls0);
+  const int sides = min(CP_LS, 2 * a.layers - ls0);
   for (uint32_t u = tid; u < sides * upr; u += PGS_NT) {
     const uint32_t ls = u / upr;
     uint8_t* const at = pgs_side(a.pool, a.layer_bytes, a.side_bytes, ls0 + ls) + (int64_t)(u - ls * upr) * 16;
@@ -72,7 +86,7 @@ __global__ void __launch_bounds__(PGS_NT) compact_paged_kernel(CompactArgs a) {
         if (i + k < keep) v[k] = *reinterpret_cast<const uint4*>(at + sFrom[i + k]);
 #pragma unroll
       for (int k = 0; k < PGS_UN; ++k)
-        if (i + k < keep) *reinterpret_cast<uint4*>(at + sTo[i + k]) = v[k];
+        if (i + k < keep) store_nt(at + sTo[i + k], v[k]);
     }
   }
 }
@@ -82,6 +96,7 @@ __global__ void __launch_bounds__(PGS_NT) compact_paged_kernel(CompactArgs a) {
 // joins them and lists the pages whose bit is clear, by ascending id.
 constexpr int FP_NT = 512;
 constexpr int FP_SEG = 8192;  // pages that a workgroup of the second kernel lists
+constexpr int64_t FP_JOIN = 1 << 22;  // words read by all workgroups of the list, of which the join is cheaper
 
 __global__ void __launch_bounds__(FP_NT) free_pages_mark_kernel(FreePagesArgs a) {
   __shared__ uint32_t sBits[FREE_RANGE / 32];
@@ -113,6 +128,17 @@ __global__ void __launch_bounds__(FP_NT) free_pages_mark_kernel(FreePagesArgs a)
   for (int w = tid; w < words; w += FP_NT) out[w] = sBits[w];
 }
 
+// Many pages: the parts are joined once, in the place of the first, and not by every workgroup of
+// the list.
+__global__ void __launch_bounds__(FP_NT) free_pages_join_kernel(FreePagesArgs a) {
+  const int64_t w = (int64_t)blockIdx.x * FP_NT + threadIdx.x;
+  if (w >= a.words) return;
+  uint32_t held = 0;
+#pragma unroll 8
+  for (int p = 0; p < a.parts; ++p) held |= a.bits[p * a.words + w];
+  a.bits[w] = held;
+}
+
 __global__ void __launch_bounds__(FP_NT) free_pages_list_kernel(FreePagesArgs a) {
   constexpr int SW = FP_SEG / 32, NW = FP_NT / kWave;
   static_assert(SW <= FP_NT, "a word per thread");
@@ -123,6 +149,7 @@ __global__ void __launch_bounds__(FP_NT) free_pages_list_kernel(FreePagesArgs a)
   // free pages of word w
   auto word = [&](int64_t w) {
     uint32_t held = 0;
+#pragma unroll 8
     for (int p = 0; p < a.parts; ++p) held |= a.bits[p * a.words + w];
     const int64_t left = a.num_blocks - w * 32;
     return ~held & (left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1u);
@@ -189,6 +216,7 @@ __device__ __forceinline__ FkRow fk_row(const ForkArgs& a, int64_t i) {
 }
 
 // a wave per new row: its own pages in own[i], and whether it copies its first
+constexpr int FK_UN = 4;  // rows of a lane at a time
 constexpr int32_t FK_COPY = 1 << 30, FK_BAD = (int32_t)0x80000000;
 __global__ void __launch_bounds__(PGS_NT) fork_rows_kernel(ForkArgs a) {
   const int lane = threadIdx.x & (kWave - 1);
@@ -202,11 +230,26 @@ __global__ void __launch_bounds__(PGS_NT) fork_rows_kernel(ForkArgs a) {
     const int32_t page = a.table[r.p * a.max_blocks + r.whole];
     ok = page >= 0;
     int other = 0;
-    for (int64_t j = lane; ok && j < a.batch; j += kWave) {
-      const FkRow o = fk_row(a, j);
-      const bool holds = j != i && o.ok && o.p >= 0 &&
-                         (o.whole > r.whole || (o.whole == r.whole && o.part > 0 && j < i));
-      other |= holds && a.table[o.p * a.max_blocks + r.whole] == page;
+    for (int64_t j0 = lane; ok && j0 < a.batch; j0 += FK_UN * kWave) {  // three loads, one behind another
+      int64_t p[FK_UN], len[FK_UN];
+      int32_t g[FK_UN];
+      bool holds[FK_UN];
+#pragma unroll
+      for (int k = 0; k < FK_UN; ++k) p[k] = a.parent[min(j0 + k * kWave, a.batch - 1)];
+#pragma unroll
+      for (int k = 0; k < FK_UN; ++k) {
+        holds[k] = p[k] >= 0 && p[k] < a.old_batch && j0 + k * kWave < a.batch && j0 + k * kWave != i;
+        len[k] = a.kv_len[holds[k] ? p[k] : r.p];
+      }
+#pragma unroll
+      for (int k = 0; k < FK_UN; ++k) {
+        // the row's page in this column: whole if its tokens pass the page, else filled in part
+        holds[k] &= len[k] <= a.max_blocks * a.bs && (len[k] >= (r.whole + 1) * a.bs ||
+                                                      (len[k] > r.whole * a.bs && j0 + k * kWave < i));
+        g[k] = a.table[(holds[k] ? p[k] : r.p) * a.max_blocks + r.whole];
+      }
+#pragma unroll
+      for (int k = 0; k < FK_UN; ++k) other |= holds[k] && g[k] == page;
     }
     copy = __any(other);
   }
@@ -266,9 +309,11 @@ __global__ void __launch_bounds__(PGS_NT) fork_tables_kernel(ForkArgs a) {
 
 // ---- copies of pages: entry e's first tokens[e] tokens from page to page, in every layer and
 // side. They lie one behind another on both sides.
-constexpr int CY_LS = 8;
+constexpr int CY_LS = 1;
 __global__ void __launch_bounds__(PGS_NT) copy_pages_kernel(CopyPagesArgs a) {
-  const int64_t e = blockIdx.x;
+  int ls0;
+  const int64_t e = pgs_item(a.n, CY_LS, ls0);
+  if (ls0 >= 2 * a.layers) return;  // uniform
   const int32_t from = a.copies[e], to = a.copies[a.n + e], tokens = a.copies[2 * a.n + e];
   if (from < 0 || to < 0 || tokens == 0) return;  // uniform
   if (from >= a.num_blocks || to >= a.num_blocks || tokens < 0 || tokens > a.bs) {
@@ -277,7 +322,7 @@ __global__ void __launch_bounds__(PGS_NT) copy_pages_kernel(CopyPagesArgs a) {
   }
   const int64_t page = a.bs * a.row_bytes;
   const uint32_t upr = (uint32_t)(tokens * (a.row_bytes / 16));
-  const int ls0 = (int)blockIdx.y * CY_LS, sides = min(CY_LS, 2 * a.layers - ls0);
+  const int sides = min(CY_LS, 2 * a.layers - ls0);
   for (uint32_t u0 = threadIdx.x; u0 < sides * upr; u0 += PGS_NT * PGS_UN) {
     uint4 v[PGS_UN];
     uint8_t* dst[PGS_UN];
@@ -293,28 +338,35 @@ __global__ void __launch_bounds__(PGS_NT) copy_pages_kernel(CopyPagesArgs a) {
     }
 #pragma unroll
     for (int k = 0; k < PGS_UN; ++k)
-      if (dst[k]) *reinterpret_cast<uint4*>(dst[k]) = v[k];
+      if (dst[k]) store_nt(dst[k], v[k]);
   }
 }
 
 // ---------------------------------------------------------------- launches
 hipError_t launch_compact_paged(const CompactArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)a.batch, (unsigned)((2 * a.layers + CP_LS - 1) / CP_LS));
+  const dim3 grid = pgs_grid(a.batch, a.layers, CP_LS);
   hipLaunchKernelGGL(compact_paged_kernel, grid, dim3(PGS_NT), 0, s, a);
   return hipGetLastError();
 }
 
-int free_pages_parts(int64_t entries) {  // a workgroup for every 4,096 entries
-  return (int)std::max<int64_t>(1, std::min<int64_t>(64, entries / 4096));
+int free_pages_parts(int64_t entries) {  // a workgroup for every 1,024 entries
+  return (int)std::max<int64_t>(1, std::min<int64_t>(64, entries / 1024));
 }
 
 hipError_t launch_free_pages(const FreePagesArgs& a, hipStream_t s) {
   const unsigned ranges = (unsigned)((a.num_blocks + FREE_RANGE - 1) / FREE_RANGE);
   hipLaunchKernelGGL(free_pages_mark_kernel, dim3(ranges, (unsigned)a.parts), dim3(FP_NT), 0, s, a);
-  const hipError_t e = hipGetLastError();
+  hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(free_pages_list_kernel, dim3((unsigned)((a.num_blocks + FP_SEG - 1) / FP_SEG)),
-                     dim3(FP_NT), 0, s, a);
+  const int64_t segments = (a.num_blocks + FP_SEG - 1) / FP_SEG;
+  FreePagesArgs b = a;
+  if (a.parts > 1 && a.parts * a.words * segments > FP_JOIN) {
+    hipLaunchKernelGGL(free_pages_join_kernel, dim3((unsigned)((a.words + FP_NT - 1) / FP_NT)), dim3(FP_NT), 0, s, a);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    b.parts = 1;
+  }
+  hipLaunchKernelGGL(free_pages_list_kernel, dim3((unsigned)segments), dim3(FP_NT), 0, s, b);
   return hipGetLastError();
 }
 
@@ -328,7 +380,7 @@ hipError_t launch_fork_tables(const ForkArgs& a, hipStream_t s) {
 }
 
 hipError_t launch_copy_pages(const CopyPagesArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)a.n, (unsigned)((2 * a.layers + CY_LS - 1) / CY_LS));
+  const dim3 grid = pgs_grid(a.n, a.layers, CY_LS);
   hipLaunchKernelGGL(copy_pages_kernel, grid, dim3(PGS_NT), 0, s, a);
   return hipGetLastError();
 }

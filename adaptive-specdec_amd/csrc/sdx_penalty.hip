@@ -34,8 +34,6 @@ constexpr int PN_UN = 8;   // history tokens in flight per thread
 constexpr uint32_t PN_SEEN = 0x80000000u, PN_COUNT = (1u << 20) - 1;
 static_assert(PN_HISTORY + TREE_MAX_NODES <= (int64_t)PN_COUNT && PN_MAX_BIAS < 2047, "fields of a word");
 
-typedef uint32_t pn_u4 __attribute__((ext_vector_type(4)));
-
 template <int DT>
 struct PnType;
 template <>
@@ -322,7 +320,7 @@ __global__ void __launch_bounds__(PN_NT) __attribute__((amdgpu_waves_per_eu(4)))
               }
             }
           }
-          __builtin_nontemporal_store(__builtin_bit_cast(pn_u4, x[k]), reinterpret_cast<pn_u4*>(dst + v));
+          store_nt(dst + v, x[k]);
         }
       }
       // the row's ends, where a unit is not whole

@@ -420,17 +420,17 @@ tree_attn_kernel(TreeAttnArgs a) {
           for (int db = 0; db < D / 32; ++db)
 #pragma unroll
             for (int e4 = 0; e4 < 4; ++e4)
-              *reinterpret_cast<uint2*>(to + 32 * db + 8 * e4) =
-                  make_uint2(pa_pack<FMT>(st.o[db][4 * e4] * f, st.o[db][4 * e4 + 1] * f),
-                             pa_pack<FMT>(st.o[db][4 * e4 + 2] * f, st.o[db][4 * e4 + 3] * f));
+              store_nt(to + 32 * db + 8 * e4,
+                       make_uint2(pa_pack<FMT>(st.o[db][4 * e4] * f, st.o[db][4 * e4 + 1] * f),
+                                  pa_pack<FMT>(st.o[db][4 * e4 + 2] * f, st.o[db][4 * e4 + 3] * f)));
         } else {
           float* const to = a.part_o + ((int64_t)u.part * TA_ROWS + i) * D + 4 * hi;
 #pragma unroll
           for (int db = 0; db < D / 32; ++db)
 #pragma unroll
             for (int e4 = 0; e4 < 4; ++e4)
-              *reinterpret_cast<float4*>(to + 32 * db + 8 * e4) = make_float4(
-                  st.o[db][4 * e4], st.o[db][4 * e4 + 1], st.o[db][4 * e4 + 2], st.o[db][4 * e4 + 3]);
+              store_nt(to + 32 * db + 8 * e4, make_float4(st.o[db][4 * e4], st.o[db][4 * e4 + 1],
+                                                          st.o[db][4 * e4 + 2], st.o[db][4 * e4 + 3]));
           if (hi == 0) a.part_ml[(int64_t)u.part * TA_ROWS + i] = make_float2(st.m, st.l);
         }
       }
@@ -521,8 +521,8 @@ __global__ void __launch_bounds__(PA_NT) tree_attn_join_kernel(TreeAttnArgs a) {
       const float f = l > 0.0f || l != l ? 1.0f / l : 0.0f;
       const uint32_t r = x.r0 + i, j = r / (uint32_t)a.group;
       const int64_t qrow = (int64_t)(x.t0 + j) * a.hq + x.kvh * a.group + (r - j * a.group);
-      *reinterpret_cast<uint2*>(a.out + qrow * D + d4 * 4) =
-          make_uint2(pa_pack<FMT>(o.x * f, o.y * f), pa_pack<FMT>(o.z * f, o.w * f));
+      store_nt(a.out + qrow * D + d4 * 4,
+               make_uint2(pa_pack<FMT>(o.x * f, o.y * f), pa_pack<FMT>(o.z * f, o.w * f)));
     }
   }
 }
