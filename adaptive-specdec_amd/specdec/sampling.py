@@ -210,17 +210,25 @@ def _rows_of(name, t, rows, cols, dtype):
         raise ValueError(f"{name} must be [{rows}, {'...' if cols is None else cols}], got {tuple(t.shape)}")
     if t.dtype is not dtype:
         t = t.to(dtype)
-    if t.shape[1] and (t.stride(1) != 1 or (rows > 1 and t.stride(0) < t.shape[1])):
-        t = t.contiguous()
-    return t, t.stride(0) if rows > 1 else t.shape[1]
+    ld, unit = t.stride()
+    n = t.shape[1]
+    if n and (unit != 1 or (rows > 1 and ld < n)):
+        return t.contiguous(), n
+    return t, ld if rows > 1 else n
 
 
-def _per_row(name, t, batch):
+def _per_row(name, t, batch, dtype=torch.float32):
     if t is None:
         return None
     if t.numel() != batch:
         raise ValueError(f"{name} must be [{batch}], got {tuple(t.shape)}")
-    return _lib.as_dtype(t, torch.float32)
+    return t if t.dtype is dtype and t.is_contiguous() else t.to(dtype).contiguous()
+
+
+def _whole(name, t):
+    if t is not None and t.dtype is not torch.int64 and (t.dtype.is_floating_point or t.dtype.is_complex or
+                                                         t.dtype is torch.bool):
+        raise TypeError(f"{name} must be whole numbers, got {t.dtype}")
 
 
 def penalize_logits(logits, history=None, history_len=None, cu_rows=None, *, prompt_len=None,
@@ -251,10 +259,10 @@ def penalize_logits(logits, history=None, history_len=None, cu_rows=None, *, pro
     if logits.dim() != 2:
         raise ValueError(f"logits must be [rows, V], got {tuple(logits.shape)}")
     dt = _lib.dtype_code(logits)
-    for name, t in (("history", history), ("bias_ids", bias_ids), ("node_tokens", node_tokens),
-                    ("tree_mask", tree_mask), ("allowed", allowed)):
-        if t is not None and (t.dtype.is_floating_point or t.dtype.is_complex or t.dtype is torch.bool):
-            raise TypeError(f"{name} must be whole numbers, got {t.dtype}")
+    _whole("history", history)
+    _whole("bias_ids", bias_ids)
+    _whole("node_tokens", node_tokens)
+    _whole("tree_mask", tree_mask)
     if error is not None and (error.dtype != torch.int32 or error.numel() < 1):
         raise TypeError("error must be an int32 device tensor of one element")
     R, V = logits.shape
@@ -274,12 +282,11 @@ def penalize_logits(logits, history=None, history_len=None, cu_rows=None, *, pro
     hist, hist_ld, hl, pl = None, 0, None, None
     if history is not None:
         hist, hist_ld = _rows_of("history", history, B, None, torch.int64)
-        hl = _lib.as_dtype(history_len, torch.int64)
-        pl = None if prompt_len is None else _lib.as_dtype(prompt_len, torch.int64)
-        if hl.numel() != B or (pl is not None and pl.numel() != B):
-            raise ValueError(f"history_len and prompt_len must be [{B}]")
-    rep, freq, pres = (_per_row(n, t, B) for n, t in (("repetition", repetition), ("frequency", frequency),
-                                                      ("presence", presence)))
+        hl = _per_row("history_len", history_len, B, torch.int64)
+        pl = _per_row("prompt_len", prompt_len, B, torch.int64)
+    rep = _per_row("repetition", repetition, B)
+    freq = _per_row("frequency", frequency, B)
+    pres = _per_row("presence", presence, B)
     bi = bv = None
     if bias_ids is not None:
         if bias_ids.dim() != 2 or bias_ids.shape[0] != B or bias.shape != bias_ids.shape:
