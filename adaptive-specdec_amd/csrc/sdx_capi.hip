@@ -1464,7 +1464,6 @@ int sdx_prefix_attention_paged(const void* q, int dtype, int64_t num_tokens, int
 // ------------------------------------------------------------------ attention of trees
 static size_t tree_attn_ws(Carve& c, int64_t tokens, int64_t batch, int32_t hq, int32_t hkv, int32_t d,
                            sdx::TreeAttnArgs* a) {
-  a->head = c.take<uint32_t>(64);
   a->max_items = sdx::tree_attn_items(tokens, batch, hkv, hq / hkv);
   a->items = c.take<sdx::TreeAttnItem>((size_t)a->max_items);
   a->part_ml = c.take<float2>((size_t)2 * sdx::TREE_ATTN_GRID * sdx::TREE_ATTN_ROWS);

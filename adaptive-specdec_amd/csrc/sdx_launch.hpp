@@ -642,6 +642,10 @@ struct TreeAttnItem {  // query rows of a row, and the workgroups that have its 
   int32_t t0, kvh, r0, m;      // the row's first token, KV head, first query row, query rows
   int32_t first, parts, pad[2];
 };
+struct TreeAttnDiv {  // a division by multiplication
+  uint32_t mul;
+  int32_t shift;
+};
 struct TreeAttnArgs {
   const uint16_t* q;           // [tokens, hq, d] bf16 or fp16
   const int64_t* cu_q;         // [batch + 1] node offsets
@@ -652,10 +656,10 @@ struct TreeAttnArgs {
   const int64_t* mask;         // [tokens, words]
   int64_t batch, tokens, max_blocks, num_blocks;
   int32_t hq, hkv, group, bs, words;
+  TreeAttnDiv by_bs, by_group; // (set by the launch)
   float scale_log2;            // softmax scale * log2(e)
   uint16_t* out;               // [tokens, hq, d]
   int32_t* error;
-  uint32_t* head;              // [64] the items
   TreeAttnItem* items;         // [max_items]
   int64_t max_items;
   float2* part_ml;             // [2 TREE_ATTN_GRID, TREE_ATTN_ROWS] max and sum of each part's query rows

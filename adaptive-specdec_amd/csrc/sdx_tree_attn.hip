@@ -54,6 +54,17 @@ __device__ __forceinline__ uint32_t ta_items(const TreeAttnArgs& a, const TaRow&
   return (uint32_t)(r.qt * a.hkv);
 }
 
+// x / d for x < 2^30, with l = ceil(log2 d): mul = floor(2^(30 + l) / d) + 1 is off by at most d, and
+// x d <= 2^(30 + l)
+__device__ __forceinline__ uint32_t ta_div(uint32_t x, const TreeAttnDiv& d) {
+  return (uint32_t)(((uint64_t)x * d.mul) >> d.shift);
+}
+static TreeAttnDiv ta_divide_by(int32_t d) {
+  int l = 0;
+  while ((int64_t)1 << l < d) ++l;
+  return TreeAttnDiv{(uint32_t)(((uint64_t)1 << (30 + l)) / d + 1), 30 + l};
+}
+
 // a value that is the same in all lanes, as a scalar
 __device__ __forceinline__ uint64_t ta_uniform(uint64_t x) {
   return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32 |
@@ -135,10 +146,10 @@ struct TaUnit {
 };
 // token of query row i of the unit
 __device__ __forceinline__ int64_t ta_token(const TreeAttnArgs& a, const TaUnit& u, int i) {
-  return u.t0 + (int32_t)((uint32_t)(u.r0 + i) / (uint32_t)a.group);
+  return u.t0 + (int32_t)ta_div(u.r0 + i, a.by_group);
 }
 __device__ __forceinline__ int64_t ta_qrow(const TreeAttnArgs& a, const TaUnit& u, int i) {
-  const uint32_t r = u.r0 + i, j = r / (uint32_t)a.group;
+  const uint32_t r = u.r0 + i, j = ta_div(r, a.by_group);
   return (int64_t)(u.t0 + j) * a.hq + u.kvh * a.group + (r - j * a.group);
 }
 // the word of query row i's mask for nodes 64 k ..
@@ -210,68 +221,102 @@ tree_attn_kernel(TreeAttnArgs a) {
   // Neighbours on the line share an XCD (workgroup index % 8), whose L2 their keys go through.
   const uint32_t wg = blockIdx.x % 8 * (TA_GRID / 8) + blockIdx.x / 8;
   uint32_t total, step, pos = 0, from = 0;  // from: where row b starts
-  uint32_t item0 = 0;
+  uint32_t item0 = 0, items;
   int64_t b = 0;
-  {
+  TaRow row = {};
+  // Up to 64 rows, that is a row per lane, each wave does it by itself (a third of what the barriers
+  // and the long code of any number of rows take, 2 us)
+  bool quick = a.batch <= kWave;
+  if (quick) {
+    row = lane < a.batch ? ta_row(a, lane) : TaRow{0, 0, 0, 0, 0, 0, true};
+    const uint32_t n = ta_items(a, row);
+    const uint64_t tiles = (uint64_t)n * row.len();
+    quick = !__any(tiles >> 25 != 0);
+    if (quick) {  // uniform
+      const uint32_t line = (uint32_t)tiles, li = wave_incl_scan_u32(line, lane), ii = wave_incl_scan_u32(n, lane);
+      items = rdlane(ii, kWave - 1);
+      const bool over = items > (uint64_t)a.max_items;
+      if ((__any(!row.ok) || over) && a.error && blockIdx.x == 0) *a.error = 1;
+      items = over ? 0 : items;
+      total = over ? 0 : rdlane(li, kWave - 1);
+      step = max(total / TA_GRID + (total % TA_GRID > 0), TA_LEAST);
+      pos = wg * step;
+      const uint64_t hit = __ballot(li - line <= pos && pos < li);
+      if (hit && pos < total) {
+        const int at = __ffsll((unsigned long long)hit) - 1;
+        from = rdlane(li - line, at);
+        item0 = rdlane(ii - n, at);
+        b = at;
+        row = TaRow{(int32_t)rdlane(row.t0, at), (int32_t)rdlane(row.ctx, at), (int32_t)rdlane(row.n, at),
+                    (int32_t)rdlane(row.ct, at), (int32_t)rdlane(row.kt, at), (int32_t)rdlane(row.qt, at), true};
+      } else {
+        pos = total;
+      }
+    }
+  }
+  if (!quick) {
     const bool one = a.batch <= TA_NT;
-    uint64_t line = 0, items = 0;
+    uint64_t line = 0, n = 0;
     int bad = 0;
     for (int64_t i = tid; i < a.batch; i += TA_NT) {
       const TaRow r = ta_row(a, i);
       bad |= !r.ok;
-      const uint32_t n = ta_items(a, r);
-      line += (uint64_t)n * r.len();
-      items += n;
+      line += (uint64_t)ta_items(a, r) * r.len();
+      n += ta_items(a, r);
     }
-    TaScan sc = ta_scan(line, items, sLine, sItem);
+    TaScan sc = ta_scan(line, n, sLine, sItem);
     // rows that share nodes (offsets out of order); a line of 2^32 tiles takes half a minute
     const bool over = sc.items > (uint64_t)a.max_items || sc.lines >> 32;
     if ((bad || over) && a.error && blockIdx.x == 0) *a.error = 1;
-    if (blockIdx.x == 0 && tid == 0) a.head[0] = over ? 0u : (uint32_t)sc.items;
+    items = over ? 0 : (uint32_t)sc.items;
     total = over ? 0 : (uint32_t)sc.lines;
     step = max(total / TA_GRID + (total % TA_GRID > 0), TA_LEAST);
-    pos = wg * step;
-    if ((uint64_t)wg * step >= total) return;  // uniform
+    pos = (uint32_t)min((uint64_t)wg * step, (uint64_t)total);
     uint64_t at = 0, it = 0;
-    for (int64_t b0 = 0;; b0 += TA_NT) {  // uniform; ends where the line holds pos
+    for (int64_t b0 = 0; at <= pos && pos < total; b0 += TA_NT) {  // uniform; ends where the line holds pos
       if (!one) {
         const TaRow r = b0 + tid < a.batch ? ta_row(a, b0 + tid) : TaRow{};
-        items = b0 + tid < a.batch ? ta_items(a, r) : 0;
-        line = items ? items * (uint64_t)r.len() : 0;
-        sc = ta_scan(line, items, sLine, sItem);
+        n = b0 + tid < a.batch ? ta_items(a, r) : 0;
+        line = n ? n * (uint64_t)r.len() : 0;
+        sc = ta_scan(line, n, sLine, sItem);
       }
       if (at + sc.line <= pos && pos < at + sc.line + line) {
         sAt[0] = at + sc.line;
         sAt[1] = (uint64_t)(b0 + tid) << 32 | (it + sc.item);
       }
       at += sc.lines, it += sc.items;
-      if (pos < at) break;
     }
     __syncthreads();
-    from = (uint32_t)ta_uniform(sAt[0]);
-    const uint64_t x = ta_uniform(sAt[1]);
-    item0 = (uint32_t)x;
-    b = (int64_t)(x >> 32);
+    if (pos < total) {
+      from = (uint32_t)ta_uniform(sAt[0]);
+      const uint64_t x = ta_uniform(sAt[1]);
+      item0 = (uint32_t)x;
+      b = (int64_t)(x >> 32);
+      row = ta_row(a, b);
+    }
   }
+  for (int64_t i = (int64_t)items + blockIdx.x * TA_NT + tid; i < a.max_items; i += TA_GRID * TA_NT)
+    a.items[i].parts = 0;  // records of no item
+  if (pos >= total) return;  // uniform
   const uint32_t end = min((uint64_t)total, (uint64_t)pos + step);
 
-  TaRow row = ta_row(a, b);
+  uint32_t item = (pos - from) / row.len();
   while (pos < end) {  // uniform: the items of the stretch
-    const uint32_t len = row.len(), item = (pos - from) / len;
-    const uint32_t p = from + item * len, e = min(end, p + len);
-    const uint32_t first = (p + TA_COST) / step, last = (p + len - 1) / step;
+    const uint32_t len = row.len(), p = from + item * len, e = min(end, p + len);
+    const uint32_t mine = wg * step;
+    const bool before = p + TA_COST < mine, behind = p + len - 1 >= mine + step;  // others have tiles of it
     TaUnit u;
     u.t0 = row.t0, u.ctx = row.ctx;
     u.n = row.n, u.ct = row.ct;
-    u.kvh = item / row.qt;
+    u.kvh = (int32_t)(row.qt == 1 ? item : item / (uint32_t)row.qt);
     u.r0 = (int32_t)(item - u.kvh * row.qt) * TA_ROWS;
     u.m = min(TA_ROWS, row.n * a.group - u.r0);
     u.lo = (int32_t)(max(pos - p, TA_COST) - TA_COST);
     u.hi = (int32_t)(max(e - p, TA_COST) - TA_COST);
-    u.part = first == last ? -1 : (int32_t)(2 * wg + (wg == first));
-    if (wg == first && u.lo < u.hi && tid == 0)
-      a.items[item0 + item] = TreeAttnItem{(int32_t)u.t0, u.kvh, u.r0, u.m, (int32_t)first,
-                                           (int32_t)(last - first + 1), 0, 0};
+    u.part = before || behind ? (int32_t)(2 * wg + !before) : -1;
+    if (!before && u.lo < u.hi && tid == 0)
+      a.items[item0 + item] = TreeAttnItem{u.t0, u.kvh, u.r0, u.m, (int32_t)wg,
+                                           behind ? (int32_t)((p + len - 1) / step - wg + 1) : 1, 0, 0};
     pos = e;
     const uint32_t row_end = from + ta_items(a, row) * len;
     if (u.lo < u.hi) {
@@ -288,16 +333,6 @@ tree_attn_kernel(TreeAttnArgs a) {
       st.l = 0.0f;
       const int r0 = PA_WROWS * w;  // the wave's rows
       const bool active = r0 < u.m;
-      pa_u4 qa[D / 16];
-      {
-        const uint16_t* src = a.q + (r0 + l31 < u.m ? ta_qrow(a, u, r0 + l31) * D : 0);
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          qa[ks] = *reinterpret_cast<const pa_u4*>(src + 16 * ks + 8 * hi);
-          if (r0 + l31 >= u.m) qa[ks] = (pa_u4){0, 0, 0, 0};
-        }
-      }
-      uint64_t word = u.hi > u.ct ? ta_word(a, u, r0 + l31, max(u.lo, u.ct) - u.ct) : 0;
       const int ntile = u.hi - u.lo;
       // slots of the unit's tiles, eight tiles at a time, one by each wave: page ids are loaded
       // eight tiles before they are needed here
@@ -310,13 +345,13 @@ tree_attn_kernel(TreeAttnArgs a) {
       };
       auto page_of = [&](int tile) {
         const int32_t x = key(tile);
-        return x >= 0 ? table[(uint32_t)x / (uint32_t)a.bs] : 0;
+        return x >= 0 ? table[ta_div(x, a.by_bs)] : 0;
       };
       auto put_slot = [&](int tile, int32_t page) {
         const int32_t x = key(tile);
         uint32_t s = PA_NOSLOT;
         if (x >= 0) {
-          if (page >= 0 && page < a.num_blocks) s = (uint32_t)page * (uint32_t)a.bs + (uint32_t)x % (uint32_t)a.bs;
+          if (page >= 0 && page < a.num_blocks) s = (uint32_t)page * (uint32_t)a.bs + (x - ta_div(x, a.by_bs) * (uint32_t)a.bs);
           bad |= s == PA_NOSLOT;
         }
         sSlot[(tile % TA_RING) * PA_TILE + lane] = s;
@@ -349,8 +384,19 @@ tree_attn_kernel(TreeAttnArgs a) {
         }
       };
       __syncthreads();  // the unit before is done with LDS
-      put_slot(w, page_of(w));
+      // pages, then queries and masks: the keys wait for the pages alone
+      const int32_t page0 = page_of(w);
       int32_t page = page_of(TA_NW + w);
+      const int row_i = min(r0 + l31, u.m - 1);  // rows past the item's are computed like its last, and not stored
+      pa_u4 qa[D / 16];
+      {
+        const uint16_t* const src = a.q + ta_qrow(a, u, row_i) * D + 8 * hi;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) qa[ks] = *reinterpret_cast<const pa_u4*>(src + 16 * ks);
+      }
+      const int64_t* const words = a.mask + ta_token(a, u, row_i) * a.words;
+      uint64_t word = u.hi > u.ct ? words[max(u.lo, u.ct) - u.ct] : 0;
+      put_slot(w, page0);
       if (tid == 0) sOdd = 0;
       __syncthreads();
       // PT tiles between two barriers, half of LDS. The loads of the other half lie between the
@@ -396,8 +442,8 @@ tree_attn_kernel(TreeAttnArgs a) {
             if (g < u.ct) {
               ta_mask(s, (1ull << (u.ctx - g * PA_TILE)) - 1, hi);
             } else {
-              ta_mask(s, word, hi);
-              if (g + 1 < u.hi) word = ta_word(a, u, r0 + l31, g + 1 - u.ct);
+              ta_mask(s, word & ta_valid(u.n, g - u.ct), hi);
+              if (g + 1 < u.hi) word = words[g + 1 - u.ct];
             }
           }
           pa_softmax<D, FMT, 2>(st, s, a.scale_log2);
@@ -436,7 +482,9 @@ tree_attn_kernel(TreeAttnArgs a) {
       }
       if (bad && a.error) *a.error = 1;
     }
+    ++item;
     if (pos == row_end) {  // the next row that has nodes
+      item = 0;
       from = pos;
       item0 += ta_items(a, row);
       while (++b < a.batch) {
@@ -455,9 +503,8 @@ __global__ void __launch_bounds__(PA_NT) tree_attn_join_kernel(TreeAttnArgs a) {
   constexpr int DL = D / 4, SL = PA_NT / DL / RB, UN = SL > 1 ? 4 : 2;
   __shared__ float4 sO[SL][RB][DL];
   __shared__ float2 sML[SL][RB];
-  if (blockIdx.x >= a.head[0]) return;  // uniform
   const TreeAttnItem x = a.items[blockIdx.x];
-  if (x.parts < 2) return;  // uniform: written directly
+  if (x.parts < 2) return;  // uniform: written directly, or no item
   const int tid = threadIdx.x, d4 = tid % DL, rr = tid / DL % RB, sl = tid / DL / RB;
   for (int i0 = blockIdx.y * RB; i0 < x.m; i0 += gridDim.y * RB) {  // uniform
     const int i = min(i0 + rr, x.m - 1);
@@ -551,7 +598,10 @@ static hipError_t launch_tree_attn_t(const TreeAttnArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-hipError_t launch_tree_attn(int dtype, int d, const TreeAttnArgs& a, hipStream_t s) {
+hipError_t launch_tree_attn(int dtype, int d, const TreeAttnArgs& b, hipStream_t s) {
+  TreeAttnArgs a = b;
+  a.by_bs = ta_divide_by(a.bs);
+  a.by_group = ta_divide_by(a.group);
   if (dtype == SDX_BF16)
     return d == 64 ? launch_tree_attn_t<64, SDX_BF16>(a, s) : launch_tree_attn_t<128, SDX_BF16>(a, s);
   return d == 64 ? launch_tree_attn_t<64, SDX_F16>(a, s) : launch_tree_attn_t<128, SDX_F16>(a, s);
