@@ -1189,7 +1189,7 @@ int sdx_compact_paged(void* pool, int64_t layer_stride, int64_t side_stride, int
                       int64_t row_elems, int64_t num_blocks, int32_t block_size,
                       const int32_t* block_table, int64_t batch, int64_t max_blocks,
                       const int64_t* kv_start, const int64_t* path, int64_t max_path,
-                      const int64_t* keep, int32_t* error, sdx_stream_t stream) {
+                      const int64_t* keep, int64_t* kept, int32_t* error, sdx_stream_t stream) {
   const int rc = pool_args("sdx_compact_paged", pool, layer_stride, side_stride, dtype, layers, row_elems,
                            num_blocks, block_size);
   if (rc != SDX_OK) return rc;
@@ -1203,7 +1203,7 @@ int sdx_compact_paged(void* pool, int64_t layer_stride, int64_t side_stride, int
   const int64_t es = (int64_t)dsize(dtype);
   sdx::CompactArgs a{(uint8_t*)pool, layer_stride * es, side_stride * es, row_elems * es, num_blocks,
                      block_table, kv_start, path, keep, batch, max_blocks, block_size, max_path,
-                     layers, error};
+                     layers, kept, error};
   return hip_status(sdx::launch_compact_paged(a, (hipStream_t)stream), "compact_paged");
 }
 
@@ -1213,7 +1213,8 @@ static bool free_fits(int64_t batch, int64_t max_blocks, int64_t num_blocks) {
 }
 size_t sdx_free_pages_workspace(int64_t batch, int64_t max_blocks, int64_t num_blocks) {
   if (!free_fits(batch, max_blocks, num_blocks)) return 0;
-  return (size_t)sdx::free_pages_parts(batch * max_blocks) * ((num_blocks + 31) / 32) * sizeof(uint32_t);
+  const int64_t words = (num_blocks + 31) / 32;
+  return ((size_t)sdx::free_pages_parts(batch * max_blocks, words) * words * sizeof(uint32_t) + 15) & ~(size_t)15;
 }
 int sdx_free_pages(const int32_t* block_table, int64_t batch, int64_t max_blocks, const int64_t* kv_len,
                    int32_t block_size, int64_t num_blocks, int32_t* free_blocks, int64_t* num_free,
@@ -1228,13 +1229,13 @@ int sdx_free_pages(const int32_t* block_table, int64_t batch, int64_t max_blocks
     return fail(SDX_EWORKSPACE, "sdx_free_pages: needs a 16-byte aligned workspace of %zu bytes (got %zu)",
                 need, workspace_bytes);
   sdx::FreePagesArgs a{block_table, kv_len, batch, max_blocks, block_size, num_blocks,
-                       sdx::free_pages_parts(batch * max_blocks), (num_blocks + 31) / 32,
+                       sdx::free_pages_parts(batch * max_blocks, (num_blocks + 31) / 32), (num_blocks + 31) / 32,
                        (uint32_t*)workspace, free_blocks, num_free, error};
   return hip_status(sdx::launch_free_pages(a, (hipStream_t)stream), "free_pages");
 }
 
 size_t sdx_fork_block_tables_workspace(int64_t batch) {
-  return batch < 0 || batch > (1 << 23) ? 0 : (size_t)std::max<int64_t>(batch, 1) * sizeof(int32_t);
+  return batch < 0 || batch > (1 << 18) ? 0 : (size_t)std::max<int64_t>(batch, 1) * sizeof(int32_t);
 }
 int sdx_fork_block_tables(const int32_t* block_table, int64_t old_batch, int64_t max_blocks,
                           const int64_t* kv_len, const int64_t* parent, const int64_t* room,
@@ -1246,8 +1247,8 @@ int sdx_fork_block_tables(const int32_t* block_table, int64_t old_batch, int64_t
       (old_batch > 0 && (!block_table || !kv_len)) || (max_free > 0 && !free_blocks) ||
       (batch > 0 && (!parent || !room || !out || !copies || !used)))
     return fail(SDX_EINVAL, "sdx_fork_block_tables: bad arguments");
-  if (batch > (1 << 23) || max_blocks > (1 << 27))
-    return fail(SDX_EUNSUPPORTED, "sdx_fork_block_tables: more than 2^23 rows or 2^27 blocks");
+  if (batch > (1 << 18) || max_blocks > (1 << 27))
+    return fail(SDX_EUNSUPPORTED, "sdx_fork_block_tables: more than 2^18 new rows or 2^27 blocks");
   if (batch == 0) return SDX_OK;
   if (out == block_table)
     return fail(SDX_EINVAL, "sdx_fork_block_tables: the new tables may not lie over the old ones");

@@ -592,6 +592,7 @@ struct CompactArgs {
   const int64_t* keep;          // [batch]
   int64_t batch, max_blocks, bs, max_path;
   int32_t layers;
+  int64_t* kept;                // [batch] or null: keep, 0 in rows that are refused
   int32_t* error;
 };
 hipError_t launch_compact_paged(const CompactArgs& a, hipStream_t s);
@@ -607,7 +608,7 @@ struct FreePagesArgs {
   int64_t* num_free;
   int32_t* error;
 };
-int free_pages_parts(int64_t entries);
+int free_pages_parts(int64_t entries, int64_t words);
 hipError_t launch_free_pages(const FreePagesArgs& a, hipStream_t s);
 struct ForkArgs {
   const int32_t* table;         // [old_batch, max_blocks]

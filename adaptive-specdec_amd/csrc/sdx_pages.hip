@@ -47,7 +47,11 @@ __global__ void __launch_bounds__(PGS_NT) compact_paged_kernel(CompactArgs a) {
   const int64_t* const path = a.path + b * a.max_path;
   const int32_t* const table = a.table + b * a.max_blocks;
   int bad = keep < 0 || keep > a.max_path || start < 0 || start > a.max_blocks * a.bs;
-  if (!bad && keep == 0) return;  // uniform
+  const bool tell = a.kept && ls0 == 0 && tid == 0;
+  if (!bad && keep == 0) {  // uniform
+    if (tell) a.kept[b] = 0;
+    return;
+  }
   int stay = 0;  // (the row's first tokens stay: path ascends)
   if (!bad) {
     auto slot = [&](int64_t pos) -> int64_t {
@@ -67,7 +71,9 @@ __global__ void __launch_bounds__(PGS_NT) compact_paged_kernel(CompactArgs a) {
     }
   }
   if (tid == 0) sN = 0;
-  if (__syncthreads_or(bad)) {
+  bad = __syncthreads_or(bad);
+  if (tell) a.kept[b] = bad ? 0 : keep;
+  if (bad) {  // uniform
     if (tid == 0 && a.error) *a.error = 1;
     return;
   }
@@ -349,8 +355,9 @@ hipError_t launch_compact_paged(const CompactArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-int free_pages_parts(int64_t entries) {  // a workgroup for every 1,024 entries
-  return (int)std::max<int64_t>(1, std::min<int64_t>(64, entries / 1024));
+// a workgroup for every 1,024 entries, as far as their bits stay under 16 MB
+int free_pages_parts(int64_t entries, int64_t words) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>({64, entries / 1024, (1 << 22) / words}));
 }
 
 hipError_t launch_free_pages(const FreePagesArgs& a, hipStream_t s) {

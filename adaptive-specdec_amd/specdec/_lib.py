@@ -84,7 +84,8 @@ _SIGS = {
     "sdx_tree_attention_workspace": (SZ, [I64, I64, I32, I32, I32]),
     "sdx_tree_layout": (INT, [P, I64, P, P, I32, P, I64, I32, I64, I64, P, P, P, P, P]),
     "sdx_tree_accept": (INT, [P, P, P, I64, P, I64, P, I64, P, P, P, P, P]),
-    "sdx_compact_paged": (INT, [P, I64, I64, INT, I32, I64, I64, I32, P, I64, I64, P, P, I64, P, P, P]),
+    "sdx_compact_paged": (INT, [P, I64, I64, INT, I32, I64, I64, I32, P, I64, I64, P, P, I64, P, P, P,
+                                P]),
     "sdx_free_pages": (INT, [P, I64, I64, P, I32, I64, P, P, P, SZ, P, P]),
     "sdx_free_pages_workspace": (SZ, [I64, I64, I64]),
     "sdx_fork_block_tables": (INT, [P, I64, I64, P, P, P, I64, I32, P, I64, P, P, P, P, P, SZ, P, P]),

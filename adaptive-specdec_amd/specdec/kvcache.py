@@ -313,9 +313,10 @@ class PagedKVCache:
     def compact(self, path, keep):
         """Keep a tree's accepted nodes (path [B, P], keep [B] of `specdec.tree.tree_accept`), which
         were appended from lengths[b] on: moves them together (`compact_paged`) and adds keep to the
-        lengths."""
-        compact_paged(self.pool, self.block_table, self.lengths, path, keep, error=self.error)
-        self.lengths += keep
+        lengths. Rows that are refused keep their lengths, and `error` is set."""
+        kept = torch.empty_like(self.lengths)
+        compact_paged(self.pool, self.block_table, self.lengths, path, keep, kept=kept, error=self.error)
+        self.lengths += kept
 
     def rollback(self, n):
         """lengths -= n (device [B] int64); all-or-nothing, `error` set if any row
@@ -457,17 +458,18 @@ def _table(block_table, what="block_table"):
     return _lib.as_dtype(block_table, torch.int32)
 
 
-def compact_paged(pool, block_table, kv_start, path, keep, error=None):
+def compact_paged(pool, block_table, kv_start, path, keep, kept=None, error=None):
     """Move the K/V of a tree's accepted nodes together, in every layer and side of pool [L, 2,
     num_blocks, block_size, row_elems] (contiguous; in place).
 
     Row b's token at position kv_start[b] + path[b, i] goes to kv_start[b] + i for i < keep[b]
     (kv_start, keep [B], path [B, P] int64, P at most 512, ascending in every row as
     `specdec.tree.tree_accept` gives it). Rows whose path, lengths or pages are out of range are
-    left as they are and set `error` (an int32 [1] device tensor) when given. Rows must not share
-    the pages behind kv_start.
+    left as they are and set `error` (an int32 [1] device tensor) when given; kept (int64 [B], when
+    given) receives keep, 0 in those rows: what the lengths go up by. Rows must not share the pages
+    behind kv_start.
     """
-    _lib.one_gpu(pool, block_table, kv_start, path, keep, error)
+    _lib.one_gpu(pool, block_table, kv_start, path, keep, kept, error)
     _error_word(error)
     L, nb, bs, re, side = _pool_shape(pool)
     bt = _table(block_table)
@@ -475,14 +477,18 @@ def compact_paged(pool, block_table, kv_start, path, keep, error=None):
     if path.dim() != 2 or path.shape[0] != B or kv_start.numel() != B or keep.numel() != B:
         raise ValueError(f"block_table of {B} rows needs kv_start [{B}], path [{B}, P] and keep [{B}], got "
                          f"{kv_start.numel()}, {tuple(path.shape)} and {keep.numel()}")
+    if kept is not None and (kept.dtype != torch.int64 or kept.numel() != B or not kept.is_contiguous()):
+        raise ValueError(f"kept must be a contiguous int64 [{B}]")
     st, pt, kp = (_lib.as_dtype(t, torch.int64) for t in (kv_start, path, keep))
-    if B == 0 or pt.shape[1] == 0:
+    if B == 0:
         return
+    if pt.shape[1] == 0:
+        raise ValueError("path must have a column at least")
     with _lib.on_device(pool):
         rc = _lib.lib().sdx_compact_paged(
             _lib.ptr(pool), 2 * side, side, _lib.dtype_code(pool), L, re, nb, bs, _lib.ptr(bt), B,
-            bt.shape[1], _lib.ptr(st), _lib.ptr(pt), pt.shape[1], _lib.ptr(kp), _lib.ptr(error),
-            _lib.stream_of(pool))
+            bt.shape[1], _lib.ptr(st), _lib.ptr(pt), pt.shape[1], _lib.ptr(kp), _lib.ptr(kept),
+            _lib.ptr(error), _lib.stream_of(pool))
     _lib.check(rc, "compact_paged")
 
 

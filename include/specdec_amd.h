@@ -488,21 +488,22 @@ int sdx_tree_accept(const int64_t* tokens, const int32_t* parents, const int64_t
  * kv_start[b] + path[b, i] goes to kv_start[b] + i, for i < keep[b]. path [batch, max_path] int64
  * (512 at most) ascends strictly from 0 or more, as sdx_tree_accept writes it; what lies behind
  * keep[b] is not read. kv_start, keep int64 [batch]. A row whose path, lengths or pages are out of
- * range is left as it is, all of it, and sets *error (nullable). Rows must not share the pages that
- * are written. One kernel, in place. */
+ * range is left as it is, all of it, and sets *error (nullable). kept (int64 [batch], nullable) = keep,
+ * 0 in such rows: what the rows' lengths go up by. Rows must not share the pages that are written. One
+ * kernel, in place. */
 int sdx_compact_paged(void* pool, int64_t layer_stride, int64_t side_stride, int dtype, int32_t layers,
                       int64_t row_elems, int64_t num_blocks, int32_t block_size,
                       const int32_t* block_table, int64_t batch, int64_t max_blocks,
                       const int64_t* kv_start, const int64_t* path, int64_t max_path,
-                      const int64_t* keep, int32_t* error, sdx_stream_t stream);
+                      const int64_t* keep, int64_t* kept, int32_t* error, sdx_stream_t stream);
 
 /* The pages that no row holds: free_blocks [num_blocks] int32 = their ids ascending, -1 behind the
  * last; *num_free (int64) how many. Row b of block_table [batch, max_blocks] int32 holds the pages of
  * its kv_len[b] (int64) tokens, ceil(kv_len[b] / block_size) entries, or without kv_len every entry
  * that is not negative. Pages outside [0, num_blocks) among those, and lengths out of range, set
  * *error (nullable). Any number of rows may hold a page: nothing is counted between calls, a row's
- * pages are given back by leaving it out. Two kernels; `workspace` as the query says, 16-byte aligned,
- * no initial contents. Up to 2^30 pages and 2^31 entries. */
+ * pages are given back by leaving it out. Two kernels, three for many pages; `workspace` as the query says, 16-byte
+ * aligned, no initial contents. Up to 2^30 pages and 2^31 entries. */
 int sdx_free_pages(const int32_t* block_table, int64_t batch, int64_t max_blocks, const int64_t* kv_len,
                    int32_t block_size, int64_t num_blocks, int32_t* free_blocks, int64_t* num_free,
                    void* workspace, size_t workspace_bytes, int32_t* error, sdx_stream_t stream);
@@ -519,8 +520,8 @@ size_t sdx_free_pages_workspace(int64_t batch, int64_t max_blocks, int64_t num_b
  * first *num_free (device int64; null: max_free) of them; *used (int64) = how many. out is written
  * whole, -1 behind a row's last page, and may not lie over block_table. All or nothing: where a parent, a
  * length, a page of an old row or the free pages are out of range, out and copies are -1 (tokens 0), *used 0
- * and *error (nullable) 1. Two kernels; `workspace` as the query says. The time of a row's look at the
- * others grows with the rows. Up to 2^23 rows and 2^27 columns. */
+ * and *error (nullable) 1. Two kernels; `workspace` as the query says. Every row
+ * looks at all others: 384 rows take 10 us. Up to 2^18 new rows and 2^27 columns. */
 int sdx_fork_block_tables(const int32_t* block_table, int64_t old_batch, int64_t max_blocks,
                           const int64_t* kv_len, const int64_t* parent, const int64_t* room,
                           int64_t batch, int32_t block_size, const int32_t* free_blocks,

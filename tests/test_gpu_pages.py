@@ -81,9 +81,10 @@ def test_compact_refuses_rows():
     pool = make_pool(2, 2, B * mb, bs, 64, torch.bfloat16)
     before, want = pool.clone(), pool.cpu().clone()
     assert not OT.compact(want, table, start, path, keep)
-    err = new_error()
-    compact_paged(pool, dev(table, torch.int32), dev(start), dev(path), dev(keep), error=err)
+    err, kept = new_error(), dev([9] * B)
+    compact_paged(pool, dev(table, torch.int32), dev(start), dev(path), dev(keep), kept=kept, error=err)
     assert err.item() == 1 and torch.equal(pool.cpu(), want) and not torch.equal(pool, before)
+    assert kept.tolist() == [4] + [0] * 8
     # without an error word nothing else happens either
     pool2 = before.clone()
     compact_paged(pool2, dev(table, torch.int32), dev(start), dev(path), dev(keep))
@@ -100,6 +101,8 @@ def test_cache_method_moves_and_commits():
     assert OT.compact(want, c.block_table.cpu().numpy(), [30, 3], path.cpu().numpy(), [3, 2])
     c.compact(path, keep)
     assert torch.equal(c.pool, want) and c.lengths.tolist() == [33, 5] and c.error.item() == 0
+    c.compact(dev([[0, 1, 2], [0, 1, 1]]), dev([0, 3]))       # nothing of row 0, row 1 is refused
+    assert torch.equal(c.pool, want) and c.lengths.tolist() == [33, 5] and c.error.item() == 1
 
 
 @pytest.mark.parametrize("B,mb,nb,bs,lengths", [

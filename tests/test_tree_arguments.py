@@ -45,7 +45,7 @@ def test_page_statuses():
 
     def compact(pool=FAKE, dtype=BF16, layers=2, re=64, nb=8, bs=16, table=FAKE, B=2, mb=4, P=4, stride=4096):
         return L.sdx_compact_paged(pool, 2 * stride, stride, dtype, layers, re, nb, bs, table, B, mb, FAKE,
-                                   FAKE, P, FAKE, None, None)
+                                   FAKE, P, FAKE, None, None, None)
 
     def copy(pool=FAKE, dtype=BF16, layers=2, re=64, nb=8, bs=16, n=3, copies=FAKE, stride=4096):
         return L.sdx_copy_pages(pool, 2 * stride, stride, dtype, layers, re, nb, bs, copies, n, None, None)
