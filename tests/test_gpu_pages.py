@@ -109,6 +109,8 @@ def test_cache_method_moves_and_commits():
     (1, 1, 1, 16, True), (1, 1, 1, 16, False), (3, 5, 31, 16, True), (3, 5, 33, 7, False),
     (64, 300, 20011, 16, True), (700, 90, 63001, 8, True), (5, 40, 8192, 16, False),
     (2, 3, 8193, 16, True), (4, 2000, 600007, 16, True), (0, 4, 40, 16, True),
+    # the ends of the form of one kernel
+    (23, 89, 16384, 16, True), (23, 89, 16385, 16, True), (32, 64, 16384, 16, False), (1, 5, 16383, 16, False),
 ])
 def test_free_pages(B, mb, nb, bs, lengths):
     rng = np.random.default_rng(B + nb)
