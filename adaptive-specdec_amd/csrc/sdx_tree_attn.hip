@@ -14,6 +14,19 @@
 // line from the lengths by itself (8 bytes a row, a scan). A stretch's first and last item may
 // be parts, so there is room for two parts a workgroup, which leave (O, max, sum) in fp32 for a
 // second kernel to join; whole items are written directly.
+//
+// Tiles go to LDS without a register in between, half of LDS ahead; 256 query rows a workgroup,
+// since a second tile of a row's queries would read its keys from HBM once more; two waves per
+// SIMD, 32 query rows each, of which one has matrix products while the other has exponentials.
+//
+// Measured, in graphs:
+//   32 trees of up to 64 nodes, contexts of up to 8,192, 32 heads on 8 of 128, bf16: 250 us, 3.4
+//     TB/s and 680 TFLOP/s (large copies and products reach 5.2 and 1,254: 165 us by the bytes,
+//     135 by the products). Without its loads the kernel takes 200, the loads alone 206: they
+//     share each CU's issue and LDS, and tiles are waited for at the barriers
+//   24 trees of up to 33, contexts of up to 1,531, 14 heads on 2 of 64, fp16: 23.9 us (3.3 by the bytes)
+//   1 tree of 26 behind 2,011 keys, 32 heads on 8 of 128: 17.1 us (1.7): two launches, loads that
+//     wait for one another (lengths, pages, keys), instructions that are fetched once, the join
 #include <algorithm>
 #include <type_traits>
 
@@ -27,8 +40,12 @@ constexpr int TA_NW = TA_NT / kWave;
 constexpr int TA_ROWS = TREE_ATTN_ROWS;  // query rows of an item, 32 per wave
 constexpr int TA_RING = 2 * TA_NW;       // tiles of slots
 static_assert(TA_ROWS == TA_NW * PA_WROWS, "every wave has rows of a full item");
-constexpr uint32_t TA_COST = 4;          // tiles that an item costs beside its own
-constexpr uint32_t TA_LEAST = 2;         // tiles of a stretch, at least
+// Tiles that an item costs beside its own. The cases above: 0 takes 255, 26.4 and 20.7 us, 4 takes
+// 253, 23.9 and 17.1, 8 takes 257, 23.9 and 16.8.
+constexpr uint32_t TA_COST = 4;
+// Tiles of a stretch, at least: fewer parts of short items to join. The last case: 1 takes 17.3 us, 2
+// takes 17.1, 4 takes 19.6; 9 trees of up to 70, 1,186 keys: 25.3, 21.9, 23.8.
+constexpr uint32_t TA_LEAST = 2;
 
 struct TaRow {
   int32_t t0, ctx;      // first node's token; keys in front of the nodes
@@ -591,7 +608,9 @@ static hipError_t launch_tree_attn_t(const TreeAttnArgs& a, hipStream_t s) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int64_t items = a.max_items;
-  // few items have many parts: slices of a workgroup share them
+  // Few items have many parts: slices of a workgroup share them. The cases of the file's head, whose
+  // bounds are 464, 84 and 8 items: one thread for all parts of its columns 253, 23.7 and 20.6 us, rows
+  // in twos 267, 26.0 and 16.8, one by one 285, 31.0 and 17.2
   if (items <= 16) launch_join<D, FMT, 1>(a, items, s);
   else if (items <= 64) launch_join<D, FMT, 2>(a, items, s);
   else launch_join<D, FMT, PA_NT / (D / 4)>(a, items, s);
