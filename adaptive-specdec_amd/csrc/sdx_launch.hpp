@@ -594,6 +594,7 @@ struct CompactArgs {
   int32_t layers;
   int64_t* kept;                // [batch] or null: keep, 0 in rows that are refused
   int32_t* error;
+  int64_t first, count;         // rows of a launch
 };
 hipError_t launch_compact_paged(const CompactArgs& a, hipStream_t s);
 constexpr int FREE_RANGE = 1 << 18;  // pages whose bits fit a workgroup's LDS
@@ -632,6 +633,7 @@ struct CopyPagesArgs {
   int64_t n;
   int32_t layers;
   int32_t* error;
+  int64_t first, count;         // entries of a launch
 };
 hipError_t launch_copy_pages(const CopyPagesArgs& a, hipStream_t s);
 

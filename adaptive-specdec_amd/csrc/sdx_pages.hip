@@ -26,9 +26,19 @@ __device__ __forceinline__ int64_t pgs_item(int64_t n, int LS, int& ls0) {
   ls0 = (int)(g * 8 + blockIdx.x % 8) * LS;
   return k - g * (uint32_t)n;
 }
-static dim3 pgs_grid(int64_t n, int32_t layers, int LS) {
-  const int64_t groups = (2 * layers + LS - 1) / LS;
-  return dim3((unsigned)(n * ((groups + 7) / 8 * 8)));
+// Launches over n items, each of at most 2^23 workgroups (a grid's threads have to stay under 2^32):
+// run(grid, first item, items).
+template <typename F>
+static hipError_t pgs_launch(int64_t n, int32_t layers, int LS, F run) {
+  const int64_t groups = ((2 * (int64_t)layers + LS - 1) / LS + 7) / 8 * 8;  // 2^16 at most
+  const int64_t each = ((int64_t)1 << 23) / groups;
+  for (int64_t first = 0; first < n; first += each) {
+    const int64_t count = std::min(each, n - first);
+    run(dim3((unsigned)(count * groups)), first, count);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 // ---- compact: row b's tokens start + path[i] to start + i for i < keep, ascending. A thread
@@ -46,7 +56,7 @@ __global__ void __launch_bounds__(PGS_NT) compact_paged_kernel(CompactArgs a) {
   __shared__ int sN;
   const int tid = threadIdx.x;
   int ls0;
-  const int64_t b = pgs_item(a.batch, CP_LS, ls0);
+  const int64_t b = a.first + pgs_item(a.count, CP_LS, ls0);
   if (ls0 >= 2 * a.layers) return;  // uniform
   const int64_t keep = a.keep[b], start = a.start[b];
   const int64_t* const path = a.path + b * a.max_path;
@@ -360,7 +370,7 @@ __global__ void __launch_bounds__(PGS_NT) fork_tables_kernel(ForkArgs a) {
 constexpr int CY_LS = 1;  // 2: 42 us in place of 39
 __global__ void __launch_bounds__(PGS_NT) copy_pages_kernel(CopyPagesArgs a) {
   int ls0;
-  const int64_t e = pgs_item(a.n, CY_LS, ls0);
+  const int64_t e = a.first + pgs_item(a.count, CY_LS, ls0);
   if (ls0 >= 2 * a.layers) return;  // uniform
   const int32_t from = a.copies[e], to = a.copies[a.n + e], tokens = a.copies[2 * a.n + e];
   if (from < 0 || to < 0 || tokens == 0) return;  // uniform
@@ -392,9 +402,11 @@ __global__ void __launch_bounds__(PGS_NT) copy_pages_kernel(CopyPagesArgs a) {
 
 // ---------------------------------------------------------------- launches
 hipError_t launch_compact_paged(const CompactArgs& a, hipStream_t s) {
-  const dim3 grid = pgs_grid(a.batch, a.layers, CP_LS);
-  hipLaunchKernelGGL(compact_paged_kernel, grid, dim3(PGS_NT), 0, s, a);
-  return hipGetLastError();
+  return pgs_launch(a.batch, a.layers, CP_LS, [&](dim3 grid, int64_t first, int64_t count) {
+    CompactArgs b = a;
+    b.first = first, b.count = count;
+    hipLaunchKernelGGL(compact_paged_kernel, grid, dim3(PGS_NT), 0, s, b);
+  });
 }
 
 // a workgroup for every 1,024 entries, as far as their bits stay under 16 MB
@@ -435,9 +447,11 @@ hipError_t launch_fork_tables(const ForkArgs& a, hipStream_t s) {
 }
 
 hipError_t launch_copy_pages(const CopyPagesArgs& a, hipStream_t s) {
-  const dim3 grid = pgs_grid(a.n, a.layers, CY_LS);
-  hipLaunchKernelGGL(copy_pages_kernel, grid, dim3(PGS_NT), 0, s, a);
-  return hipGetLastError();
+  return pgs_launch(a.n, a.layers, CY_LS, [&](dim3 grid, int64_t first, int64_t count) {
+    CopyPagesArgs b = a;
+    b.first = first, b.count = count;
+    hipLaunchKernelGGL(copy_pages_kernel, grid, dim3(PGS_NT), 0, s, b);
+  });
 }
 
 }  // namespace sdx

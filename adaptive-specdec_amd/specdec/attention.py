@@ -173,7 +173,7 @@ def tree_attention_paged(q, cu_q, k_pool, v_pool, block_table, kv_len, tree_mask
     its last, included; tree_mask [T, words] int64 of `specdec.tree.tree_layout` (n_b up to 64
     words and 512). Node i sees the kv_len[b] - n_b keys in front of the nodes and every node
     j whose bit j % 64 of word j / 64 is set. Returns out [T, Hq, d] of q's type, 0 for a node that
-    sees nothing. Rows out of range are skipped and set `error` (an int32 [1] device tensor) when given, and so do
+    sees nothing; nodes behind cu_q[B] are left as they were. Rows out of range are skipped and set `error` (an int32 [1] device tensor) when given, and so do
     page ids outside the pool. `workspace` (uint8, `tree_attention_workspace`) holds fp32 parts and serves one
     call at a time; None: the calling thread's own for the current stream, kept for its next calls."""
     _lib.one_gpu(q, cu_q, k_pool, v_pool, block_table, kv_len, tree_mask, out, error, workspace)

@@ -300,6 +300,8 @@ def penalize_logits(logits, history=None, history_len=None, cu_rows=None, *, pro
         if allowed.dtype is not torch.int32:
             raise TypeError(f"allowed must be int32 words, got {allowed.dtype}")
         al, al_ld = _rows_of("allowed", allowed, R, None, torch.int32)
+    # (kept by name: what a temporary held could be taken by another thread before the launch)
+    cu = None if cu_rows is None else _lib.as_dtype(cu_rows, torch.int64)
     tk = tm = None
     if node_tokens is not None:
         if node_tokens.numel() != R:
@@ -314,8 +316,7 @@ def penalize_logits(logits, history=None, history_len=None, cu_rows=None, *, pro
     with _lib.on_device(x):
         rc = _lib.lib().sdx_penalize_logits(
             _lib.ptr(x), dt, R, V, ld, _lib.ptr(out), out.stride(0) if R > 1 else V, B,
-            None if cu_rows is None else _lib.ptr(_lib.as_dtype(cu_rows, torch.int64)),
-            _lib.ptr(hist), hist_ld, 0 if hist is None else hist.shape[1], _lib.ptr(hl), _lib.ptr(pl),
+            _lib.ptr(cu), _lib.ptr(hist), hist_ld, 0 if hist is None else hist.shape[1], _lib.ptr(hl), _lib.ptr(pl),
             _lib.ptr(rep), _lib.ptr(freq), _lib.ptr(pres), _lib.ptr(bi), _lib.ptr(bv),
             0 if bi is None else bi.shape[1], _lib.ptr(al), al_ld, _lib.ptr(tk), _lib.ptr(tm),
             0 if tm is None else tm.shape[1], _lib.ptr(error), _lib.stream_of(x))

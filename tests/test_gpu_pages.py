@@ -288,3 +288,29 @@ def test_beams_as_a_graph():
         assert len(set(last)) == B and err.item() == 0
         for x, y in zip(out, step()):
             assert torch.equal(x, y)
+
+
+def test_more_items_than_a_grid_holds():
+    """2.2 million entries and rows, of which those at the ends do something, in one layer: more
+    workgroups than a launch takes."""
+    n, bs, re = 2_200_000, 4, 8
+    pool = make_pool(3, 1, 40, bs, re, torch.bfloat16)
+    want = pool.clone()
+    copies = torch.full((3, n), -1, dtype=torch.int32, device=DEV)
+    at = dev([0, 1_048_575, 1_048_576, 2_097_151, 2_097_152, n - 1])
+    copies[:, at] = dev([np.arange(6), np.arange(10, 16), [4, 1, 2, 3, 4, 1]], torch.int32)
+    for i, t in enumerate([4, 1, 2, 3, 4, 1]):
+        want[:, :, 10 + i, :t] = want[:, :, i, :t]
+    err = new_error()
+    copy_pages(pool, copies, error=err)
+    assert torch.equal(pool, want) and err.item() == 0
+    table = torch.full((n, 1), -1, dtype=torch.int32, device=DEV)
+    start, keep = (torch.zeros(n, dtype=torch.int64, device=DEV) for _ in range(2))
+    path = torch.full((n, 1), 2, dtype=torch.int64, device=DEV)
+    table[at, 0] = dev(np.arange(20, 26), torch.int32)
+    start[at] = 1
+    keep[at] = 1
+    want[:, :, 20:26, 1] = want[:, :, 20:26, 3]
+    kept = torch.full((n,), -9, dtype=torch.int64, device=DEV)
+    compact_paged(pool, table, start, path, keep, kept=kept, error=err)
+    assert torch.equal(pool, want) and torch.equal(kept, keep) and err.item() == 0
