@@ -24,8 +24,10 @@
 //
 // Measured, bf16, V = 151,936: 256 rows that decode, histories of up to 2,048 and 4 biases 44.2 us
 // (159 MB, 3.6 TB/s); 8 trees of 32 nodes under grammars, histories of up to 8,192 34.6 us (122 MB,
-// 3.5 TB/s); a copy reaches 5.2 TB/s, and the rest is the scans, which nothing overlaps in a
-// workgroup that has one row. 8 fp32 rows of 50,257: 6.8 us, of which an empty launch is 3.6.
+// 3.5 TB/s). Without histories the same 256 rows take 26 us (6.0 TB/s), with 2,048 tokens each 38:
+// their loads, counting and the tokens' own changes have a few us each. Not faster: histories and
+// biases asked for a unit ahead (spilled registers), the tokens' changes in LDS by a thread per 32
+// (another 16 KB, three workgroups a CU in place of four), atomics of several slots at once. 8 fp32 rows of 50,257: 6.8 us, of which an empty launch is 3.6.
 #include <algorithm>
 
 #include "sdx_launch.hpp"
@@ -190,20 +192,15 @@ __global__ void __launch_bounds__(PN_NT) __attribute__((amdgpu_waves_per_eu(4)))
       p.freq = a.frequency ? a.frequency[b] : 0.0f;
       p.pres = a.presence ? a.presence[b] : 0.0f;
       // the first tokens are asked for before the words are cleared
-      const int64_t* const h = a.history + b * a.history_ld;
+      const uint8_t* const h = reinterpret_cast<const uint8_t*>(a.history + b * a.history_ld);
       const int n = ok ? (int)len : 0;
-      uint32_t t[PN_UN];  // places in the words
+      uint2 y[PN_UN];  // tokens
       auto fetch = [&](int i0) {
-        int64_t y[PN_UN];
 #pragma unroll
-        for (int k = 0; k < PN_UN; ++k) y[k] = h[min(i0 + k * PN_NT, n - 1)];
-#pragma unroll
-        for (int k = 0; k < PN_UN; ++k) {
-          const uint64_t z = (uint64_t)(y[k] - vb);
-          t[k] = z < nb && i0 + k * PN_NT < n ? (uint32_t)z : ~0u;
-        }
+        for (int k = 0; k < PN_UN; ++k)
+          y[k] = *reinterpret_cast<const uint2*>(h + min((uint32_t)(tid + i0 + k * PN_NT) * 8u, (uint32_t)(n - 1) * 8u));
       };
-      if (n > 0) fetch(tid);
+      if (n > 0) fetch(0);
       uint32_t mine = 0;
       __syncthreads();  // the words are read no more
       for (int i = tid * 4; i < S + E; i += PN_NT * 4)
@@ -217,13 +214,14 @@ __global__ void __launch_bounds__(PN_NT) __attribute__((amdgpu_waves_per_eu(4)))
         }
       __syncthreads();
       if (ok) {
-        for (int i0 = tid; i0 < n;) {
+        for (int i0 = 0; i0 < n;) {  // uniform. A wave's instruction takes four clocks: few of them per token
 #pragma unroll
           for (int k = 0; k < PN_UN; ++k) {
-            if (t[k] == ~0u) continue;
-            if (i0 + k * PN_NT < prompt) atomicOr(&sWord[t[k]], PN_SEEN);
-            else atomicAdd(&sWord[t[k]], 1u);
-            atomicOr(&sBit[t[k] / 32], 1u << (t[k] % 32));
+            const uint32_t t = y[k].x - (uint32_t)vb;
+            if (t >= (uint32_t)nb || y[k].y != 0 || tid >= n - i0 - k * PN_NT) continue;
+            if (tid < (int)prompt - i0 - k * PN_NT) atomicOr(&sWord[t], PN_SEEN);
+            else atomicAdd(&sWord[t], 1u);
+            atomicOr(&sBit[t / 32], 1u << (t % 32));
           }
           i0 += PN_UN * PN_NT;
           if (i0 < n) fetch(i0);
