@@ -105,6 +105,32 @@ def test_matches_float64(dtype, ns, V, kw):
     assert err.item() == 0 and torch.equal(x, before)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V,ns,kw", [
+    (24579, [3] * 30, dict(tree=True, grammar=True, biases=3, H=300)),     # slices of many rows
+    (2048, [1] * 300, dict(path=False, H=90)), (2041, [2] * 130, dict(biases=2)), (2040, [2] * 130, dict()),
+    (8192, [4, 0, 251], dict(tree=True, H=2500, ids=3000)), (8193, [1] * 127, dict(grammar=True)),
+])
+def test_many_rows(dtype, V, ns, kw):
+    x, c, sees = make(V, ns, V, dtype, **kw)
+    check(x, c, sees, call(x, c))
+    wide = torch.full((sum(ns), V + 13), 7.0, device=DEV, dtype=dtype)     # odd strides, rows off alignment
+    view = wide[:, 5:5 + V]
+    view.copy_(x)
+    check(x, c, sees, call(view, c, out=view))
+    assert (wide[:, :5] == 7).all() and (wide[:, 5 + V:] == 7).all()
+
+
+def test_ids_alike_in_their_low_bits():
+    x, c, sees = make(5, [2, 1], 5000, torch.float32, H=64, biases=4)
+    for k in ("history", "node_tokens", "bias_ids"):
+        flat = c[k].reshape(-1)
+        flat[1::3] += np.int64(1) << 32
+        flat[2::7] -= np.int64(1) << 32
+        flat[::5] = -1 - flat[::5] % 9
+    check(x, c, sees, call(x, c))
+
+
 def test_large_vocabulary_and_long_history():
     x, c, sees = make(3, [9, 4], 262144, torch.bfloat16, H=40000, ids=9000, tree=True, grammar=True, biases=5)
     check(x, c, sees, call(x, c))
