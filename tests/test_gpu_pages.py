@@ -155,7 +155,9 @@ def random_tables(rng, B, mb, nb, bs, kv):
 
 
 @pytest.mark.parametrize("B,N,mb,bs", [(1, 1, 1, 16), (1, 9, 4, 16), (6, 6, 5, 7), (40, 33, 12, 16),
-                                       (3, 200, 9, 1), (130, 300, 30, 32), (5, 0, 3, 16)])
+                                       (3, 200, 9, 1), (130, 300, 30, 32), (5, 0, 3, 16),
+                                       # the ends of the form of one workgroup
+                                       (9, 16, 512, 3), (9, 17, 512, 3), (9, 16, 513, 3), (30, 15, 40, 16)])
 def test_fork(B, N, mb, bs):
     rng = np.random.default_rng(B + N)
     kv = rng.integers(0, mb * bs + 1, B)
