@@ -446,9 +446,10 @@ def append_paged_slots(pool, staged, slots, error=None):
 
 
 def _pool_shape(pool):
-    if pool.dim() != 5 or pool.shape[1] != 2 or not pool.is_contiguous():
+    shape = pool.shape
+    if len(shape) != 5 or shape[1] != 2 or not pool.is_contiguous():
         raise ValueError("pool must be a contiguous [L, 2, num_blocks, block_size, row_elems]")
-    L, _, nb, bs, re = pool.shape
+    L, _, nb, bs, re = shape
     return L, nb, bs, re, nb * bs * re
 
 
@@ -479,7 +480,8 @@ def compact_paged(pool, block_table, kv_start, path, keep, kept=None, error=None
                          f"{kv_start.numel()}, {tuple(path.shape)} and {keep.numel()}")
     if kept is not None and (kept.dtype != torch.int64 or kept.numel() != B or not kept.is_contiguous()):
         raise ValueError(f"kept must be a contiguous int64 [{B}]")
-    st, pt, kp = (_lib.as_dtype(t, torch.int64) for t in (kv_start, path, keep))
+    st, pt = _lib.as_dtype(kv_start, torch.int64), _lib.as_dtype(path, torch.int64)
+    kp = _lib.as_dtype(keep, torch.int64)
     if B == 0:
         return
     if pt.shape[1] == 0:
@@ -514,8 +516,7 @@ def free_page_list(block_table, num_blocks, kv_len=None, block_size=None, error=
             raise ValueError(f"kv_len must be [{B}], got {kl.numel()}")
     if num_blocks < 1:
         raise ValueError(f"num_blocks must be positive, got {num_blocks}")
-    free = torch.empty(num_blocks, dtype=torch.int32, device=bt.device)
-    num = torch.empty(1, dtype=torch.int64, device=bt.device)
+    free, num = bt.new_empty(num_blocks), bt.new_empty(1, dtype=torch.int64)
     with _lib.on_device(bt):
         need = _lib.workspace_bytes("sdx_free_pages_workspace", B, max(mb, 1), num_blocks)
         ws = _lib.cached_workspace(need, bt.device, "free_pages")
@@ -546,7 +547,8 @@ def fork_block_tables(block_table, kv_len, parent, room, free_blocks, block_size
     _error_word(error)
     bt = _table(block_table)
     B, mb = bt.shape
-    kl, pa, ro = (_lib.as_dtype(t, torch.int64) for t in (kv_len, parent, room))
+    kl, pa = _lib.as_dtype(kv_len, torch.int64), _lib.as_dtype(parent, torch.int64)
+    ro = _lib.as_dtype(room, torch.int64)
     fb = _lib.as_dtype(free_blocks, torch.int32)
     nf = None if num_free is None else _lib.as_dtype(num_free, torch.int64)
     N = pa.numel()
@@ -554,16 +556,16 @@ def fork_block_tables(block_table, kv_len, parent, room, free_blocks, block_size
         raise ValueError(f"block_table of {B} rows needs kv_len [{B}], {N} parents room [{N}] and num_free "
                          f"[1], got {kl.numel()} and {ro.numel()}")
     if out is None:
-        out = torch.empty((N, mb), dtype=torch.int32, device=bt.device)
+        out = bt.new_empty((N, mb))
     elif out.dtype != torch.int32 or tuple(out.shape) != (N, mb) or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous int32 [{N}, {mb}]")
     a0, b0 = out.data_ptr(), bt.data_ptr()
     if a0 < b0 + bt.numel() * 4 and b0 < a0 + out.numel() * 4:
         raise ValueError("out may not lie over block_table: rows read each other's entries")
-    copies = torch.empty((3, N), dtype=torch.int32, device=bt.device)
+    copies = bt.new_empty((3, N))
     if N == 0:
         return out, copies, torch.zeros(1, dtype=torch.int64, device=bt.device)
-    used = torch.empty(1, dtype=torch.int64, device=bt.device)
+    used = pa.new_empty(1)
     with _lib.on_device(bt):
         need = _lib.workspace_bytes("sdx_fork_block_tables_workspace", N)
         ws = _lib.cached_workspace(need, bt.device, "fork_tables")

@@ -271,7 +271,7 @@ def penalize_logits(logits, history=None, history_len=None, cu_rows=None, *, pro
         raise ValueError(f"{R} rows of no batch row")
     x, ld = _rows_of("logits", logits, R, V, logits.dtype)
     if out is None:
-        out = torch.empty((R, V), dtype=x.dtype, device=x.device)
+        out = x.new_empty((R, V))
     elif out.dtype != logits.dtype or out.shape != logits.shape or (V > 1 and out.stride(1) != 1) or \
             (R > 1 and out.stride(0) < V):
         raise ValueError("out must be of logits' shape and type, its rows contiguous")

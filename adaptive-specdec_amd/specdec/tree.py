@@ -32,7 +32,8 @@ def _offsets(cu_q, batch, T):
 
 
 def _whole(name, t):
-    if t is not None and (t.dtype.is_floating_point or t.dtype.is_complex or t.dtype is torch.bool):
+    if t is not None and t.dtype is not torch.int64 and (t.dtype.is_floating_point or t.dtype.is_complex or
+                                                         t.dtype is torch.bool):
         raise TypeError(f"{name} must be whole numbers, got {t.dtype}")
 
 
@@ -70,12 +71,8 @@ def tree_layout(parents, cu_q, kv_len, block_table=None, block_size=None, max_no
         if block_table.dim() != 2 or block_table.shape[0] != B:
             raise ValueError(f"block_table must be [{B}, max_blocks], got {tuple(block_table.shape)}")
         bt = _lib.as_dtype(block_table, torch.int32)
-    dev = parents.device
-    mask = torch.empty((T, (max_nodes + 63) // 64), dtype=torch.int64, device=dev)
-    if bt is None:
-        pos, slots = torch.empty(T, dtype=torch.int64, device=dev), None
-    else:
-        pos, slots = torch.empty((2, T), dtype=torch.int64, device=dev).unbind(0)
+    mask, pos = kl.new_empty((T, (max_nodes + 63) // 64)), kl.new_empty(T)
+    slots = None if bt is None else kl.new_empty(T)
     if T:
         with _lib.on_device(up):
             rc = _lib.lib().sdx_tree_layout(
@@ -117,8 +114,7 @@ def tree_accept(tokens, parents, choice, cu_q, max_path, active=None, error=None
         if active.numel() != B:
             raise ValueError(f"active must be [{B}], got {active.numel()} rows")
         act = (active != 0).to(torch.uint8).contiguous()
-    path = torch.empty((B, max_path), dtype=torch.int64, device=tokens.device)
-    keep, y = torch.empty((2, B), dtype=torch.int64, device=tokens.device).unbind(0)
+    path, keep, y = tk.new_empty((B, max_path)), tk.new_empty(B), tk.new_empty(B)
     if B:
         with _lib.on_device(tk):
             rc = _lib.lib().sdx_tree_accept(
