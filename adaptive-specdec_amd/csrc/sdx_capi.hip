@@ -1235,7 +1235,7 @@ int sdx_free_pages(const int32_t* block_table, int64_t batch, int64_t max_blocks
 }
 
 size_t sdx_fork_block_tables_workspace(int64_t batch) {
-  return batch < 0 || batch > (1 << 18) ? 0 : (size_t)std::max<int64_t>(batch, 1) * sizeof(int32_t);
+  return batch < 0 || batch > (1 << 18) ? 0 : (size_t)std::max<int64_t>(batch, 1) * 2 * sizeof(int32_t);
 }
 int sdx_fork_block_tables(const int32_t* block_table, int64_t old_batch, int64_t max_blocks,
                           const int64_t* kv_len, const int64_t* parent, const int64_t* room,
@@ -1257,7 +1257,7 @@ int sdx_fork_block_tables(const int32_t* block_table, int64_t old_batch, int64_t
     return fail(SDX_EWORKSPACE, "sdx_fork_block_tables: needs a 16-byte aligned workspace of %zu bytes "
                                 "(got %zu)", need, workspace_bytes);
   sdx::ForkArgs a{block_table, kv_len, parent, room, free_blocks, num_free, old_batch, batch, max_blocks,
-                  block_size, max_free, (int32_t*)workspace, out, copies, used, error};
+                  block_size, max_free, (int32_t*)workspace, (int32_t*)workspace + batch, out, copies, used, error};
   return hip_status(sdx::launch_fork_tables(a, (hipStream_t)stream), "fork_tables");
 }
 

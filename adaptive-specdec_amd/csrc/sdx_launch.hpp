@@ -620,6 +620,7 @@ struct ForkArgs {
   const int64_t* num_free;
   int64_t old_batch, batch, max_blocks, bs, max_free;
   int32_t* own;                 // [batch] pages taken, and flags
+  int32_t* gap;                 // [batch] first entry of the row's share of free_blocks that is no page
   int32_t* out;                 // [batch, max_blocks]
   int32_t* copies;              // [3, batch]
   int64_t* used;

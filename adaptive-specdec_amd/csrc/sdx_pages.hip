@@ -314,12 +314,50 @@ __device__ __forceinline__ int32_t fk_own(const ForkArgs& a, int64_t i, int lane
   return ok ? (int32_t)(need - kept) | (copy ? FK_COPY : 0) : FK_BAD;
 }
 
+// Free pages are taken in front of the first entry that is no page (free_page_list leaves -1 behind
+// its last one). All rows together take batch * max_blocks at most, so a wave per new row looks at
+// max_blocks of them, whatever the pool has: row i's first that is no page, as an index of its
+// share, or FK_NONE.
+constexpr int32_t FK_NONE = 0x7FFFFFFF;
+__device__ __forceinline__ int64_t fk_have(const ForkArgs& a) {
+  return a.num_free ? min(*a.num_free, a.max_free) : a.max_free;
+}
+struct FkGap {
+  int64_t first, most, have;
+  int32_t g[FK_UN];  // the share's first entries
+};
+// asked for ahead of what the row takes: none of these loads waits for another
+__device__ __forceinline__ FkGap fk_ask(const ForkArgs& a, int64_t i, int lane) {
+  FkGap r;
+  r.first = i * a.max_blocks;
+  r.most = min(a.max_free - r.first, a.max_blocks);
+  r.have = fk_have(a);
+#pragma unroll
+  for (int k = 0; k < FK_UN; ++k)
+    r.g[k] = r.most > 0 ? a.free_blocks[r.first + min((int64_t)k * kWave + lane, r.most - 1)] : 0;
+  return r;
+}
+__device__ __forceinline__ int32_t fk_gap(const ForkArgs& a, FkGap& r, int lane) {
+  const int64_t n = min(r.have - r.first, r.most);
+  for (int64_t c0 = 0; c0 < n;) {  // uniform
+#pragma unroll
+    for (int k = 0; k < FK_UN; ++k) {
+      const uint64_t none = __ballot(c0 + k * kWave + lane < n && r.g[k] < 0);
+      if (none) return (int32_t)(c0 + k * kWave) + __ffsll((unsigned long long)none) - 1;
+    }
+    c0 += FK_UN * kWave;
+    if (c0 >= n) break;
+#pragma unroll
+    for (int k = 0; k < FK_UN; ++k) r.g[k] = a.free_blocks[r.first + min(c0 + k * kWave + lane, n - 1)];
+  }
+  return FK_NONE;
+}
+
 // New row i's table and copy, by `step` threads, of which this is thread t: x from fk_own, `before`
 // the pages of the rows in front of it, all the rows' pages.
 __device__ __forceinline__ void fk_put(const ForkArgs& a, int64_t i, int32_t x, uint64_t before, uint64_t total,
                                        bool bad, int t, int step) {
-  const int64_t have = a.num_free ? min(*a.num_free, a.max_free) : a.max_free;
-  bad |= (int64_t)total > have;
+  bad |= (int64_t)total > fk_have(a);
   const FkRow r = fk_row(a, i);
   const bool copy = x & FK_COPY;
   const int64_t kept = r.whole + (r.part > 0 && !copy), end = kept + (x & (FK_COPY - 1));
@@ -347,17 +385,18 @@ __device__ __forceinline__ void fk_put(const ForkArgs& a, int64_t i, int32_t x, 
 constexpr int FK_SMALL = 16;
 constexpr int64_t FK_SMALL_BLOCKS = 512;
 __global__ void __launch_bounds__(FK_SMALL * kWave) fork_small_kernel(ForkArgs a) {
-  __shared__ int32_t sOwn[FK_SMALL];
+  __shared__ int32_t sOwn[FK_SMALL], sGap[FK_SMALL];
   const int lane = threadIdx.x & (kWave - 1), i = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   if (i < a.batch) {  // uniform per wave
-    const int32_t x = fk_own(a, i, lane);
-    if (lane == 0) sOwn[i] = x;
+    FkGap ask = fk_ask(a, i, lane);
+    const int32_t x = fk_own(a, i, lane), gap = fk_gap(a, ask, lane);
+    if (lane == 0) sOwn[i] = x, sGap[i] = gap;
   }
   __syncthreads();
-  const int32_t x = lane < a.batch ? sOwn[lane] : 0;
-  const bool bad = __any(x < 0);
+  const int32_t x = lane < a.batch ? sOwn[lane] : 0, gap = lane < a.batch ? sGap[lane] : FK_NONE;
   const uint32_t n = (uint32_t)x & (FK_COPY - 1), inc = wave_incl_scan_u32(n, lane);
   const uint32_t total = rdlane(inc, kWave - 1);
+  const bool bad = __any(x < 0 || (gap != FK_NONE && lane * a.max_blocks + gap < (int64_t)total));
   if (i < a.batch)
     fk_put(a, i, (int32_t)rdlane((uint32_t)x, i), rdlane(inc - n, i), total, bad, lane, kWave);
 }
@@ -367,8 +406,9 @@ __global__ void __launch_bounds__(PGS_NT) fork_rows_kernel(ForkArgs a) {
   const int lane = threadIdx.x & (kWave - 1);
   const int64_t i = (int64_t)blockIdx.x * (PGS_NT / kWave) + threadIdx.x / kWave;
   if (i >= a.batch) return;  // uniform per wave
-  const int32_t x = fk_own(a, i, lane);
-  if (lane == 0) a.own[i] = x;
+  FkGap ask = fk_ask(a, i, lane);
+  const int32_t x = fk_own(a, i, lane), gap = fk_gap(a, ask, lane);
+  if (lane == 0) a.own[i] = x, a.gap[i] = gap;
 }
 
 __global__ void __launch_bounds__(PGS_NT) fork_tables_kernel(ForkArgs a) {
@@ -377,10 +417,12 @@ __global__ void __launch_bounds__(PGS_NT) fork_tables_kernel(ForkArgs a) {
   const int tid = threadIdx.x;
   const int64_t i = blockIdx.x;
   uint64_t total = 0, before = 0;
+  int64_t none = INT64_MAX;  // first entry that is no page
   int bad = 0;
   for (int64_t j = tid; j < a.batch; j += PGS_NT) {
-    const int32_t x = a.own[j];
+    const int32_t x = a.own[j], gap = a.gap[j];
     bad |= x < 0;
+    if (gap != FK_NONE) none = min(none, j * a.max_blocks + gap);
     const uint64_t n = (uint32_t)x & (FK_COPY - 1);
     total += n;
     if (j < i) before += n;
@@ -392,6 +434,7 @@ __global__ void __launch_bounds__(PGS_NT) fork_tables_kernel(ForkArgs a) {
   total = before = 0;
 #pragma unroll
   for (int w = 0; w < NW; ++w) total += sSum[w][0], before += sSum[w][1];
+  bad |= __syncthreads_or(none < (int64_t)total);
   fk_put(a, i, a.own[i], before, total, bad != 0, tid, PGS_NT);
 }
 

@@ -538,9 +538,9 @@ def fork_block_tables(block_table, kv_len, parent, room, free_blocks, block_size
     less) tokens. It shares the old row's whole pages; a last page filled in part goes to the first
     new row that goes on in it, unless another holds it whole, and the others get a new page and
     an entry in copies. New pages are free_blocks (int32) in order, the first num_free (int64 [1] on
-    the device; None: all) of them, as `free_page_list` gives both. Returns (table [N, max_blocks] int32,
-    -1 behind a row's last page; copies [3, N] int32 for `copy_pages`; used [1] int64, the pages
-    taken). All or nothing: parents, lengths, pages or free pages that do not fit give a table of
+    the device; None: all) of them as far as none is negative, as `free_page_list` gives both.
+    Returns (table [N, max_blocks] int32, -1 behind a row's last page; copies [3, N] int32 for
+    `copy_pages`; used [1] int64, the pages taken). All or nothing: parents, lengths, pages or free pages that do not fit give a table of
     -1, no copies and used 0, and set `error` (an int32 [1] device tensor) when given.
     """
     _lib.one_gpu(block_table, kv_len, parent, room, free_blocks, num_free, out, error)

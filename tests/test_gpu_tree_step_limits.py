@@ -1,0 +1,63 @@
+"""Calls at the edges of the operators around steps over trees: what cannot be right is refused or
+reported, never cut, skipped or taken for something else."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import tree as OT
+from specdec.kvcache import fork_block_tables, free_page_list
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def dev(x, dtype=None):
+    return torch.as_tensor(np.asarray(x), device=DEV, dtype=dtype)
+
+
+def new_error():
+    return torch.zeros(1, dtype=torch.int32, device=DEV)
+
+
+# ---- free pages that are none
+
+@pytest.mark.parametrize("N,mb,bs", [(3, 4, 16), (16, 512, 3), (17, 40, 16), (300, 9, 4), (5, 700, 2)])
+def test_a_fork_takes_pages_in_front_of_the_first_that_is_none(N, mb, bs):
+    """The list of free_page_list, -1 behind its pages, without their number or with a number that is
+    too large; a negative entry among the pages. What fits in front of it is given, else nothing."""
+    rng = np.random.default_rng(N)
+    B = N
+    kv = rng.integers(1, mb * bs + 1, B)
+    need = -(-kv // bs)
+    ids = rng.permutation(int(need.sum()))
+    table = np.full((B, mb), -1)
+    at = 0
+    for b in range(B):
+        table[b, :need[b]] = ids[at:at + need[b]]
+        at += need[b]
+    parent = rng.integers(0, B, N)                       # some twice: copies
+    room = np.minimum(kv[parent] + rng.integers(0, 3 * bs + 1, N), mb * bs)
+    most = N * mb
+    _, _, used, ok = OT.fork(table, kv, parent, room, list(range(at, at + most)), bs)
+    assert ok and used > 0
+    bt, rest = dev(table, torch.int32), (dev(kv), dev(parent), dev(room))
+    for have in (used, used - 1):                        # pages that are free
+        pages = np.arange(at, at + have)
+        nb = at + have
+        want, copies, u, ok = OT.fork(table, kv, parent, room, pages, bs)
+        assert ok == (have == used)
+        free, num = free_page_list(bt, nb, kv_len=rest[0], block_size=bs)
+        assert num.item() == have and free.numel() > have
+        for n in (None, num, num + 1, num * 0 + nb):
+            err = new_error()
+            got, gc, gu = fork_block_tables(bt, *rest, free, bs, num_free=n, error=err)
+            assert got.tolist() == want.tolist() and gc.tolist() == copies.tolist()
+            assert gu.item() == u and err.item() == (0 if ok else 1)
+    pages = np.arange(at, at + used)
+    for hole in {0, used // 2, used - 1}:
+        p = pages.copy()
+        p[hole] = -1
+        err = new_error()
+        got, gc, gu = fork_block_tables(bt, *rest, dev(p, torch.int32), bs, error=err)
+        assert (got == -1).all() and (gc[:2] == -1).all() and (gc[2] == 0).all()
+        assert gu.item() == 0 and err.item() == 1
