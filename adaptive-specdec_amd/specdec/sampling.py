@@ -308,8 +308,9 @@ def penalize_logits(logits, history=None, history_len=None, cu_rows=None, *, pro
             raise ValueError(f"node_tokens must be [{R}], got {tuple(node_tokens.shape)}")
         tk = _lib.as_dtype(node_tokens, torch.int64)
     if tree_mask is not None:
-        if tree_mask.dim() != 2 or tree_mask.shape[0] != R or tree_mask.dtype is not torch.int64:
-            raise ValueError(f"tree_mask must be int64 [{R}, words], got {tuple(tree_mask.shape)}")
+        if tree_mask.dim() != 2 or tree_mask.shape[0] != R or tree_mask.shape[1] < 1 or \
+                tree_mask.dtype is not torch.int64:
+            raise ValueError(f"tree_mask must be int64 [{R}, words], a word at least, got {tuple(tree_mask.shape)}")
         tm = tree_mask.contiguous()
     if R == 0 or V == 0:
         return out

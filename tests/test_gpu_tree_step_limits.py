@@ -6,6 +6,7 @@ import torch
 
 from oracle import tree as OT
 from specdec.kvcache import fork_block_tables, free_page_list
+from specdec.sampling import penalize_logits
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -61,3 +62,15 @@ def test_a_fork_takes_pages_in_front_of_the_first_that_is_none(N, mb, bs):
         got, gc, gu = fork_block_tables(bt, *rest, dev(p, torch.int32), bs, error=err)
         assert (got == -1).all() and (gc[:2] == -1).all() and (gc[2] == 0).all()
         assert gu.item() == 0 and err.item() == 1
+
+
+# ---- masks without columns
+
+def test_a_mask_of_no_columns_is_no_chain():
+    x = torch.randn((4, 100), device=DEV)
+    c = dict(cu_rows=dev([0, 4]), frequency=torch.ones(1, device=DEV), node_tokens=dev([1, 2, 3, 4]))
+    for R in (4, 0):
+        y, tok = x[:R], c["node_tokens"][:R]
+        with pytest.raises(ValueError, match="words"):
+            penalize_logits(y, **{**c, "cu_rows": dev([0, R]), "node_tokens": tok},
+                            tree_mask=torch.zeros((R, 0), dtype=torch.int64, device=DEV))
