@@ -314,10 +314,12 @@ def penalize_logits(logits, history=None, history_len=None, cu_rows=None, *, pro
         tm = tree_mask.contiguous()
     if R == 0 or V == 0:
         return out
+    # (a history of no columns has no address; its lengths are looked at all the same, its tokens never)
+    hp = _lib.ptr(hist) or _lib.ptr(hl)
     with _lib.on_device(x):
         rc = _lib.lib().sdx_penalize_logits(
             _lib.ptr(x), dt, R, V, ld, _lib.ptr(out), out.stride(0) if R > 1 else V, B,
-            _lib.ptr(cu), _lib.ptr(hist), hist_ld, 0 if hist is None else hist.shape[1], _lib.ptr(hl), _lib.ptr(pl),
+            _lib.ptr(cu), hp, hist_ld, 0 if hist is None else hist.shape[1], _lib.ptr(hl), _lib.ptr(pl),
             _lib.ptr(rep), _lib.ptr(freq), _lib.ptr(pres), _lib.ptr(bi), _lib.ptr(bv),
             0 if bi is None else bi.shape[1], _lib.ptr(al), al_ld, _lib.ptr(tk), _lib.ptr(tm),
             0 if tm is None else tm.shape[1], _lib.ptr(error), _lib.stream_of(x))

@@ -74,3 +74,21 @@ def test_a_mask_of_no_columns_is_no_chain():
         with pytest.raises(ValueError, match="words"):
             penalize_logits(y, **{**c, "cu_rows": dev([0, R]), "node_tokens": tok},
                             tree_mask=torch.zeros((R, 0), dtype=torch.int64, device=DEV))
+
+
+# ---- histories without columns
+
+def test_lengths_of_a_history_of_no_columns():
+    x = torch.randn((3, 100), device=DEV)
+    h = torch.zeros((3, 0), dtype=torch.int64, device=DEV)
+    rep = torch.full((3,), 2.0, device=DEV)
+    tok = dev([1, 2, 3])
+    err = new_error()
+    got = penalize_logits(x, h, dev([0, 0, 0]), repetition=rep, node_tokens=tok, error=err)
+    assert err.item() == 0 and torch.equal(got, penalize_logits(x, repetition=rep, node_tokens=tok))
+    for lens, prompt in (([0, 1, 0], None), ([0, -1, 0], None), ([0, 0, 0], [0, 1, 0])):
+        err = new_error()
+        out = penalize_logits(x, h, dev(lens), prompt_len=None if prompt is None else dev(prompt), repetition=rep,
+                              node_tokens=tok, error=err)
+        assert err.item() == 1 and torch.equal(out[1], x[1])
+        assert torch.equal(out[0::2], got[0::2])
