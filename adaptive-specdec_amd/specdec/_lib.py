@@ -212,6 +212,15 @@ def as_dtype(t, dtype):
     return t.to(dtype).contiguous()
 
 
+def as_int32(t):
+    """Whole numbers t as a contiguous int32 tensor (t itself where it is one). What 32 bits do not hold
+    becomes their largest or smallest number, which is out of every range that the kernels check: cut to
+    its low bits it could be another, valid one."""
+    if t.dtype is torch.int32 or t.dtype.itemsize < 4:
+        return as_dtype(t, torch.int32)
+    return t.to(torch.int64).clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32).contiguous()
+
+
 def workspace(nbytes, device, prepare=True):
     """A new workspace of at least `nbytes`; with `prepare`, prepared by
     sdx_workspace_init on the current stream (zero-filled, header word set: the

@@ -215,7 +215,7 @@ def tree_attention_paged(q, cu_q, k_pool, v_pool, block_table, kv_len, tree_mask
         q = q.clone()
     cu = _lib.as_dtype(cu_q, torch.int64)
     kl = _lib.as_dtype(kv_len, torch.int64)
-    bt = _lib.as_dtype(block_table, torch.int32)
+    bt = _lib.as_int32(block_table)
     tm = tree_mask.contiguous()
     with _lib.on_device(q):
         if workspace is None:

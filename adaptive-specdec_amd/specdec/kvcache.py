@@ -456,7 +456,7 @@ def _pool_shape(pool):
 def _table(block_table, what="block_table"):
     if block_table.dim() != 2:
         raise ValueError(f"{what} must be [B, max_blocks], got {tuple(block_table.shape)}")
-    return _lib.as_dtype(block_table, torch.int32)
+    return _lib.as_int32(block_table)
 
 
 def compact_paged(pool, block_table, kv_start, path, keep, kept=None, error=None):
@@ -549,7 +549,7 @@ def fork_block_tables(block_table, kv_len, parent, room, free_blocks, block_size
     B, mb = bt.shape
     kl, pa = _lib.as_dtype(kv_len, torch.int64), _lib.as_dtype(parent, torch.int64)
     ro = _lib.as_dtype(room, torch.int64)
-    fb = _lib.as_dtype(free_blocks, torch.int32)
+    fb = _lib.as_int32(free_blocks)
     nf = None if num_free is None else _lib.as_dtype(num_free, torch.int64)
     N = pa.numel()
     if kl.numel() != B or ro.numel() != N or (nf is not None and nf.numel() != 1):
@@ -588,7 +588,7 @@ def copy_pages(pool, copies, error=None):
     L, nb, bs, re, side = _pool_shape(pool)
     if copies.dim() != 2 or copies.shape[0] != 3:
         raise ValueError(f"copies must be [3, N], got {tuple(copies.shape)}")
-    c = _lib.as_dtype(copies, torch.int32)
+    c = _lib.as_int32(copies)
     if c.shape[1] == 0:
         return
     with _lib.on_device(pool):

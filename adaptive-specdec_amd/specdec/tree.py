@@ -63,14 +63,14 @@ def tree_layout(parents, cu_q, kv_len, block_table=None, block_size=None, max_no
     if not 1 <= max_nodes <= MAX_NODES:
         raise ValueError(f"max_nodes must lie in [1, {MAX_NODES}], got {max_nodes}")
     T, B = parents.numel(), kv_len.numel()
-    up = _lib.as_dtype(parents, torch.int32)
+    up = _lib.as_int32(parents)
     cu = _offsets(cu_q, B, T)
     kl = _lib.as_dtype(kv_len, torch.int64)
     bt = None
     if block_table is not None:
         if block_table.dim() != 2 or block_table.shape[0] != B:
             raise ValueError(f"block_table must be [{B}, max_blocks], got {tuple(block_table.shape)}")
-        bt = _lib.as_dtype(block_table, torch.int32)
+        bt = _lib.as_int32(block_table)
     mask, pos = kl.new_empty((T, (max_nodes + 63) // 64)), kl.new_empty(T)
     slots = None if bt is None else kl.new_empty(T)
     if T:
@@ -108,7 +108,7 @@ def tree_accept(tokens, parents, choice, cu_q, max_path, active=None, error=None
     if not 1 <= max_path <= MAX_NODES:
         raise ValueError(f"max_path must lie in [1, {MAX_NODES}], got {max_path}")
     tk, ch = _lib.as_dtype(tokens, torch.int64), _lib.as_dtype(choice, torch.int64)
-    up, cu = _lib.as_dtype(parents, torch.int32), _lib.as_dtype(cu_q, torch.int64)
+    up, cu = _lib.as_int32(parents), _lib.as_dtype(cu_q, torch.int64)
     act = None
     if active is not None:
         if active.numel() != B:

@@ -5,8 +5,10 @@ import pytest
 import torch
 
 from oracle import tree as OT
-from specdec.kvcache import fork_block_tables, free_page_list
+from specdec.attention import tree_attention_paged
+from specdec.kvcache import compact_paged, copy_pages, fork_block_tables, free_page_list
 from specdec.sampling import penalize_logits
+from specdec.tree import tree_accept, tree_layout
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -92,3 +94,45 @@ def test_lengths_of_a_history_of_no_columns():
                               node_tokens=tok, error=err)
         assert err.item() == 1 and torch.equal(out[1], x[1])
         assert torch.equal(out[0::2], got[0::2])
+
+
+# ---- whole numbers that 32 bits do not hold
+
+@pytest.mark.parametrize("far", [1 << 32, (1 << 32) + 1, -(1 << 32), (1 << 40) - 1, -(1 << 33) - 1])
+def test_numbers_past_32_bits_are_out_of_range(far):
+    up = dev([-1, 0, far, 0])
+    table = dev([[2, 1]], torch.int32)
+    err = new_error()
+    mask, pos, slots = tree_layout(up, dev([0, 4]), dev([9]), table, 16, error=err)
+    assert err.item() == 1 and (mask == 0).all() and (pos == 0).all() and (slots == -1).all()
+    path, keep, _ = tree_accept(dev([5, 6, 7, 8]), up, dev([7, 7, 7, 7]), dev([0, 4]), 4)
+    assert path.tolist() == [[0, -1, -1, -1]] and keep.tolist() == [1]     # node 2 is nobody's child
+    # pages
+    wide = torch.tensor([[2, far]], device=DEV)
+    err = new_error()
+    free_page_list(wide, 4, kv_len=dev([20]), block_size=16, error=err)
+    assert err.item() == 1
+    pool = torch.randn((1, 2, 4, 16, 8), device=DEV).half()
+    before = pool.clone()
+    err = new_error()
+    compact_paged(pool, wide, dev([14]), dev([[1, 3]]), dev([2]), error=err)
+    assert err.item() == 1 and torch.equal(pool, before)
+    for row in range(3):                                   # a source, a target, a number of tokens
+        copies = dev([[1], [2], [3]])
+        copies[row] = far
+        err = new_error()
+        copy_pages(pool, copies, error=err)
+        # negative pages are entries that are skipped
+        assert torch.equal(pool, before) and err.item() == (0 if row < 2 and far < 0 else 1)
+    q = torch.randn((4, 1, 64), device=DEV).half()
+    kp = torch.randn((4, 16, 64), device=DEV).half()
+    err = new_error()
+    tree_attention_paged(q, dev([0, 4]), kp, kp, wide, dev([20]), torch.full((4, 1), 15, device=DEV), error=err)
+    assert err.item() == 1
+    if far < 0:                                            # a new table without holes
+        err = new_error()
+        got, _, used = fork_block_tables(table, dev([20]), dev([0]), dev([32]), dev([far]), 16,
+                                         error=err)
+        assert used.item() == 0 and err.item() == 0 and got.tolist() == [[2, 1]]
+        got, _, used = fork_block_tables(table, dev([16]), dev([0]), dev([17]), dev([far]), 16, error=err)
+        assert used.item() == 0 and err.item() == 1 and (got == -1).all()
