@@ -212,12 +212,32 @@ def as_dtype(t, dtype):
     return t.to(dtype).contiguous()
 
 
-def as_int32(t):
+_WHOLE = frozenset({torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8, torch.uint16, torch.uint32})
+
+
+def whole(name, t):
+    """t, which holds whole numbers by its type: fractions, NaN and truth values would be cut to numbers
+    that nobody meant."""
+    if t.dtype not in _WHOLE:
+        raise TypeError(f"{name} must be whole numbers, got {t.dtype}")
+    return t
+
+
+def as_int64(name, t):
+    """Whole numbers t as a contiguous int64 tensor (t itself where it is one)."""
+    if t.dtype is torch.int64 and t.is_contiguous():
+        return t
+    return whole(name, t).to(torch.int64).contiguous()
+
+
+def as_int32(name, t):
     """Whole numbers t as a contiguous int32 tensor (t itself where it is one). What 32 bits do not hold
     becomes their largest or smallest number, which is out of every range that the kernels check: cut to
     its low bits it could be another, valid one."""
-    if t.dtype is torch.int32 or t.dtype.itemsize < 4:
-        return as_dtype(t, torch.int32)
+    if t.dtype is torch.int32 and t.is_contiguous():
+        return t
+    if whole(name, t).dtype.itemsize < 4:
+        return t.to(torch.int32).contiguous()
     return t.to(torch.int64).clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32).contiguous()
 
 

@@ -213,9 +213,9 @@ def tree_attention_paged(q, cu_q, k_pool, v_pool, block_table, kv_len, tree_mask
     q = q.contiguous()
     if q.data_ptr() % 16:
         q = q.clone()
-    cu = _lib.as_dtype(cu_q, torch.int64)
-    kl = _lib.as_dtype(kv_len, torch.int64)
-    bt = _lib.as_int32(block_table)
+    cu = _lib.as_int64("cu_q", cu_q)
+    kl = _lib.as_int64("kv_len", kv_len)
+    bt = _lib.as_int32("block_table", block_table)
     tm = tree_mask.contiguous()
     with _lib.on_device(q):
         if workspace is None:

@@ -456,7 +456,7 @@ def _pool_shape(pool):
 def _table(block_table, what="block_table"):
     if block_table.dim() != 2:
         raise ValueError(f"{what} must be [B, max_blocks], got {tuple(block_table.shape)}")
-    return _lib.as_int32(block_table)
+    return _lib.as_int32(what, block_table)
 
 
 def compact_paged(pool, block_table, kv_start, path, keep, kept=None, error=None):
@@ -480,8 +480,8 @@ def compact_paged(pool, block_table, kv_start, path, keep, kept=None, error=None
                          f"{kv_start.numel()}, {tuple(path.shape)} and {keep.numel()}")
     if kept is not None and (kept.dtype != torch.int64 or kept.numel() != B or not kept.is_contiguous()):
         raise ValueError(f"kept must be a contiguous int64 [{B}]")
-    st, pt = _lib.as_dtype(kv_start, torch.int64), _lib.as_dtype(path, torch.int64)
-    kp = _lib.as_dtype(keep, torch.int64)
+    st, pt = _lib.as_int64("kv_start", kv_start), _lib.as_int64("path", path)
+    kp = _lib.as_int64("keep", keep)
     if B == 0:
         return
     if pt.shape[1] == 0:
@@ -511,7 +511,7 @@ def free_page_list(block_table, num_blocks, kv_len=None, block_size=None, error=
     B, mb = bt.shape
     kl = None
     if kv_len is not None:
-        kl = _lib.as_dtype(kv_len, torch.int64)
+        kl = _lib.as_int64("kv_len", kv_len)
         if kl.numel() != B:
             raise ValueError(f"kv_len must be [{B}], got {kl.numel()}")
     if num_blocks < 1:
@@ -547,10 +547,10 @@ def fork_block_tables(block_table, kv_len, parent, room, free_blocks, block_size
     _error_word(error)
     bt = _table(block_table)
     B, mb = bt.shape
-    kl, pa = _lib.as_dtype(kv_len, torch.int64), _lib.as_dtype(parent, torch.int64)
-    ro = _lib.as_dtype(room, torch.int64)
-    fb = _lib.as_int32(free_blocks)
-    nf = None if num_free is None else _lib.as_dtype(num_free, torch.int64)
+    kl, pa = _lib.as_int64("kv_len", kv_len), _lib.as_int64("parent", parent)
+    ro = _lib.as_int64("room", room)
+    fb = _lib.as_int32("free_blocks", free_blocks)
+    nf = None if num_free is None else _lib.as_int64("num_free", num_free)
     N = pa.numel()
     if kl.numel() != B or ro.numel() != N or (nf is not None and nf.numel() != 1):
         raise ValueError(f"block_table of {B} rows needs kv_len [{B}], {N} parents room [{N}] and num_free "
@@ -588,7 +588,7 @@ def copy_pages(pool, copies, error=None):
     L, nb, bs, re, side = _pool_shape(pool)
     if copies.dim() != 2 or copies.shape[0] != 3:
         raise ValueError(f"copies must be [3, N], got {tuple(copies.shape)}")
-    c = _lib.as_int32(copies)
+    c = _lib.as_int32("copies", copies)
     if c.shape[1] == 0:
         return
     with _lib.on_device(pool):

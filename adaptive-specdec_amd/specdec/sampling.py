@@ -209,7 +209,7 @@ def _rows_of(name, t, rows, cols, dtype):
     if t.dim() != 2 or t.shape[0] != rows or (cols is not None and t.shape[1] != cols):
         raise ValueError(f"{name} must be [{rows}, {'...' if cols is None else cols}], got {tuple(t.shape)}")
     if t.dtype is not dtype:
-        t = t.to(dtype)
+        t = _lib.whole(name, t).to(dtype)
     ld, unit = t.stride()
     n = t.shape[1]
     if n and (unit != 1 or (rows > 1 and ld < n)):
@@ -222,13 +222,9 @@ def _per_row(name, t, batch, dtype=torch.float32):
         return None
     if t.numel() != batch:
         raise ValueError(f"{name} must be [{batch}], got {tuple(t.shape)}")
+    if dtype is torch.int64:
+        return _lib.as_int64(name, t)
     return t if t.dtype is dtype and t.is_contiguous() else t.to(dtype).contiguous()
-
-
-def _whole(name, t):
-    if t is not None and t.dtype is not torch.int64 and (t.dtype.is_floating_point or t.dtype.is_complex or
-                                                         t.dtype is torch.bool):
-        raise TypeError(f"{name} must be whole numbers, got {t.dtype}")
 
 
 def penalize_logits(logits, history=None, history_len=None, cu_rows=None, *, prompt_len=None,
@@ -259,10 +255,6 @@ def penalize_logits(logits, history=None, history_len=None, cu_rows=None, *, pro
     if logits.dim() != 2:
         raise ValueError(f"logits must be [rows, V], got {tuple(logits.shape)}")
     dt = _lib.dtype_code(logits)
-    _whole("history", history)
-    _whole("bias_ids", bias_ids)
-    _whole("node_tokens", node_tokens)
-    _whole("tree_mask", tree_mask)
     if error is not None and (error.dtype != torch.int32 or error.numel() < 1):
         raise TypeError("error must be an int32 device tensor of one element")
     R, V = logits.shape
@@ -292,7 +284,7 @@ def penalize_logits(logits, history=None, history_len=None, cu_rows=None, *, pro
         if bias_ids.dim() != 2 or bias_ids.shape[0] != B or bias.shape != bias_ids.shape:
             raise ValueError(f"bias_ids and bias must be [{B}, n], got {tuple(bias_ids.shape)} and "
                              f"{tuple(bias.shape)}")
-        bi, bv = _lib.as_dtype(bias_ids, torch.int64), _lib.as_dtype(bias, torch.float32)
+        bi, bv = _lib.as_int64("bias_ids", bias_ids), _lib.as_dtype(bias, torch.float32)
     al, al_ld = None, 0
     if allowed is not None:
         if allowed.dim() == 2 and allowed.shape[1] < (V + 31) // 32:
@@ -301,15 +293,15 @@ def penalize_logits(logits, history=None, history_len=None, cu_rows=None, *, pro
             raise TypeError(f"allowed must be int32 words, got {allowed.dtype}")
         al, al_ld = _rows_of("allowed", allowed, R, None, torch.int32)
     # (kept by name: what a temporary held could be taken by another thread before the launch)
-    cu = None if cu_rows is None else _lib.as_dtype(cu_rows, torch.int64)
+    cu = None if cu_rows is None else _lib.as_int64("cu_rows", cu_rows)
     tk = tm = None
     if node_tokens is not None:
         if node_tokens.numel() != R:
             raise ValueError(f"node_tokens must be [{R}], got {tuple(node_tokens.shape)}")
-        tk = _lib.as_dtype(node_tokens, torch.int64)
+        tk = _lib.as_int64("node_tokens", node_tokens)
     if tree_mask is not None:
         if tree_mask.dim() != 2 or tree_mask.shape[0] != R or tree_mask.shape[1] < 1 or \
-                tree_mask.dtype is not torch.int64:
+                _lib.whole("tree_mask", tree_mask).dtype is not torch.int64:
             raise ValueError(f"tree_mask must be int64 [{R}, words], a word at least, got {tuple(tree_mask.shape)}")
         tm = tree_mask.contiguous()
     if R == 0 or V == 0:

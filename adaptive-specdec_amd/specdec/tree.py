@@ -28,13 +28,7 @@ MAX_NODES = 512   # of a row
 def _offsets(cu_q, batch, T):
     if cu_q.numel() != batch + 1:
         raise ValueError(f"{batch} rows need cu_q [{batch + 1}], got {cu_q.numel()} offsets")
-    return _lib.as_dtype(cu_q, torch.int64)
-
-
-def _whole(name, t):
-    if t is not None and t.dtype is not torch.int64 and (t.dtype.is_floating_point or t.dtype.is_complex or
-                                                         t.dtype is torch.bool):
-        raise TypeError(f"{name} must be whole numbers, got {t.dtype}")
+    return _lib.as_int64("cu_q", cu_q)
 
 
 def tree_layout(parents, cu_q, kv_len, block_table=None, block_size=None, max_nodes=64,
@@ -52,7 +46,6 @@ def tree_layout(parents, cu_q, kv_len, block_table=None, block_size=None, max_no
     and slots without a page, which set `error` (an int32 [1] device tensor) when given.
     """
     _lib.one_gpu(parents, cu_q, kv_len, block_table, error)
-    _whole("parents", parents)
     if error is not None and (error.dtype != torch.int32 or error.numel() < 1):
         raise TypeError("error must be an int32 device tensor of one element")
     if parents.dim() != 1:
@@ -63,14 +56,14 @@ def tree_layout(parents, cu_q, kv_len, block_table=None, block_size=None, max_no
     if not 1 <= max_nodes <= MAX_NODES:
         raise ValueError(f"max_nodes must lie in [1, {MAX_NODES}], got {max_nodes}")
     T, B = parents.numel(), kv_len.numel()
-    up = _lib.as_int32(parents)
+    up = _lib.as_int32("parents", parents)
     cu = _offsets(cu_q, B, T)
-    kl = _lib.as_dtype(kv_len, torch.int64)
+    kl = _lib.as_int64("kv_len", kv_len)
     bt = None
     if block_table is not None:
         if block_table.dim() != 2 or block_table.shape[0] != B:
             raise ValueError(f"block_table must be [{B}, max_blocks], got {tuple(block_table.shape)}")
-        bt = _lib.as_int32(block_table)
+        bt = _lib.as_int32("block_table", block_table)
     mask, pos = kl.new_empty((T, (max_nodes + 63) // 64)), kl.new_empty(T)
     slots = None if bt is None else kl.new_empty(T)
     if T:
@@ -96,8 +89,6 @@ def tree_accept(tokens, parents, choice, cu_q, max_path, active=None, error=None
     range set `error` (an int32 [1] device tensor) when given.
     """
     _lib.one_gpu(tokens, parents, choice, cu_q, active, error)
-    for name, t in (("tokens", tokens), ("parents", parents), ("choice", choice)):
-        _whole(name, t)
     if error is not None and (error.dtype != torch.int32 or error.numel() < 1):
         raise TypeError("error must be an int32 device tensor of one element")
     T, B = tokens.numel(), cu_q.numel() - 1
@@ -107,8 +98,8 @@ def tree_accept(tokens, parents, choice, cu_q, max_path, active=None, error=None
     max_path = int(max_path)
     if not 1 <= max_path <= MAX_NODES:
         raise ValueError(f"max_path must lie in [1, {MAX_NODES}], got {max_path}")
-    tk, ch = _lib.as_dtype(tokens, torch.int64), _lib.as_dtype(choice, torch.int64)
-    up, cu = _lib.as_int32(parents), _lib.as_dtype(cu_q, torch.int64)
+    tk, ch = _lib.as_int64("tokens", tokens), _lib.as_int64("choice", choice)
+    up, cu = _lib.as_int32("parents", parents), _lib.as_int64("cu_q", cu_q)
     act = None
     if active is not None:
         if active.numel() != B:

@@ -136,3 +136,42 @@ def test_numbers_past_32_bits_are_out_of_range(far):
         assert used.item() == 0 and err.item() == 0 and got.tolist() == [[2, 1]]
         got, _, used = fork_block_tables(table, dev([16]), dev([0]), dev([17]), dev([far]), 16, error=err)
         assert used.item() == 0 and err.item() == 1 and (got == -1).all()
+
+
+# ---- numbers that are not whole
+
+def test_only_whole_numbers_are_taken_for_whole_numbers():
+    i64 = lambda *x: dev(x, torch.int64)  # noqa: E731
+    pool = torch.zeros((1, 2, 4, 16, 8), dtype=torch.half, device=DEV)
+    table = dev([[0, 1], [2, -1]], torch.int32)
+    q = torch.zeros((3, 1, 64), dtype=torch.half, device=DEV)
+    kp = torch.zeros((4, 16, 64), dtype=torch.half, device=DEV)
+    x = torch.zeros((3, 10), device=DEV)
+    cu, kv = i64(0, 2, 3), i64(20, 3)
+    calls = [
+        (tree_layout, dict(parents=dev([-1, 0, -1], torch.int32), cu_q=cu, kv_len=kv, block_table=table,
+                           block_size=16), ("parents", "cu_q", "kv_len", "block_table")),
+        (tree_accept, dict(tokens=i64(1, 2, 3), parents=dev([-1, 0, -1], torch.int32), choice=i64(2, 5, 6), cu_q=cu,
+                           max_path=4), ("tokens", "parents", "choice", "cu_q")),
+        (compact_paged, dict(pool=pool, block_table=table, kv_start=kv - 2, path=dev([[0, 1], [0, 1]]), keep=i64(2, 1)),
+         ("block_table", "kv_start", "path", "keep")),
+        (free_page_list, dict(block_table=table, num_blocks=4, kv_len=kv, block_size=16),
+         ("block_table", "kv_len")),
+        (fork_block_tables, dict(block_table=table, kv_len=kv, parent=i64(0, 1), room=i64(21, 4),
+                                 free_blocks=dev([3], torch.int32), block_size=16, num_free=i64(1)),
+         ("block_table", "kv_len", "parent", "room", "free_blocks", "num_free")),
+        (copy_pages, dict(pool=pool, copies=dev([[0], [3], [5]], torch.int32)), ("copies",)),
+        (tree_attention_paged, dict(q=q, cu_q=cu, k_pool=kp, v_pool=kp, block_table=table, kv_len=kv,
+                                    tree_mask=torch.ones((3, 1), dtype=torch.int64, device=DEV)),
+         ("cu_q", "kv_len", "block_table")),
+        (penalize_logits, dict(logits=x, history=i64(1, 2).view(2, 1), history_len=i64(1, 1), cu_rows=cu,
+                               prompt_len=i64(0, 1), node_tokens=i64(1, 2, 3), bias_ids=i64(1, 2).view(2, 1),
+                               bias=torch.ones((2, 1), device=DEV)),
+         ("history", "history_len", "cu_rows", "prompt_len", "node_tokens", "bias_ids")),
+    ]
+    for call, args, names in calls:
+        call(**args)
+        for name in names:
+            for dtype in (torch.float32, torch.bool, torch.bfloat16):
+                with pytest.raises(TypeError, match=name):
+                    call(**{**args, name: args[name].to(dtype)})
