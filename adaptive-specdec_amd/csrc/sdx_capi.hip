@@ -1171,6 +1171,10 @@ int sdx_tree_accept(const int64_t* tokens, const int32_t* parents, const int64_t
 }
 
 // ------------------------------------------------------------------ pages of the cache
+// x's first nx bytes and y's first ny have some in common
+static bool overlap(const void* x, size_t nx, const void* y, size_t ny) {
+  return x && y && (const char*)x < (const char*)y + ny && (const char*)y < (const char*)x + nx;
+}
 // pool arguments that compact and copy share
 static int pool_args(const char* who, const void* pool, int64_t layer_stride, int64_t side_stride, int dtype,
                      int32_t layers, int64_t row_elems, int64_t num_blocks, int32_t block_size) {
@@ -1200,6 +1204,13 @@ int sdx_compact_paged(void* pool, int64_t layer_stride, int64_t side_stride, int
     return fail(SDX_EUNSUPPORTED, "sdx_compact_paged: more than 2^23 rows, 2^31 blocks or paths of more "
                                   "than %d tokens", sdx::TREE_MAX_NODES);
   if (batch == 0) return SDX_OK;
+  // a row's workgroups all read its lengths and path, and one of them writes kept (keep itself may
+  // become kept: a row that is refused then has 0 of it for the others, which move nothing either)
+  const size_t n = (size_t)batch * sizeof(int64_t);
+  if (overlap(kept, n, kv_start, n) || overlap(kept, n, path, n * max_path) ||
+      (kept != keep && overlap(kept, n, keep, n)) ||
+      overlap(kept, n, block_table, (size_t)batch * max_blocks * sizeof(int32_t)))
+    return fail(SDX_EINVAL, "sdx_compact_paged: kept may be keep itself or lies apart from what is read");
   const int64_t es = (int64_t)dsize(dtype);
   sdx::CompactArgs a{(uint8_t*)pool, layer_stride * es, side_stride * es, row_elems * es, num_blocks,
                      block_table, kv_start, path, keep, batch, max_blocks, block_size, max_path,

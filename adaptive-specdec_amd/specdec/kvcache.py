@@ -467,8 +467,8 @@ def compact_paged(pool, block_table, kv_start, path, keep, kept=None, error=None
     (kv_start, keep [B], path [B, P] int64, P at most 512, ascending in every row as
     `specdec.tree.tree_accept` gives it). Rows whose path, lengths or pages are out of range are
     left as they are and set `error` (an int32 [1] device tensor) when given; kept (int64 [B], when
-    given) receives keep, 0 in those rows: what the lengths go up by. Rows must not share the pages
-    behind kv_start.
+    given; keep itself, or apart from the other arguments) receives keep, 0 in those rows: what the
+    lengths go up by. Rows must not share the pages behind kv_start.
     """
     _lib.one_gpu(pool, block_table, kv_start, path, keep, kept, error)
     _error_word(error)

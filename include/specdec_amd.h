@@ -489,8 +489,8 @@ int sdx_tree_accept(const int64_t* tokens, const int32_t* parents, const int64_t
  * (512 at most) ascends strictly from 0 or more, as sdx_tree_accept writes it; what lies behind
  * keep[b] is not read. kv_start, keep int64 [batch]. A row whose path, lengths or pages are out of
  * range is left as it is, all of it, and sets *error (nullable). kept (int64 [batch], nullable) = keep,
- * 0 in such rows: what the rows' lengths go up by. Rows must not share the pages that are written. One
- * kernel, in place. */
+ * 0 in such rows: what the rows' lengths go up by; it may be keep itself, else lies apart from what is
+ * read. Rows must not share the pages that are written. One kernel, in place. */
 int sdx_compact_paged(void* pool, int64_t layer_stride, int64_t side_stride, int dtype, int32_t layers,
                       int64_t row_elems, int64_t num_blocks, int32_t block_size,
                       const int32_t* block_table, int64_t batch, int64_t max_blocks,

@@ -175,3 +175,26 @@ def test_only_whole_numbers_are_taken_for_whole_numbers():
             for dtype in (torch.float32, torch.bool, torch.bfloat16):
                 with pytest.raises(TypeError, match=name):
                     call(**{**args, name: args[name].to(dtype)})
+
+
+# ---- counts written over counts
+
+def test_kept_may_be_keep_itself():
+    """Rows that are refused have 0 in it then, and move nothing."""
+    L, B, mb, bs = 9, 40, 3, 16
+    g = torch.Generator(device=DEV).manual_seed(2)
+    pool = torch.randn((L, 2, B * mb, bs, 64), generator=g, device=DEV).half()
+    table = np.arange(B * mb).reshape(B, mb)
+    start, path, keep = np.full(B, 20), np.tile([1, 2, 5, 9], (B, 1)), np.full(B, 4)
+    path[::3, 2] = 2                                     # does not ascend
+    keep[5] = 0
+    want = pool.cpu().clone()
+    assert not OT.compact(want, table, start, path, keep)
+    k, err = dev(keep), new_error()
+    compact_paged(pool, dev(table, torch.int32), dev(start), dev(path), k, kept=k, error=err)
+    assert torch.equal(pool.cpu(), want) and err.item() == 1
+    assert k.tolist() == [0 if b % 3 == 0 else int(keep[b]) for b in range(B)]
+    s = dev(start)
+    with pytest.raises(RuntimeError, match="apart"):
+        compact_paged(pool, dev(table, torch.int32), s, dev(path), dev(keep), kept=s)
+    assert torch.equal(pool.cpu(), want) and s.tolist() == start.tolist()
