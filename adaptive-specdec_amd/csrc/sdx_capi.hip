@@ -1261,12 +1261,24 @@ int sdx_fork_block_tables(const int32_t* block_table, int64_t old_batch, int64_t
   if (batch > (1 << 18) || max_blocks > (1 << 27))
     return fail(SDX_EUNSUPPORTED, "sdx_fork_block_tables: more than 2^18 new rows or 2^27 blocks");
   if (batch == 0) return SDX_OK;
-  if (out == block_table)
+  if (overlap(out, (size_t)batch * max_blocks * sizeof(int32_t), block_table,
+              (size_t)old_batch * max_blocks * sizeof(int32_t)))
     return fail(SDX_EINVAL, "sdx_fork_block_tables: the new tables may not lie over the old ones");
   const size_t need = sdx_fork_block_tables_workspace(batch);
   if (!workspace || !aligned16(workspace) || workspace_bytes < need)
     return fail(SDX_EWORKSPACE, "sdx_fork_block_tables: needs a 16-byte aligned workspace of %zu bytes "
                                 "(got %zu)", need, workspace_bytes);
+  // every workgroup reads all of these, and writes its part of those
+  const struct { const void* at; size_t bytes; } read[] = {
+      {block_table, (size_t)old_batch * max_blocks * sizeof(int32_t)}, {kv_len, (size_t)old_batch * sizeof(int64_t)},
+      {parent, (size_t)batch * sizeof(int64_t)}, {room, (size_t)batch * sizeof(int64_t)},
+      {free_blocks, (size_t)max_free * sizeof(int32_t)}, {num_free, sizeof(int64_t)}},
+      written[] = {{out, (size_t)batch * max_blocks * sizeof(int32_t)},
+                   {copies, (size_t)batch * 3 * sizeof(int32_t)}, {used, sizeof(int64_t)}};
+  for (const auto& r : read)
+    for (const auto& w : written)
+      if (overlap(r.at, r.bytes, w.at, w.bytes))
+        return fail(SDX_EINVAL, "sdx_fork_block_tables: out, copies and used may not lie over what is read");
   sdx::ForkArgs a{block_table, kv_len, parent, room, free_blocks, num_free, old_batch, batch, max_blocks,
                   block_size, max_free, (int32_t*)workspace, (int32_t*)workspace + batch, out, copies, used, error};
   return hip_status(sdx::launch_fork_tables(a, (hipStream_t)stream), "fork_tables");

@@ -518,8 +518,8 @@ size_t sdx_free_pages_workspace(int64_t batch, int64_t max_blocks, int64_t num_b
  * of copies [3, batch] int32: the page, the new page and the tokens to copy (-1, -1, 0: none), as
  * sdx_copy_pages takes them. New pages come from free_blocks [max_free] int32, row after row, in order, the
  * first *num_free (device int64; null: max_free) of them as far as none is negative; *used (int64) =
- * how many. out is written whole, -1 behind a row's last page, and may not lie over block_table. All or
- * nothing: where a parent, a length, a page of an old row or the free pages are out of range, out and
+ * how many. out is written whole, -1 behind a row's last page; out, copies and used may not lie over
+ * the other arguments. All or nothing: where a parent, a length, a page of an old row or the free pages are out of range, out and
  * copies are -1 (tokens 0), *used 0 and *error (nullable) 1. Two kernels; `workspace` as the query says. Every row
  * looks at all others: 384 rows take 10 us. Up to 2^18 new rows and 2^27 columns. */
 int sdx_fork_block_tables(const int32_t* block_table, int64_t old_batch, int64_t max_blocks,

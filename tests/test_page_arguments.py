@@ -23,3 +23,28 @@ def test_compact_does_not_write_what_it_reads():
             if kept != keep:
                 assert call(kept) == EINVAL, (at, kept)
                 assert b"kept may be keep itself" in L.sdx_last_error()
+
+
+def test_forked_tables_do_not_lie_over_what_is_read():
+    """Every row reads the old tables, the parents and the number of free pages while others write theirs."""
+    from specdec import _lib
+    L = _lib.lib()
+    B, mb, N, free = 6, 4, 5, 7
+    base = dict(table=(1 << 20, 4 * B * mb), kv=(2 << 20, 8 * B), parent=(3 << 20, 8 * N), room=(4 << 20, 8 * N),
+                free=(5 << 20, 4 * free), num=(6 << 20, 8))
+    apart = dict(out=7 << 20, copies=8 << 20, used=9 << 20)
+    p = ctypes.c_void_p
+    ws = L.sdx_fork_block_tables_workspace(N)
+
+    def call(**over):
+        w = {**apart, **over}
+        at = {k: p(v[0]) for k, v in base.items()}
+        return L.sdx_fork_block_tables(at["table"], B, mb, at["kv"], at["parent"], at["room"], N, 16, at["free"], free,
+                                       at["num"], p(w["out"]), p(w["copies"]), p(w["used"]), p(10 << 20), ws, None,
+                                       None)
+
+    for name, size in (("out", 4 * N * mb), ("copies", 12 * N), ("used", 8)):
+        for at, n in base.values():
+            for where in (at, at + n - 4, at - size + 4):
+                assert call(**{name: where}) == EINVAL, (name, at, where)
+                assert b"may not lie over" in L.sdx_last_error()
