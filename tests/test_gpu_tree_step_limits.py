@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from oracle import tree as OT
-from specdec.attention import tree_attention_paged
+from specdec.attention import tree_attention_paged, tree_attention_workspace
 from specdec.kvcache import compact_paged, copy_pages, fork_block_tables, free_page_list
 from specdec.sampling import penalize_logits
 from specdec.tree import tree_accept, tree_layout
@@ -20,6 +20,22 @@ def dev(x, dtype=None):
 
 def new_error():
     return torch.zeros(1, dtype=torch.int32, device=DEV)
+
+
+def attention_case(n, start, d=64, pad=0, bs=16):
+    """n: nodes per row, start: keys in front of them."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    n, start = np.asarray(n), np.asarray(start)
+    cu, kv = np.concatenate([[0], np.cumsum(n)]), n + start
+    mb = int(-(-kv.max() // bs)) + 1
+    B, T = len(n), int(cu[-1]) + pad
+    table = np.arange(B * mb).reshape(B, mb)
+    parents = [max(i // 2 - 1, -1) for m in n for i in range(m)] + [-1] * pad
+    mask = tree_layout(dev(parents, torch.int32), dev(cu), dev(kv),
+                       max_nodes=max(64, -(-int(n.max()) // 64) * 64))[0]
+    rnd = lambda *s: torch.randn(s, generator=g, device=DEV).half()  # noqa: E731
+    return dict(q=rnd(T, 8, d), cu_q=dev(cu), k_pool=rnd(B * mb, bs, 2 * d), v_pool=rnd(B * mb, bs, 2 * d),
+                block_table=dev(table, torch.int32), kv_len=dev(kv), tree_mask=mask)
 
 
 # ---- free pages that are none
@@ -175,6 +191,33 @@ def test_only_whole_numbers_are_taken_for_whole_numbers():
             for dtype in (torch.float32, torch.bool, torch.bfloat16):
                 with pytest.raises(TypeError, match=name):
                     call(**{**args, name: args[name].to(dtype)})
+
+
+# ---- rows that share their nodes
+
+def shared_nodes(B):
+    """Offsets 0, 256, 0, 256, ...: every row with nodes has all of them."""
+    c = attention_case([64] * 4, [30] * 4)
+    cu = torch.zeros(B + 1, dtype=torch.int64, device=DEV)
+    cu[1::2] = 256
+    return dict(c, cu_q=cu, kv_len=torch.full((B,), 350, device=DEV),
+                block_table=c["block_table"][:1].repeat(B, 4), tree_mask=c["tree_mask"].repeat(1, 4))
+
+
+@pytest.mark.parametrize("B", [40, 64, 70, 600, 1100])
+def test_rows_that_share_their_nodes_compute_nothing(B):
+    """More items than the workspace has records for, laid out by each wave (to 64 rows), by the
+    workgroup, and in several rounds of it: no output, and nothing behind the workspace."""
+    c = shared_nodes(B)
+    T, hq, d = c["q"].shape
+    hkv = c["k_pool"].shape[2] // d
+    need = tree_attention_workspace(T, B, hq, hkv, d).numel()
+    room = torch.full((need + (1 << 20),), 0x5A, dtype=torch.uint8, device=DEV)
+    items = hkv * sum(-(-256 * (hq // hkv) // 256) for b in range(0, B, 2))
+    assert items > hkv * (T * (hq // hkv) // 256 + min(B, T))
+    err, out = new_error(), torch.full_like(c["q"], 7.0)
+    tree_attention_paged(**c, out=out, workspace=room[:need], error=err)
+    assert err.item() == 1 and (out == 7).all() and (room[need:] == 0x5A).all()
 
 
 # ---- counts written over counts
