@@ -206,7 +206,7 @@ __device__ __forceinline__ void ta_add_odd(PaState<D>& st, const TreeAttnArgs& a
 // 16 bytes of each lane from its own address to the 1 KB at LDS byte `to`, lane after lane, without
 // a register in between. The compiler does not count it: ta_wait waits for it.
 __device__ __forceinline__ void ta_load_lds(const uint8_t* from, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory", "m0");
 }
 __device__ __forceinline__ void ta_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
