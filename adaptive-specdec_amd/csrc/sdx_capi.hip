@@ -1490,6 +1490,7 @@ static size_t tree_attn_ws(Carve& c, int64_t tokens, int64_t batch, int32_t hq, 
                            sdx::TreeAttnArgs* a) {
   a->max_items = sdx::tree_attn_items(tokens, batch, hkv, hq / hkv);
   a->items = c.take<sdx::TreeAttnItem>((size_t)a->max_items);
+  a->left = c.take<int32_t>(1);
   a->part_ml = c.take<float2>((size_t)2 * sdx::TREE_ATTN_GRID * sdx::TREE_ATTN_ROWS);
   a->part_o = c.take<float>((size_t)2 * sdx::TREE_ATTN_GRID * sdx::TREE_ATTN_ROWS * d);
   return c.used;
@@ -1506,13 +1507,12 @@ size_t sdx_tree_attention_workspace(int64_t num_tokens, int64_t batch, int32_t n
   return tree_attn_ws(c, num_tokens, batch, num_q_heads, num_kv_heads, head_dim, &a);
 }
 
-int sdx_tree_attention_paged(const void* q, int dtype, int64_t num_tokens, int64_t batch,
-                             const int64_t* cu_q, int32_t num_q_heads, int32_t num_kv_heads,
-                             int32_t head_dim, const void* k_pool, const void* v_pool,
-                             int64_t num_blocks, int32_t block_size, const int32_t* block_table,
-                             int64_t max_blocks, const int64_t* kv_len, const int64_t* tree_mask,
-                             int32_t mask_words, float scale, void* workspace, size_t workspace_bytes,
-                             void* out, int32_t* error, sdx_stream_t stream) {
+static int tree_attention(bool whole, const void* q, int dtype, int64_t num_tokens, int64_t batch,
+                          const int64_t* cu_q, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                          const void* k_pool, const void* v_pool, int64_t num_blocks, int32_t block_size,
+                          const int32_t* block_table, int64_t max_blocks, const int64_t* kv_len,
+                          const int64_t* tree_mask, int32_t mask_words, float scale, void* workspace,
+                          size_t workspace_bytes, void* out, int32_t* error, sdx_stream_t stream) {
   if (num_tokens < 0 || batch < 0 || num_q_heads < 1 || num_kv_heads < 1 || block_size < 1 ||
       max_blocks < 1 || num_blocks < 1 || mask_words < 1 || !(scale > 0.0f) ||
       !(scale * 1.4426950408889634f < INFINITY))
@@ -1545,8 +1545,30 @@ int sdx_tree_attention_paged(const void* q, int dtype, int64_t num_tokens, int64
   a.batch = batch; a.tokens = num_tokens; a.max_blocks = max_blocks; a.num_blocks = num_blocks;
   a.hq = num_q_heads; a.hkv = num_kv_heads; a.group = num_q_heads / num_kv_heads; a.bs = block_size;
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.out = (uint16_t*)out; a.error = error;
+  a.out = (uint16_t*)out; a.whole = whole; a.error = error;
   return hip_status(sdx::launch_tree_attn(dtype, head_dim, a, (hipStream_t)stream), "tree_attn");
+}
+int sdx_tree_attention_paged(const void* q, int dtype, int64_t num_tokens, int64_t batch,
+                             const int64_t* cu_q, int32_t num_q_heads, int32_t num_kv_heads,
+                             int32_t head_dim, const void* k_pool, const void* v_pool,
+                             int64_t num_blocks, int32_t block_size, const int32_t* block_table,
+                             int64_t max_blocks, const int64_t* kv_len, const int64_t* tree_mask,
+                             int32_t mask_words, float scale, void* workspace, size_t workspace_bytes,
+                             void* out, int32_t* error, sdx_stream_t stream) {
+  return tree_attention(false, q, dtype, num_tokens, batch, cu_q, num_q_heads, num_kv_heads, head_dim, k_pool,
+                        v_pool, num_blocks, block_size, block_table, max_blocks, kv_len, tree_mask, mask_words,
+                        scale, workspace, workspace_bytes, out, error, stream);
+}
+int sdx_tree_attention_paged_whole(const void* q, int dtype, int64_t num_tokens, int64_t batch,
+                                   const int64_t* cu_q, int32_t num_q_heads, int32_t num_kv_heads,
+                                   int32_t head_dim, const void* k_pool, const void* v_pool,
+                                   int64_t num_blocks, int32_t block_size, const int32_t* block_table,
+                                   int64_t max_blocks, const int64_t* kv_len, const int64_t* tree_mask,
+                                   int32_t mask_words, float scale, void* workspace, size_t workspace_bytes,
+                                   void* out, int32_t* error, sdx_stream_t stream) {
+  return tree_attention(true, q, dtype, num_tokens, batch, cu_q, num_q_heads, num_kv_heads, head_dim, k_pool,
+                        v_pool, num_blocks, block_size, block_table, max_blocks, kv_len, tree_mask, mask_words,
+                        scale, workspace, workspace_bytes, out, error, stream);
 }
 
 }  // extern "C"

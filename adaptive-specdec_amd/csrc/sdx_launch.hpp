@@ -663,9 +663,11 @@ struct TreeAttnArgs {
   TreeAttnDiv by_bs, by_group; // (set by the launch)
   float scale_log2;            // softmax scale * log2(e)
   uint16_t* out;               // [tokens, hq, d]
+  bool whole;                  // 0 where nothing is computed, else left as it was
   int32_t* error;
   TreeAttnItem* items;         // [max_items]
   int64_t max_items;
+  int32_t* left;               // with whole: 1 rows are refused, 2 all are
   float2* part_ml;             // [2 TREE_ATTN_GRID, TREE_ATTN_ROWS] max and sum of each part's query rows
   float* part_o;               // [2 TREE_ATTN_GRID, TREE_ATTN_ROWS, d]
 };

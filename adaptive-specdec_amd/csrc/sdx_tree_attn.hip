@@ -51,7 +51,7 @@ struct TaRow {
   int32_t t0, ctx;      // first node's token; keys in front of the nodes
   int32_t n, ct, kt;    // nodes; tiles of the cache, and with the nodes'
   int32_t qt;           // tiles of query rows
-  bool ok;
+  bool ok, back;        // back: its offsets descend
   __device__ __forceinline__ uint32_t len() const { return (uint32_t)kt + TA_COST; }
 };
 __device__ __forceinline__ TaRow ta_row(const TreeAttnArgs& a, int64_t b) {
@@ -59,6 +59,7 @@ __device__ __forceinline__ TaRow ta_row(const TreeAttnArgs& a, int64_t b) {
   const int64_t t0 = a.cu_q[b], t1 = a.cu_q[b + 1], kv = a.kv_len[b], n = t1 - t0;
   r.ok = t0 >= 0 && n >= 0 && t1 <= a.tokens && n <= min(a.words * 64, TREE_MAX_NODES) && kv >= n &&
          kv <= a.max_blocks * a.bs;  // 2^30 keys, 2^23 tokens at most
+  r.back = n < 0;
   r.t0 = (int32_t)t0;
   r.n = r.ok ? (int32_t)n : 0;
   r.ctx = r.ok ? (int32_t)(kv - n) : 0;
@@ -241,19 +242,23 @@ tree_attn_kernel(TreeAttnArgs a) {
   uint32_t item0 = 0, items;
   int64_t b = 0;
   TaRow row = {};
+  // for an output that is written whole: rows are refused, all of them are (offsets that descend may
+  // name a token twice)
+  bool refused = false, none = false;
   // Up to 64 rows, that is a row per lane, each wave does it by itself (a third of what the barriers
   // and the long code of any number of rows take, 2 us)
   bool quick = a.batch <= kWave;
   if (quick) {
-    row = lane < a.batch ? ta_row(a, lane) : TaRow{0, 0, 0, 0, 0, 0, true};
+    row = lane < a.batch ? ta_row(a, lane) : TaRow{0, 0, 0, 0, 0, 0, true, false};
     const uint32_t n = ta_items(a, row);
     const uint64_t tiles = (uint64_t)n * row.len();
     quick = !__any(tiles >> 25 != 0);
     if (quick) {  // uniform
       const uint32_t line = (uint32_t)tiles, li = wave_incl_scan_u32(line, lane), ii = wave_incl_scan_u32(n, lane);
       items = rdlane(ii, kWave - 1);
-      const bool over = items > (uint64_t)a.max_items;
-      if ((__any(!row.ok) || over) && a.error && blockIdx.x == 0) *a.error = 1;
+      const bool over = items > (uint64_t)a.max_items || (a.whole && __any(row.back));
+      refused = __any(!row.ok), none = over;
+      if ((refused || over) && a.error && blockIdx.x == 0) *a.error = 1;
       items = over ? 0 : items;
       total = over ? 0 : rdlane(li, kWave - 1);
       step = max(total / TA_GRID + (total % TA_GRID > 0), TA_LEAST);
@@ -265,7 +270,7 @@ tree_attn_kernel(TreeAttnArgs a) {
         item0 = rdlane(ii - n, at);
         b = at;
         row = TaRow{(int32_t)rdlane(row.t0, at), (int32_t)rdlane(row.ctx, at), (int32_t)rdlane(row.n, at),
-                    (int32_t)rdlane(row.ct, at), (int32_t)rdlane(row.kt, at), (int32_t)rdlane(row.qt, at), true};
+                    (int32_t)rdlane(row.ct, at), (int32_t)rdlane(row.kt, at), (int32_t)rdlane(row.qt, at), true, false};
       } else {
         pos = total;
       }
@@ -274,16 +279,21 @@ tree_attn_kernel(TreeAttnArgs a) {
   if (!quick) {
     const bool one = a.batch <= TA_NT;
     uint64_t line = 0, n = 0;
-    int bad = 0;
+    int bad = 0, back = 0;
     for (int64_t i = tid; i < a.batch; i += TA_NT) {
       const TaRow r = ta_row(a, i);
       bad |= !r.ok;
+      back |= r.back;
       line += (uint64_t)ta_items(a, r) * r.len();
       n += ta_items(a, r);
     }
     TaScan sc = ta_scan(line, n, sLine, sItem);
     // rows that share nodes (offsets out of order); a line of 2^32 tiles takes half a minute
-    const bool over = sc.items > (uint64_t)a.max_items || sc.lines >> 32;
+    bool over = sc.items > (uint64_t)a.max_items || sc.lines >> 32;
+    if (a.whole) {  // uniform
+      refused = __syncthreads_or(bad);
+      none = over = over || (refused && __syncthreads_or(back));
+    }
     if ((bad || over) && a.error && blockIdx.x == 0) *a.error = 1;
     items = over ? 0 : (uint32_t)sc.items;
     total = over ? 0 : (uint32_t)sc.lines;
@@ -314,6 +324,7 @@ tree_attn_kernel(TreeAttnArgs a) {
   }
   for (int64_t i = (int64_t)items + blockIdx.x * TA_NT + tid; i < a.max_items; i += TA_GRID * TA_NT)
     a.items[i].parts = 0;  // records of no item
+  if (a.whole && blockIdx.x == 0 && tid == 0) *a.left = none ? 2 : refused;
   if (pos >= total) return;  // uniform
   const uint32_t end = min((uint64_t)total, (uint64_t)pos + step);
 
@@ -512,14 +523,41 @@ tree_attn_kernel(TreeAttnArgs a) {
   }
 }
 
+// Tokens t0 .. t1 - 1 of out become 0, by `parts` workgroups, of which this is one.
+template <int D>
+__device__ __forceinline__ void ta_zero(const TreeAttnArgs& a, int64_t t0, int64_t t1, uint32_t part, uint32_t parts) {
+  const int64_t units = (int64_t)a.hq * (D / 8);  // of 16 bytes
+  t0 = max(t0, (int64_t)0), t1 = min(t1, a.tokens);
+  if (t0 >= t1) return;  // uniform
+  for (int64_t u = t0 * units + part * PA_NT + threadIdx.x; u < t1 * units; u += parts * PA_NT)
+    store_nt(a.out + u * 8, make_uint4(0, 0, 0, 0));
+}
+// What nothing is computed for: tokens in front of the rows and behind them, those of refused rows.
+template <int D>
+__device__ __forceinline__ void ta_rest(const TreeAttnArgs& a, uint32_t part, uint32_t parts) {
+  const int32_t left = *a.left;
+  ta_zero<D>(a, 0, left > 1 ? a.tokens : a.cu_q[0], part, parts);
+  ta_zero<D>(a, a.cu_q[a.batch], a.tokens, part, parts);
+  for (int64_t i = part; left == 1 && i < a.batch; i += parts)
+    if (!ta_row(a, i).ok) ta_zero<D>(a, a.cu_q[i], a.cu_q[i + 1], 0, 1);
+}
+
 // Join of the items that are split: out = sum_c w_c O_c, w_c = 2^(m_c - m) / sum 2^(m_c - m) l_c.
 // A workgroup has RB query rows of an item at a time; 256 / (D / 4 RB) slices of D / 4 threads
-// share a row's parts, each with a running maximum of its own, and are joined in LDS.
+// share a row's parts, each with a running maximum of its own, and are joined in LDS. TA_REST
+// workgroups behind those of the items write the rest of an output that is written whole: there they
+// hold nobody up (one tree of 26: without them 17.1 us, with them 17.4, in the kernel before 17.9).
+constexpr int TA_REST = 256;
 template <int D, int FMT, int RB>
 __global__ void __launch_bounds__(PA_NT) tree_attn_join_kernel(TreeAttnArgs a) {
   constexpr int DL = D / 4, SL = PA_NT / DL / RB, UN = SL > 1 ? 4 : 2;
   __shared__ float4 sO[SL][RB][DL];
   __shared__ float2 sML[SL][RB];
+  if (blockIdx.x >= a.max_items) {  // uniform
+    ta_rest<D>(a, (blockIdx.x - (uint32_t)a.max_items) * gridDim.y + blockIdx.y,
+               (gridDim.x - (uint32_t)a.max_items) * gridDim.y);
+    return;
+  }
   const TreeAttnItem x = a.items[blockIdx.x];
   if (x.parts < 2) return;  // uniform: written directly, or no item
   const int tid = threadIdx.x, d4 = tid % DL, rr = tid / DL % RB, sl = tid / DL / RB;
@@ -599,7 +637,8 @@ int64_t tree_attn_items(int64_t tokens, int64_t batch, int32_t hkv, int32_t grou
 template <int D, int FMT, int RB>
 static void launch_join(const TreeAttnArgs& a, int64_t items, hipStream_t s) {
   const unsigned blocks = RB >= 8 ? TA_ROWS / RB / 2 : TA_ROWS / RB;
-  hipLaunchKernelGGL((tree_attn_join_kernel<D, FMT, RB>), dim3((unsigned)items, blocks), dim3(PA_NT), 0, s, a);
+  const unsigned columns = (unsigned)items + (a.whole ? TA_REST / blocks : 0);
+  hipLaunchKernelGGL((tree_attn_join_kernel<D, FMT, RB>), dim3(columns, blocks), dim3(PA_NT), 0, s, a);
 }
 
 template <int D, int FMT>

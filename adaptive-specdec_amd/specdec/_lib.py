@@ -81,6 +81,8 @@ _SIGS = {
                                   I32, P, I64, P, P, I32, P, P]),
     "sdx_tree_attention_paged": (INT, [P, INT, I64, I64, P, I32, I32, I32, P, P, I64, I32, P, I64, P, P, I32, F,
                                        P, SZ, P, P, P]),
+    "sdx_tree_attention_paged_whole": (INT, [P, INT, I64, I64, P, I32, I32, I32, P, P, I64, I32, P, I64, P, P,
+                                             I32, F, P, SZ, P, P, P]),
     "sdx_tree_attention_workspace": (SZ, [I64, I64, I32, I32, I32]),
     "sdx_tree_layout": (INT, [P, I64, P, P, I32, P, I64, I32, I64, I64, P, P, P, P, P]),
     "sdx_tree_accept": (INT, [P, P, P, I64, P, I64, P, I64, P, P, P, P, P]),

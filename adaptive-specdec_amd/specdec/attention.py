@@ -173,9 +173,11 @@ def tree_attention_paged(q, cu_q, k_pool, v_pool, block_table, kv_len, tree_mask
     its last, included; tree_mask [T, words] int64 of `specdec.tree.tree_layout` (n_b up to 64
     words and 512). Node i sees the kv_len[b] - n_b keys in front of the nodes and every node
     j whose bit j % 64 of word j / 64 is set. Returns out [T, Hq, d] of q's type, 0 for a node that
-    sees nothing; nodes behind cu_q[B] are left as they were. Rows out of range are skipped and set `error` (an int32 [1] device tensor) when given, and so do
-    page ids outside the pool. `workspace` (uint8, `tree_attention_workspace`) holds fp32 parts and serves one
-    call at a time; None: the calling thread's own for the current stream, kept for its next calls."""
+    sees nothing. Rows out of range are skipped and set `error` (an int32 [1] device tensor) when
+    given, and so do page ids outside the pool. The nodes of such rows and those behind cu_q[B] are left
+    as they were in an `out` that is given, and are 0 in one that is allocated here (where offsets that
+    descend skip all rows). `workspace` (uint8, `tree_attention_workspace`) holds fp32 parts and serves
+    one call at a time; None: the calling thread's own for the current stream, kept for its next calls."""
     _lib.one_gpu(q, cu_q, k_pool, v_pool, block_table, kv_len, tree_mask, out, error, workspace)
     if q.dtype not in (torch.bfloat16, torch.float16) or k_pool.dtype != q.dtype or \
             v_pool.dtype != q.dtype:
@@ -201,8 +203,10 @@ def tree_attention_paged(q, cu_q, k_pool, v_pool, block_table, kv_len, tree_mask
             tree_mask.shape[1] < 1:
         raise ValueError(f"tree_attention_paged: tree_mask must be int64 [{T}, words], got "
                          f"{tree_mask.dtype} {tuple(tree_mask.shape)}")
+    call = _lib.lib().sdx_tree_attention_paged
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        call = _lib.lib().sdx_tree_attention_paged_whole
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError("tree_attention_paged: out must be contiguous, of q's shape and type")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
@@ -221,7 +225,7 @@ def tree_attention_paged(q, cu_q, k_pool, v_pool, block_table, kv_len, tree_mask
         if workspace is None:
             need = _lib.workspace_bytes("sdx_tree_attention_workspace", T, B, hq, hkv, d)
             workspace = _lib.cached_workspace(need, q.device, "tree_attn")
-        rc = _lib.lib().sdx_tree_attention_paged(
+        rc = call(
             _lib.ptr(q), _lib.dtype_code(q), T, B, _lib.ptr(cu), hq, hkv, d, _lib.ptr(k_pool),
             _lib.ptr(v_pool), nb, bs, _lib.ptr(bt), bt.shape[1], _lib.ptr(kl), _lib.ptr(tm), tm.shape[1],
             scale, _lib.ptr(workspace), workspace.numel(), _lib.ptr(out), _lib.ptr(error),

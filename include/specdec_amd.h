@@ -628,6 +628,15 @@ int sdx_tree_attention_paged(const void* q, int dtype, int64_t num_tokens, int64
                              int64_t max_blocks, const int64_t* kv_len, const int64_t* tree_mask,
                              int32_t mask_words, float scale, void* workspace, size_t workspace_bytes,
                              void* out, int32_t* error, sdx_stream_t stream);
+/* The same, with out written whole: 0 for tokens of no row and of rows that are refused, for memory
+ * that holds something else. Offsets that descend refuse all rows here. */
+int sdx_tree_attention_paged_whole(const void* q, int dtype, int64_t num_tokens, int64_t batch,
+                                   const int64_t* cu_q, int32_t num_q_heads, int32_t num_kv_heads,
+                                   int32_t head_dim, const void* k_pool, const void* v_pool,
+                                   int64_t num_blocks, int32_t block_size, const int32_t* block_table,
+                                   int64_t max_blocks, const int64_t* kv_len, const int64_t* tree_mask,
+                                   int32_t mask_words, float scale, void* workspace, size_t workspace_bytes,
+                                   void* out, int32_t* error, sdx_stream_t stream);
 size_t sdx_tree_attention_workspace(int64_t num_tokens, int64_t batch, int32_t num_q_heads,
                                     int32_t num_kv_heads, int32_t head_dim);
 

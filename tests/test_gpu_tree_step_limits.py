@@ -193,6 +193,67 @@ def test_only_whole_numbers_are_taken_for_whole_numbers():
                     call(**{**args, name: args[name].to(dtype)})
 
 
+# ---- outputs that nothing is computed for
+
+def call_over_nan(c, **more):
+    """The call, with NaN in all memory that it allocates."""
+    torch.use_deterministic_algorithms(True, warn_only=True)
+    try:
+        assert torch.empty_like(c["q"]).isnan().all()
+        return tree_attention_paged(**c, **more)
+    finally:
+        torch.use_deterministic_algorithms(False)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n,start", [([5, 9, 4], [100, 20, 0]), ([3] * 70, [5] * 70), ([1] * 600, [7] * 600),
+                                     ([0, 0], [4, 4]), ([300], [50])])
+def test_an_allocated_output_is_0_where_nothing_is_computed(n, start, d):
+    c = attention_case(n, start, d=d, pad=37)
+    T = int(c["cu_q"][-1])
+    want = torch.full_like(c["q"], 7.0)
+    tree_attention_paged(**c, out=want)
+    assert (want[T:] == 7).all()                          # a given one is left as it was
+    want[T:] = 0
+    assert torch.equal(call_over_nan(c), want)
+    if T == 0:
+        return
+    # a row that is refused, a token in front of the first row
+    b = len(n) - 1
+    a, e = c["cu_q"].tolist()[b:b + 2]
+    bad = dict(c, kv_len=c["kv_len"].clone())
+    bad["kv_len"][b] = -3
+    err = new_error()
+    got = call_over_nan(bad, error=err)
+    assert err.item() == 1 and (got[a:e] == 0).all() and (got[T:] == 0).all()
+    given = torch.full_like(c["q"], 7.0)
+    tree_attention_paged(**bad, out=given)
+    assert (given[a:e] == 7).all() and torch.equal(given[:a], got[:a])
+    if n[0] > 1:
+        assert (call_over_nan(dict(c, cu_q=c["cu_q"].clamp(min=1)))[0] == 0).all()
+
+
+def test_an_allocated_output_of_rows_that_share_nodes_is_0():
+    c = shared_nodes(40)
+    assert (call_over_nan(c) == 0).all()
+
+
+def test_padding_of_an_allocated_output_in_a_graph():
+    c = attention_case([5, 9], [100, 20], pad=9)
+    call_over_nan(c)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = tree_attention_paged(**c)
+    for last in (14, 11, 5, 14):
+        c["cu_q"][2] = last
+        c["kv_len"][1] = 20 + last - 5
+        out.fill_(float("nan"))
+        g.replay()
+        torch.cuda.synchronize()
+        assert (out[last:] == 0).all() and torch.equal(out, tree_attention_paged(**c))
+
+
 # ---- rows that share their nodes
 
 def shared_nodes(B):

@@ -1,8 +1,9 @@
-"""CPU checks of arguments of the page operators that lie over one another: the C entry points
-return their status before anything is launched (the pointers are never dereferenced)."""
+"""CPU checks of arguments of the page operators that lie over one another, and of the attention that
+writes its output whole: the C entry points return their status before anything is launched (the
+pointers are never dereferenced)."""
 import ctypes
 
-OK, EINVAL = 0, -1
+OK, EINVAL, EUNSUP, EWS = 0, -1, -2, -4
 
 
 def test_compact_does_not_write_what_it_reads():
@@ -48,3 +49,20 @@ def test_forked_tables_do_not_lie_over_what_is_read():
             for where in (at, at + n - 4, at - size + 4):
                 assert call(**{name: where}) == EINVAL, (name, at, where)
                 assert b"may not lie over" in L.sdx_last_error()
+
+
+def test_the_attention_that_writes_its_output_whole_refuses_alike():
+    from specdec import _lib
+    L = _lib.lib()
+    fake, off = ctypes.c_void_p(4096), ctypes.c_void_p(4104)
+
+    def call(T=3, B=2, hq=4, hkv=2, d=64, mb=4, scale=0.1, out=fake, nbytes=None):
+        need = L.sdx_tree_attention_workspace(max(T, 1), max(B, 1), max(hq, 1), max(hkv, 1), d)
+        return L.sdx_tree_attention_paged_whole(
+            fake, 1, T, B, fake, hq, hkv, d, fake, fake, 8, 16, fake, mb, fake, fake, 1, scale, fake,
+            need if nbytes is None else nbytes, out, None, None)
+
+    assert call(T=0) == OK
+    for bad in (dict(T=-1), dict(B=0), dict(hq=3), dict(scale=0.0), dict(out=None), dict(out=off)):
+        assert call(**bad) == EINVAL, bad
+    assert call(d=96) == EUNSUP and call(mb=1 << 28) == EUNSUP and call(nbytes=64) == EWS
