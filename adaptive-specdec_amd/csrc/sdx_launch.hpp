@@ -605,11 +605,13 @@ struct FreePagesArgs {
   int32_t parts;
   int64_t words;                // of 32 pages
   uint32_t* bits;               // [parts, words]
+  uint32_t* counts;             // [segments] free pages of each
   int32_t* free_blocks;         // [num_blocks]
   int64_t* num_free;
   int32_t* error;
 };
 int free_pages_parts(int64_t entries, int64_t words);
+int64_t free_pages_segments(int64_t num_blocks);
 hipError_t launch_free_pages(const FreePagesArgs& a, hipStream_t s);
 struct ForkArgs {
   const int32_t* table;         // [old_batch, max_blocks]

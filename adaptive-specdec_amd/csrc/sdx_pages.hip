@@ -118,7 +118,10 @@ __global__ void __launch_bounds__(PGS_NT) compact_paged_kernel(CompactArgs a) {
 // few dependent loads and of two launches.
 constexpr int FP_NT = 512;
 constexpr int FP_SEG = 8192;  // pages that a workgroup of the second kernel lists
-constexpr int64_t FP_JOIN = 1 << 22;  // words read by all workgroups of the list, of which the join is cheaper
+// Words that all workgroups of the list read (a square of the pages), beyond which a kernel that counts
+// is cheaper. 320 entries, without it and with it: 2^18 pages 13.9 and 10.5 us, 2^20 30.4 and 11.0, 2^24 787
+// and 35; 115,200 entries and 2^15 pages 15.3 and 13.0; 2^17 pages of 320 entries (at the rule) 10.7 without.
+constexpr int64_t FP_JOIN = 1 << 16;
 
 // The bits of pages base .. in sBits, from the workgroup's share of the tables.
 __device__ __forceinline__ void fp_mark(const FreePagesArgs& a, int64_t base, int words, uint32_t* sBits) {
@@ -156,15 +159,32 @@ __global__ void __launch_bounds__(FP_NT) free_pages_mark_kernel(FreePagesArgs a)
   for (int w = tid; w < words; w += FP_NT) out[w] = sBits[w];
 }
 
-// Many pages: the parts are joined once, in the place of the first, and not by every workgroup of
-// the list.
-__global__ void __launch_bounds__(FP_NT) free_pages_join_kernel(FreePagesArgs a) {
-  const int64_t w = (int64_t)blockIdx.x * FP_NT + threadIdx.x;
-  if (w >= a.words) return;
+// Many pages: the parts are joined once, in the place of the first, and every segment's free pages
+// counted, a workgroup each; a workgroup of the list then adds up counts and not all pages.
+constexpr int FP_SW = FP_SEG / 32;  // words of a segment
+__device__ __forceinline__ uint32_t fp_free(const FreePagesArgs& a, int64_t w) {  // word w's free pages
   uint32_t held = 0;
 #pragma unroll 8
   for (int p = 0; p < a.parts; ++p) held |= a.bits[p * a.words + w];
-  a.bits[w] = held;
+  const int64_t left = a.num_blocks - w * 32;
+  return ~held & (left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1u);
+}
+__global__ void __launch_bounds__(FP_SW) free_pages_count_kernel(FreePagesArgs a) {
+  constexpr int NW = FP_SW / kWave;
+  __shared__ uint32_t sSum[NW];
+  const int tid = threadIdx.x;
+  const int64_t w = (int64_t)blockIdx.x * FP_SW + tid;
+  const uint32_t mine = w < a.words ? fp_free(a, w) : 0u;
+  if (w < a.words) a.bits[w] = ~mine;
+  const uint32_t n = (uint32_t)wave_sum_u64(__popc(mine));
+  if (tid % kWave == 0) sSum[tid / kWave] = n;
+  __syncthreads();
+  if (tid == 0) {
+    uint32_t sum = 0;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) sum += sSum[k];
+    a.counts[blockIdx.x] = sum;
+  }
 }
 
 // Few pages and few entries: one workgroup, a word per thread, does both.
@@ -195,28 +215,29 @@ __global__ void __launch_bounds__(FP_NT) free_pages_small_kernel(FreePagesArgs a
   }
 }
 
+template <bool COUNTED>
 __global__ void __launch_bounds__(FP_NT) free_pages_list_kernel(FreePagesArgs a) {
-  constexpr int SW = FP_SEG / 32, NW = FP_NT / kWave;
+  constexpr int SW = FP_SW, NW = FP_NT / kWave;
   static_assert(SW <= FP_NT, "a word per thread");
   __shared__ uint32_t sFree[SW], sAt[SW], sWave[NW];
   __shared__ uint64_t sSum[NW][2];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wv = tid / kWave;
   const int64_t w0 = (int64_t)blockIdx.x * SW;
-  // free pages of word w
-  auto word = [&](int64_t w) {
-    uint32_t held = 0;
-#pragma unroll 8
-    for (int p = 0; p < a.parts; ++p) held |= a.bits[p * a.words + w];
-    const int64_t left = a.num_blocks - w * 32;
-    return ~held & (left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1u);
-  };
   uint64_t before = 0, total = 0;
-  for (int64_t w = tid; w < a.words; w += FP_NT) {
-    const uint32_t n = (uint32_t)__popc(word(w));
-    total += n;
-    if (w < w0) before += n;
+  if constexpr (COUNTED) {
+    for (int64_t k = tid; k < gridDim.x; k += FP_NT) {
+      const uint32_t n = a.counts[k];
+      total += n;
+      if (k < blockIdx.x) before += n;
+    }
+  } else {
+    for (int64_t w = tid; w < a.words; w += FP_NT) {
+      const uint32_t n = (uint32_t)__popc(fp_free(a, w));
+      total += n;
+      if (w < w0) before += n;
+    }
   }
-  const uint32_t mine = tid < SW && w0 + tid < a.words ? word(w0 + tid) : 0u;
+  const uint32_t mine = tid < SW && w0 + tid < a.words ? fp_free(a, w0 + tid) : 0u;
   const uint32_t n = (uint32_t)__popc(mine);
   const uint32_t inc = wave_incl_scan_u32(n, lane);
   total = wave_sum_u64(total);
@@ -489,6 +510,8 @@ int free_pages_parts(int64_t entries, int64_t words) {
   return (int)std::max<int64_t>(1, std::min<int64_t>({64, entries / 1024, (1 << 22) / words}));
 }
 
+int64_t free_pages_segments(int64_t num_blocks) { return (num_blocks + FP_SEG - 1) / FP_SEG; }
+
 hipError_t launch_free_pages(const FreePagesArgs& a, hipStream_t s) {
   // One part (under 2,048 entries) and a word per thread: in one kernel 912 entries and 900 pages take
   // 3.2 us, in two 4.9; at the end of the rule, 16,384 pages, 7.3 and 7.5.
@@ -500,15 +523,17 @@ hipError_t launch_free_pages(const FreePagesArgs& a, hipStream_t s) {
   hipLaunchKernelGGL(free_pages_mark_kernel, dim3(ranges, (unsigned)a.parts), dim3(FP_NT), 0, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int64_t segments = (a.num_blocks + FP_SEG - 1) / FP_SEG;
-  FreePagesArgs b = a;
-  if (a.parts > 1 && a.parts * a.words * segments > FP_JOIN) {
-    hipLaunchKernelGGL(free_pages_join_kernel, dim3((unsigned)((a.words + FP_NT - 1) / FP_NT)), dim3(FP_NT), 0, s, a);
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    b.parts = 1;
+  const int64_t segments = free_pages_segments(a.num_blocks);
+  if (a.parts * a.words * segments <= FP_JOIN) {
+    hipLaunchKernelGGL(free_pages_list_kernel<false>, dim3((unsigned)segments), dim3(FP_NT), 0, s, a);
+    return hipGetLastError();
   }
-  hipLaunchKernelGGL(free_pages_list_kernel, dim3((unsigned)segments), dim3(FP_NT), 0, s, b);
+  hipLaunchKernelGGL(free_pages_count_kernel, dim3((unsigned)segments), dim3(FP_SW), 0, s, a);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  FreePagesArgs b = a;
+  b.parts = 1;
+  hipLaunchKernelGGL(free_pages_list_kernel<true>, dim3((unsigned)segments), dim3(FP_NT), 0, s, b);
   return hipGetLastError();
 }
 

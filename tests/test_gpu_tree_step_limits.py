@@ -302,3 +302,24 @@ def test_kept_may_be_keep_itself():
     with pytest.raises(RuntimeError, match="apart"):
         compact_paged(pool, dev(table, torch.int32), s, dev(path), dev(keep), kept=s)
     assert torch.equal(pool.cpu(), want) and s.tolist() == start.tolist()
+
+
+# ---- lists of many pages
+
+@pytest.mark.parametrize("nb,B,mb", [(1 << 17, 8, 40), ((1 << 17) + 1, 8, 40), (20_000, 70, 300), (3_000_017, 40, 100),
+                                     (1_300_000, 900, 300), (20_000_003, 5, 7)])
+def test_free_pages_of_large_pools(nb, B, mb):
+    """At the ends of the forms: segments that are added up page by page, and by their counts."""
+    g = torch.Generator(device=DEV).manual_seed(nb)
+    table = torch.randint(0, nb, (B, mb), generator=g, device=DEV)
+    table[0, 0], table[-1, -1], table[0, 1:3] = nb - 1, 0, 8191
+    kv = torch.randint(0, mb * 16 + 1, (B,), generator=g, device=DEV)
+    kv[0], kv[-1] = mb * 16, mb * 16
+    held = torch.zeros(nb, dtype=torch.bool, device=DEV)
+    at = torch.arange(mb, device=DEV) < ((kv + 15) // 16)[:, None]
+    held[table[at]] = True
+    want = (~held).nonzero().view(-1)
+    err = new_error()
+    free, num = free_page_list(table.int(), nb, kv_len=kv, block_size=16, error=err)
+    assert err.item() == 0 and num.item() == want.numel()
+    assert torch.equal(free[:want.numel()].long(), want) and (free[want.numel():] == -1).all()

@@ -66,3 +66,19 @@ def test_the_attention_that_writes_its_output_whole_refuses_alike():
     for bad in (dict(T=-1), dict(B=0), dict(hq=3), dict(scale=0.0), dict(out=None), dict(out=off)):
         assert call(**bad) == EINVAL, bad
     assert call(d=96) == EUNSUP and call(mb=1 << 28) == EUNSUP and call(nbytes=64) == EWS
+
+
+def test_free_pages_of_many_pages_and_entries():
+    """The tables are gone through once for every 2^18 pages: large pools behind large tables are refused,
+    each of them by itself is not."""
+    from specdec import _lib
+    L = _lib.lib()
+    fake = ctypes.c_void_p(4096)
+
+    def call(B, mb, nb, nbytes=16):                    # (a workspace that is too small: nothing is launched)
+        return L.sdx_free_pages(fake, B, mb, fake, 16, nb, fake, fake, fake, nbytes, None, None)
+
+    assert call(1 << 15, 1 << 16, 1 << 23) == EWS and call(1 << 15, 1 << 16, (1 << 23) + 1) == EUNSUP
+    assert call(1 << 8, 1 << 16, 1 << 30) == EWS and call((1 << 8) + 1, 1 << 16, 1 << 30) == EUNSUP
+    assert L.sdx_free_pages_workspace(1 << 8, 1 << 16, 1 << 30) > 0
+    assert L.sdx_free_pages_workspace((1 << 8) + 1, 1 << 16, 1 << 30) == 0
