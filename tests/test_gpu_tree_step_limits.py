@@ -323,3 +323,56 @@ def test_free_pages_of_large_pools(nb, B, mb):
     free, num = free_page_list(table.int(), nb, kv_len=kv, block_size=16, error=err)
     assert err.item() == 0 and num.item() == want.numel()
     assert torch.equal(free[:want.numel()].long(), want) and (free[want.numel():] == -1).all()
+
+
+# ---- sizes past 32 bits
+
+def test_pages_past_32_bits_are_moved_and_copied():
+    """Sides of 2.6 GB, a pool of 10 GB: pages at its ends and where 2^32 and 2^33 bytes lie."""
+    L, nb, bs, re = 2, 40000, 16, 2048
+    pool = torch.zeros((L, 2, nb, bs, re), dtype=torch.bfloat16, device=DEV)
+    page = bs * re * 2
+    assert pool.numel() * 2 > 2 ** 33
+    near = sorted({p for e in (31, 32, 33) for s in range(4) for p in range((2 ** e - s * nb * page) // page - 1,
+                                                                            (2 ** e - s * nb * page) // page + 2)
+                   if 0 <= p < nb} | {0, 1, nb - 2, nb - 1})
+    assert len(near) >= 8
+    small = torch.randn((L, 2, len(near), bs, re), device=DEV).bfloat16()
+    pool[:, :, near] = small
+    n = len(near) // 2
+    table = np.arange(2 * n).reshape(n, 2)[:, ::-1]        # rows of two pages, in the small pool and in the large
+    start, path, keep = np.full(n, 10), np.tile([0, 3, 4, 7, 20], (n, 1)), np.full(n, 5)
+    want = small.cpu()
+    assert OT.compact(want, table, start, path, keep)
+    err = new_error()
+    compact_paged(pool, dev(np.asarray(near)[table], torch.int32), dev(start), dev(path), dev(keep), error=err)
+    assert torch.equal(pool[:, :, near].cpu(), want) and err.item() == 0
+    half = len(near) // 2
+    copies = np.stack([np.arange(half), np.arange(half, 2 * half), 1 + np.arange(half) % bs])
+    for s, d, t in copies.T:
+        want[:, :, d, :t] = want[:, :, s, :t]
+    copies[:2] = np.asarray(near)[copies[:2]]
+    copy_pages(pool, dev(copies, torch.int32), error=err)
+    assert torch.equal(pool[:, :, near].cpu(), want) and err.item() == 0
+    pool[:, :, near] = 0
+    assert not pool.any()                                 # nothing else
+
+
+def test_logits_past_32_bits_of_elements():
+    R, V = 17000, 131071                                  # 2.2e9 logits, rows off alignment
+    assert R * V > 2 ** 31
+    g = torch.Generator(device=DEV).manual_seed(1)
+    line = torch.randn(V, generator=g, device=DEV).bfloat16()
+    x = line.repeat(R, 1)
+    hist = torch.randint(0, V, (R, 4), generator=g, device=DEV)
+    c = dict(history_len=torch.full((R,), 4, device=DEV), repetition=torch.full((R,), 1.3, device=DEV),
+             presence=torch.full((R,), 0.5, device=DEV))
+    err = new_error()
+    assert penalize_logits(x, hist, **c, out=x, error=err) is x and err.item() == 0
+    rows = [0, 1, R // 2, 2 ** 31 // V - 1, 2 ** 31 // V, 2 ** 31 // V + 1, R - 2, R - 1]
+    few = penalize_logits(line.repeat(len(rows), 1), hist[rows], **{k: v[rows] for k, v in c.items()})
+    assert torch.equal(x[rows], few)
+    changed = torch.zeros(R, dtype=torch.int64, device=DEV)
+    for r0 in range(0, R, 1000):
+        changed[r0:r0 + 1000] = (x[r0:r0 + 1000] != line).sum(1)
+    assert (changed <= 4).all() and (changed > 0).all()
