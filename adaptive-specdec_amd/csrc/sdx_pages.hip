@@ -19,8 +19,9 @@ __device__ __forceinline__ uint8_t* pgs_side(uint8_t* pool, int64_t layer_bytes,
 
 // Work on n items in every (layer, side): groups of LS sides go to the XCDs in turn (workgroup % 8),
 // so that an XCD's translations are those of its own sides. 64 rows of up to 64 nodes in 64 layers
-// of 8 heads of 128 are compacted in 14.8 us, without it in 17.6; the pages of 48 groups of 8 beams
-// are freed, forked and copied in 39 us, without it in 55. The workgroup's item, and its first side.
+// of 8 heads of 128 are compacted in 14.8 us, without it in 17.6; when the pages of 48 groups of 8 beams
+// were freed, forked and copied in 39 us (now 40), they took 55 without it. The workgroup's item, and
+// its first side.
 __device__ __forceinline__ int64_t pgs_item(int64_t n, int LS, int& ls0) {
   const uint32_t k = blockIdx.x / 8, g = k / (uint32_t)n;
   ls0 = (int)(g * 8 + blockIdx.x % 8) * LS;
@@ -121,7 +122,7 @@ constexpr int FP_SEG = 8192;  // pages that a workgroup of the second kernel lis
 // Words that all workgroups of the list read (a square of the pages), beyond which a kernel that counts
 // is cheaper. 320 entries, without it and with it: 2^18 pages 13.9 and 10.5 us, 2^20 30.4 and 11.0, 2^24 787
 // and 35; 115,200 entries and 2^15 pages 15.3 and 13.0; 2^17 pages of 320 entries (at the rule) 10.7 without.
-constexpr int64_t FP_JOIN = 1 << 16;
+constexpr int64_t FP_COUNT = 1 << 16;
 
 // The bits of pages base .. in sBits, from the workgroup's share of the tables.
 __device__ __forceinline__ void fp_mark(const FreePagesArgs& a, int64_t base, int words, uint32_t* sBits) {
@@ -338,7 +339,7 @@ __device__ __forceinline__ int32_t fk_own(const ForkArgs& a, int64_t i, int lane
 // Free pages are taken in front of the first entry that is no page (free_page_list leaves -1 behind
 // its last one). All rows together take batch * max_blocks at most, so a wave per new row looks at
 // max_blocks of them, whatever the pool has: row i's first that is no page, as an index of its
-// share, or FK_NONE.
+// share, or FK_NONE. 1 us of a call: 16 rows of 60 pages 5.2 us without it and 6.1, 384 rows 7.8 and 8.9.
 constexpr int32_t FK_NONE = 0x7FFFFFFF;
 __device__ __forceinline__ int64_t fk_have(const ForkArgs& a) {
   return a.num_free ? min(*a.num_free, a.max_free) : a.max_free;
@@ -400,9 +401,8 @@ __device__ __forceinline__ void fk_put(const ForkArgs& a, int64_t i, int32_t x, 
   }
 }
 
-// Few rows: one workgroup, a wave per row, in place of two launches. 16 rows of 60 pages: 5.1 us and
-// 6.4, 4 rows 4.4 and 6.4; with two rows a wave, 32 of them, 8.2 and 6.3, and 16 rows of 1,024 pages
-// 8.7 and 7.8.
+// Few rows: one workgroup, a wave per row, in place of two launches. 16 rows of 60 pages: 6.1 us and
+// 7.4, 4 rows 4.8 and 7.1, 16 rows of 512 pages 8.3 and 8.6, of 1,024 11.1 and 10.1.
 constexpr int FK_SMALL = 16;
 constexpr int64_t FK_SMALL_BLOCKS = 512;
 __global__ void __launch_bounds__(FK_SMALL * kWave) fork_small_kernel(ForkArgs a) {
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(PGS_NT) fork_tables_kernel(ForkArgs a) {
 // ---- copies of pages: entry e's first tokens[e] tokens from page to page, in every layer and
 // side. They lie one behind another on both sides. Bound by HBM, stored past the L2 as above:
 // 139 copies of 1,149 tokens from 727, in 36 layers of 4 heads of 128, take 25 us (138 MB, 5.5
-// TB/s); beams freed, forked and copied through it take 63 us, not 39.
+// TB/s); beams freed, forked and copied through it took 63 us, not 39.
 constexpr int CY_LS = 1;  // 2: 42 us in place of 39
 __global__ void __launch_bounds__(PGS_NT) copy_pages_kernel(CopyPagesArgs a) {
   int ls0;
@@ -524,7 +524,7 @@ hipError_t launch_free_pages(const FreePagesArgs& a, hipStream_t s) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int64_t segments = free_pages_segments(a.num_blocks);
-  if (a.parts * a.words * segments <= FP_JOIN) {
+  if (a.parts * a.words * segments <= FP_COUNT) {
     hipLaunchKernelGGL(free_pages_list_kernel<false>, dim3((unsigned)segments), dim3(FP_NT), 0, s, a);
     return hipGetLastError();
   }

@@ -24,9 +24,12 @@
 //     TB/s and 680 TFLOP/s (large copies and products reach 5.2 and 1,254: 165 us by the bytes,
 //     135 by the products). Without its loads the kernel takes 200, the loads alone 206: they
 //     share each CU's issue and LDS, and tiles are waited for at the barriers
-//   24 trees of up to 33, contexts of up to 1,531, 14 heads on 2 of 64, fp16: 23.9 us (3.3 by the bytes)
-//   1 tree of 26 behind 2,011 keys, 32 heads on 8 of 128: 17.1 us (1.7): two launches, loads that
+//   24 trees of up to 33, contexts of up to 1,531, 14 heads on 2 of 64, fp16: 23.6 us (3.3 by the bytes)
+//   1 tree of 26 behind 2,011 keys, 32 heads on 8 of 128: 17.4 us (1.7): two launches, loads that
 //     wait for one another (lengths, pages, keys), instructions that are fetched once, the join
+//   More than 256 query rows a KV head read its keys once for every 256: 32 trees behind 8,192 keys each
+//     on 8 heads of 128, 64 nodes of 32 heads 348 us (219 by the bytes), 64 of 64 heads 657 (438 by the
+//     products), 65 of 32 heads 519 (223 by the products)
 #include <algorithm>
 #include <type_traits>
 

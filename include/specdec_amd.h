@@ -522,8 +522,9 @@ size_t sdx_free_pages_workspace(int64_t batch, int64_t max_blocks, int64_t num_b
  * first *num_free (device int64; null: max_free) of them as far as none is negative; *used (int64) =
  * how many. out is written whole, -1 behind a row's last page; out, copies and used may not lie over
  * the other arguments. All or nothing: where a parent, a length, a page of an old row or the free pages are out of range, out and
- * copies are -1 (tokens 0), *used 0 and *error (nullable) 1. Two kernels; `workspace` as the query says. Every row
- * looks at all others: 384 rows take 10 us. Up to 2^18 new rows and 2^27 columns. */
+ * copies are -1 (tokens 0), *used 0 and *error (nullable) 1. One kernel to 16 rows of up to 512 columns,
+ * else two; `workspace` as the query says. Every row looks at all others: 384 rows take 11 us. Up to 2^18
+ * new rows and 2^27 columns. */
 int sdx_fork_block_tables(const int32_t* block_table, int64_t old_batch, int64_t max_blocks,
                           const int64_t* kv_len, const int64_t* parent, const int64_t* room,
                           int64_t batch, int32_t block_size, const int32_t* free_blocks,
