@@ -1173,7 +1173,7 @@ int sdx_tree_accept(const int64_t* tokens, const int32_t* parents, const int64_t
 // ------------------------------------------------------------------ pages of the cache
 // x's first nx bytes and y's first ny have some in common
 static bool overlap(const void* x, size_t nx, const void* y, size_t ny) {
-  return x && y && (const char*)x < (const char*)y + ny && (const char*)y < (const char*)x + nx;
+  return x && y && nx && ny && (const char*)x < (const char*)y + ny && (const char*)y < (const char*)x + nx;
 }
 // pool arguments that compact and copy share
 static int pool_args(const char* who, const void* pool, int64_t layer_stride, int64_t side_stride, int dtype,

@@ -376,3 +376,17 @@ def test_logits_past_32_bits_of_elements():
     for r0 in range(0, R, 1000):
         changed[r0:r0 + 1000] = (x[r0:r0 + 1000] != line).sum(1)
     assert (changed <= 4).all() and (changed > 0).all()
+
+
+# ---- arguments that hold nothing
+
+def test_an_empty_list_lies_over_nothing():
+    """No free pages, as an empty slice of the memory that the new table is written to."""
+    out = torch.full((2, 4), 9, dtype=torch.int32, device=DEV)
+    err = new_error()
+    got, copies, used = fork_block_tables(dev([[5, 6, -1, -1]], torch.int32), dev([20]), dev([0, -1]), dev([32, 0]),
+                                          out.view(-1)[3:3], 16, out=out, error=err)
+    assert err.item() == 0 and used.item() == 0 and got.tolist() == [[5, 6, -1, -1], [-1] * 4]
+    with pytest.raises(RuntimeError, match="lie over"):
+        fork_block_tables(dev([[5, 6, -1, -1]], torch.int32), dev([20]), dev([0, -1]), dev([32, 0]),
+                          out.view(-1)[3:4], 16, out=out, error=err)
